@@ -307,6 +307,46 @@ uint32_t ptwm_b200_crc32_by_runs(const uint8_t* data, size_t len, size_t run);
 int64_t ptwm_b200_fit_shared_states_host(const uint8_t* const* planes, const uint64_t* lens, const uint32_t* row_lens, size_t n, uint8_t* out, size_t cap,
                                          uint32_t state_lens[8]);
 
+/* ---- 3. operators on decoded weights ------------------------------------- */
+
+/* Enqueued on `stream` (a cudaStream_t as an integer; 0 or 1 = the legacy default stream) and not waited for; no call
+ * allocates or synchronises, so all of them can be captured into a CUDA graph.  dtype codes: 1 fp32, 4 fp16, 6 bf16,
+ * 29 E4M3.  How 8-bit values are scaled: */
+#define PTWM_B200_SCALE_NONE  0u
+#define PTWM_B200_SCALE_ROW   1u   /* one fp32 per row */
+#define PTWM_B200_SCALE_BLOCK 2u   /* one E8M0 code per 32 values of a row */
+
+/* Root-mean-square norm of rows of `cols` values with the residual's addition:
+ *   h = x + residual, rounded to the rows' type (not written without a residual, where h = x)
+ *   y = h / sqrt(mean(h^2) + eps) * weight, sums in fp32, rounded once
+ * in the rows' type, or (scaled != SCALE_NONE) as E4M3 values with scales: per row max|y| / 448, per block the smallest
+ * power of two that keeps the block within 448.  A maximum that is not finite makes its scale and values NaN; zeros have scale 0
+ * (row) or 2^-127 (block).  All rows lie back to back; h may be x or residual. */
+int64_t ptwm_b200_rms_norm(uint64_t x, uint64_t residual, uint64_t weight, uint64_t h, uint64_t y, uint64_t scales, uint64_t rows, uint64_t cols,
+                           uint32_t dtype, uint32_t weight_dtype, uint32_t scaled, float eps, uint32_t device_ordinal, uint64_t stream);
+/* Its gradient, for an output in the rows' type: dx (the residual's as well) and dweight from h, the gradient dy of y and
+ * the gradient dh of h (0: none).  dx or dweight may be 0.  `scratch` is needed for dweight, and sums run in an order that
+ * depends on the sizes alone. */
+uint64_t ptwm_b200_rms_norm_grad_scratch_bytes(uint64_t rows, uint64_t cols);
+int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t dy, uint64_t dh, uint64_t dx, uint64_t dweight, uint64_t scratch, uint64_t scratch_bytes,
+                                uint64_t rows, uint64_t cols, uint32_t dtype, uint32_t weight_dtype, float eps, uint32_t device_ordinal, uint64_t stream);
+
+/* A matrix of E2M1 values with group scales in device memory:
+ * W[n][k] = e2m1(values[n * value_pitch + k / 2], low nibble for even k) * scale(scales[n * scale_pitch + k / group]) [* *global_scale].
+ * group 32: E8M0 scales (MXFP4); group 16: E4M3 scales (NVFP4).  Pointers and pitches are multiples of 16 bytes. */
+typedef struct ptwm_b200_scaled_weight {
+    uint64_t values, scales, global_scale;   /* device pointers; global_scale: one fp32, or 0 */
+    uint64_t rows, cols;
+    uint32_t value_pitch, scale_pitch;       /* bytes */
+    uint32_t group, reserved;
+} ptwm_b200_scaled_weight;
+
+/* y[m][n] = sum over k of x[m][k] W[n][k] for `tokens` rows x of w->cols values, sums in fp32, rounded once to y_dtype. */
+int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t x_scales, uint64_t y, uint64_t tokens, uint32_t x_dtype, uint32_t x_scaled,
+                         uint32_t y_dtype, uint32_t device_ordinal, uint64_t stream);
+/* dx[m][k] = sum over n of dy[m][n] W[n][k]: the gradient that goes back to the tokens. */
+int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* w, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dtype, uint32_t device_ordinal, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,10 +13,11 @@ import subprocess
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PTWM_B200_LIB") or os.path.join(_HERE, "libptwm_b200.so")  # PTWM_B200_LIB: load another build of the same library
 _SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("unity.cu", "ptwm_b200.cu", "encoder.cu", "kernels.cuh", "encode.cuh", "encode_tables.cuh", "noalloc.cu",
-                                                      "format.hpp", "host_common.hpp", "slice_copy.hpp", "plan.h")] + [
+                                                      "format.hpp", "host_common.hpp", "errors.hpp", "slice_copy.hpp", "plan.h", "operators.cu", "number_types.cuh", "rms_norm.cuh", "matvec.cuh")] + [
     os.path.join(_HERE, "..", "include", "ptwm_b200.h")]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-pthread", "-shared"]
+_UNITS = ("unity.cu", "operators.cu")  # translation units, compiled side by side
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -25,7 +26,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     stale = force or not os.path.exists(LIB_PATH) or any(os.path.getmtime(s) > os.path.getmtime(LIB_PATH) for s in srcs)
     if stale:
         nvcc = os.environ.get("NVCC", "nvcc")
-        cmd = [nvcc, *NVCC_FLAGS, "-o", LIB_PATH, os.path.join(_HERE, "csrc", "unity.cu")]
+        cmd = [nvcc, *NVCC_FLAGS, "--threads", str(len(_UNITS)), "-o", LIB_PATH, *(os.path.join(_HERE, "csrc", u) for u in _UNITS)]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         res = subprocess.run(cmd, capture_output=True, text=True)
@@ -51,6 +52,11 @@ class EncodeTensor(C.Structure):
 class EncodeOptions(C.Structure):
     _fields_ = [("chunk_size", C.c_uint32), ("menu", C.c_uint32), ("forced_codec", C.c_int32), ("emit_plane_crc", C.c_uint8),
                 ("emit_payload_hash", C.c_uint8), ("candidates", C.c_uint8), ("reserved", C.c_uint8 * 1)]
+
+
+class ScaledWeightArgs(C.Structure):
+    _fields_ = [("values", C.c_uint64), ("scales", C.c_uint64), ("global_scale", C.c_uint64), ("rows", C.c_uint64), ("cols", C.c_uint64),
+                ("value_pitch", C.c_uint32), ("scale_pitch", C.c_uint32), ("group", C.c_uint32), ("reserved", C.c_uint32)]
 
 
 ALLOC_FN = C.CFUNCTYPE(C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint64)
@@ -92,6 +98,11 @@ _SIGNATURES = {
     "ptwm_b200_crc32_by_runs": (C.c_uint32, [C.c_char_p, C.c_size_t, C.c_size_t]),
     "ptwm_b200_fit_shared_states_host": (C.c_int64, [C.POINTER(C.c_char_p), C.POINTER(C.c_uint64), C.POINTER(C.c_uint32), C.c_size_t, C.c_void_p, C.c_size_t,
                                                      C.POINTER(C.c_uint32)]),
+    "ptwm_b200_rms_norm": (C.c_int64, [C.c_uint64] * 8 + [C.c_uint32] * 3 + [C.c_float, C.c_uint32, C.c_uint64]),
+    "ptwm_b200_rms_norm_grad_scratch_bytes": (C.c_uint64, [C.c_uint64, C.c_uint64]),
+    "ptwm_b200_rms_norm_grad": (C.c_int64, [C.c_uint64] * 10 + [C.c_uint32] * 2 + [C.c_float, C.c_uint32, C.c_uint64]),
+    "ptwm_b200_matvec": (C.c_int64, [C.c_void_p] + [C.c_uint64] * 4 + [C.c_uint32] * 4 + [C.c_uint64]),
+    "ptwm_b200_matvec_grad": (C.c_int64, [C.c_void_p] + [C.c_uint64] * 3 + [C.c_uint32] * 2 + [C.c_uint64]),
     "ptwm_hardware_backend_v1_cuda_stream_handle": (C.c_uint64, [C.c_uint32]),
     "ptwm_plane_codec_v1_cuda_stream_handle": (C.c_uint64, [C.c_uint32]),
     "ptwm_hardware_backend_v1_dispatch_decode_cuda": (C.c_int64, [C.c_uint8, C.c_void_p, C.c_size_t, C.c_char_p, C.c_size_t, C.c_uint64, C.c_size_t,

@@ -371,6 +371,24 @@ class ContainerHandle:
         plan.run(self.blob_on_device(), out, scratch, flags=self._flags())
         return [(self._infos[i]["name"], v) for i, v in zip(plan.indices, plan.views(out))]
 
+    # -- weights to apply --------------------------------------------------------
+    def scaled_weight(self, name: str, *, expert: Optional[int] = None):
+        """The microscaled matrix ``name`` as a ``ScaledWeight``, its values and scales decoded in one pass; which tensors
+        these are: ``operators.scaled_names``."""
+        from .operators import ScaledWeight, scaled_names
+        values, scales, top = scaled_names(name, self.__contains__)
+        got = dict(self.decode_model([n for n in (values, scales, top) if n is not None]))
+        return ScaledWeight(got[values], got[scales], None if top is None else got[top], expert=expert)
+
+    def projection(self, norm: str, names: Sequence[str], *, eps: float = 1e-6, quant: Optional[str] = None):
+        """The norm vector ``norm`` and the microscaled matrices ``names`` that read it, decoded in one pass, as a ``Projection``."""
+        from .operators import Projection, ScaledWeight, scaled_names
+        parts = [scaled_names(n, self.__contains__) for n in names]
+        if norm not in self:
+            raise KeyError(norm)
+        got = dict(self.decode_model(dict.fromkeys([norm, *(t for p in parts for t in p if t is not None)])))
+        weights = [ScaledWeight(got[v], got[s], None if top is None else got[top]) for v, s, top in parts]
+        return Projection(got[norm], weights, eps=eps, quant=quant)
 
     def decode_model_streamed(self, names: Optional[Iterable[str]] = None, pieces: int = 8,
                               indices: Optional[Sequence[int]] = None) -> list[tuple[str, torch.Tensor]]:
@@ -525,6 +543,10 @@ class TensorIndex:
         if self._handle.shape(name) is None:
             raise TypeError(f"tensor {name!r} has no shape metadata; cannot reconstruct a torch.Tensor. Call get_bytes().")
         return self._handle.decode(name)
+
+    def get_scaled_weight(self, name: str, *, expert: Optional[int] = None):
+        """The microscaled matrix ``name`` (its values and scales together) as a ``ScaledWeight``."""
+        return self._handle.scaled_weight(name, expert=expert)
 
     def stream_tensors(self, names: Optional[Iterable[str]] = None) -> Iterator[tuple[str, torch.Tensor]]:
         for name in (list(names) if names is not None else self.names()):

@@ -1,5 +1,5 @@
-// Helpers shared by the translation units of libptwm_b200.so: error string,
-// CUDA error macro, device guard and the per-device persistent state.
+// Helpers shared by the container code of libptwm_b200.so: device memory and
+// the per-device persistent state.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -10,26 +10,9 @@
 
 #include "../../include/ptwm_b200.h"
 #include "kernels.cuh"
+#include "errors.hpp"
 
 namespace ptwm {
-
-// Last error of the calling thread (returned by ptwm_b200_last_error).
-std::string& last_error_ref();
-inline int64_t fail(int64_t rc, const std::string& m) { last_error_ref() = m; return rc; }
-
-#define CUDA_TRY(expr)                                                                                        \
-    do {                                                                                                      \
-        cudaError_t e_ = (expr);                                                                              \
-        if (e_ != cudaSuccess) return ::ptwm::fail(PTWM_RC_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e_)); \
-    } while (0)
-
-// Makes `dev` current for the scope and restores the previous device.
-struct DeviceGuard {
-    int prev = -1;
-    cudaError_t err;
-    explicit DeviceGuard(int dev) { err = cudaGetDevice(&prev); if (err == cudaSuccess && prev != dev) err = cudaSetDevice(dev); }
-    ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
-};
 
 // Device memory.  An encode's comes from the allocator the program registered (ptwm_b200_set_allocator), else from cudaMalloc: it
 // takes work memory several times the size of the tensors; handed out and taken back by the driver that was 55 of the 64 ms

@@ -1,0 +1,93 @@
+// Products of a matrix of E2M1 nibbles with group scales (MXFP4: E8M0 per 32, NVFP4: E4M3 per 16 and one fp32) with tokens.
+//
+//   W[n][k] = e2m1(values[n][k]) * scale[n][k / group] (* global)
+//   y[m][n] = sum_k x[m][k] W[n][k]          dx[m][k] = sum_n dy[m][n] W[n][k]
+// Sums are fp32, with one rounding at the end.
+#pragma once
+#include "number_types.cuh"
+
+namespace ptwm {
+
+struct ScaledMatrix {
+    const uint8_t* values;       // [rows][value_pitch], two to a byte, the even one in the low nibble
+    const uint8_t* scales;       // [rows][scale_pitch]
+    const float* global_scale;   // or null
+    uint64_t rows, cols;
+    uint32_t value_pitch, scale_pitch;
+    uint32_t group;              // 32: E8M0; 16: E4M3
+};
+struct TokenArgs {
+    const void* x;
+    const void* scales;
+    uint64_t tokens;
+    uint32_t scaled;
+    void* y;
+};
+
+__device__ __forceinline__ float group_scale(const ScaledMatrix& w, uint64_t row, uint64_t k) {
+    const uint8_t s = w.scales[row * w.scale_pitch + k / w.group];
+    return w.group == 32 ? e8m0_f32(s) : e4m3_f32(s);
+}
+
+template <class T> __device__ __forceinline__ float token_value(const TokenArgs& t, uint64_t m, uint64_t k, uint64_t cols) {
+    return to_f32(static_cast<const T*>(t.x)[m * cols + k]);
+}
+template <> __device__ __forceinline__ float token_value<uint8_t>(const TokenArgs& t, uint64_t m, uint64_t k, uint64_t cols) {
+    const float v = e4m3_f32(static_cast<const uint8_t*>(t.x)[m * cols + k]);
+    return t.scaled == SCALE_ROW ? v : v * e8m0_f32(static_cast<const uint8_t*>(t.scales)[m * (cols / 32) + k / 32]);
+}
+
+// A warp per row of the matrix and eight tokens; a lane takes every 32nd byte.
+template <class T, class Y> __global__ void __launch_bounds__(256) matvec_kernel(ScaledMatrix w, TokenArgs t) {
+    const uint64_t n = uint64_t(blockIdx.x) * 8 + threadIdx.x / 32, m0 = uint64_t(blockIdx.y) * 8;
+    const uint32_t lane = threadIdx.x & 31;
+    if (n >= w.rows) return;
+    const int count = int(t.tokens - m0 < 8 ? t.tokens - m0 : 8);
+    float sum[8] = {};
+    for (uint64_t b = lane; b < w.cols / 2; b += 32) {
+        const uint32_t v = w.values[n * w.value_pitch + b];
+        const float s = group_scale(w, n, 2 * b), lo = e2m1_f32(v & 15) * s, hi = e2m1_f32(v >> 4) * s;
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+            if (m < count) sum[m] += token_value<T>(t, m0 + m, 2 * b, w.cols) * lo + token_value<T>(t, m0 + m, 2 * b + 1, w.cols) * hi;
+    }
+    const float global = w.global_scale ? *w.global_scale : 1.0f;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+        for (int o = 16; o; o >>= 1) sum[m] += __shfl_xor_sync(0xFFFFFFFFu, sum[m], o);
+        if (lane == 0 && m < count) {
+            float v = sum[m] * global;
+            if (t.scaled == SCALE_ROW) v *= static_cast<const float*>(t.scales)[m0 + m];
+            static_cast<Y*>(t.y)[(m0 + m) * w.rows + n] = from_f32<Y>(v);
+        }
+    }
+}
+
+// A thread per byte of a row (two columns) and eight tokens, down all rows.
+template <class T> __global__ void __launch_bounds__(128) matvec_grad_kernel(ScaledMatrix w, TokenArgs t) {
+    const uint64_t b = uint64_t(blockIdx.x) * 128 + threadIdx.x, m0 = uint64_t(blockIdx.y) * 8;
+    if (b >= w.cols / 2) return;
+    const int count = int(t.tokens - m0 < 8 ? t.tokens - m0 : 8);
+    float lo[8] = {}, hi[8] = {};
+    for (uint64_t n = 0; n < w.rows; ++n) {
+        const uint32_t v = w.values[n * w.value_pitch + b];
+        const float s = group_scale(w, n, 2 * b), a = e2m1_f32(v & 15) * s, c = e2m1_f32(v >> 4) * s;
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+            if (m < count) {
+                const float d = to_f32(static_cast<const T*>(t.x)[(m0 + m) * w.rows + n]);
+                lo[m] += d * a;
+                hi[m] += d * c;
+            }
+    }
+    const float global = w.global_scale ? *w.global_scale : 1.0f;
+#pragma unroll
+    for (int m = 0; m < 8; ++m)
+        if (m < count) {
+            T* y = static_cast<T*>(t.y) + (m0 + m) * w.cols + 2 * b;
+            y[0] = from_f32<T>(lo[m] * global);
+            y[1] = from_f32<T>(hi[m] * global);
+        }
+}
+
+}  // namespace ptwm

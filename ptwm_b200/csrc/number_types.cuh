@@ -1,0 +1,36 @@
+// The number types of the operators: fp32, fp16, bf16 (public dtype codes 1, 4, 6), E4M3 with scales, and E2M1 nibbles.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace ptwm {
+
+enum : uint32_t { DT_FP32 = 1, DT_FP16 = 4, DT_BF16 = 6, DT_E4M3 = 29 };
+enum : uint32_t { SCALE_NONE = 0, SCALE_ROW = 1, SCALE_BLOCK = 2 };  // how 8-bit values are scaled: not, fp32 per row, E8M0 per 32
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// 2^(e - 127) of an E8M0 code; 255 is NaN.  Code 0 is the subnormal 2^-127.
+__device__ __forceinline__ float e8m0_f32(uint32_t e) { return e == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float(e ? e << 23 : 0x00400000u); }
+
+__device__ __forceinline__ float e4m3_f32(uint8_t v) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3))); }
+// Nearest E4M3 value, ties to even; beyond 448 it is 448, NaN stays NaN.
+__device__ __forceinline__ uint8_t f32_e4m3(float v) { return uint8_t(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3)); }
+
+// E2M1: a sign, two bits of exponent with bias 1, one of mantissa; 0 and 0.5 are its subnormals.
+__device__ __forceinline__ float e2m1_f32(uint32_t c) {
+    const uint32_t e = (c >> 1) & 3, m = c & 1;
+    const float v = e ? __uint_as_float(((126 + e) << 23) | (m << 22)) : 0.5f * float(m);
+    return (c & 8) ? -v : v;
+}
+
+}  // namespace ptwm

@@ -437,6 +437,14 @@ class SafeOpen:
             raise KeyError(name)
         return self._container.decode(name)
 
+    def get_scaled_weight(self, name: str, *, expert: Optional[int] = None):
+        """The microscaled matrix ``name`` (its values and scales together) as a ``ScaledWeight``."""
+        if self._container is not None:
+            return self._container.scaled_weight(name, expert=expert)
+        from .operators import ScaledWeight, scaled_names
+        values, scales, top = scaled_names(name, set(self.keys()).__contains__)
+        return ScaledWeight(self.get_tensor(values), self.get_tensor(scales), None if top is None else self.get_tensor(top), expert=expert)
+
     def get_slice(self, name: str) -> Any:
         if self._container is not None:
             raise NotImplementedError("get_slice is not supported on .ptwm/ptwm-shell containers")

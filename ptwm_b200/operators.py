@@ -1,0 +1,335 @@
+"""Operators that apply decoded weights on CUDA: ``rms_norm`` and ``matvec``.
+
+What a container decodes to includes norm vectors and, for microscaled models, matrices of 4-bit values with a scale per
+group, which torch cannot multiply by.  ``ScaledWeight`` is a handle on such a matrix where it lies, ``matvec`` multiplies
+it with one token or many, and ``rms_norm`` is the norm in front of it, with the residual's addition and, if asked for, an
+output in 8 bits with scales (``ScaledActivations``) that ``matvec`` reads.  ``Projection`` is a norm and the matrices that
+read it.
+
+Every call runs on the current stream of its tensors' device, allocates its results with torch, waits for nothing and can be
+captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Any, Callable, Mapping, Optional, Sequence
+
+import torch
+
+from . import _lib
+from .container import _check, stream_handle
+
+__all__ = ["Projection", "ScaledActivations", "ScaledWeight", "matvec", "rms_norm"]
+
+_PLAIN = {torch.float32: 1, torch.float16: 4, torch.bfloat16: 6}
+_E4M3 = 29
+_QUANT = {None: 0, "row": 1, "block": 2}
+_U8 = (torch.uint8,) + ((torch.float4_e2m1fn_x2,) if hasattr(torch, "float4_e2m1fn_x2") else ())
+_E8M0 = torch.float8_e8m0fnu
+
+
+def _on_cuda(what: str, t: Any, device: Optional[torch.device] = None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} is a tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{what} lives in host memory; move it to CUDA first")
+    if device is not None and t.device != device:
+        raise ValueError(f"{what} lives on {t.device}, the others on {device}")
+
+
+class ScaledActivations:
+    """Rows of E4M3 values with their scales: fp32 per row (``scales`` has the rows' leading dimensions) or E8M0 per 32
+    values (one more dimension, a 32nd of the columns)."""
+
+    __slots__ = ("values", "scales", "quant")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor) -> None:
+        _on_cuda("values", values)
+        _on_cuda("scales", scales, values.device)
+        if values.dtype != torch.float8_e4m3fn or values.dim() < 1:
+            raise TypeError(f"values are rows of float8_e4m3fn, got {values.dtype} with {values.dim()} dimensions")
+        if scales.dtype == torch.uint8:
+            scales = scales.view(_E8M0)
+        if scales.dtype == torch.float32:
+            quant, want = "row", values.shape[:-1]
+        elif scales.dtype == _E8M0:
+            quant, want = "block", (*values.shape[:-1], values.shape[-1] // 32)
+            if values.shape[-1] % 32:
+                raise ValueError(f"block scales need whole blocks of 32 values, got rows of {values.shape[-1]}")
+        else:
+            raise TypeError(f"scales are float32 per row or float8_e8m0fnu (uint8) per 32 values, got {scales.dtype}")
+        if tuple(scales.shape) != tuple(want):
+            raise ValueError(f"scales have shape {tuple(scales.shape)}, expected {tuple(want)}")
+        self.values, self.scales, self.quant = values, scales, quant
+
+    @classmethod
+    def _of(cls, values: torch.Tensor, scales: torch.Tensor, quant: str) -> "ScaledActivations":
+        self = object.__new__(cls)
+        self.values, self.scales, self.quant = values, scales, quant
+        return self
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    def __repr__(self) -> str:
+        return f"ScaledActivations(shape={tuple(self.shape)}, quant={self.quant!r}, device={self.device})"
+
+
+def scaled_names(name: str, has: Callable[[str], bool]) -> tuple[str, str, Optional[str]]:
+    """The tensors that make up the microscaled matrix ``name``: values, scales and fp32 scale, as ModelOpt names them
+    (``name.weight``, ``.weight_scale``, ``.weight_scale_2``), as gpt-oss does (``name_blocks``, ``name_scales``), or
+    ``name``, ``name_scale``, ``name_scale_2``.  Raises KeyError where no such set is there."""
+    for values, scales, top in ((f"{name}.weight", f"{name}.weight_scale", f"{name}.weight_scale_2"), (f"{name}_blocks", f"{name}_scales", None),
+                                (name, f"{name}_scale", f"{name}_scale_2")):
+        if has(values) and has(scales):
+            return values, scales, top if top is not None and has(top) else None
+    raise KeyError(name)
+
+
+class ScaledWeight:
+    """A matrix of 4-bit values with group scales, where it lies in device memory.
+
+    ``values``: E2M1 codes, two to a byte with the even column in the low nibble: uint8 or float4_e2m1fn_x2 of shape
+    [rows, cols / 2], or [rows, cols / 32, 16].  ``scales``: E8M0 (uint8 or float8_e8m0fnu) of shape [rows, cols / 32], which
+    is MXFP4, or float8_e4m3fn of shape [rows, cols / 16], NVFP4, with ``global_scale`` as one fp32 number in device memory
+    (1 where it is None).  ``expert`` picks one matrix of a stack of them.
+
+    The tensors are kept and read in place; only one whose rows are not contiguous or do not start at multiples of 16
+    bytes is copied, once, here."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, global_scale: Optional[torch.Tensor] = None, *, expert: Optional[int] = None) -> None:
+        _on_cuda("values", values)
+        _on_cuda("scales", scales, values.device)
+        if values.dtype not in _U8:
+            raise TypeError(f"values are packed nibbles (uint8 or float4_e2m1fn_x2), got {values.dtype}")
+        if scales.dtype in (torch.uint8, _E8M0):
+            self.kind, self.group = "mxfp4", 32
+        elif scales.dtype == torch.float8_e4m3fn:
+            self.kind, self.group = "nvfp4", 16
+        else:
+            raise TypeError(f"scales are E8M0 (uint8 or float8_e8m0fnu) or float8_e4m3fn, got {scales.dtype}")
+        values, scales = values.view(torch.uint8), scales.view(torch.uint8)
+        if expert is not None:
+            values, scales = values[expert], scales[expert]
+        if values.dim() == 3 and values.shape[-1] == 16 and scales.dim() == 2:
+            values = values.reshape(values.shape[0], -1)
+        if values.dim() != 2 or scales.dim() != 2:
+            raise ValueError(f"one matrix of values and one of scales are wanted, got shapes {tuple(values.shape)} and {tuple(scales.shape)}"
+                             + ("; pick one of a stack with expert=" if values.dim() > 2 else ""))
+        self.rows, self.cols = values.shape[0], 2 * values.shape[1]
+        if not self.rows or not self.cols or self.cols % self.group or tuple(scales.shape) != (self.rows, self.cols // self.group):
+            raise ValueError(f"{self.kind}: values of {self.rows} x {self.cols} want scales of {self.rows} x {self.cols}/{self.group}, got {tuple(scales.shape)}")
+        if global_scale is not None:
+            _on_cuda("global_scale", global_scale, values.device)
+            if self.kind != "nvfp4":
+                raise ValueError("only NVFP4 matrices have a global scale")
+            if global_scale.dtype != torch.float32 or global_scale.numel() != 1:
+                raise TypeError(f"global_scale is one float32 number, got {global_scale.dtype} of shape {tuple(global_scale.shape)}")
+        self.device = values.device
+        self._values, self._scales, self._global = self._aligned(values), self._aligned(scales), global_scale
+        self._args = _lib.ScaledWeightArgs(self._values.data_ptr(), self._scales.data_ptr(), 0 if global_scale is None else global_scale.data_ptr(),
+                                           self.rows, self.cols, self._values.stride(0), self._scales.stride(0), self.group, 0)
+        self._ref = C.addressof(self._args)
+        self._ordinal = self.device.index
+
+    @staticmethod
+    def _aligned(t: torch.Tensor) -> torch.Tensor:
+        """``t`` where its rows can be read as they lie, else a copy whose rows start at multiples of 16 bytes."""
+        wide = t.shape[0] == 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1])
+        if wide and (t.shape[1] == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0 and t.stride(0) < 1 << 32:
+            if t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1]:
+                return t
+        pitch = (t.shape[1] + 15) // 16 * 16
+        copy = torch.zeros(t.shape[0], pitch, dtype=torch.uint8, device=t.device)
+        copy[:, :t.shape[1]] = t
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(t.device).synchronize()  # the handle may be used on another stream next
+        return copy[:, :t.shape[1]]
+
+    @classmethod
+    def from_state(cls, state: Mapping[str, torch.Tensor], name: str, *, expert: Optional[int] = None) -> "ScaledWeight":
+        """The matrix ``name`` of a state dict (``load_file``, ``dict(handle.decode_model())``); see ``scaled_names``."""
+        values, scales, top = scaled_names(name, state.__contains__)
+        return cls(state[values], state[scales], None if top is None else state[top], expert=expert)
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.rows, self.cols
+
+    def __repr__(self) -> str:
+        return f"ScaledWeight({self.kind}, {self.rows} x {self.cols}, device={self.device})"
+
+
+# ---- rms_norm -------------------------------------------------------------------------------------
+def _norm(x, weight, residual, eps: float, quant: Optional[str]):
+    """(y or ScaledActivations, h) of checked, contiguous tensors."""
+    cols = x.shape[-1]
+    device = x.device.index
+    h = x if residual is None else torch.empty_like(x)
+    scales = None
+    if quant is None:
+        y = torch.empty_like(x)
+    else:
+        y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        scales = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quant == "row" else
+                  torch.empty((*x.shape[:-1], cols // 32), dtype=_E8M0, device=x.device))
+    _check(_lib.lib().ptwm_b200_rms_norm(x.data_ptr(), 0 if residual is None else residual.data_ptr(), weight.data_ptr(), h.data_ptr(), y.data_ptr(),
+                                         0 if scales is None else scales.data_ptr(), x.numel() // cols, cols, _PLAIN[x.dtype], _PLAIN[weight.dtype],
+                                         _QUANT[quant], eps, device, stream_handle(device)))
+    return (y if quant is None else ScaledActivations._of(y, scales, quant)), h
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, h = _norm(x, weight, residual, eps, None)
+        ctx.save_for_backward(h, weight)
+        ctx.eps, ctx.has_residual = eps, residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, h) if residual is not None else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[0] or ctx.needs_input_grad[2], ctx.needs_input_grad[1]
+        if dy is None:  # only the residual stream was used
+            dx = dh
+            dw = torch.zeros_like(weight) if need_w and dh is not None else None
+        else:
+            dy = dy.contiguous()
+            dh = None if dh is None else dh.contiguous()
+            cols, device = h.shape[-1], h.device.index
+            rows = h.numel() // cols
+            dx = torch.empty_like(h) if need_x else None
+            dw = torch.empty_like(weight) if need_w else None
+            L = _lib.lib()
+            size = L.ptwm_b200_rms_norm_grad_scratch_bytes(rows, cols) if need_w else 0
+            scratch = torch.empty(size, dtype=torch.uint8, device=h.device) if size else None
+            _check(L.ptwm_b200_rms_norm_grad(h.data_ptr(), weight.data_ptr(), dy.data_ptr(), 0 if dh is None else dh.data_ptr(), 0 if dx is None else dx.data_ptr(),
+                                             0 if dw is None else dw.data_ptr(), 0 if scratch is None else scratch.data_ptr(), size, rows, cols, _PLAIN[h.dtype],
+                                             _PLAIN[weight.dtype], ctx.eps, device, stream_handle(device)))
+        return (dx if ctx.needs_input_grad[0] else None), dw, (dx if ctx.has_residual and ctx.needs_input_grad[2] else None), None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residual: Optional[torch.Tensor] = None, quant: Optional[str] = None):
+    """Root-mean-square norm over the last dimension, with the residual's addition.
+
+    ``h = x + residual`` (rounded to x's type; without a residual ``h = x``), then
+    ``y = h / sqrt(mean(h^2) + eps) * weight`` with fp32 sums and one rounding.  x and residual are fp32, fp16 or bf16 of one
+    shape and type, weight is a vector of any of these types.  Returns ``y``, or ``(y, h)`` with a residual.
+
+    ``quant``: None for y in x's type; "row" or "block" for ``ScaledActivations``, E4M3 values with a fp32 scale per row
+    (max|y| / 448) or an E8M0 scale per 32 values (the smallest power of two that keeps them within 448).  A row or block
+    that is not finite has NaN for scale and values.
+
+    Without ``quant`` there are gradients for x, residual and weight."""
+    _on_cuda("x", x)
+    _on_cuda("weight", weight, x.device)
+    if x.dtype not in _PLAIN or weight.dtype not in _PLAIN:
+        raise TypeError(f"x and weight are float32, float16 or bfloat16, got {x.dtype} and {weight.dtype}")
+    if quant not in _QUANT:
+        raise ValueError(f"quant is None, 'row' or 'block', got {quant!r}")
+    if x.dim() < 1 or x.shape[-1] == 0 or weight.shape != x.shape[-1:]:
+        raise ValueError(f"weight of shape {tuple(weight.shape)} does not fit rows of x, shape {tuple(x.shape)}")
+    if quant == "block" and x.shape[-1] % 32:
+        raise ValueError(f"block scales need whole blocks of 32 values, got rows of {x.shape[-1]}")
+    if residual is not None:
+        _on_cuda("residual", residual, x.device)
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}, x {x.dtype} {tuple(x.shape)}; they have to be alike")
+    grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))
+    if grad and quant is not None:
+        raise ValueError("an 8-bit output has no gradient: call under torch.no_grad() or detach the inputs")
+    x, weight = x.contiguous(), weight.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    if grad:
+        return _RmsNorm.apply(x, weight, residual, float(eps))
+    y, h = _norm(x, weight, residual, eps, quant)
+    return y if residual is None else (y, h)
+
+
+# ---- matvec ---------------------------------------------------------------------------------------
+def _product(x, scales, quant, weight: ScaledWeight, out_dtype: torch.dtype) -> torch.Tensor:
+    device = weight._ordinal
+    y = torch.empty((*x.shape[:-1], weight.rows), dtype=out_dtype, device=x.device)
+    _check(_lib.lib().ptwm_b200_matvec(weight._ref, x.data_ptr(), 0 if scales is None else scales.data_ptr(), y.data_ptr(), x.numel() // weight.cols,
+                                       _E4M3 if scales is not None else _PLAIN[x.dtype], _QUANT[quant], _PLAIN[out_dtype], device, stream_handle(device)))
+    return y
+
+
+class _Matvec(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, out_dtype):
+        ctx.weight, ctx.dtype = weight, x.dtype
+        return _product(x, None, None, weight, out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        w = ctx.weight
+        dy = dy.to(ctx.dtype).contiguous()
+        dx = torch.empty((*dy.shape[:-1], w.cols), dtype=ctx.dtype, device=dy.device)
+        _check(_lib.lib().ptwm_b200_matvec_grad(w._ref, dy.data_ptr(), dx.data_ptr(), dy.numel() // w.rows, _PLAIN[ctx.dtype], w._ordinal, stream_handle(w._ordinal)))
+        return dx, None, None
+
+
+def matvec(x, weight: ScaledWeight, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``y[..., n] = sum_k x[..., k] W[n, k]`` with a 4-bit matrix, for one token or many.
+
+    x is fp32, fp16 or bf16 of shape [..., cols], or ``ScaledActivations``.  Sums are fp32, rounded once to ``out_dtype``
+    (x's type; bf16 for ScaledActivations).  The gradient goes back to a plain x; the matrix has none."""
+    if not isinstance(weight, ScaledWeight):
+        raise TypeError(f"weight is a ScaledWeight, got {type(weight).__name__}")
+    scales = quant = None
+    if isinstance(x, ScaledActivations):
+        scales, quant, x = x.scales, x.quant, x.values
+        out_dtype = out_dtype or torch.bfloat16
+        if not scales.is_contiguous():
+            scales = scales.contiguous()
+    else:
+        _on_cuda("x", x)
+        if x.dtype not in _PLAIN:
+            raise TypeError(f"x is float32, float16, bfloat16 or ScaledActivations, got {x.dtype}")
+        out_dtype = out_dtype or x.dtype
+    if out_dtype not in _PLAIN:
+        raise TypeError(f"out_dtype is float32, float16 or bfloat16, got {out_dtype}")
+    if x.device != weight.device:
+        raise ValueError(f"x lives on {x.device}, the weight on {weight.device}")
+    if x.dim() < 1 or x.shape[-1] != weight.cols:
+        raise ValueError(f"x of shape {tuple(x.shape)} does not fit a matrix of {weight.rows} x {weight.cols}")
+    if not x.is_contiguous():
+        x = x.contiguous()
+    if scales is None and x.requires_grad and torch.is_grad_enabled():
+        return _Matvec.apply(x, weight, out_dtype)
+    return _product(x, scales, quant, weight, out_dtype)
+
+
+class Projection:
+    """A norm and the matrices that read its output, such as the gate and up projections of a feed-forward block.
+
+    ``projection(x, residual)`` returns ``([W x' for W in weights], h)`` with ``x', h = rms_norm(x, norm, eps,
+    residual=residual, quant=quant)``; ``h`` is x where there is no residual."""
+
+    def __init__(self, norm: torch.Tensor, weights: Sequence[ScaledWeight], *, eps: float = 1e-6, quant: Optional[str] = None) -> None:
+        self.norm, self.weights, self.eps, self.quant = norm, list(weights), eps, quant
+        _on_cuda("norm", norm)
+        if quant not in _QUANT:
+            raise ValueError(f"quant is None, 'row' or 'block', got {quant!r}")
+        if norm.dim() != 1:
+            raise ValueError(f"norm is a vector, got shape {tuple(norm.shape)}")
+        for w in self.weights:
+            if not isinstance(w, ScaledWeight):
+                raise TypeError(f"weights are ScaledWeights, got {type(w).__name__}")
+            if w.cols != norm.shape[0] or w.device != norm.device:
+                raise ValueError(f"a norm of {norm.shape[0]} on {norm.device} does not fit {w!r}")
+
+    def __call__(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> tuple[list[torch.Tensor], torch.Tensor]:
+        got = rms_norm(x, self.norm, self.eps, residual=residual, quant=self.quant)
+        y, h = (got, x) if residual is None else got
+        return [matvec(y, w, out_dtype=x.dtype) for w in self.weights], h

@@ -1,0 +1,639 @@
+"""rms_norm and matvec against their definitions in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import oracle
+import ptwm_b200
+from ptwm_b200 import Projection, ScaledActivations, ScaledWeight, matvec, rms_norm
+from _data import mixed_model, specs_mxfp4, specs_nvfp4, spec_norm
+
+pytestmark = pytest.mark.gpu
+DT = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+E2M1 = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0], dtype=torch.float64)
+F32 = 2.0 ** -24  # half a step of fp32
+
+
+@pytest.fixture(autouse=True)
+def _cuda(cuda_device):
+    torch.cuda.set_device(cuda_device)
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _floor(dtype):  # half the smallest step there is
+    return torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+
+
+# ---- rms_norm ----------------------------------------------------------------------------------------
+def _norm64(x, weight, eps, residual):
+    h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    h64 = h.double()
+    rms = (h64.square().mean(-1, keepdim=True) + eps).sqrt()
+    return h, h64 / rms * weight.double()
+
+
+def _norm_slack(cols):
+    """Relative error of y before its rounding: a sum of positive terms in which a term goes through at most cols / 32 + 16
+    additions (half of that after the root), the mean, the root (2 steps) and two products."""
+    return ((cols / 32 + 16) / 2 + 8) * F32
+
+
+def _inputs(rows, cols, dtype, seed, residual=True, weight_dtype=None):
+    g = _gen(seed)
+    x = (torch.randn(rows, cols, generator=g, device="cuda") * 3).to(dtype)
+    res = (torch.randn(rows, cols, generator=g, device="cuda") * 2).to(dtype) if residual else None
+    w = (1 + 0.1 * torch.randn(cols, generator=g, device="cuda")).to(weight_dtype or dtype)
+    return x, res, w
+
+
+ROWS_COLS = [(1, 1), (3, 7), (1, 32), (5, 96), (2, 1000), (17, 1024), (1, 4096), (333, 4095), (7, 8200), (2, 10501), (3, 16384), (2, 40000), (1200, 64)]
+
+
+@pytest.mark.parametrize("rows, cols", ROWS_COLS)
+@pytest.mark.parametrize("dtype, weight_dtype", [("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp32"), ("fp32", "bf16")])
+@pytest.mark.parametrize("residual", [True, False])
+def test_norm_plain(rows, cols, dtype, weight_dtype, residual):
+    x, res, w = _inputs(rows, cols, DT[dtype], rows + cols, residual, DT[weight_dtype])
+    got = rms_norm(x, w, 1e-5, residual=res)
+    y, h = got if residual else (got, None)
+    want_h, want = _norm64(x, w, 1e-5, res)
+    if residual:
+        assert torch.equal(h, want_h)
+    assert y.dtype == x.dtype and y.shape == x.shape
+    tol = (_half_step(x.dtype) + _norm_slack(cols)) * want.abs() + _floor(x.dtype)
+    assert bool(((y.double() - want).abs() <= tol).all())
+
+
+def _check_8(values, scales, want, rel, step):
+    """E4M3 values times scales against want: half a step of E4M3, relative 2^-4 or, below its normal numbers, 2^-10 of the scale."""
+    back = values.double() * scales
+    tol = torch.maximum(2.0 ** -4 * want.abs(), 2.0 ** -10 * scales) * (1 + 2.0 ** -10) + rel * want.abs()
+    assert bool(((back - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("rows, cols", ROWS_COLS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_norm_row_scales(rows, cols, dtype):
+    x, res, w = _inputs(rows, cols, DT[dtype], 2 * rows + cols)
+    y, h = rms_norm(x, w, 1e-5, residual=res, quant="row")
+    want_h, want = _norm64(x, w, 1e-5, res)
+    assert torch.equal(h, want_h) and y.quant == "row" and y.shape == x.shape
+    s = want.abs().amax(-1) / 448
+    assert bool(((y.scales.double() - s).abs() <= (_norm_slack(cols) + 2 * F32) * s).all())
+    _check_8(y.values, y.scales.double()[:, None], want, 2 * _norm_slack(cols), None)
+
+
+@pytest.mark.parametrize("rows, cols", [rc for rc in ROWS_COLS if rc[1] % 32 == 0])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_norm_block_scales(rows, cols, dtype):
+    x, res, w = _inputs(rows, cols, DT[dtype], 3 * rows + cols)
+    w = w * torch.where(torch.arange(cols, device="cuda") % 3 == 0, 2.0 ** -9, 1.0).to(w.dtype)
+    y, h = rms_norm(x, w, 1e-5, residual=res, quant="block")
+    want_h, want = _norm64(x, w, 1e-5, res)
+    assert torch.equal(h, want_h) and y.quant == "block" and y.scales.shape == (rows, cols // 32)
+    most = want.reshape(rows, -1, 32).abs().amax(-1)
+    slack = _norm_slack(cols)
+    lo, hi = (torch.ceil(torch.log2(most * f / 448)).clamp(-127, 127) + 127 for f in (1 - slack, 1 + slack))
+    e = y.scales.view(torch.uint8).double()
+    assert bool(((e >= lo) & (e <= hi)).all())
+    _check_8(y.values, torch.exp2(e - 127).repeat_interleave(32, 1), want, 2 * slack, None)
+
+
+@pytest.mark.parametrize("quant", [None, "row", "block"])
+def test_norm_of_zeros_infinities_and_nan(quant):
+    cols = 4096
+    x = torch.randn(6, cols, generator=_gen(1), device="cuda").to(torch.bfloat16)
+    x[1] = 0
+    x[2, 77] = math.inf
+    x[3, 4095] = math.nan
+    x[4] = 1e-30
+    w = torch.ones(cols, device="cuda", dtype=torch.bfloat16)
+    got = rms_norm(x, w, 0.0 if quant is None else 1e-6, quant=quant)
+    if quant is None:
+        y = got.double()
+        assert bool(torch.isnan(y[1]).all())  # 0 / 0: no eps
+        assert bool(torch.isnan(y[3]).all()) and math.isnan(y[2, 77]) and bool((y[2, :77] == 0).all())
+    else:
+        s = got.scales.view(torch.uint8).int() if quant == "block" else got.scales
+        v = got.values.float()
+        assert bool((v[1] == 0).all()) and bool((s[1] == 0).all())
+        if quant == "row":
+            assert bool(torch.isnan(s[2:4]).all()) and bool(torch.isnan(v[2:4]).all())
+        else:
+            assert s[2, 77 // 32] == 255 and bool(torch.isnan(v[2, 64:96]).all()) and bool((v[2, :64] == 0).all())
+            assert bool((s[3] == 255).all()) and bool(torch.isnan(v[3]).all())
+        assert bool((v[4] > 0).all())
+    plain = rms_norm(x[5:], w, 1e-6, quant=quant)  # a row does not know its neighbours
+    again = rms_norm(x, w, 1e-6, quant=quant)
+    if quant is None:
+        assert torch.equal(plain[0], again[5])
+    else:
+        assert torch.equal(plain.values.view(torch.uint8)[0], again.values.view(torch.uint8)[5])
+
+
+def test_norm_strides_offsets_and_empty_rows():
+    base = torch.randn(9, 517, generator=_gen(2), device="cuda").to(torch.bfloat16)
+    w = torch.randn(1030, generator=_gen(3), device="cuda").to(torch.bfloat16)
+    for x, weight in [(base[:, 1:513], w[3:515]), (base.t(), w[1:10]), (base[::2, ::2], w[::3][:259]), (base[1:].reshape(2, 4, 517), w[:517]), (base.flatten()[1:4097].view(4, 1024), w[5:1029])]:
+        y = rms_norm(x, weight, 1e-5)
+        _, want = _norm64(x, weight, 1e-5, None)
+        assert y.shape == x.shape
+        assert bool(((y.double() - want).abs() <= (_half_step(x.dtype) + _norm_slack(x.shape[-1])) * want.abs()).all())
+    for quant in (None, "row", "block"):
+        y, h = rms_norm(base[:0, :512], w[:512], residual=base[:0, :512], quant=quant)
+        assert y.shape == (0, 512) and h.shape == (0, 512)
+
+
+@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 7), (5, 96), (1, 4096), (700, 1000), (333, 4095), (2, 10501), (3, 16384), (2, 40000)])
+@pytest.mark.parametrize("dtype, weight_dtype", [("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp32")])
+@pytest.mark.parametrize("residual", [True, False])
+def test_norm_gradient(rows, cols, dtype, weight_dtype, residual):
+    x, res, w = _inputs(rows, cols, DT[dtype], rows * 5 + cols, residual, DT[weight_dtype])
+    leaves = [t.requires_grad_() for t in (x, w, res) if t is not None]
+    g = _gen(9)
+    dy = torch.randn(rows, cols, generator=g, device="cuda").to(x.dtype)
+    dh = torch.randn(rows, cols, generator=g, device="cuda").to(x.dtype)
+    got = rms_norm(x, w, 1e-5, residual=res)
+    grads = torch.autograd.grad(got, leaves, (dy, dh) if residual else dy)
+    h = (x.float() + res.float()).to(x.dtype).double().detach() if residual else x.double().detach()
+    r = (h.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+    gw = dy.double() * w.double().detach()
+    parts = [r * gw, h * r ** 3 * (gw * h).mean(-1, keepdim=True)] + ([dh.double()] if residual else [])
+    want = parts[0] - parts[1] + (parts[2] if residual else 0)
+    # fp32 errors of each part: the dot product's go with the sum of its magnitudes; then one rounding
+    size = parts[0].abs() + (h * r ** 3).abs() * (gw * h).abs().mean(-1, keepdim=True) + want.abs()
+    tol = _half_step(x.dtype) * want.abs() + 4 * _norm_slack(cols) * size + _floor(x.dtype)
+    assert bool(((grads[0].double() - want).abs() <= tol).all())
+    if residual:
+        assert torch.equal(grads[2], grads[0])
+    terms = dy.double() * h * r
+    tol = _half_step(w.dtype) * terms.sum(0).abs() + ((rows + 16) * F32 + 2 * _norm_slack(cols)) * terms.abs().sum(0) + _floor(w.dtype)
+    assert grads[1].dtype == w.dtype and bool(((grads[1].double() - terms.sum(0)).abs() <= tol).all())
+
+
+def test_norm_gradient_against_differences():
+    x, res, w = _inputs(3, 40, torch.float32, 4)
+    c1, c2 = (torch.randn(3, 40, generator=_gen(s), device="cuda") for s in (5, 6))
+
+    def loss64(x, res, w):
+        h = x.double() + res.double()
+        y = h * (h.square().mean(-1, keepdim=True) + 1e-5).rsqrt() * w.double()
+        return ((y * c1.double()).sum() + (h * c2.double()).sum()).item()
+
+    for t in (x, res, w):
+        t.requires_grad_()
+    y, h = rms_norm(x, w, 1e-5, residual=res)
+    ((y * c1).sum() + (h * c2).sum()).backward()
+    step = 2.0 ** -8
+    for t in (x, res, w):
+        flat, grad = t.detach().clone().flatten(), t.grad.flatten()
+        for i in range(0, flat.numel(), 7):
+            args = []
+            for sign in (1, -1):
+                moved = flat.double().clone()
+                moved[i] += sign * step
+                args.append([moved.view(t.shape) if o is t else o.detach().double() for o in (x, res, w)])
+            slope = (loss64(*args[0]) - loss64(*args[1])) / (2 * step)
+            # third derivatives of order one: an error of some step^2
+            assert abs(slope - grad[i].item()) <= 8 * step ** 2 * (1 + abs(slope))
+
+
+def test_norm_gradient_of_one_output_and_of_some_inputs():
+    x, res, w = _inputs(4, 64, torch.float32, 8)
+    x.requires_grad_()
+    y, h = rms_norm(x, w, residual=res)
+    assert torch.equal(torch.autograd.grad(h.sum(), x)[0], torch.ones_like(x))
+    y, h = rms_norm(x, w, residual=res)
+    only, = torch.autograd.grad(y.sum(), x)
+    w.requires_grad_()
+    y, h = rms_norm(x.detach(), w, residual=res)
+    dw, = torch.autograd.grad(y.sum(), w)
+    y, h = rms_norm(x, w, residual=res)
+    a, b = torch.autograd.grad(y.sum(), (x, w))
+    assert torch.equal(a, only) and torch.equal(b, dw)
+    empty = torch.empty(0, 64, device="cuda", requires_grad=True)
+    a, b = torch.autograd.grad(rms_norm(empty, w).sum(), (empty, w))
+    assert a.shape == (0, 64) and bool((b == 0).all())
+    with pytest.raises(ValueError, match="no gradient"):
+        rms_norm(x, w, quant="row")
+    with torch.no_grad():
+        rms_norm(x, w, quant="row")
+
+
+# ---- matvec ------------------------------------------------------------------------------------------
+def _weight64(values, scales, top):
+    codes = torch.stack((values & 15, values >> 4), -1).reshape(values.shape[0], -1)
+    w = E2M1.to(values.device)[codes.long()]
+    group = w.shape[1] // scales.shape[1]
+    s = torch.exp2(scales.double() - 127) if scales.dtype == torch.uint8 else scales.double()
+    if scales.dtype == torch.uint8:
+        s = torch.where(scales == 255, torch.full_like(s, math.nan), s)
+    return w * s.repeat_interleave(group, 1) * (1.0 if top is None else top.double().item())
+
+
+def _matrix(n, k, kind, seed, lo=-3, hi=3):
+    """Any codes; scales are powers of two between 2^lo and 2^hi."""
+    g = _gen(seed)
+    values = torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    if kind == "mxfp4":
+        return values, torch.randint(127 + lo, 128 + hi, (n, k // 32), generator=g, device="cuda", dtype=torch.uint8), None
+    return values, torch.exp2(torch.randint(lo, hi + 1, (n, k // 16), generator=g, device="cuda").float()).to(torch.float8_e4m3fn), torch.tensor([0.25], device="cuda")
+
+
+SIZES = [(1, 32), (3, 64), (16, 32), (33, 96), (64, 512), (130, 1024), (127, 2080), (200, 4096), (129, 14336), (1000, 288)]
+TOKENS = [1, 2, 7, 8, 9, 16, 33, 64, 100, 129, 300]
+
+
+def _integers(tokens, k, dtype, seed):
+    return torch.randint(-2, 3, (tokens, k), generator=_gen(seed), device="cuda").to(dtype)
+
+
+@pytest.mark.parametrize("n, k", SIZES)
+@pytest.mark.parametrize("tokens", TOKENS)
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_matvec_of_whole_numbers_is_exact(n, k, tokens, kind, dtype):
+    # products are multiples of 1/16 (1/64 with the global scale) below 2^7; sums of 14336 of them fit 24 bits, whatever their order
+    k = k + 16 if kind == "nvfp4" and k % 64 == 32 else k  # rows that end inside a pair of groups
+    w = _matrix(n, k, kind, n + k)
+    x = _integers(tokens, k, DT[dtype], tokens)
+    want = (x.double() @ _weight64(*w).T)
+    y = matvec(x, ScaledWeight(*w), out_dtype=torch.float32)
+    assert y.shape == (tokens, n) and torch.equal(y.double(), want)
+    y = matvec(x, ScaledWeight(*w))
+    assert torch.equal(y, want.float().to(x.dtype))
+
+
+@pytest.mark.parametrize("n, k", SIZES)
+@pytest.mark.parametrize("tokens", TOKENS)
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("quant", ["row", "block"])
+def test_matvec_of_8_bit_whole_numbers_is_exact(n, k, tokens, kind, quant):
+    w = _matrix(n, k, kind, n + k)
+    x = _integers(tokens, k, torch.float8_e4m3fn, tokens + 1)
+    g = _gen(11)
+    if quant == "row":
+        scales = torch.exp2(torch.randint(-2, 3, (tokens,), generator=g, device="cuda").float())
+        x64 = x.double() * scales.double()[:, None]
+    else:
+        scales = torch.randint(126, 129, (tokens, k // 32), generator=g, device="cuda", dtype=torch.uint8)
+        x64 = x.double() * torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
+    want = x64 @ _weight64(*w).T
+    y = matvec(ScaledActivations(x, scales), ScaledWeight(*w), out_dtype=torch.float32)
+    assert torch.equal(y.double(), want)
+    assert torch.equal(matvec(ScaledActivations(x, scales), ScaledWeight(*w)), want.float().to(torch.bfloat16))
+
+
+def _check_product(y, x64, w64, dtype):
+    """One rounding, and a fp32 sum: each of its terms goes through at most k additions, which tensor cores round towards zero
+    (twice half a step); 8 more for products, parts of x and scales."""
+    want = x64 @ w64.T
+    tol = _half_step(dtype) * want.abs() + (w64.shape[1] + 8) * 2 * F32 * (x64.abs() @ w64.abs().T) + _floor(dtype)
+    assert bool(((y.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("tokens", [1, 5, 8, 40, 200])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_matvec_of_normal_values(kind, tokens, dtype):
+    specs = (specs_mxfp4 if kind == "mxfp4" else specs_nvfp4)("w", 300, 1056, 3)
+    values, scales = (torch.frombuffer(bytearray(s.raw), dtype=torch.uint8).cuda().reshape(300, -1) for s in specs[:2])
+    top = torch.frombuffer(bytearray(specs[2].raw), dtype=torch.float32).cuda() if kind == "nvfp4" else None
+    scales = scales.view(torch.float8_e4m3fn) if kind == "nvfp4" else scales
+    x = (torch.randn(tokens, 1056, generator=_gen(tokens), device="cuda") * 10).to(DT[dtype])
+    w64 = _weight64(values, scales, top)
+    _check_product(matvec(x, ScaledWeight(values, scales, top)), x.double(), w64, x.dtype)
+    # sums that nearly cancel keep their small part: fp32 output against the same bound
+    _check_product(matvec(x, ScaledWeight(values, scales, top), out_dtype=torch.float32), x.double(), w64, torch.float32)
+    for quant in ("row", "block"):
+        y = rms_norm(x, torch.ones(1056, device="cuda"), quant=quant)
+        s = y.scales.double()[:, None] if quant == "row" else torch.exp2(y.scales.view(torch.uint8).double() - 127).repeat_interleave(32, 1)
+        _check_product(matvec(y, ScaledWeight(values, scales, top), out_dtype=torch.float32), y.values.double() * s, w64, torch.float32)
+
+
+@pytest.mark.parametrize("tokens", [1, 6, 30, 150])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_matvec_far_apart_magnitudes(tokens, dtype):
+    """Tokens and groups of very different size: each is held against its own row, not against the largest."""
+    n, k = 70, 512
+    values, scales, _ = _matrix(n, k, "mxfp4", 5, -60, 20)
+    span = 12 if dtype == "fp16" else 60
+    x = torch.randn(tokens, k, generator=_gen(6), device="cuda") * torch.exp2(torch.randint(-span, span // 2, (tokens, 1), generator=_gen(7), device="cuda").float())
+    x = x.to(DT[dtype])
+    y = matvec(x, ScaledWeight(values, scales), out_dtype=torch.float32)
+    _check_product(y, x.double(), _weight64(values, scales, None), torch.float32)
+
+
+@pytest.mark.parametrize("tokens", [1, 4, 20, 140])
+def test_matvec_extreme_scales(tokens):
+    """E8M0 from 2^-127 to 2^127, NaN scales, E4M3 subnormals and its largest, infinities and NaN in x."""
+    n, k = 40, 256
+    g = _gen(8)
+    values = torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.full((n, k // 32), 127, device="cuda", dtype=torch.uint8)
+    scales[0], scales[1], scales[2, 3], scales[3] = 0, 240, 255, 9
+    x = torch.randint(-2, 3, (tokens, k), generator=g, device="cuda").float()
+    w64 = _weight64(values, scales, None)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = matvec(x.to(dtype), ScaledWeight(values, scales), out_dtype=torch.float32)
+        want = (x.double() @ w64.T).float()
+        assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.nan_to_num(y)[:, 1:], torch.nan_to_num(want)[:, 1:])
+        # row 0 is made of terms around the smallest normal number, where a unit may take what is below for zero
+        assert bool(((y - want)[:, 0].abs() <= k * 2.0 ** -126).all())
+    nv = torch.tensor([2.0 ** -9, 3 * 2.0 ** -9, 448.0, 2.0 ** -6], device="cuda").to(torch.float8_e4m3fn).repeat(n, k // 64)
+    y = matvec(x, ScaledWeight(values, nv))
+    _check_product(y, x.double(), _weight64(values, nv, None), torch.float32)
+    nv = nv.clone()
+    nv.view(torch.uint8)[5, 2] = 0x7F
+    assert bool(torch.isnan(matvec(x, ScaledWeight(values, nv))[:, 5]).all())
+    # an infinity meets no zero in row 4: everything there is infinite with the code's sign; a NaN makes its token's sums NaN
+    values[4] = 0x22
+    ok = ScaledWeight(values, torch.full_like(scales, 127))
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        z = x.to(dtype).clone()
+        z[tokens - 1, 9] = -math.inf
+        z[tokens - 1, 10] = 60000.0
+        y = matvec(z, ok)
+        assert y[tokens - 1, 4] == -math.inf and (tokens == 1 or bool(torch.isfinite(y[:-1]).all()))
+        z[tokens - 1, 200] = math.nan
+        y = matvec(z, ok)
+        assert bool(torch.isnan(y[tokens - 1]).all()) and (tokens == 1 or bool(torch.isfinite(y[:-1]).all()))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("tokens", [1, 3, 24, 200])
+def test_matvec_largest_and_smallest_tokens(dtype, tokens):
+    """Tokens at the ends of their type's range, where parts or scaled copies of them could overflow or vanish."""
+    n, k = 32, 128
+    values, scales, _ = _matrix(n, k, "mxfp4", 4, -4, -4)
+    most = torch.finfo(DT[dtype]).max
+    for size in (most, 2.0 ** -126, 2.0 ** -120):
+        x = torch.zeros(tokens, k, device="cuda", dtype=DT[dtype])
+        x[:, 5] = size
+        x[0, 70] = -size
+        y = matvec(x, ScaledWeight(values, scales), out_dtype=torch.float32)
+        want = x.double() @ _weight64(values, scales, None).T
+        tol = 2.0 ** -20 * (x.double().abs() @ _weight64(values, scales, None).abs().T) + 2 * 2.0 ** -126  # what is below the normal numbers may count as zero
+        assert bool(((y.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("n, k", SIZES)
+@pytest.mark.parametrize("tokens", [1, 7, 16, 65, 130, 300])
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_matvec_gradient_of_whole_numbers_is_exact(n, k, tokens, kind, dtype):
+    k = k + 16 if kind == "nvfp4" and k % 64 == 32 else k
+    w = _matrix(n, k, kind, n + k)
+    x = _integers(tokens, k, DT[dtype], 1).requires_grad_()
+    dy = _integers(tokens, n, DT[dtype], 2)
+    dx, = torch.autograd.grad(matvec(x, ScaledWeight(*w)), x, dy)
+    want = dy.double() @ _weight64(*w)
+    assert dx.shape == x.shape and dx.dtype == x.dtype and torch.equal(dx, want.float().to(x.dtype))
+
+
+def test_matvec_gradient_against_differences_and_between_types():
+    w = _matrix(48, 96, "nvfp4", 3)
+    handle = ScaledWeight(*w)
+    x = torch.randn(5, 96, generator=_gen(1), device="cuda").requires_grad_()
+    c = torch.randn(5, 48, generator=_gen(2), device="cuda")
+    (matvec(x, handle) * c).sum().backward()
+    w64 = _weight64(*w)
+    for i in range(0, 480, 17):  # linear: the difference of two sums is the slope, but for rounding
+        m, k = divmod(i, 96)
+        step = torch.zeros(5, 96, device="cuda")
+        step[m, k] = 1.0
+        slope = ((matvec((x + step).detach(), handle).double() - matvec((x - step).detach(), handle).double()) * c.double()).sum().item() / 2
+        size = ((x.detach().abs() + 1).double() @ w64.abs().T * c.abs().double()).sum().item()
+        assert abs(slope - x.grad[m, k].item()) <= 2 * 104 * 2 * F32 * size
+    xb = x.detach().to(torch.bfloat16).requires_grad_()
+    y = matvec(xb, handle, out_dtype=torch.float32)
+    dx, = torch.autograd.grad(y, xb, c.to(torch.bfloat16).float())
+    assert y.dtype == torch.float32 and dx.dtype == torch.bfloat16
+    _check_product(dx, c.to(torch.bfloat16).double(), w64.T.contiguous(), torch.bfloat16)
+
+
+def test_matvec_layouts_of_matrix_and_tokens():
+    values, scales, _ = _matrix(96, 1024, "mxfp4", 3)
+    x = _integers(6, 1024, torch.bfloat16, 3)
+    want = matvec(x, ScaledWeight(values, scales))
+    assert torch.equal(matvec(x, ScaledWeight(values.reshape(96, 32, 16), scales)), want)
+    assert torch.equal(matvec(x, ScaledWeight(values, scales.view(torch.float8_e8m0fnu))), want)
+    if hasattr(torch, "float4_e2m1fn_x2"):
+        assert torch.equal(matvec(x, ScaledWeight(values.view(torch.float4_e2m1fn_x2), scales)), want)
+    stack = torch.stack((torch.zeros_like(values), values)).reshape(2, 96, 32, 16)
+    assert torch.equal(matvec(x, ScaledWeight(stack, torch.stack((scales, scales)), expert=1)), want)
+    # views: rows with room behind them, every second row, transposed storage, an odd offset
+    room = torch.zeros(96, 1024, dtype=torch.uint8, device="cuda")
+    room[:, 16:528] = values
+    assert torch.equal(matvec(x, ScaledWeight(room[:, 16:528], scales)), want)
+    twice = values.repeat_interleave(2, 0)
+    assert torch.equal(matvec(x, ScaledWeight(twice[::2], scales.repeat_interleave(2, 0)[1::2])), want)
+    assert torch.equal(matvec(x, ScaledWeight(values.t().contiguous().t(), scales.t().contiguous().t())), want)
+    odd = torch.zeros(96 * 512 + 1, dtype=torch.uint8, device="cuda")
+    odd[1:] = values.flatten()
+    assert torch.equal(matvec(x, ScaledWeight(odd[1:].view(96, 512), scales)), want)
+    one = ScaledWeight(values[5:6], scales[5:6])
+    assert torch.equal(matvec(x, one), want[:, 5:6])
+    # tokens: strided, offset by one element, more dimensions, one vector, none
+    assert torch.equal(matvec(x.t().contiguous().t(), ScaledWeight(values, scales)), want)
+    flat = torch.zeros(6 * 1024 + 1, dtype=torch.bfloat16, device="cuda")
+    flat[1:] = x.flatten()
+    assert torch.equal(matvec(flat[1:].view(6, 1024), ScaledWeight(values, scales)), want)
+    assert torch.equal(matvec(x.view(2, 3, 1024), ScaledWeight(values, scales)), want.view(2, 3, 96))
+    assert torch.equal(matvec(x[2], ScaledWeight(values, scales)), want[2])
+    assert matvec(x[:0], ScaledWeight(values, scales)).shape == (0, 96)
+    e = x[:0].clone().requires_grad_()
+    assert torch.autograd.grad(matvec(e, ScaledWeight(values, scales)).sum(), e)[0].shape == (0, 1024)
+    q = x.to(torch.float8_e4m3fn)
+    both = torch.ones(6, 2, device="cuda")
+    assert torch.equal(matvec(ScaledActivations(q.t().contiguous().t(), both[:, 0]), ScaledWeight(values, scales)), want)
+
+
+def test_a_token_does_not_depend_on_its_neighbours():
+    """The same token gives the same bits beside others that hold infinities, as long as as many are asked for."""
+    w = ScaledWeight(*_matrix(200, 2048, "nvfp4", 3))
+    for tokens in (2, 8, 40, 200):
+        x = torch.randn(tokens, 2048, generator=_gen(3), device="cuda").to(torch.bfloat16)
+        a = matvec(x, w)
+        assert torch.equal(a, matvec(x, w))
+        z = x.clone()
+        z[1:] = math.inf
+        assert torch.equal(matvec(z, w)[0], a[0])
+
+
+def test_refusals():
+    values, scales, top = _matrix(64, 128, "nvfp4", 1)
+    mx_values, mx_scales, _ = _matrix(64, 128, "mxfp4", 1)
+    w = ScaledWeight(values, scales, top)
+    x = torch.zeros(2, 128, device="cuda")
+    for bad in [lambda: ScaledWeight(values.float(), scales), lambda: ScaledWeight(values, scales.float()), lambda: ScaledWeight(values, scales, top.double()),
+                lambda: ScaledWeight(values, scales, torch.ones(2, device="cuda")), lambda: matvec(x.double(), w), lambda: matvec(x, w, out_dtype=torch.float64),
+                lambda: rms_norm(x.double(), x[0]), lambda: ScaledActivations(x, x[:, 0]), lambda: ScaledActivations(x.to(torch.float8_e4m3fn), x[:, 0].half()),
+                lambda: matvec(x, values)]:
+        with pytest.raises(TypeError):
+            bad()
+    for bad in [lambda: ScaledWeight(values, scales[:, :-1]), lambda: ScaledWeight(values[:, :-4], scales), lambda: ScaledWeight(mx_values, mx_scales, top),
+                lambda: ScaledWeight(values[None], scales[None]), lambda: ScaledWeight(values[:0], scales[:0]), lambda: ScaledWeight(values, scales, top.cpu()),
+                lambda: matvec(x[:, :64], w), lambda: matvec(x.cpu(), w), lambda: rms_norm(x, x[0, :64]), lambda: rms_norm(x, x[0], quant="int8"),
+                lambda: rms_norm(x[:, :40], x[0, :40], quant="block"), lambda: rms_norm(x, x[0], residual=x[:1]), lambda: rms_norm(x, x[0], residual=x.half()),
+                lambda: rms_norm(x[:, :0], x[0, :0]), lambda: ScaledActivations(x.to(torch.float8_e4m3fn), x[:, :2]), lambda: ScaledActivations(x[:, :40].to(torch.float8_e4m3fn), mx_scales[:2, :1]),
+                lambda: Projection(x[0, :64], [w]), lambda: Projection(x, [w]), lambda: Projection(x[0], [w], quant="int8")]:
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(IndexError):
+        ScaledWeight(values[None], scales[None], expert=1)
+
+
+# ---- streams, graphs, containers ------------------------------------------------------------------------
+def test_streams_and_overlapping_calls():
+    w = ScaledWeight(*_matrix(1024, 2048, "mxfp4", 3))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    xs = [_integers(t, 2048, torch.bfloat16, t) for t in (1, 16, 100)]
+    want = [matvec(x, w) for x in xs]
+    norm = torch.ones(2048, device="cuda")
+    want_norm = [rms_norm(x, norm, quant="row").values.view(torch.uint8) for x in xs]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(20):
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append((matvec(x, w), rms_norm(x, norm, quant="row").values.view(torch.uint8)))
+    torch.cuda.synchronize()
+    for i, (y, q) in enumerate(got):
+        assert torch.equal(y, want[i % 3]) and torch.equal(q, want_norm[i % 3])
+
+
+@pytest.mark.parametrize("tokens", [1, 12, 130])
+def test_captured_and_replayed(tokens):
+    w = ScaledWeight(*_matrix(512, 1024, "nvfp4", 3))
+    norm = torch.ones(1024, device="cuda", dtype=torch.bfloat16)
+    p = Projection(norm, [w, w], quant="block")
+    x = torch.randn(tokens, 1024, generator=_gen(1), device="cuda").to(torch.bfloat16)
+    res = torch.randn(tokens, 1024, generator=_gen(2), device="cuda").to(torch.bfloat16)
+    p(x, res)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs of the same handles, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = p(x, res)
+        graphs.append((g, out))
+    for seed in (3, 4):
+        x.copy_(torch.randn(tokens, 1024, generator=_gen(seed), device="cuda"))
+        for g, _ in graphs:
+            g.replay()
+        (y1, y2), h = p(x, res)
+        for _, ((z1, z2), k) in graphs:
+            assert torch.equal(z1, y1) and torch.equal(z2, y2) and torch.equal(k, h)
+
+
+def test_gradients_captured_and_replayed():
+    w = ScaledWeight(*_matrix(256, 512, "mxfp4", 3))
+    norm = torch.ones(512, device="cuda", requires_grad=True)
+    x = torch.randn(40, 512, generator=_gen(1), device="cuda", requires_grad=True)
+    res = torch.randn(40, 512, generator=_gen(2), device="cuda", requires_grad=True)
+    dy = torch.randn(40, 256, generator=_gen(3), device="cuda")
+
+    def step():
+        (y,), h = Projection(norm, [w])(x, res)
+        return torch.autograd.grad((y, h), (x, norm, res), (dy, torch.ones_like(h)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    with torch.no_grad():
+        x.copy_(torch.randn(40, 512, generator=_gen(5), device="cuda"))
+    g.replay()
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
+
+
+def test_nothing_is_written_outside_the_results():
+    w = ScaledWeight(*_matrix(100, 512, "mxfp4", 3))
+    room = torch.full((1 << 22,), 7, dtype=torch.uint8, device="cuda")
+    L, stream = ptwm_b200._lib.lib(), 1
+    x = _integers(11, 512, torch.float32, 2)
+    torch.cuda.synchronize()
+    at = room.data_ptr() + 4096
+    assert L.ptwm_b200_matvec(w._ref, x.data_ptr(), 0, at, 11, 1, 0, 1, 0, stream) == 0
+    torch.cuda.synchronize()
+    end = 4096 + 11 * 100 * 4
+    assert bool((room[:4096] == 7).all()) and bool((room[end:] == 7).all())
+    room.fill_(7)
+    assert L.ptwm_b200_matvec_grad(w._ref, x.data_ptr(), at, 9, 1, 0, stream) == 0  # any 9 x 100 numbers do as a gradient
+    torch.cuda.synchronize()
+    end = 4096 + 9 * 512 * 4
+    assert bool((room[:4096] == 7).all()) and bool((room[end:] == 7).all())
+    room.fill_(7)
+    wt = torch.ones(511, device="cuda")
+    assert L.ptwm_b200_rms_norm(x.data_ptr(), 0, wt.data_ptr(), 0, at, room.data_ptr() + (1 << 20), 3, 511, 1, 1, 1, 1e-6, 0, stream) == 0
+    torch.cuda.synchronize()
+    assert bool((room[:4096] == 7).all()) and bool((room[4096 + 3 * 511:1 << 20] == 7).all()) and bool((room[(1 << 20) + 12:] == 7).all())
+
+
+def test_weights_straight_from_a_container(tmp_path):
+    specs = mixed_model()
+    specs += [spec_norm("blk.norm2.weight", 256, 21)]
+    for spec in specs_nvfp4("blk.nv2", 160, 256, 22):
+        specs.append(spec)
+    blob = oracle.write_container(specs, chunk_size=4096, emit_crc=True, emit_hash=True, menu=(oracle.IDENTITY, oracle.HUFFMAN, oracle.RANS, oracle.O1SAC))
+    path = tmp_path / "m.ptwm"
+    path.write_bytes(blob)
+    raw = {s.name: s for s in specs}
+    handle = ptwm_b200.ContainerHandle(blob)
+    state = ptwm_b200.load_file(path)
+    index, opened = ptwm_b200.TensorIndex(path), ptwm_b200.SafeOpen(path)
+    x = torch.randn(3, 256, generator=_gen(1), device="cuda").to(torch.bfloat16)
+    for name, values, scales, top in (("blk.mx", "blk.mx_blocks", "blk.mx_scales", None), ("blk.nv", "blk.nv.weight", "blk.nv.weight_scale", "blk.nv.weight_scale_2")):
+        v = torch.from_numpy(np.frombuffer(raw[values].raw, dtype=np.uint8).copy()).reshape(raw[values].shape)
+        s = torch.from_numpy(np.frombuffer(raw[scales].raw, dtype=np.uint8).copy()).reshape(raw[scales].shape)
+        g = None if top is None else torch.from_numpy(np.frombuffer(raw[top].raw, dtype=np.float32).copy())
+        w64 = _weight64(v, s if top is None else s.view(torch.float8_e4m3fn), g).cuda()
+        w = handle.scaled_weight(name)
+        assert w.shape == (96, 256) and w.kind == ("mxfp4" if top is None else "nvfp4")
+        y = matvec(x, w)
+        _check_product(y, x.double(), w64, torch.bfloat16)
+        for other in (ScaledWeight.from_state(state, name), index.get_scaled_weight(name), opened.get_scaled_weight(name)):
+            assert torch.equal(matvec(x, other), y)
+    with pytest.raises(KeyError):
+        handle.scaled_weight("blk.q")
+    # a norm and the two matrices behind it, as a block of a model runs them
+    p = handle.projection("blk.norm2.weight", ["blk.nv", "blk.nv2"], eps=1e-5, quant="block")
+    res = torch.randn(3, 256, generator=_gen(2), device="cuda").to(torch.bfloat16)
+    (a, b), h = p(x, res)
+    q, k = rms_norm(x, handle.decode("blk.norm2.weight"), 1e-5, residual=res, quant="block")
+    assert torch.equal(h, k) and torch.equal(a, matvec(q, handle.scaled_weight("blk.nv"))) and torch.equal(b, matvec(q, handle.scaled_weight("blk.nv2")))
+    assert a.shape == (3, 96) and b.shape == (3, 160) and a.dtype == torch.bfloat16
+    with pytest.raises(KeyError):
+        handle.projection("blk.none", ["blk.nv"])
+
+
+def test_tensor_sizes_beyond_32_bits():
+    """Offsets into x and y that pass 2^31 elements."""
+    rows, cols = 262145, 8224
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[-1] = torch.randn(cols, generator=_gen(1), device="cuda")
+    w = torch.ones(cols, dtype=torch.bfloat16, device="cuda")
+    y = rms_norm(x, w, quant="block")
+    one = rms_norm(x[-1:], w, quant="block")
+    assert torch.equal(y.values.view(torch.uint8)[-1], one.values.view(torch.uint8)[0]) and torch.equal(y.scales.view(torch.uint8)[-1], one.scales.view(torch.uint8)[0])
+    m = ScaledWeight(*_matrix(16, cols, "mxfp4", 2))
+    got = matvec(y, m)
+    assert bool((got[:-200] == 0).all())
+    want = matvec(one, m, out_dtype=torch.float32).double()
+    assert bool(((got[-1].double() - want[0]).abs() <= 2.0 ** -7 * want[0].abs() + 1e-3 * want.abs().max()).all())

@@ -1,0 +1,88 @@
+"""Refusals of the operators that apply decoded weights, without a GPU: the C ABI looks at its arguments before it touches a
+device, and the Python side before it calls."""
+import ctypes as C
+
+import pytest
+import torch
+
+import ptwm_b200
+from ptwm_b200 import _lib
+from ptwm_b200.operators import scaled_names
+
+INVALID, SMALL, UNSUPPORTED = -1, -2, -5
+A = 1 << 20  # an aligned address nobody reads
+
+
+@pytest.fixture(scope="module")
+def L():
+    ptwm_b200.build()
+    return _lib.lib()
+
+
+def _weight(**over):
+    a = dict(values=A, scales=A, global_scale=0, rows=64, cols=64, value_pitch=32, scale_pitch=16, group=32, reserved=0)
+    a.update(over)
+    return _lib.ScaledWeightArgs(**a)
+
+
+@pytest.mark.parametrize("over, rc", [
+    (dict(values=0), INVALID), (dict(scales=0), INVALID), (dict(group=8), INVALID), (dict(rows=0), INVALID), (dict(cols=0), INVALID), (dict(cols=48), INVALID),
+    (dict(value_pitch=24), INVALID), (dict(values=A + 8), INVALID), (dict(scales=A + 4), INVALID), (dict(scale_pitch=8), INVALID), (dict(value_pitch=16), INVALID),
+    (dict(cols=1024, value_pitch=512), INVALID), (dict(rows=(1 << 30) + 1), UNSUPPORTED)])
+def test_matrices_that_are_none(L, over, rc):
+    w = _weight(**over)
+    assert L.ptwm_b200_matvec(C.addressof(w), A, 0, A, 1, 6, 0, 6, 0, 1) == rc
+    assert L.ptwm_b200_matvec_grad(C.addressof(w), A, A, 1, 6, 0, 1) == rc
+    assert _lib.last_error().startswith("scaled weight")
+
+
+def test_tokens_that_are_none(L):
+    w = _weight()
+    p = C.addressof(w)
+    nv = _weight(cols=48, group=16, value_pitch=32)
+    for args, rc in [((p, A, 0, A, 1, 6, 0, 13), UNSUPPORTED), ((p, A, 0, A, 1, 13, 0, 6), UNSUPPORTED), ((p, A, A, A, 1, 6, 1, 6), UNSUPPORTED), ((p, A, 0, A, 1, 29, 1, 6), UNSUPPORTED),
+                     ((p, A, A, A, 1, 29, 0, 6), UNSUPPORTED), ((p, A, A, A, 1, 29, 3, 6), UNSUPPORTED), ((p, 0, 0, A, 1, 6, 0, 6), INVALID), ((p, A, 0, 0, 1, 6, 0, 6), INVALID),
+                     ((p, A, 0, A, (1 << 19) + 1, 6, 0, 6), UNSUPPORTED), ((C.addressof(nv), A, A, A, 1, 29, 2, 6), INVALID), ((None, A, 0, A, 1, 6, 0, 6), INVALID)]:
+        assert L.ptwm_b200_matvec(*args, 0, 1) == rc, args
+    assert L.ptwm_b200_matvec(p, 0, 0, 0, 0, 6, 0, 6, 0, 1) == 0  # no tokens: nothing to do, on any machine
+    for args, rc in [((p, A, A, 1, 29), UNSUPPORTED), ((p, 0, A, 1, 6), INVALID), ((p, A, 0, 1, 6), INVALID)]:
+        assert L.ptwm_b200_matvec_grad(*args, 0, 1) == rc, args
+
+
+def test_norms_that_are_none(L):
+    for args, rc in [((A, 0, A, 0, A, 0, 4, 64, 29, 6, 0), UNSUPPORTED), ((A, 0, A, 0, A, 0, 4, 64, 6, 13, 0), UNSUPPORTED), ((A, 0, A, 0, A, A, 4, 64, 6, 6, 3), INVALID),
+                     ((A, 0, A, 0, A, 0, 4, 0, 6, 6, 0), INVALID), ((A, 0, A, 0, A, A, 4, 48, 6, 6, 2), INVALID), ((0, 0, A, 0, A, 0, 4, 64, 6, 6, 0), INVALID),
+                     ((A, 0, 0, 0, A, 0, 4, 64, 6, 6, 0), INVALID), ((A, 0, A, 0, 0, 0, 4, 64, 6, 6, 0), INVALID), ((A, A, A, 0, A, 0, 4, 64, 6, 6, 0), INVALID),
+                     ((A, 0, A, 0, A, 0, 4, 64, 6, 6, 1), INVALID), ((A, 0, A, 0, A, 0, 1 << 31, 64, 6, 6, 0), UNSUPPORTED)]:
+        assert L.ptwm_b200_rms_norm(*args, 1e-6, 0, 1) == rc, args
+    assert L.ptwm_b200_rms_norm(0, 0, 0, 0, 0, 0, 0, 64, 6, 6, 0, 1e-6, 0, 1) == 0
+    need = L.ptwm_b200_rms_norm_grad_scratch_bytes(1000, 64)
+    assert need >= 64 * 4
+    for args, rc in [((A, A, A, 0, A, 0, 0, 0, 4, 64, 29, 6), UNSUPPORTED), ((A, A, A, 0, 0, 0, 0, 0, 4, 64, 6, 6), INVALID), ((A, A, 0, 0, A, 0, 0, 0, 4, 64, 6, 6), INVALID),
+                     ((A, A, A, 0, A, A, 0, 0, 1000, 64, 6, 6), SMALL), ((A, A, A, 0, A, A, A, need - 1, 1000, 64, 6, 6), SMALL), ((A, A, A, 0, A, 0, 0, 0, 4, 0, 6, 6), UNSUPPORTED)]:
+        assert L.ptwm_b200_rms_norm_grad(*args, 1e-6, 0, 1) == rc, args
+
+
+def test_tensors_in_host_memory_are_refused():
+    x = torch.zeros(2, 64)
+    with pytest.raises(ValueError, match="host memory"):
+        ptwm_b200.rms_norm(x, torch.ones(64))
+    with pytest.raises(ValueError, match="host memory"):
+        ptwm_b200.ScaledWeight(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="host memory"):
+        ptwm_b200.ScaledActivations(x.to(torch.float8_e4m3fn), torch.zeros(2))
+    with pytest.raises(TypeError, match="ScaledWeight"):
+        ptwm_b200.matvec(x, torch.zeros(4, 32, dtype=torch.uint8))
+    with pytest.raises(TypeError, match="tensor"):
+        ptwm_b200.rms_norm([1.0], torch.ones(1))
+
+
+def test_names_of_a_microscaled_matrix():
+    def of(*names):
+        return set(names).__contains__
+    assert scaled_names("a", of("a.weight", "a.weight_scale", "a.weight_scale_2")) == ("a.weight", "a.weight_scale", "a.weight_scale_2")
+    assert scaled_names("a", of("a.weight", "a.weight_scale")) == ("a.weight", "a.weight_scale", None)
+    assert scaled_names("a", of("a_blocks", "a_scales", "a_bias")) == ("a_blocks", "a_scales", None)
+    assert scaled_names("a", of("a", "a_scale", "a_scale_2")) == ("a", "a_scale", "a_scale_2")
+    with pytest.raises(KeyError):
+        scaled_names("a", of("a", "a_blocks", "b_scale"))
