@@ -13,7 +13,7 @@ import subprocess
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PTWM_B200_LIB") or os.path.join(_HERE, "libptwm_b200.so")  # PTWM_B200_LIB: load another build of the same library
 _SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("unity.cu", "ptwm_b200.cu", "encoder.cu", "kernels.cuh", "encode.cuh", "encode_tables.cuh", "noalloc.cu",
-                                                      "format.hpp", "host_common.hpp", "errors.hpp", "slice_copy.hpp", "plan.h", "operators.cu", "number_types.cuh", "rms_norm.cuh", "matvec.cuh")] + [
+                                                      "format.hpp", "host_common.hpp", "errors.hpp", "slice_copy.hpp", "plan.h", "operators.cu", "number_types.cuh", "rms_norm.cuh", "matvec.cuh", "matvec_tiles.cuh", "tensor_core.cuh")] + [
     os.path.join(_HERE, "..", "include", "ptwm_b200.h")]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-pthread", "-shared"]
@@ -101,8 +101,10 @@ _SIGNATURES = {
     "ptwm_b200_rms_norm": (C.c_int64, [C.c_uint64] * 8 + [C.c_uint32] * 3 + [C.c_float, C.c_uint32, C.c_uint64]),
     "ptwm_b200_rms_norm_grad_scratch_bytes": (C.c_uint64, [C.c_uint64, C.c_uint64]),
     "ptwm_b200_rms_norm_grad": (C.c_int64, [C.c_uint64] * 10 + [C.c_uint32] * 2 + [C.c_float, C.c_uint32, C.c_uint64]),
-    "ptwm_b200_matvec": (C.c_int64, [C.c_void_p] + [C.c_uint64] * 4 + [C.c_uint32] * 4 + [C.c_uint64]),
-    "ptwm_b200_matvec_grad": (C.c_int64, [C.c_void_p] + [C.c_uint64] * 3 + [C.c_uint32] * 2 + [C.c_uint64]),
+    "ptwm_b200_matvec_scratch_bytes": (C.c_uint64, [C.c_void_p] + [C.c_uint64] * 2 + [C.c_uint32] * 2),
+    "ptwm_b200_matvec": (C.c_int64, [C.c_void_p] + [C.c_uint64] * 4 + [C.c_uint32] * 3 + [C.c_uint64] * 2 + [C.c_uint32, C.c_uint64]),
+    "ptwm_b200_matvec_grad": (C.c_int64, [C.c_void_p] + [C.c_uint64] * 3 + [C.c_uint32] + [C.c_uint64] * 2 + [C.c_uint32, C.c_uint64]),
+    "ptwm_b200_operator_status": (C.c_int64, [C.c_uint32]),
     "ptwm_hardware_backend_v1_cuda_stream_handle": (C.c_uint64, [C.c_uint32]),
     "ptwm_plane_codec_v1_cuda_stream_handle": (C.c_uint64, [C.c_uint32]),
     "ptwm_hardware_backend_v1_dispatch_decode_cuda": (C.c_int64, [C.c_uint8, C.c_void_p, C.c_size_t, C.c_char_p, C.c_size_t, C.c_uint64, C.c_size_t,

@@ -63,31 +63,4 @@ template <class T, class Y> __global__ void __launch_bounds__(256) matvec_kernel
     }
 }
 
-// A thread per byte of a row (two columns) and eight tokens, down all rows.
-template <class T> __global__ void __launch_bounds__(128) matvec_grad_kernel(ScaledMatrix w, TokenArgs t) {
-    const uint64_t b = uint64_t(blockIdx.x) * 128 + threadIdx.x, m0 = uint64_t(blockIdx.y) * 8;
-    if (b >= w.cols / 2) return;
-    const int count = int(t.tokens - m0 < 8 ? t.tokens - m0 : 8);
-    float lo[8] = {}, hi[8] = {};
-    for (uint64_t n = 0; n < w.rows; ++n) {
-        const uint32_t v = w.values[n * w.value_pitch + b];
-        const float s = group_scale(w, n, 2 * b), a = e2m1_f32(v & 15) * s, c = e2m1_f32(v >> 4) * s;
-#pragma unroll
-        for (int m = 0; m < 8; ++m)
-            if (m < count) {
-                const float d = to_f32(static_cast<const T*>(t.x)[(m0 + m) * w.rows + n]);
-                lo[m] += d * a;
-                hi[m] += d * c;
-            }
-    }
-    const float global = w.global_scale ? *w.global_scale : 1.0f;
-#pragma unroll
-    for (int m = 0; m < 8; ++m)
-        if (m < count) {
-            T* y = static_cast<T*>(t.y) + (m0 + m) * w.cols + 2 * b;
-            y[0] = from_f32<T>(lo[m] * global);
-            y[1] = from_f32<T>(hi[m] * global);
-        }
-}
-
 }  // namespace ptwm

@@ -1,0 +1,261 @@
+// Products of a 4-bit matrix with more than a few tokens, on tensor cores.
+//
+//   forward:   D[n][m] = sum_k W[n][k] x[m][k]       gradient: D[k][m] = sum_n W[n][k] dy[m][n]
+// A block makes a tile of 128 rows of D (n, or k) and up to 256 tokens.  The matrix stays packed until it is in shared memory:
+// TMA brings boxes of nibbles and scales, eight warps turn them into bf16 (exactly: a nibble times its scale has at most six
+// significant bits) in the swizzled lines the tensor cores read, and one thread issues the MMAs.  Tokens come as bf16 by TMA.
+// Tokens of other types are bf16 parts that add up to them: E4M3 is one, fp16 two, fp32 three (token_parts_kernel); each part is
+// multiplied with the same converted tile, and all sums meet in the same fp32 accumulator.  In the gradient the contraction
+// runs down the rows of the matrix, so the converted tile is MN-major: the same lines, another descriptor.
+#pragma once
+#include "matvec.cuh"
+#include "tensor_core.cuh"
+
+namespace ptwm {
+
+constexpr uint32_t TILE_ROWS = 128;                 // rows of D to a block
+constexpr uint32_t STEP = 64;                       // contraction to a converted tile: one 128-byte line of bf16
+constexpr uint32_t RAW_STAGES = 6, RAW_BYTES = 8192, SCALES_BYTES = 8192, A_STAGES = 4, A_BYTES = TILE_ROWS * STEP * 2;
+constexpr uint32_t TILES_THREADS = 352;             // warp 0: TMA of the matrix, 1: MMA, 2: TMA of the tokens, 3 to 10: conversion, then the results
+constexpr uint32_t TILES_HEAD = 1024;               // barriers and the like, in front of the buffers
+
+struct TilesArgs {
+    uint64_t rows;             // of D: n, or k in the gradient
+    uint64_t contraction;      // k, or n
+    uint64_t tokens;
+    uint64_t part_rows;        // rows from one part of the tokens to the next
+    uint32_t parts;
+    uint32_t tile_tokens;      // a multiple of 16, at most 256
+    uint32_t b_stages;
+    uint32_t group;
+    const float* global_scale;
+    const float* token_scale;  // or null
+    void* y;
+    uint32_t* status;
+};
+
+// Bytes of dynamic shared memory; 1024 more to align them.
+inline uint32_t tiles_smem(uint32_t tile_tokens, uint32_t b_stages) {
+    return 1024 + TILES_HEAD + RAW_STAGES * RAW_BYTES + SCALES_BYTES + A_STAGES * A_BYTES + b_stages * tile_tokens * STEP * 2;
+}
+
+// Eight nibbles -> eight bf16 in their order, times `scale`.  A word takes the even nibble of a byte to its low half and the odd one
+// to its high half; a product puts their signs at bit 15 and the other three bits at 8..6, which reads as the number times 2^-126;
+// `scale` is the group's times 2^126.  Every step is exact.
+__device__ __forceinline__ void nibbles_to_bf16(uint32_t w, uint32_t scale, uint32_t (&out)[4]) {
+    const uint32_t odd = w >> 4;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t v = __byte_perm(w, odd, i | i << 4 | (4 + i) << 8 | (4 + i) << 12) & 0x000F000Fu;
+        const uint32_t bits = (v * 0x1040u) & 0x81C081C0u;
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(out[i]) : "r"(bits), "r"(scale));
+    }
+}
+
+// Scale of a group as a pair of bf16.  MXFP4: 2^(e - 127) 2^126, and for e above 128 the rest in *more (else 1).  NVFP4: s 2^126 would
+// pass bf16's range, so it is s 2^116, and the results are multiplied by 2^10.
+__device__ __forceinline__ uint32_t mx_scale(uint32_t e, uint32_t* more) {
+    const uint32_t hi = e > 128 ? 254 : e + 126, rest = e > 128 ? e - 1 : 127;
+    *more = e == 255 ? 0x7FC07FC0u : rest * 0x00800080u;
+    return hi * 0x00800080u;
+}
+__device__ __forceinline__ uint32_t nv_scale(uint32_t s) {
+    const __nv_bfloat16 b = __float2bfloat16_rn(e4m3_f32(uint8_t(s)) * 0x1p116f);
+    uint16_t u;
+    memcpy(&u, &b, 2);
+    return u * 0x00010001u;
+}
+constexpr float NV_REST = 1024.0f;
+
+template <bool GRAD> struct TilesShared {
+    static constexpr uint32_t raw = TILES_HEAD, scales = raw + RAW_STAGES * RAW_BYTES, a = scales + SCALES_BYTES, b = a + A_STAGES * A_BYTES;
+    static constexpr uint32_t raw_rows = GRAD ? STEP : TILE_ROWS, scale_bytes = raw_rows * 16, scale_slots = SCALES_BYTES / scale_bytes;
+    // barriers: raw full / empty, a full / empty, b full / empty, accumulator full
+    static constexpr uint32_t raw_full = 0, raw_empty = 64, a_full = 128, a_empty = 192, b_full = 256, b_empty = 320, done = 384, tmem = 392, failed = 396;
+};
+
+// Nibbles of one thread (16 bytes: 32 values) -> four 16-byte pieces of bf16.
+__device__ __forceinline__ void convert32(const uint4& v, uint32_t group, uint32_t s, uint4 (&out)[4]) {
+    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+    uint32_t more = 0x3F803F80u;
+    const uint32_t s0 = group == 32 ? mx_scale(s & 255, &more) : nv_scale(s & 255), s1 = group == 32 ? s0 : nv_scale(s >> 8 & 255);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t o[4];
+        nibbles_to_bf16(words[i], i < 2 ? s0 : s1, o);
+        if (more != 0x3F803F80u) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[j]) : "r"(more));
+        }
+        out[i] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+template <class Y, bool GRAD>
+__global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __grid_constant__ CUtensorMap values, const __grid_constant__ CUtensorMap scales,
+                                                                        const __grid_constant__ CUtensorMap tokens, const TilesArgs t) {
+    using S = TilesShared<GRAD>;
+    extern __shared__ uint8_t dynamic[];
+    uint8_t* base = dynamic + (1024 - (smem_u32(dynamic) & 1023)) % 1024;
+    const uint32_t sb = smem_u32(base);
+    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(base + S::failed);
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint32_t row0 = blockIdx.x * TILE_ROWS, token0 = blockIdx.y * t.tile_tokens;
+    const uint32_t steps = uint32_t((t.contraction + STEP - 1) / STEP);
+    // A raw stage is 128 k of 128 rows (two steps) forward, and 64 rows (one step) of the tile's 128 k in the gradient.
+    const uint32_t raws = GRAD ? steps : (steps + 1) / 2;
+    // A box of scales is 16 bytes of each row: 512 k (MXFP4) or 256 (NVFP4), so several raw stages forward, one in the gradient.
+    const uint32_t scale_raws = GRAD ? 1 : t.group == 32 ? 4 : 2;
+    const uint32_t cols = t.tile_tokens <= 32 ? 32 : t.tile_tokens <= 64 ? 64 : t.tile_tokens <= 128 ? 128 : 256;
+    const uint32_t b_bytes = t.tile_tokens * STEP * 2;
+
+    if (threadIdx.x == 0) {
+        *failed = 0;
+        for (uint32_t i = 0; i < RAW_STAGES; ++i) { mbar_init(sb + S::raw_full + 8 * i, 1); mbar_init(sb + S::raw_empty + 8 * i, 8); }
+        for (uint32_t i = 0; i < A_STAGES; ++i) { mbar_init(sb + S::a_full + 8 * i, 8); mbar_init(sb + S::a_empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < t.b_stages; ++i) { mbar_init(sb + S::b_full + 8 * i, 1); mbar_init(sb + S::b_empty + 8 * i, 1); }
+        mbar_init(sb + S::done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(sb + S::tmem, cols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(base + S::tmem);
+
+    if (warp == 0) {
+        if (elect_one()) {
+            for (uint32_t raw = 0; raw < raws && !*failed; ++raw) {
+                const uint32_t st = raw % RAW_STAGES, full = sb + S::raw_full + 8 * st;
+                if (raw >= RAW_STAGES) mbar_wait(sb + S::raw_empty + 8 * st, (raw / RAW_STAGES - 1) & 1, failed);
+                if (*failed) break;
+                const bool with_scales = raw % scale_raws == 0;
+                mbar_expect(full, S::raw_rows * (with_scales ? 80 : 64));
+                if (GRAD) tma_load(sb + S::raw + st * RAW_BYTES, &values, full, int32_t(row0 / 2), int32_t(raw * STEP));
+                else tma_load(sb + S::raw + st * RAW_BYTES, &values, full, int32_t(raw * 64), int32_t(row0));
+                if (with_scales) {
+                    // its slot was last read for raw stages before raw - RAW_STAGES: there are enough slots for those in between
+                    const uint32_t dst = sb + S::scales + raw / scale_raws % S::scale_slots * S::scale_bytes;
+                    if (GRAD) tma_load(dst, &scales, full, int32_t(row0 / t.group & ~15u), int32_t(raw * STEP));
+                    else tma_load(dst, &scales, full, int32_t(raw / scale_raws * 16), int32_t(row0));
+                }
+            }
+            // every load has been waited for by those who use it, unless something failed: then what is under way gets time to land
+            if (*failed) let_copies_land();
+        }
+    } else if (warp == 2) {
+        if (elect_one()) {
+            for (uint32_t b = 0; b < steps * t.parts && !*failed; ++b) {
+                const uint32_t st = b % t.b_stages, full = sb + S::b_full + 8 * st;
+                if (b >= t.b_stages) mbar_wait(sb + S::b_empty + 8 * st, (b / t.b_stages - 1) & 1, failed);
+                if (*failed) break;
+                mbar_expect(full, b_bytes);
+                tma_load(sb + S::b + st * b_bytes, &tokens, full, int32_t(b / t.parts * STEP), int32_t(b % t.parts * t.part_rows + token0));
+            }
+            if (*failed) let_copies_land();
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t idesc = instruction_desc(t.tile_tokens, GRAD);
+            for (uint32_t step = 0, b = 0; step < steps && !*failed; ++step) {
+                const uint32_t as = step % A_STAGES;
+                mbar_wait(sb + S::a_full + 8 * as, step / A_STAGES & 1, failed);
+                for (uint32_t p = 0; p < t.parts; ++p, ++b) {
+                    const uint32_t bs = b % t.b_stages;
+                    mbar_wait(sb + S::b_full + 8 * bs, b / t.b_stages & 1, failed);
+                    if (*failed) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (uint32_t k = 0; k < STEP / 16; ++k) {
+                        const uint32_t a_addr = sb + S::a + as * A_BYTES + (GRAD ? k * 2048 : k * 32);
+                        const uint64_t ad = GRAD ? operand_desc(a_addr, 8192, 1024) : operand_desc(a_addr, 16, 1024);
+                        mma_f16(tmem, ad, operand_desc(sb + S::b + bs * b_bytes + k * 32, 16, 1024), idesc, (b | k) != 0);
+                    }
+                    tc_commit(sb + S::b_empty + 8 * bs);
+                }
+                if (!*failed) tc_commit(sb + S::a_empty + 8 * as);
+            }
+            tc_commit(sb + S::done);
+        }
+    } else {
+        const uint32_t c = threadIdx.x - 96;
+        // this thread's 16 bytes of a raw stage: forward row c / 2 and half c % 2 of either step's 32 bytes; in the gradient row (c % 128) / 2 and
+        // one quarter of its 64 bytes, so that eight neighbours store to eight different 16-byte banks
+        const uint32_t row = GRAD ? c % 128 / 2 : c / 2, quarter = GRAD ? c % 2 + c / 128 * 2 : c % 2;
+        const uint32_t first_group = GRAD ? row0 / t.group & 15u : 0;
+        const uint32_t out = GRAD ? (quarter / 2) * 8192 + row / 8 * 1024 + row % 8 * 128 : row / 8 * 1024 + row % 8 * 128;
+        for (uint32_t step = 0; step < steps && !*failed; ++step) {
+            const uint32_t raw = GRAD ? step : step / 2, st = raw % RAW_STAGES, as = step % A_STAGES;
+            const uint32_t q = GRAD ? quarter : step % 2 * 2 + quarter;  // which 32 of the 128 k
+            mbar_wait(sb + S::raw_full + 8 * st, raw / RAW_STAGES & 1, failed);
+            const uint4 v = *reinterpret_cast<const uint4*>(base + S::raw + st * RAW_BYTES + row * 64 + q * 16);
+            const uint8_t* sp = base + S::scales + raw / scale_raws % S::scale_slots * S::scale_bytes + row * 16;
+            const uint32_t g = first_group + raw % scale_raws * (128 / t.group);
+            const uint32_t s = t.group == 32 ? sp[g + q] : *reinterpret_cast<const uint16_t*>(sp + g + 2 * q);
+            uint4 o[4];
+            convert32(v, t.group, s, o);
+            if (step >= A_STAGES) mbar_wait(sb + S::a_empty + 8 * as, (step / A_STAGES - 1) & 1, failed);
+            uint8_t* dst = base + S::a + as * A_BYTES + out;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + (((quarter % 2 * 4 + j) ^ (row % 8)) * 16)) = o[j];
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(sb + S::a_full + 8 * as);
+                if (GRAD || step % 2 || step + 1 == steps) mbar_arrive(sb + S::raw_empty + 8 * st);
+            }
+        }
+        // results: a warp reaches the 32 lanes (rows of D) that its number modulo 4 names; the two warps of a quarter share the tokens
+        mbar_wait(sb + S::done, 0, failed);
+        tc_fence_after();
+        const uint32_t lanes = warp % 4 * 32;
+        const uint64_t n = row0 + lanes + lane;
+        float factor = t.group == 32 ? 1.0f : NV_REST;
+        if (t.global_scale) factor *= *t.global_scale;
+        if (*failed) factor = __uint_as_float(0x7FC00000u);
+        const uint32_t half = (t.tile_tokens / 16 + 1) / 2 * 16, from = warp < 7 ? 0 : half, to = warp < 7 ? half : t.tile_tokens;
+        for (uint32_t m = from; m < to; m += 16) {
+            uint32_t v[16];
+            tmem_load16(tmem + (lanes << 16) + m, v);
+            if (n < t.rows) {
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) {
+                    const uint64_t token = token0 + m + j;
+                    if (token < t.tokens) {
+                        const float f = __uint_as_float(v[j]) * factor;
+                        static_cast<Y*>(t.y)[token * t.rows + n] = from_f32<Y>(t.token_scale ? f * t.token_scale[token] : f);
+                    }
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free(tmem, cols);
+    }
+    if (threadIdx.x == 0 && *failed) atomicExch(t.status, 1u);
+}
+
+// Tokens as bf16 parts whose sum they are: part p of token m is row p * part_rows + m of `out`, `pitch` values long, with zeros behind
+// `cols`.  E4M3 (times its block's scale) fits one bf16, fp16 two, fp32 three (each takes the next eight bits).  What is not finite is
+// its first part alone.
+template <class T>
+__global__ void __launch_bounds__(256) token_parts_kernel(TokenArgs t, uint64_t cols, __nv_bfloat16* out, uint32_t pitch, uint64_t part_rows) {
+    constexpr int PARTS = sizeof(T) == 4 ? 3 : sizeof(T) == 1 ? 1 : std::is_same<T, __half>::value ? 2 : 1;
+    const uint64_t m = blockIdx.x;
+    for (uint64_t k = uint64_t(blockIdx.y) * 256 + threadIdx.x; k < pitch; k += uint64_t(gridDim.y) * 256) {
+        float rest = k < cols ? token_value<T>(t, m, k, cols) : 0.0f;
+        const bool finite = (__float_as_uint(rest) & 0x7F800000u) != 0x7F800000u;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            // cut, not rounded: a value near the largest stays finite
+            const __nv_bfloat16 b = finite ? __float2bfloat16_rz(rest) : __float2bfloat16_rn(rest);
+            out[(p * part_rows + m) * pitch + k] = b;
+            rest = finite ? rest - __bfloat162float(b) : 0.0f;
+        }
+    }
+}
+
+}  // namespace ptwm

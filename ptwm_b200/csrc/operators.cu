@@ -1,9 +1,13 @@
 // Host side of the operators that apply decoded weights: rms_norm and matvec with 4-bit weights.  A translation unit of its
 // own; every call enqueues its kernels on the caller's stream and returns.
 #include <algorithm>
+#include <map>
+#include <mutex>
+#include <type_traits>
 
 #include "errors.hpp"
 #include "matvec.cuh"
+#include "matvec_tiles.cuh"
 #include "rms_norm.cuh"
 
 using namespace ptwm;
@@ -33,7 +37,113 @@ int64_t matrix_of(const ptwm_b200_scaled_weight* w, ScaledMatrix* out) {
     return 0;
 }
 
+// Where a wait inside a kernel gave up, per device: read by ptwm_b200_operator_status.
+__device__ uint32_t g_operator_status;
+
+struct PerDevice { uint32_t* status = nullptr; bool attributes = false; };
+std::mutex g_devices_mu;
+std::map<int, PerDevice> g_devices;
+
+template <class Y, bool GRAD> cudaError_t allow_tiles() {
+    return cudaFuncSetAttribute(matvec_tiles_kernel<Y, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(tiles_smem(256, 3)));
+}
+
+// Once per device, with that device current.
+int64_t device_of(int device, PerDevice* out) {
+    std::lock_guard<std::mutex> g(g_devices_mu);
+    PerDevice& d = g_devices[device];
+    if (!d.attributes) {
+        void* p = nullptr;
+        CUDA_TRY(cudaGetSymbolAddress(&p, g_operator_status));
+        d.status = static_cast<uint32_t*>(p);
+        CUDA_TRY((allow_tiles<float, false>()));
+        CUDA_TRY((allow_tiles<__half, false>()));
+        CUDA_TRY((allow_tiles<__nv_bfloat16, false>()));
+        CUDA_TRY((allow_tiles<float, true>()));
+        CUDA_TRY((allow_tiles<__half, true>()));
+        CUDA_TRY((allow_tiles<__nv_bfloat16, true>()));
+        d.attributes = true;
+    }
+    *out = d;
+    return 0;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled f = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return f;
+}
+
+// Map of a 2-D tensor of bytes or bf16: rows of `inner` values `pitch` bytes apart, loaded in boxes.
+int64_t tensor_map(CUtensorMap* map, bool bf16, const void* p, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_inner, uint32_t box_rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return fail(PTWM_RC_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t dims[2] = {inner, rows}, strides[1] = {pitch};
+    const cuuint32_t box[2] = {box_inner, box_rows}, steps[2] = {1, 1};
+    const CUresult e = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              bf16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (e != CUDA_SUCCESS) return fail(PTWM_RC_CUDA, "cuTensorMapEncodeTiled: error " + std::to_string(int(e)));
+    return 0;
+}
+
+// How the tokens of a product reach the tensor cores: as they are, or as parts in scratch.
+struct Parts { uint32_t parts; uint64_t pitch; uint64_t bytes; };
+Parts parts_of(uint64_t x, uint64_t tokens, uint64_t contraction, uint32_t dtype) {
+    const uint32_t parts = dtype == DT_FP32 ? 3 : dtype == DT_FP16 ? 2 : 1;
+    if (dtype == DT_BF16 && x % 16 == 0 && contraction % 8 == 0) return {1, contraction, 0};
+    const uint64_t pitch = (contraction + 7) / 8 * 8;
+    return {parts, pitch, parts * tokens * pitch * 2};
+}
+
+// More tokens than this go to the tensor-core tiles.
+constexpr uint64_t FEW_TOKENS = 8;
+
+template <bool GRAD>
+int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, int device, const PerDevice& dev, cudaStream_t st) {
+    const uint64_t rows = GRAD ? w.cols : w.rows, contraction = GRAD ? w.rows : w.cols;
+    const Parts p = parts_of(reinterpret_cast<uintptr_t>(x.x), x.tokens, contraction, x_dtype);
+    if (p.bytes > scratch_bytes || (p.bytes && !scratch)) return fail(PTWM_RC_BUFFER_TOO_SMALL, "matvec: scratch too small");
+    const void* tokens = x.x;
+    if (p.bytes) {
+        auto* out = at<__nv_bfloat16>(scratch);
+        const dim3 grid(uint32_t(x.tokens), uint32_t(std::min<uint64_t>((p.pitch + 255) / 256, 64)));
+        if (x_dtype == DT_E4M3) token_parts_kernel<uint8_t><<<grid, 256, 0, st>>>(x, contraction, out, uint32_t(p.pitch), x.tokens);
+        else with_type(x_dtype, [&](auto v) { token_parts_kernel<decltype(v)><<<grid, 256, 0, st>>>(x, contraction, out, uint32_t(p.pitch), x.tokens); });
+        CUDA_TRY(cudaGetLastError());
+        tokens = out;
+    }
+    const uint64_t tiles = (x.tokens + 255) / 256;
+    TilesArgs t{rows, contraction, x.tokens, x.tokens, p.parts, uint32_t(((x.tokens + tiles - 1) / tiles + 15) / 16 * 16), 0, w.group, w.global_scale,
+                x.scaled == SCALE_ROW ? static_cast<const float*>(x.scales) : nullptr, x.y, dev.status};
+    const uint32_t b_bytes = t.tile_tokens * STEP * 2;
+    t.b_stages = std::min<uint32_t>(8, 3 * 256 * STEP * 2 / b_bytes);
+    CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
+    CUtensorMap values, scales, tmap;
+    int64_t rc = tensor_map(&values, false, w.values, w.cols / 2, w.rows, w.value_pitch, 64, GRAD ? STEP : TILE_ROWS);
+    if (rc == 0) rc = tensor_map(&scales, false, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 16, GRAD ? STEP : TILE_ROWS);
+    if (rc == 0) rc = tensor_map(&tmap, true, tokens, contraction, p.parts * x.tokens, p.pitch * 2, STEP, t.tile_tokens);
+    if (rc < 0) return rc;
+    const dim3 grid(uint32_t((rows + TILE_ROWS - 1) / TILE_ROWS), uint32_t((x.tokens + t.tile_tokens - 1) / t.tile_tokens));
+    with_type(y_dtype, [&](auto o) { matvec_tiles_kernel<decltype(o), GRAD><<<grid, TILES_THREADS, tiles_smem(t.tile_tokens, t.b_stages), st>>>(values, scales, tmap, t); });
+    CUDA_TRY(cudaGetLastError());
+    return 0;
+}
+
 }  // namespace
+
+extern "C" int64_t ptwm_b200_operator_status(uint32_t device) {
+    DeviceGuard guard{int(device)};
+    if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
+    uint32_t v = 0;
+    CUDA_TRY(cudaMemcpyFromSymbol(&v, g_operator_status, 4));
+    return v;
+}
 
 extern "C" int64_t ptwm_b200_rms_norm(uint64_t x, uint64_t residual, uint64_t weight, uint64_t h, uint64_t y, uint64_t scales, uint64_t rows, uint64_t cols,
                                       uint32_t dtype, uint32_t weight_dtype, uint32_t scaled, float eps, uint32_t device, uint64_t stream) {
@@ -79,8 +189,12 @@ extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t
     return 0;
 }
 
+extern "C" uint64_t ptwm_b200_matvec_scratch_bytes(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t tokens, uint32_t x_dtype, uint32_t grad) {
+    return !w || (!grad && tokens <= FEW_TOKENS) ? 0 : parts_of(x, tokens, grad ? w->rows : w->cols, x_dtype).bytes;
+}
+
 extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint64_t x, uint64_t x_scales, uint64_t y, uint64_t tokens, uint32_t x_dtype, uint32_t x_scaled,
-                                    uint32_t y_dtype, uint32_t device, uint64_t stream) {
+                                    uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, uint32_t device, uint64_t stream) {
     ScaledMatrix w;
     if (const int64_t rc = matrix_of(weight, &w); rc < 0) return rc;
     if (!plain_type(y_dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec: the output is fp32, fp16 or bf16");
@@ -93,6 +207,11 @@ extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint6
     DeviceGuard guard{int(device)};
     if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
     const TokenArgs t{at<void>(x), at<void>(x_scales), tokens, x_scaled, at<void>(y)};
+    if (tokens > FEW_TOKENS) {
+        PerDevice dev;
+        if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
+        return launch_tiles<false>(w, t, x_dtype, y_dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
+    }
     const dim3 grid(uint32_t((w.rows + 7) / 8), uint32_t((tokens + 7) / 8));
     with_type(y_dtype, [&](auto o) {
         if (x_dtype == DT_E4M3) matvec_kernel<uint8_t, decltype(o)><<<grid, 256, 0, stream_of(stream)>>>(w, t);
@@ -102,7 +221,8 @@ extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint6
     return 0;
 }
 
-extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dtype, uint32_t device, uint64_t stream) {
+extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dtype, uint64_t scratch, uint64_t scratch_bytes,
+                                         uint32_t device, uint64_t stream) {
     ScaledMatrix w;
     if (const int64_t rc = matrix_of(weight, &w); rc < 0) return rc;
     if (!plain_type(dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec_grad: gradients are fp32, fp16 or bf16");
@@ -112,8 +232,7 @@ extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, 
     DeviceGuard guard{int(device)};
     if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
     const TokenArgs t{at<void>(dy), nullptr, tokens, SCALE_NONE, at<void>(dx)};
-    const dim3 grid(uint32_t((w.cols / 2 + 127) / 128), uint32_t((tokens + 7) / 8));
-    with_type(dtype, [&](auto v) { matvec_grad_kernel<decltype(v)><<<grid, 128, 0, stream_of(stream)>>>(w, t); });
-    CUDA_TRY(cudaGetLastError());
-    return 0;
+    PerDevice dev;
+    if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
+    return launch_tiles<true>(w, t, dtype, dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
 }

@@ -256,11 +256,17 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residu
 
 # ---- matvec ---------------------------------------------------------------------------------------
 def _product(x, scales, quant, weight: ScaledWeight, out_dtype: torch.dtype) -> torch.Tensor:
-    device = weight._ordinal
+    device, tokens, code = weight._ordinal, x.numel() // weight.cols, _E4M3 if scales is not None else _PLAIN[x.dtype]
     y = torch.empty((*x.shape[:-1], weight.rows), dtype=out_dtype, device=x.device)
-    _check(_lib.lib().ptwm_b200_matvec(weight._ref, x.data_ptr(), 0 if scales is None else scales.data_ptr(), y.data_ptr(), x.numel() // weight.cols,
-                                       _E4M3 if scales is not None else _PLAIN[x.dtype], _QUANT[quant], _PLAIN[out_dtype], device, stream_handle(device)))
+    scratch, size = _scratch(weight, x, tokens, code, 0)
+    _check(_lib.lib().ptwm_b200_matvec(weight._ref, x.data_ptr(), 0 if scales is None else scales.data_ptr(), y.data_ptr(), tokens, code, _QUANT[quant], _PLAIN[out_dtype],
+                                       0 if scratch is None else scratch.data_ptr(), size, device, stream_handle(device)))
     return y
+
+
+def _scratch(weight: ScaledWeight, x: torch.Tensor, tokens: int, code: int, grad: int):
+    size = _lib.lib().ptwm_b200_matvec_scratch_bytes(weight._ref, x.data_ptr(), tokens, code, grad)
+    return (torch.empty(size, dtype=torch.uint8, device=x.device) if size else None), size
 
 
 class _Matvec(torch.autograd.Function):
@@ -275,7 +281,10 @@ class _Matvec(torch.autograd.Function):
         w = ctx.weight
         dy = dy.to(ctx.dtype).contiguous()
         dx = torch.empty((*dy.shape[:-1], w.cols), dtype=ctx.dtype, device=dy.device)
-        _check(_lib.lib().ptwm_b200_matvec_grad(w._ref, dy.data_ptr(), dx.data_ptr(), dy.numel() // w.rows, _PLAIN[ctx.dtype], w._ordinal, stream_handle(w._ordinal)))
+        tokens, code = dy.numel() // w.rows, _PLAIN[ctx.dtype]
+        scratch, size = _scratch(w, dy, tokens, code, 1)
+        _check(_lib.lib().ptwm_b200_matvec_grad(w._ref, dy.data_ptr(), dx.data_ptr(), tokens, code, 0 if scratch is None else scratch.data_ptr(), size, w._ordinal,
+                                                stream_handle(w._ordinal)))
         return dx, None, None
 
 

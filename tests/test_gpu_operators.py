@@ -570,20 +570,33 @@ def test_nothing_is_written_outside_the_results():
     x = _integers(11, 512, torch.float32, 2)
     torch.cuda.synchronize()
     at = room.data_ptr() + 4096
-    assert L.ptwm_b200_matvec(w._ref, x.data_ptr(), 0, at, 11, 1, 0, 1, 0, stream) == 0
+    assert L.ptwm_b200_matvec(w._ref, x.data_ptr(), 0, at, 8, 1, 0, 1, 0, 0, 0, stream) == 0
     torch.cuda.synchronize()
-    end = 4096 + 11 * 100 * 4
+    end = 4096 + 8 * 100 * 4
     assert bool((room[:4096] == 7).all()) and bool((room[end:] == 7).all())
+    for call, cols, tokens in ((L.ptwm_b200_matvec, 100, 11), (L.ptwm_b200_matvec_grad, 512, 9)):  # any 9 x 100 numbers do as a gradient
+        room.fill_(7)
+        grad = int(call is L.ptwm_b200_matvec_grad)
+        size = L.ptwm_b200_matvec_scratch_bytes(w._ref, x.data_ptr(), tokens, 1, grad)
+        there = room.data_ptr() + (1 << 21)
+        more = () if grad else (0,)
+        types = (1,) if grad else (1, 0, 1)
+        torch.cuda.synchronize()
+        assert call(w._ref, x.data_ptr(), *more, at, tokens, *types, there, size - 1, 0, stream) == -2
+        assert call(w._ref, x.data_ptr(), *more, at, tokens, *types, there, size, 0, stream) == 0
+        torch.cuda.synchronize()
+        end = 4096 + tokens * cols * 4
+        assert bool((room[:4096] == 7).all()) and bool((room[end:1 << 21] == 7).all()) and bool((room[(1 << 21) + size:] == 7).all())
     room.fill_(7)
-    assert L.ptwm_b200_matvec_grad(w._ref, x.data_ptr(), at, 9, 1, 0, stream) == 0  # any 9 x 100 numbers do as a gradient
     torch.cuda.synchronize()
-    end = 4096 + 9 * 512 * 4
-    assert bool((room[:4096] == 7).all()) and bool((room[end:] == 7).all())
-    room.fill_(7)
     wt = torch.ones(511, device="cuda")
     assert L.ptwm_b200_rms_norm(x.data_ptr(), 0, wt.data_ptr(), 0, at, room.data_ptr() + (1 << 20), 3, 511, 1, 1, 1, 1e-6, 0, stream) == 0
     torch.cuda.synchronize()
     assert bool((room[:4096] == 7).all()) and bool((room[4096 + 3 * 511:1 << 20] == 7).all()) and bool((room[(1 << 20) + 12:] == 7).all())
+
+
+def test_no_wait_has_given_up():
+    assert ptwm_b200._lib.lib().ptwm_b200_operator_status(0) == 0
 
 
 def test_weights_straight_from_a_container(tmp_path):

@@ -31,8 +31,8 @@ def _weight(**over):
     (dict(cols=1024, value_pitch=512), INVALID), (dict(rows=(1 << 30) + 1), UNSUPPORTED)])
 def test_matrices_that_are_none(L, over, rc):
     w = _weight(**over)
-    assert L.ptwm_b200_matvec(C.addressof(w), A, 0, A, 1, 6, 0, 6, 0, 1) == rc
-    assert L.ptwm_b200_matvec_grad(C.addressof(w), A, A, 1, 6, 0, 1) == rc
+    assert L.ptwm_b200_matvec(C.addressof(w), A, 0, A, 1, 6, 0, 6, 0, 0, 0, 1) == rc
+    assert L.ptwm_b200_matvec_grad(C.addressof(w), A, A, 1, 6, 0, 0, 0, 1) == rc
     assert _lib.last_error().startswith("scaled weight")
 
 
@@ -43,10 +43,10 @@ def test_tokens_that_are_none(L):
     for args, rc in [((p, A, 0, A, 1, 6, 0, 13), UNSUPPORTED), ((p, A, 0, A, 1, 13, 0, 6), UNSUPPORTED), ((p, A, A, A, 1, 6, 1, 6), UNSUPPORTED), ((p, A, 0, A, 1, 29, 1, 6), UNSUPPORTED),
                      ((p, A, A, A, 1, 29, 0, 6), UNSUPPORTED), ((p, A, A, A, 1, 29, 3, 6), UNSUPPORTED), ((p, 0, 0, A, 1, 6, 0, 6), INVALID), ((p, A, 0, 0, 1, 6, 0, 6), INVALID),
                      ((p, A, 0, A, (1 << 19) + 1, 6, 0, 6), UNSUPPORTED), ((C.addressof(nv), A, A, A, 1, 29, 2, 6), INVALID), ((None, A, 0, A, 1, 6, 0, 6), INVALID)]:
-        assert L.ptwm_b200_matvec(*args, 0, 1) == rc, args
-    assert L.ptwm_b200_matvec(p, 0, 0, 0, 0, 6, 0, 6, 0, 1) == 0  # no tokens: nothing to do, on any machine
+        assert L.ptwm_b200_matvec(*args, 0, 0, 0, 1) == rc, args
+    assert L.ptwm_b200_matvec(p, 0, 0, 0, 0, 6, 0, 6, 0, 0, 0, 1) == 0  # no tokens: nothing to do, on any machine
     for args, rc in [((p, A, A, 1, 29), UNSUPPORTED), ((p, 0, A, 1, 6), INVALID), ((p, A, 0, 1, 6), INVALID)]:
-        assert L.ptwm_b200_matvec_grad(*args, 0, 1) == rc, args
+        assert L.ptwm_b200_matvec_grad(*args, 0, 0, 0, 1) == rc, args
 
 
 def test_norms_that_are_none(L):
