@@ -37,30 +37,4 @@ template <> __device__ __forceinline__ float token_value<uint8_t>(const TokenArg
     return t.scaled == SCALE_ROW ? v : v * e8m0_f32(static_cast<const uint8_t*>(t.scales)[m * (cols / 32) + k / 32]);
 }
 
-// A warp per row of the matrix and eight tokens; a lane takes every 32nd byte.
-template <class T, class Y> __global__ void __launch_bounds__(256) matvec_kernel(ScaledMatrix w, TokenArgs t) {
-    const uint64_t n = uint64_t(blockIdx.x) * 8 + threadIdx.x / 32, m0 = uint64_t(blockIdx.y) * 8;
-    const uint32_t lane = threadIdx.x & 31;
-    if (n >= w.rows) return;
-    const int count = int(t.tokens - m0 < 8 ? t.tokens - m0 : 8);
-    float sum[8] = {};
-    for (uint64_t b = lane; b < w.cols / 2; b += 32) {
-        const uint32_t v = w.values[n * w.value_pitch + b];
-        const float s = group_scale(w, n, 2 * b), lo = e2m1_f32(v & 15) * s, hi = e2m1_f32(v >> 4) * s;
-#pragma unroll
-        for (int m = 0; m < 8; ++m)
-            if (m < count) sum[m] += token_value<T>(t, m0 + m, 2 * b, w.cols) * lo + token_value<T>(t, m0 + m, 2 * b + 1, w.cols) * hi;
-    }
-    const float global = w.global_scale ? *w.global_scale : 1.0f;
-#pragma unroll
-    for (int m = 0; m < 8; ++m) {
-        for (int o = 16; o; o >>= 1) sum[m] += __shfl_xor_sync(0xFFFFFFFFu, sum[m], o);
-        if (lane == 0 && m < count) {
-            float v = sum[m] * global;
-            if (t.scaled == SCALE_ROW) v *= static_cast<const float*>(t.scales)[m0 + m];
-            static_cast<Y*>(t.y)[(m0 + m) * w.rows + n] = from_f32<Y>(v);
-        }
-    }
-}
-
 }  // namespace ptwm

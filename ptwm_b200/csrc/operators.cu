@@ -7,6 +7,7 @@
 
 #include "errors.hpp"
 #include "matvec.cuh"
+#include "matvec_few.cuh"
 #include "matvec_tiles.cuh"
 #include "rms_norm.cuh"
 
@@ -37,6 +38,44 @@ int64_t matrix_of(const ptwm_b200_scaled_weight* w, ScaledMatrix* out) {
     return 0;
 }
 
+constexpr uint32_t SMEM_MOST = 227 * 1024;
+
+// How the columns of a product with few tokens are split; depth 0: not at all, its tokens do not fit shared memory.
+struct FewSplit { uint32_t wk, ranks, depth, smem; };
+FewSplit few_split(uint64_t rows, uint32_t boxes, uint32_t tokens) {
+    // Enough warps for the whole GPU, but a box for each; first within a block, then over a cluster.
+    const uint64_t tiles = (rows + 15) / 16, wanted = 148 * 16;
+    uint32_t wk = 1, ranks = 1;
+    while (wk < 8 && wk * 2 <= boxes && tiles * wk * 2 <= wanted) wk *= 2;
+    while (wk == 8 && ranks < 8 && ranks * 16 <= boxes && tiles * wk * ranks * 2 <= wanted) ranks *= 2;
+    auto share = [&] { return (boxes + ranks - 1) / ranks; };
+    while (ranks < 8 && tokens * few_pitch(share()) > 64 * 1024) ranks *= 2;
+    const uint32_t per_warp = (share() + wk - 1) / wk;
+    const uint32_t depth = std::min<uint32_t>(4, std::max<uint32_t>(per_warp, 1));
+    const uint32_t smem = few_smem(tokens, share(), depth);
+    return {wk, ranks, smem <= SMEM_MOST ? depth : 0, smem};
+}
+bool goes_to_few(const ScaledMatrix& w, uint64_t tokens) {
+    return tokens <= FEW_TOKENS && few_split(w.rows, uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), uint32_t(tokens)).depth;
+}
+
+template <class F> void with_few(uint32_t x_dtype, bool two, bool mx, F f) {
+    auto pick = [&](auto v) {
+        using T = decltype(v);
+        if (mx) two ? f(matvec_few_kernel<T, 2, true>) : f(matvec_few_kernel<T, 1, true>);
+        else two ? f(matvec_few_kernel<T, 2, false>) : f(matvec_few_kernel<T, 1, false>);
+    };
+    if (x_dtype == DT_E4M3) pick(uint8_t());
+    else with_type(x_dtype, pick);
+}
+cudaError_t allow_few() {
+    cudaError_t e = cudaSuccess;
+    for (uint32_t t : {DT_FP32, DT_FP16, DT_BF16, DT_E4M3})
+        for (int k = 0; k < 4 && e == cudaSuccess; ++k)
+            with_few(t, k & 1, k & 2, [&](auto f) { e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_MOST)); });
+    return e;
+}
+
 // Where a wait inside a kernel gave up, per device: read by ptwm_b200_operator_status.
 __device__ uint32_t g_operator_status;
 
@@ -56,6 +95,7 @@ int64_t device_of(int device, PerDevice* out) {
         void* p = nullptr;
         CUDA_TRY(cudaGetSymbolAddress(&p, g_operator_status));
         d.status = static_cast<uint32_t*>(p);
+        CUDA_TRY(allow_few());
         CUDA_TRY((allow_tiles<float, false>()));
         CUDA_TRY((allow_tiles<__half, false>()));
         CUDA_TRY((allow_tiles<__nv_bfloat16, false>()));
@@ -80,14 +120,14 @@ EncodeTiled encode_tiled() {
     return f;
 }
 
-// Map of a 2-D tensor of bytes or bf16: rows of `inner` values `pitch` bytes apart, loaded in boxes.
-int64_t tensor_map(CUtensorMap* map, bool bf16, const void* p, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_inner, uint32_t box_rows) {
+// Map of a 2-D tensor: rows of `inner` values `pitch` bytes apart, loaded in boxes.
+int64_t tensor_map(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* p, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_inner, uint32_t box_rows) {
     const EncodeTiled encode = encode_tiled();
     if (!encode) return fail(PTWM_RC_CUDA, "the driver has no cuTensorMapEncodeTiled");
     const cuuint64_t dims[2] = {inner, rows}, strides[1] = {pitch};
     const cuuint32_t box[2] = {box_inner, box_rows}, steps[2] = {1, 1};
-    const CUresult e = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              bf16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult e = encode(map, type, 2, const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (e != CUDA_SUCCESS) return fail(PTWM_RC_CUDA, "cuTensorMapEncodeTiled: error " + std::to_string(int(e)));
     return 0;
 }
@@ -100,9 +140,6 @@ Parts parts_of(uint64_t x, uint64_t tokens, uint64_t contraction, uint32_t dtype
     const uint64_t pitch = (contraction + 7) / 8 * 8;
     return {parts, pitch, parts * tokens * pitch * 2};
 }
-
-// More tokens than this go to the tensor-core tiles.
-constexpr uint64_t FEW_TOKENS = 8;
 
 template <bool GRAD>
 int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, int device, const PerDevice& dev, cudaStream_t st) {
@@ -125,13 +162,40 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     t.b_stages = std::min<uint32_t>(8, 3 * 256 * STEP * 2 / b_bytes);
     CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
     CUtensorMap values, scales, tmap;
-    int64_t rc = tensor_map(&values, false, w.values, w.cols / 2, w.rows, w.value_pitch, 64, GRAD ? STEP : TILE_ROWS);
-    if (rc == 0) rc = tensor_map(&scales, false, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 16, GRAD ? STEP : TILE_ROWS);
-    if (rc == 0) rc = tensor_map(&tmap, true, tokens, contraction, p.parts * x.tokens, p.pitch * 2, STEP, t.tile_tokens);
+    int64_t rc = tensor_map(&values, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, w.values, w.cols / 2, w.rows, w.value_pitch, 64, GRAD ? STEP : TILE_ROWS);
+    if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 16, GRAD ? STEP : TILE_ROWS);
+    if (rc == 0) rc = tensor_map(&tmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, tokens, contraction, p.parts * x.tokens, p.pitch * 2, STEP, t.tile_tokens);
     if (rc < 0) return rc;
     const dim3 grid(uint32_t((rows + TILE_ROWS - 1) / TILE_ROWS), uint32_t((x.tokens + t.tile_tokens - 1) / t.tile_tokens));
     with_type(y_dtype, [&](auto o) { matvec_tiles_kernel<decltype(o), GRAD><<<grid, TILES_THREADS, tiles_smem(t.tile_tokens, t.b_stages), st>>>(values, scales, tmap, t); });
     CUDA_TRY(cudaGetLastError());
+    return 0;
+}
+
+int64_t launch_few(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype, uint32_t y_dtype, int device, const PerDevice& dev, cudaStream_t st) {
+    const uint32_t boxes = uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), tokens = uint32_t(x.tokens);
+    const FewSplit s = few_split(w.rows, boxes, tokens);
+    const FewArgs a{x.x, x.scales, w.global_scale, x.y, dev.status, w.rows, w.cols, tokens, x.scaled, y_dtype, w.group, boxes, s.wk, s.depth, few_pitch((boxes + s.ranks - 1) / s.ranks),
+                    reinterpret_cast<uintptr_t>(x.x) % 16 == 0};
+    CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
+    CUtensorMap values, scales;
+    int64_t rc = tensor_map(&values, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.values, w.cols / 2, w.rows, w.value_pitch, BOX_COLS / 2, 16);
+    if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 16, 16);
+    if (rc < 0) return rc;
+    const uint32_t per_block = FEW_WARPS / s.wk * 16;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim = {s.ranks, 1, 1};
+    cfg.gridDim = dim3(uint32_t((w.rows + per_block - 1) / per_block) * s.ranks);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = s.smem;
+    cfg.stream = st;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaSuccess;
+    with_few(x_dtype, tokens > 8, w.group == 32, [&](auto f) { e = cudaLaunchKernelEx(&cfg, f, values, scales, a); });
+    CUDA_TRY(e);
     return 0;
 }
 
@@ -190,7 +254,9 @@ extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t
 }
 
 extern "C" uint64_t ptwm_b200_matvec_scratch_bytes(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t tokens, uint32_t x_dtype, uint32_t grad) {
-    return !w || (!grad && tokens <= FEW_TOKENS) ? 0 : parts_of(x, tokens, grad ? w->rows : w->cols, x_dtype).bytes;
+    ScaledMatrix m;
+    if (matrix_of(w, &m) < 0 || (!grad && goes_to_few(m, tokens))) return 0;
+    return parts_of(x, tokens, grad ? m.rows : m.cols, x_dtype).bytes;
 }
 
 extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint64_t x, uint64_t x_scales, uint64_t y, uint64_t tokens, uint32_t x_dtype, uint32_t x_scaled,
@@ -207,18 +273,10 @@ extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint6
     DeviceGuard guard{int(device)};
     if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
     const TokenArgs t{at<void>(x), at<void>(x_scales), tokens, x_scaled, at<void>(y)};
-    if (tokens > FEW_TOKENS) {
-        PerDevice dev;
-        if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
-        return launch_tiles<false>(w, t, x_dtype, y_dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
-    }
-    const dim3 grid(uint32_t((w.rows + 7) / 8), uint32_t((tokens + 7) / 8));
-    with_type(y_dtype, [&](auto o) {
-        if (x_dtype == DT_E4M3) matvec_kernel<uint8_t, decltype(o)><<<grid, 256, 0, stream_of(stream)>>>(w, t);
-        else with_type(x_dtype, [&](auto v) { matvec_kernel<decltype(v), decltype(o)><<<grid, 256, 0, stream_of(stream)>>>(w, t); });
-    });
-    CUDA_TRY(cudaGetLastError());
-    return 0;
+    PerDevice dev;
+    if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
+    if (goes_to_few(w, tokens)) return launch_few(w, t, x_dtype, y_dtype, int(device), dev, stream_of(stream));
+    return launch_tiles<false>(w, t, x_dtype, y_dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
 }
 
 extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dtype, uint64_t scratch, uint64_t scratch_bytes,

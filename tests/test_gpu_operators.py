@@ -333,6 +333,24 @@ def test_matvec_far_apart_magnitudes(tokens, dtype):
     _check_product(y, x.double(), _weight64(values, scales, None), torch.float32)
 
 
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("tokens", [1, 3, 16, 40])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_matvec_small_values_beside_large_ones(kind, tokens, dtype):
+    """What a token holds beside a far larger value is not lost: rows whose weight is zero there are held to their own terms."""
+    n, k = 48, 2048
+    values, scales, top = _matrix(n, k, kind, 12)
+    values[::2, 300] = 0  # columns 600 and 601
+    w = ScaledWeight(values, scales, top)
+    w64 = _weight64(values, scales, top)
+    for power in (20, 30, 36, 45, 70, 120):
+        x = torch.randn(tokens, k, generator=_gen(power), device="cuda").to(DT[dtype])
+        x[:, 600] = 2.0 ** power
+        x[tokens // 2, 601] = 2.0 ** (power // 2)
+        x[:, 1000:1010] *= 2.0 ** -20
+        _check_product(matvec(x, w, out_dtype=torch.float32), x.double(), w64, torch.float32)
+
+
 @pytest.mark.parametrize("tokens", [1, 4, 20, 140])
 def test_matvec_extreme_scales(tokens):
     """E8M0 from 2^-127 to 2^127, NaN scales, E4M3 subnormals and its largest, infinities and NaN in x."""
@@ -567,14 +585,14 @@ def test_nothing_is_written_outside_the_results():
     w = ScaledWeight(*_matrix(100, 512, "mxfp4", 3))
     room = torch.full((1 << 22,), 7, dtype=torch.uint8, device="cuda")
     L, stream = ptwm_b200._lib.lib(), 1
-    x = _integers(11, 512, torch.float32, 2)
+    x = _integers(20, 512, torch.float32, 2)
     torch.cuda.synchronize()
     at = room.data_ptr() + 4096
     assert L.ptwm_b200_matvec(w._ref, x.data_ptr(), 0, at, 8, 1, 0, 1, 0, 0, 0, stream) == 0
     torch.cuda.synchronize()
     end = 4096 + 8 * 100 * 4
     assert bool((room[:4096] == 7).all()) and bool((room[end:] == 7).all())
-    for call, cols, tokens in ((L.ptwm_b200_matvec, 100, 11), (L.ptwm_b200_matvec_grad, 512, 9)):  # any 9 x 100 numbers do as a gradient
+    for call, cols, tokens in ((L.ptwm_b200_matvec, 100, 20), (L.ptwm_b200_matvec_grad, 512, 9)):  # any 9 x 100 numbers do as a gradient
         room.fill_(7)
         grad = int(call is L.ptwm_b200_matvec_grad)
         size = L.ptwm_b200_matvec_scratch_bytes(w._ref, x.data_ptr(), tokens, 1, grad)
