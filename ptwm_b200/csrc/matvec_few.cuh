@@ -6,14 +6,17 @@
 // tiles of 128 rows first, for products that fill a sixteenth of its width.
 //   Operands are fp16.  An E2M1 number fits it; so does its product with an E4M3 scale (six significant bits, 2^-10 to 2688), which
 // NVFP4 takes before the MMA.  E8M0 scales range further: MXFP4 multiplies the sums of each group with them, in fp32.
-//   Tokens become fp16 by a power of two that takes the largest of the block's share of them to [2^14, 2^15): bf16, fp16 and E4M3
-// values down to 2^-29 of it or less are exact.  Where one is not, or tokens are fp32, what is left over goes through the same
-// products again as another part, on a finer scale, until the parts are within 2^-23 of every value: one pass for nearly all
-// bf16 tokens, two for fp32.
-//   Columns are split over the warps of a block (`wk`) and the blocks of a cluster where rows alone do not fill the GPU; the shares are
-// added in the order of the columns.
+//   Tokens become fp16 by a power of two that takes the largest of the block's share of them to [2^14, 2^15).  That is exact for bf16
+// values down to 2^-31 of it (fp16 2^-28, E4M3 2^-35).  Where the smallest is below, or tokens are fp32, what is left over goes through
+// the same products again as another part on a finer scale: one pass for nearly all bf16 tokens, two for fp32, and always as many
+// as bring the parts within 2^-23 of every value.
+//   A block per SM keeps its tokens in shared memory and takes row tiles in turn.  Its 16 warps split the columns (`wk` of them) and row
+// tiles (16 / wk) so that the longest warp has the fewest boxes; tokens that do not fit are split over the blocks of a cluster.  Shares
+// are added in the order of the columns.
 #pragma once
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "matvec.cuh"
 #include "tensor_core.cuh"
@@ -21,7 +24,7 @@
 namespace ptwm {
 
 constexpr uint32_t FEW_TOKENS = 16;
-constexpr uint32_t BOX_COLS = 256, BOX_BYTES = 16 * BOX_COLS / 2, BOX_SCALES = 16 * 16, FEW_WARPS = 8;
+constexpr uint32_t BOX_COLS = 256, BOX_BYTES = 16 * BOX_COLS / 2, BOX_SCALES = 16 * 16, FEW_WARPS = 16, FEW_HEAD = 1024;
 
 struct FewArgs {
     const void* x;
@@ -32,54 +35,117 @@ struct FewArgs {
     uint64_t rows, cols;
     uint32_t tokens, scaled, y_dtype, group;
     uint32_t boxes;      // of 256 columns
-    uint32_t wk;         // warps of a block that share a row tile; 8 / wk row tiles to a block
+    uint32_t wk;         // warps that share a row tile
     uint32_t depth;      // boxes under way per warp
     uint32_t pitch;      // bytes of a token's values in shared memory
     uint32_t wide;       // tokens can be read 8 values at a time
 };
 
 inline uint32_t few_pitch(uint32_t boxes) { return boxes * BOX_COLS * 2 + 64; }  // neighbours in different banks
-inline uint32_t few_smem(uint32_t tokens, uint32_t boxes, uint32_t depth) {
-    return 1024 + 1024 + FEW_WARPS * depth * (BOX_BYTES + BOX_SCALES) + tokens * few_pitch(boxes);
+inline uint32_t few_smem(uint32_t tokens, uint32_t boxes, uint32_t depth, uint32_t parts, uint32_t ranks, uint32_t wk) {
+    const uint32_t shares = 2 * (FEW_WARPS + (ranks > 1 ? FEW_WARPS / wk : 0)) * tokens * 64;
+    return 1024 + FEW_HEAD + FEW_WARPS * depth * (BOX_BYTES + BOX_SCALES) + shares + parts * tokens * few_pitch(boxes);
 }
 
-template <class T> __device__ __forceinline__ void load8(const FewArgs& a, uint64_t token, uint64_t k, float (&v)[8]) {
+// Eight values of a token, as they lie.
+template <class T> struct Eight { uint32_t w[sizeof(T) * 2]; };
+template <class T> __device__ __forceinline__ Eight<T> load8(const FewArgs& a, uint64_t token, uint64_t k) {
     const T* p = static_cast<const T*>(a.x) + token * a.cols + k;
+    Eight<T> e;
     if (a.wide) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 lo = reinterpret_cast<const float4*>(p)[0], hi = reinterpret_cast<const float4*>(p)[1];
-            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-        } else if constexpr (sizeof(T) == 2) {
-            const uint4 w = *reinterpret_cast<const uint4*>(p);
-            T e[8];
-            memcpy(e, &w, 16);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+        if constexpr (sizeof(T) == 1) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            e.w[0] = v.x; e.w[1] = v.y;
         } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(p);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = e4m3_f32(uint8_t((i < 4 ? w.x : w.y) >> (8 * (i & 3))));
+            for (int i = 0; i < int(sizeof(T)) * 2; i += 4) {
+                const uint4 v = reinterpret_cast<const uint4*>(p)[i / 4];
+                e.w[i] = v.x; e.w[i + 1] = v.y; e.w[i + 2] = v.z; e.w[i + 3] = v.w;
+            }
         }
     } else {
+        T v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (sizeof(T) == 1) v[i] = e4m3_f32(p[i]);
-            else v[i] = to_f32(p[i]);
+        for (int i = 0; i < 8; ++i) v[i] = p[i];
+        memcpy(&e, v, sizeof e);
+    }
+    return e;
+}
+__device__ __forceinline__ uint32_t e4m3x2_half2(uint32_t two) {
+    uint32_t h;
+    asm("{\n\t.reg .b16 e;\n\tcvt.u16.u32 e, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, e;\n\t}" : "=r"(h) : "r"(two));
+    return h;
+}
+__device__ __forceinline__ float2 half2_floats(uint32_t u) {
+    __half2 h;
+    memcpy(&h, &u, 4);
+    return __half22float2(h);
+}
+// Scale of the block of 32 that holds value k of a token (E4M3 with block scales), else 1.
+template <class T> __device__ __forceinline__ float block_of(const FewArgs& a, uint64_t token, uint64_t k) {
+    if (sizeof(T) == 1 && a.scaled == SCALE_BLOCK) return e8m0_f32(static_cast<const uint8_t*>(a.x_scales)[token * (a.cols / 32) + k / 32]);
+    return 1.0f;
+}
+template <class T> __device__ __forceinline__ void unpack8(const Eight<T>& e, float s, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(e.w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(e.w[i] << 16); v[2 * i + 1] = __uint_as_float(e.w[i] & 0xFFFF0000u); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = half2_floats(sizeof(T) == 1 ? e4m3x2_half2(e.w[i / 2] >> (16 * (i & 1))) : e.w[i % (sizeof(T) * 2)]);
+            v[2 * i] = f.x * s; v[2 * i + 1] = f.y * s;
         }
     }
-    if constexpr (sizeof(T) == 1)
-        if (a.scaled == SCALE_BLOCK) {
-            const float s = e8m0_f32(static_cast<const uint8_t*>(a.x_scales)[token * (a.cols / 32) + k / 32]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= s;
-        }
 }
 
-__device__ __forceinline__ float power_of_two(int e) {  // 2^e for -149 <= e <= 127
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { uint32_t r; asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) { uint32_t r; asm("min.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ uint32_t less_one_u16x2(uint32_t a) { uint32_t r; asm("add.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xFFFFFFFFu)); return r; }
+
+// Largest finite magnitude and smallest one that is not zero, as bits of fp32; 0 and 0xFFFFFFFF where there is none.
+struct Extremes { uint32_t most = 0, least = 0xFFFFFFFFu; };
+__device__ __forceinline__ void extremes_of(float v, Extremes& x) {
+    const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+    if (b && b < 0x7F800000u) { x.most = max(x.most, b); x.least = min(x.least, b); }
+}
+template <class T> __device__ __forceinline__ void extremes8(const Eight<T>& e, float s, Extremes& x) {
+    if constexpr (sizeof(T) == 2) {  // magnitudes compare as numbers: two at a time, and zero minus one is the largest
+        uint32_t hi = 0, lo = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t m = e.w[i] & 0x7FFF7FFFu;
+            hi = max_u16x2(hi, m);
+            lo = min_u16x2(lo, less_one_u16x2(m));
+        }
+        constexpr uint32_t INF = std::is_same<T, __half>::value ? 0x7C00 : 0x7F80;
+        const uint32_t h = max(hi & 0xFFFF, hi >> 16), l = min(lo & 0xFFFF, lo >> 16) + 1;
+        if (h < INF) {
+            auto bits = [](uint32_t u) -> uint32_t {
+                if (std::is_same<T, __nv_bfloat16>::value) return u << 16;
+                return __float_as_uint(half2_floats(u).x);
+            };
+            x.most = max(x.most, bits(h));
+            if (l <= 0xFFFF) x.least = min(x.least, bits(l));
+            return;
+        }
+    }
+    float v[8];
+    unpack8<T>(e, s, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) extremes_of(v[i], x);
+}
+
+__device__ __forceinline__ float power_of_two(int e) {  // 2^e for -149 <= e <= 127, 0 below
     return __uint_as_float(e >= -126 ? uint32_t(e + 127) << 23 : e >= -149 ? 1u << (e + 149) : 0u);
 }
-// v 2^e, exactly where the result is a number of fp32's; |e| up to 250.
-__device__ __forceinline__ float times_power(float v, int e) { return v * power_of_two(e / 2) * power_of_two(e - e / 2); }
+// What a part leaves of a value that was scaled for it, scaled for the next part: eleven bits are taken.
+__device__ __forceinline__ float after_part(float v, float finer) {
+    return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u ? 0.0f : (v - __half2float(__float2half_rn(v))) * finer;
+}
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -112,212 +178,285 @@ __device__ __forceinline__ void store_as(void* y, uint32_t dtype, uint64_t i, fl
     else static_cast<float*>(y)[i] = v;
 }
 
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+
 // NT: groups of eight tokens.  MX: E8M0 scales per 32 columns, else E4M3 per 16.
 template <class T, int NT, bool MX>
-__global__ void __launch_bounds__(256) matvec_few_kernel(const __grid_constant__ CUtensorMap values, const __grid_constant__ CUtensorMap scales, const FewArgs a) {
+__global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __grid_constant__ CUtensorMap values, const __grid_constant__ CUtensorMap scales, const FewArgs a) {
     namespace cg = cooperative_groups;
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;       // kept side by side
+    constexpr int FINER = sizeof(T) == 4 ? 12 : 39;     // powers of two from one part to the next
+    // from which power on, after scaling, values of the type are exact in the parts of a pass (fp32: to 2^-23)
+    constexpr int FLOOR = sizeof(T) == 4 || std::is_same<T, __half>::value ? -14 : sizeof(T) == 1 ? -21 : -17;
     extern __shared__ uint8_t dynamic[];
     uint8_t* base = dynamic + (1024 - (smem_u32(dynamic) & 1023)) % 1024;
-    // head: barriers of every warp and box, largest magnitude, flags
+    // head: barriers of every warp and box, extremes, flag
     uint32_t* const most = reinterpret_cast<uint32_t*>(base + 960);
-    volatile uint32_t* const failed = reinterpret_cast<uint32_t*>(base + 964);
-    uint8_t* const ring = base + 1024;
-    uint8_t* const xs = ring + FEW_WARPS * a.depth * (BOX_BYTES + BOX_SCALES);
+    uint32_t* const least = reinterpret_cast<uint32_t*>(base + 964);
+    volatile uint32_t* const failed = reinterpret_cast<uint32_t*>(base + 968);
+    uint8_t* const ring = base + FEW_HEAD;
+    float* const shares = reinterpret_cast<float*>(ring + FEW_WARPS * a.depth * (BOX_BYTES + BOX_SCALES));
+    const uint32_t per = a.tokens * 16;                 // results of a row tile
+    float* const sums = shares + 2 * FEW_WARPS * per;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    uint8_t* const xs = reinterpret_cast<uint8_t*>(sums + (ranks > 1 ? 2 * (FEW_WARPS / a.wk) * per : 0));
 
     // this block's boxes, and this warp's among them
     const uint32_t tiles = FEW_WARPS / a.wk, part = warp % a.wk;
-    const uint32_t block_lo = uint32_t(uint64_t(a.boxes) * rank / ranks), block_hi = uint32_t(uint64_t(a.boxes) * (rank + 1) / ranks), block_n = block_hi - block_lo;
+    const uint32_t block_lo = uint32_t(uint64_t(a.boxes) * rank / ranks), block_n = uint32_t(uint64_t(a.boxes) * (rank + 1) / ranks) - block_lo;
     const uint32_t lo = block_lo + block_n * part / a.wk, n = block_lo + block_n * (part + 1) / a.wk - lo;
-    const uint32_t row0 = (blockIdx.x / ranks * tiles + warp / a.wk) * 16;
-    const uint32_t mine = row0 < a.rows ? n : 0;
+    const uint32_t step = gridDim.x / ranks, groups = uint32_t((a.rows + 16 * tiles - 1) / (16 * tiles)), first_group = blockIdx.x / ranks;
+    const uint32_t turns = (groups - first_group + step - 1) / step;  // groups of row tiles for this block: first_group, + step, ...
 
     const uint32_t bars = smem_u32(base) + warp * a.depth * 8;
     const uint32_t boxes_at = smem_u32(ring) + warp * a.depth * BOX_BYTES, scales_at = smem_u32(ring) + FEW_WARPS * a.depth * BOX_BYTES + warp * a.depth * BOX_SCALES;
-    if (threadIdx.x == 0) { *most = 0; *failed = 0; }
+    if (threadIdx.x == 0) { *most = 0; *least = 0xFFFFFFFFu; *failed = 0; }
     if (lane == 0) {
         for (uint32_t i = 0; i < a.depth; ++i) mbar_init(bars + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
     }
     __syncwarp();
-    // box i of this warp (counted through all passes)
-    auto load = [&](uint32_t i) {
-        const uint32_t slot = i % a.depth, box = lo + i % n;
-        mbar_expect(bars + 8 * slot, BOX_BYTES + BOX_SCALES);
-        tma_load(boxes_at + slot * BOX_BYTES, &values, bars + 8 * slot, int32_t(box * (BOX_COLS / 2)), int32_t(row0));
+    // the next box of this warp: boxes of a row tile, as often as there are passes, then the next turn's
+    uint32_t next_box = 0, next_slot = 0, next_pass = 0, next_row = (first_group * tiles + warp / a.wk) * 16;
+    uint32_t left = turns * n;  // boxes to ask for, but for further passes
+    auto load = [&](uint32_t passes) {
+        const uint32_t bar = bars + 8 * next_slot, box = lo + next_box;
+        mbar_expect(bar, BOX_BYTES + BOX_SCALES);
+        tma_load(boxes_at + next_slot * BOX_BYTES, &values, bar, int32_t(box * (BOX_COLS / 2)), int32_t(next_row));
         // 16 bytes of scales: these 256 columns' (NVFP4), or theirs and a neighbour's (MXFP4, eight of them)
-        tma_load(scales_at + slot * BOX_SCALES, &scales, bars + 8 * slot, int32_t(MX ? box / 2 * 16 : box * 16), int32_t(row0));
+        tma_load(scales_at + next_slot * BOX_SCALES, &scales, bar, int32_t(MX ? box / 2 * 16 : box * 16), int32_t(next_row));
+        if (++next_slot == a.depth) next_slot = 0;
+        if (++next_box == n) {
+            next_box = 0;
+            if (++next_pass == passes) { next_pass = 0; next_row += step * tiles * 16; }
+        }
+        --left;
     };
-    uint32_t issued = 0;
+    // Until the passes are known only the first row tile's first pass is asked for.
     if (lane == 0)
-        for (; issued < mine && issued < a.depth; ++issued) load(issued);
+        for (uint32_t i = 0; i < n && i < a.depth; ++i) {
+            const uint32_t bar = bars + 8 * i;
+            mbar_expect(bar, BOX_BYTES + BOX_SCALES);
+            tma_load(boxes_at + i * BOX_BYTES, &values, bar, int32_t((lo + i) * (BOX_COLS / 2)), int32_t(next_row));
+            tma_load(scales_at + i * BOX_SCALES, &scales, bar, int32_t(MX ? (lo + i) / 2 * 16 : (lo + i) * 16), int32_t(next_row));
+        }
     __syncthreads();
 
-    // the largest finite magnitude of the block's share of the tokens
+    // the largest and the smallest magnitude of the block's share of the tokens
     const uint32_t pieces = a.tokens * block_n;  // of 256 values: one for a warp at a time
     {
-        uint32_t m = 0;
+        Extremes x;
         for (uint32_t i = warp; i < pieces; i += FEW_WARPS) {
+            const uint32_t token = i / block_n;
             const uint64_t k = uint64_t(block_lo + i % block_n) * BOX_COLS + lane * 8;
-            if (k < a.cols) {
-                float v[8];
-                load8<T>(a, i / block_n, k, v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-                    if (b < 0x7F800000u) m = max(m, b);
-                }
-            }
+            if (k < a.cols) extremes8<T>(load8<T>(a, token, k), block_of<T>(a, token, k), x);
         }
-        m = __reduce_max_sync(0xFFFFFFFFu, m);
-        if (lane == 0 && m) atomicMax(most, m);
+        x.most = __reduce_max_sync(0xFFFFFFFFu, x.most);
+        x.least = __reduce_min_sync(0xFFFFFFFFu, x.least);
+        if (lane == 0 && x.most) { atomicMax(most, x.most); atomicMin(least, x.least); }
     }
     __syncthreads();
-    const int shift = min(126, 141 - int(*most >> 23)), finer = sizeof(T) == 4 ? 12 : 39;
+    // 2^up takes the largest to [2^14, 2^15); a part has the bits down to 2^-24
+    const int up0 = min(126, 141 - int(*most >> 23));
+    const int bottom = *most ? max(int(*least >> 23), 1) - 127 + up0 - (*least >> 23 ? 0 : 23) : 0;
+    const uint32_t passes = 1 + (bottom < FLOOR ? uint32_t(FLOOR - bottom + FINER * PARTS - 1) / (FINER * PARTS) : 0);
+    if (lane == 0) {
+        left *= passes;
+        // what has been asked for, and the rest of the ring
+        const uint32_t done = min(n, a.depth);
+        left -= done;
+        next_box = done; next_slot = done == a.depth ? 0 : done;
+        if (next_box == n && n) {
+            next_box = 0;
+            if (++next_pass == passes) { next_pass = 0; next_row += step * tiles * 16; }
+        }
+        for (uint32_t i = done; i < a.depth && left; ++i) load(passes);
+    }
 
-    float total[NT][4] = {};
-    bool more = true;
-    for (uint32_t pass = 0; more; ++pass) {
-        // part `pass` of the tokens to shared memory
-        const int up = shift + finer * int(pass);
-        bool left = false;
+    const uint32_t part_bytes = a.tokens * a.pitch;
+    auto stage = [&](uint32_t pass) {  // the parts of a pass of the tokens to shared memory
+        const float first = power_of_two(up0);
+        constexpr float FINE = float(1ull << FINER);
         for (uint32_t i = warp; i < pieces; i += FEW_WARPS) {
             const uint32_t token = i / block_n, at = i % block_n * BOX_COLS + lane * 8;
             const uint64_t k = uint64_t(block_lo) * BOX_COLS + at;
             float v[8] = {};
-            if (k < a.cols) load8<T>(a, token, k, v);
-            uint32_t h[4];
+            if (k < a.cols) unpack8<T>(load8<T>(a, token, k), block_of<T>(a, token, k), v);
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                float part_of[2];
+            for (int j = 0; j < 8; ++j) v[j] *= first;
+            for (uint32_t p = 0; p < pass * PARTS; ++p)
 #pragma unroll
-                for (int i2 = 0; i2 < 2; ++i2) {
-                    const float x = v[j + i2];
-                    if ((__float_as_uint(x) & 0x7F800000u) == 0x7F800000u) { part_of[i2] = pass ? 0.0f : x; continue; }
-                    float rest = x;
-                    for (uint32_t p = 0; p < pass; ++p) {
-                        const int e = shift + finer * int(p);
-                        rest -= times_power(__half2float(__float2half_rn(times_power(rest, e))), -e);
-                    }
-                    part_of[i2] = times_power(rest, up);
-                    rest -= times_power(__half2float(__float2half_rn(part_of[i2])), -up);
-                    left |= fabsf(rest) > 0x1p-23f * fabsf(x);
-                }
-                h[j / 2] = pack_half(part_of[0], part_of[1]);
+                for (int j = 0; j < 8; ++j) v[j] = after_part(v[j], FINE);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                uint32_t h[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[j] = pack_half(v[2 * j], v[2 * j + 1]);
+                *reinterpret_cast<uint4*>(xs + p * part_bytes + token * a.pitch + at * 2) = make_uint4(h[0], h[1], h[2], h[3]);
+                if (p + 1 < PARTS)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = after_part(v[j], FINE);
             }
-            *reinterpret_cast<uint4*>(xs + token * a.pitch + at * 2) = make_uint4(h[0], h[1], h[2], h[3]);
         }
-        more = __syncthreads_or(left) != 0 && pass < 9;
-        const float down = power_of_two(-up);
-        float sum[NT][4] = {};
-        for (uint32_t i = 0; i < mine; ++i) {
-            const uint32_t all = pass * n + i, slot = all % a.depth;
-            mbar_wait(bars + 8 * slot, all / a.depth & 1, failed);
-            const uint8_t* box = ring + (warp * a.depth + slot) * BOX_BYTES;
-            const uint8_t* sc = ring + FEW_WARPS * a.depth * BOX_BYTES + (warp * a.depth + slot) * BOX_SCALES;
-            uint32_t s0[4], s1[4];  // scales of rows g and g + 8
-            if (MX) {
-                const uint32_t half = ((lo + i) & 1) * 8;
-                const uint2 p = *reinterpret_cast<const uint2*>(sc + g * 16 + half), q = *reinterpret_cast<const uint2*>(sc + (g + 8) * 16 + half);
-                s0[0] = p.x; s0[1] = p.y; s1[0] = q.x; s1[1] = q.y;
-            } else {
-                const uint4 p = *reinterpret_cast<const uint4*>(sc + g * 16), q = *reinterpret_cast<const uint4*>(sc + (g + 8) * 16);
-                s0[0] = p.x; s0[1] = p.y; s0[2] = p.z; s0[3] = p.w; s1[0] = q.x; s1[1] = q.y; s1[2] = q.z; s1[3] = q.w;
-            }
-            const uint8_t* xp = xs + g * a.pitch + (lo + i - block_lo) * (BOX_COLS * 2) + t * 16;
+        __syncthreads();
+    };
+    if (passes == 1) stage(0);
+
+    uint32_t tokens_at[NT];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {  // 32 columns: 16 bytes of a row, four to a lane; TMA has swizzled the 16-byte pieces
-                const uint32_t at = (uint32_t(c) ^ g) * 16 + t * 4;
-                const uint32_t w0 = *reinterpret_cast<const uint32_t*>(box + g * 128 + at), w1 = *reinterpret_cast<const uint32_t*>(box + (g + 8) * 128 + at);
-                uint32_t h0[4], h1[4];
-                nibbles_to_half(w0, h0);
-                nibbles_to_half(w1, h1);
-                float f0 = 0, f1 = 0;
+    for (int m = 0; m < NT; ++m) tokens_at[m] = smem_u32(xs) + min(m * 8 + g, a.tokens - 1) * a.pitch + t * 16;
+    uint32_t slot = 0, parity = 0;
+    for (uint32_t turn = 0; turn < turns; ++turn) {
+        const uint32_t group = first_group + turn * step;
+        float total[NT][4] = {};
+        for (uint32_t pass = 0; pass < passes; ++pass) {
+            if (passes > 1) {
+                __syncthreads();  // before these parts take the place of the last
+                stage(pass);
+            }
+            // what undoes the scaling: powers below one with the scales of a group, so that nothing overflows, the others at the end
+            const int up = up0 + FINER * PARTS * int(pass);
+            const float down = power_of_two(up > 0 ? -up : 0), rest = power_of_two(up < 0 ? -up : 0);
+            float sum[NT][4] = {}, sum2[NT][4] = {};
+            for (uint32_t i = 0; i < n; ++i) {
+                mbar_wait(bars + 8 * slot, parity, failed);
+                const uint32_t box = boxes_at + slot * BOX_BYTES + (g * 144 + t * 4);  // TMA has swizzled the 16-byte pieces of a line
+                const uint32_t sc = scales_at + slot * BOX_SCALES + g * 16;
+                uint32_t s0[4], s1[4];  // scales of rows g and g + 8
                 if (MX) {
-                    uint32_t pair;
-                    asm("{\n\t.reg .b16 e;\n\tcvt.u16.u32 e, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, e;\n\t}" : "=r"(pair) : "r"(__byte_perm(s0[c / 4], s1[c / 4], (c & 3) | (4 + (c & 3)) << 4)));
-                    f0 = __uint_as_float(pair << 16) * down;
-                    f1 = __uint_as_float(pair & 0xFFFF0000u) * down;
-                    if (down > 1.0f) {  // an overflow is for the sums to have, not for a group of zeros
-                        if (f0 > 3.4028235e38f) f0 = 3.4028235e38f;
-                        if (f1 > 3.4028235e38f) f1 = 3.4028235e38f;
-                    }
+                    const uint32_t half = ((lo + i) & 1) * 8;
+                    const uint2 p = lds64(sc + half), q = lds64(sc + 128 + half);
+                    s0[0] = p.x; s0[1] = p.y; s1[0] = q.x; s1[1] = q.y;
                 } else {
-                    const uint32_t b = (c & 1) * 2 + t / 2;  // lanes 0 and 1 hold the first group of 16 columns, 2 and 3 the second
-                    uint32_t pair;
-                    asm("{\n\t.reg .b16 e;\n\tcvt.u16.u32 e, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, e;\n\t}" : "=r"(pair) : "r"(__byte_perm(s0[c / 2], s1[c / 2], b | (4 + b) << 4)));
-                    const uint32_t p0 = __byte_perm(pair, 0, 0x1010), p1 = __byte_perm(pair, 0, 0x3232);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) { h0[j] = half2_mul(h0[j], p0); h1[j] = half2_mul(h1[j], p1); }
+                    const uint4 p = lds128(sc), q = lds128(sc + 128);
+                    s0[0] = p.x; s0[1] = p.y; s0[2] = p.z; s0[3] = p.w; s1[0] = q.x; s1[1] = q.y; s1[2] = q.z; s1[3] = q.w;
                 }
+                uint32_t xt[NT];  // where there is no token, another's values make sums that nobody stores
 #pragma unroll
-                for (int m = 0; m < NT; ++m) {
-                    uint4 b = make_uint4(0, 0, 0, 0);
-                    if (m * 8 + g < a.tokens) b = *reinterpret_cast<const uint4*>(xp + m * 8 * a.pitch + c * 64);
+                for (int m = 0; m < NT; ++m) xt[m] = tokens_at[m] + (lo + i - block_lo) * (BOX_COLS * 2);
+                const uint32_t nib = t / 2;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {  // 32 columns: 16 bytes of a row, four to a lane
+                    const uint32_t w = box ^ uint32_t(c << 4);
+                    uint32_t h0[4], h1[4];
+                    nibbles_to_half(lds32(w), h0);
+                    nibbles_to_half(lds32(w + 1024), h1);
+                    float f0 = 0, f1 = 0;
                     if (MX) {
-                        float d[4] = {};
-                        mma16816(d, h0[0], h1[0], h0[1], h1[1], b.x, b.y);
-                        mma16816(d, h0[2], h1[2], h0[3], h1[3], b.z, b.w);
-                        total[m][0] += d[0] * f0;
-                        total[m][1] += d[1] * f0;
-                        total[m][2] += d[2] * f1;
-                        total[m][3] += d[3] * f1;
+                        uint32_t pair;
+                        asm("{\n\t.reg .b16 e;\n\tcvt.u16.u32 e, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, e;\n\t}" : "=r"(pair) : "r"(__byte_perm(s0[c / 4], s1[c / 4], (c & 3) | (4 + (c & 3)) << 4)));
+                        f0 = __uint_as_float(pair << 16) * down;
+                        f1 = __uint_as_float(pair & 0xFFFF0000u) * down;
                     } else {
-                        mma16816(sum[m], h0[0], h1[0], h0[1], h1[1], b.x, b.y);
-                        mma16816(sum[m], h0[2], h1[2], h0[3], h1[3], b.z, b.w);
+                        const uint32_t b = (c & 1) * 2 + nib;  // lanes 0 and 1 hold the first group of 16 columns, 2 and 3 the second
+                        const uint32_t pair = e4m3x2_half2(__byte_perm(s0[c / 2], s1[c / 2], b | (4 + b) << 4));
+                        const uint32_t p0 = __byte_perm(pair, 0, 0x1010), p1 = __byte_perm(pair, 0, 0x3232);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { h0[j] = half2_mul(h0[j], p0); h1[j] = half2_mul(h1[j], p1); }
+                    }
+#pragma unroll
+                    for (int m = 0; m < NT; ++m) {
+                        const uint4 b = lds128(xt[m] + c * 64);
+                        uint4 b2;
+                        if (PARTS == 2) b2 = lds128(xt[m] + part_bytes + c * 64);
+                        if (MX) {
+                            float d[4];
+                            mma16816_first(d, h0[0], h1[0], h0[1], h1[1], b.x, b.y);
+                            mma16816(d, h0[2], h1[2], h0[3], h1[3], b.z, b.w);
+                            if (PARTS == 2) {
+                                float e[4];
+                                mma16816_first(e, h0[0], h1[0], h0[1], h1[1], b2.x, b2.y);
+                                mma16816(e, h0[2], h1[2], h0[3], h1[3], b2.z, b2.w);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) d[j] += e[j] * (1.0f / float(1ull << FINER));
+                            }
+                            sum[m][0] += d[0] * f0;
+                            sum[m][1] += d[1] * f0;
+                            sum[m][2] += d[2] * f1;
+                            sum[m][3] += d[3] * f1;
+                        } else {
+                            mma16816(sum[m], h0[0], h1[0], h0[1], h1[1], b.x, b.y);
+                            mma16816(sum[m], h0[2], h1[2], h0[3], h1[3], b.z, b.w);
+                            if (PARTS == 2) {
+                                mma16816(sum2[m], h0[0], h1[0], h0[1], h1[1], b2.x, b2.y);
+                                mma16816(sum2[m], h0[2], h1[2], h0[3], h1[3], b2.z, b2.w);
+                            }
+                        }
                     }
                 }
+                __syncwarp();
+                if (lane == 0 && left && !*failed) load(passes);
+                if (++slot == a.depth) { slot = 0; parity ^= 1; }
             }
-            __syncwarp();
-            if (lane == 0 && !*failed)
-                for (const uint32_t until = (pass + (more ? 2 : 1)) * n; issued < until && issued <= all + a.depth; ++issued) load(issued);
-        }
-        if (!MX)
 #pragma unroll
             for (int m = 0; m < NT; ++m)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) total[m][j] += sum[m][j] * down;
-        if (more) __syncthreads();  // before the next part overwrites this one
-    }
-    if (*failed && lane == 0) let_copies_land();
-
-    // shares of the warps, [row tile][share][token][row], then of the blocks
-    __syncthreads();
-    float* const shares = reinterpret_cast<float*>(ring);
-    constexpr uint32_t PER = NT * 8 * 16;
-#pragma unroll
-    for (int m = 0; m < NT; ++m)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) shares[warp * PER + (m * 8 + 2 * t + (j & 1)) * 16 + g + (j >> 1) * 8] = total[m][j];
-    __syncthreads();
-    float* const sums = shares + FEW_WARPS * PER;
-    const uint32_t outs = tiles * PER;
-    auto finish = [&](uint32_t e, float v) {
-        const uint32_t tile = e / PER, token = e % PER / 16;
-        const uint64_t row = uint64_t(blockIdx.x / ranks * tiles + tile) * 16 + e % 16;
-        if (token >= a.tokens || row >= a.rows) return;
-        if (a.global_scale) v *= *a.global_scale;
-        if (a.scaled == SCALE_ROW) v *= static_cast<const float*>(a.x_scales)[token];
-        store_as(a.y, a.y_dtype, token * a.rows + row, *failed ? __uint_as_float(0x7FC00000u) : v);
-    };
-    for (uint32_t e = threadIdx.x; e < outs; e += 256) {
-        float v = 0;
-        for (uint32_t p = 0; p < a.wk; ++p) v += shares[(e / PER * a.wk + p) * PER + e % PER];
-        if (ranks == 1) finish(e, v);
-        else sums[e] = v;
-    }
-    if (ranks > 1) {
-        cluster.sync();
-        for (uint32_t e = rank * 256 + threadIdx.x; e < outs; e += ranks * 256) {
-            float v = 0;
-            for (uint32_t r = 0; r < ranks; ++r) v += *cluster.map_shared_rank(sums + e, r);
-            finish(e, v);
+                for (int j = 0; j < 4; ++j) {
+                    float v = sum[m][j];
+                    if (PARTS == 2 && !MX) v += sum2[m][j] * (1.0f / float(1ull << FINER));
+                    total[m][j] += (MX ? v : v * down) * rest;
+                }
         }
-        cluster.sync();  // nobody leaves while others read its sums
+        // shares of the warps, [token][row], in one of two places: a warp comes back to it after the barrier of the next turn
+        float* const my = shares + ((turn & 1) * FEW_WARPS + warp) * per;
+#pragma unroll
+        for (int m = 0; m < NT; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t token = m * 8 + 2 * t + (j & 1);
+                if (token < a.tokens) my[token * 16 + g + (j >> 1) * 8] = total[m][j];
+            }
+        __syncthreads();
+        auto finish = [&](uint32_t e, float v) {
+            const uint32_t token = e % per / 16;
+            const uint64_t row = uint64_t(group * tiles + e / per) * 16 + e % 16;
+            if (row >= a.rows) return;
+            if (a.global_scale) v *= *a.global_scale;
+            if (a.scaled == SCALE_ROW) v *= static_cast<const float*>(a.x_scales)[token];
+            store_as(a.y, a.y_dtype, token * a.rows + row, *failed ? __uint_as_float(0x7FC00000u) : v);
+        };
+        const float* const all = shares + (turn & 1) * FEW_WARPS * per;
+        float* const mine = sums + (turn & 1) * tiles * per;
+        for (uint32_t e = threadIdx.x; e < tiles * per; e += FEW_WARPS * 32) {
+            float v = 0;
+            for (uint32_t p = 0; p < a.wk; ++p) v += all[(e / per * a.wk + p) * per + e % per];
+            if (ranks == 1) finish(e, v);
+            else mine[e] = v;
+        }
+        if (ranks > 1) {
+            cluster.sync();
+            for (uint32_t e = rank * FEW_WARPS * 32 + threadIdx.x; e < tiles * per; e += ranks * FEW_WARPS * 32) {
+                float v = 0;
+                for (uint32_t r = 0; r < ranks; ++r) v += *cluster.map_shared_rank(mine + e, r);
+                finish(e, v);
+            }
+        }
     }
+    if (ranks > 1) cluster.sync();  // nobody leaves while others read its sums
+    if (*failed && lane == 0) let_copies_land();
     if (threadIdx.x == 0 && *failed) atomicExch(a.status, 1u);
 }
 

@@ -40,23 +40,32 @@ int64_t matrix_of(const ptwm_b200_scaled_weight* w, ScaledMatrix* out) {
 
 constexpr uint32_t SMEM_MOST = 227 * 1024;
 
-// How the columns of a product with few tokens are split; depth 0: not at all, its tokens do not fit shared memory.
-struct FewSplit { uint32_t wk, ranks, depth, smem; };
-FewSplit few_split(uint64_t rows, uint32_t boxes, uint32_t tokens) {
-    // Enough warps for the whole GPU, but a box for each; first within a block, then over a cluster.
-    const uint64_t tiles = (rows + 15) / 16, wanted = 148 * 16;
-    uint32_t wk = 1, ranks = 1;
-    while (wk < 8 && wk * 2 <= boxes && tiles * wk * 2 <= wanted) wk *= 2;
-    while (wk == 8 && ranks < 8 && ranks * 16 <= boxes && tiles * wk * ranks * 2 <= wanted) ranks *= 2;
-    auto share = [&] { return (boxes + ranks - 1) / ranks; };
-    while (ranks < 8 && tokens * few_pitch(share()) > 64 * 1024) ranks *= 2;
-    const uint32_t per_warp = (share() + wk - 1) / wk;
-    const uint32_t depth = std::min<uint32_t>(4, std::max<uint32_t>(per_warp, 1));
-    const uint32_t smem = few_smem(tokens, share(), depth);
-    return {wk, ranks, smem <= SMEM_MOST ? depth : 0, smem};
+// How a product with few tokens is split; depth 0: not at all, its tokens do not fit shared memory.
+struct FewSplit { uint32_t wk, ranks, depth, smem, blocks; };
+FewSplit few_split(uint64_t rows, uint32_t boxes, uint32_t tokens, uint32_t parts) {
+    constexpr uint32_t SMS = 148;
+    const uint64_t tiles = (rows + 15) / 16;
+    for (uint32_t ranks = 1; ranks <= 8 && ranks <= boxes; ranks *= 2) {
+        const uint32_t share = (boxes + ranks - 1) / ranks;
+        // warps to a row tile: the fewest boxes for the warp that has most, and of equals the fewest shares to add
+        FewSplit best{};
+        uint64_t least = ~0ull;
+        for (uint32_t wk = 1; wk <= FEW_WARPS; wk *= 2) {
+            const uint64_t groups = (tiles + FEW_WARPS / wk - 1) / (FEW_WARPS / wk), at_once = SMS / ranks;
+            const uint64_t cost = (groups + at_once - 1) / at_once * ((share + wk - 1) / wk);
+            if (cost < least) { least = cost; best = {wk, ranks, 0, 0, uint32_t(std::min(groups, at_once) * ranks)}; }
+        }
+        for (uint32_t depth = 4; depth >= 2; --depth)
+            if (few_smem(tokens, share, depth, parts, ranks, best.wk) <= SMEM_MOST) {
+                best.depth = depth;
+                best.smem = few_smem(tokens, share, depth, parts, ranks, best.wk);
+                return best;
+            }
+    }
+    return {};
 }
-bool goes_to_few(const ScaledMatrix& w, uint64_t tokens) {
-    return tokens <= FEW_TOKENS && few_split(w.rows, uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), uint32_t(tokens)).depth;
+FewSplit few_split(const ScaledMatrix& w, uint64_t tokens, uint32_t x_dtype) {
+    return tokens > FEW_TOKENS ? FewSplit{} : few_split(w.rows, uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), uint32_t(tokens), x_dtype == DT_FP32 ? 2 : 1);
 }
 
 template <class F> void with_few(uint32_t x_dtype, bool two, bool mx, F f) {
@@ -172,9 +181,8 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     return 0;
 }
 
-int64_t launch_few(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype, uint32_t y_dtype, int device, const PerDevice& dev, cudaStream_t st) {
+int64_t launch_few(const ScaledMatrix& w, const TokenArgs& x, const FewSplit& s, uint32_t x_dtype, uint32_t y_dtype, int device, const PerDevice& dev, cudaStream_t st) {
     const uint32_t boxes = uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), tokens = uint32_t(x.tokens);
-    const FewSplit s = few_split(w.rows, boxes, tokens);
     const FewArgs a{x.x, x.scales, w.global_scale, x.y, dev.status, w.rows, w.cols, tokens, x.scaled, y_dtype, w.group, boxes, s.wk, s.depth, few_pitch((boxes + s.ranks - 1) / s.ranks),
                     reinterpret_cast<uintptr_t>(x.x) % 16 == 0};
     CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
@@ -182,13 +190,12 @@ int64_t launch_few(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype, 
     int64_t rc = tensor_map(&values, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.values, w.cols / 2, w.rows, w.value_pitch, BOX_COLS / 2, 16);
     if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 16, 16);
     if (rc < 0) return rc;
-    const uint32_t per_block = FEW_WARPS / s.wk * 16;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute cluster;
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim = {s.ranks, 1, 1};
-    cfg.gridDim = dim3(uint32_t((w.rows + per_block - 1) / per_block) * s.ranks);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(s.blocks);
+    cfg.blockDim = dim3(FEW_WARPS * 32);
     cfg.dynamicSmemBytes = s.smem;
     cfg.stream = st;
     cfg.attrs = &cluster;
@@ -255,7 +262,7 @@ extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t
 
 extern "C" uint64_t ptwm_b200_matvec_scratch_bytes(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t tokens, uint32_t x_dtype, uint32_t grad) {
     ScaledMatrix m;
-    if (matrix_of(w, &m) < 0 || (!grad && goes_to_few(m, tokens))) return 0;
+    if (matrix_of(w, &m) < 0 || (!grad && few_split(m, tokens, x_dtype).depth)) return 0;
     return parts_of(x, tokens, grad ? m.rows : m.cols, x_dtype).bytes;
 }
 
@@ -275,7 +282,7 @@ extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint6
     const TokenArgs t{at<void>(x), at<void>(x_scales), tokens, x_scaled, at<void>(y)};
     PerDevice dev;
     if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
-    if (goes_to_few(w, tokens)) return launch_few(w, t, x_dtype, y_dtype, int(device), dev, stream_of(stream));
+    if (const FewSplit s = few_split(w, tokens, x_dtype); s.depth) return launch_few(w, t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream));
     return launch_tiles<false>(w, t, x_dtype, y_dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
 }
 
