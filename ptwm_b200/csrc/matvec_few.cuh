@@ -10,9 +10,9 @@
 // values down to 2^-31 of it (fp16 2^-28, E4M3 2^-35).  Where the smallest is below, or tokens are fp32, what is left over goes through
 // the same products again as another part on a finer scale: one pass for nearly all bf16 tokens, two for fp32, and always as many
 // as bring the parts within 2^-23 of every value.
-//   A block per SM keeps its tokens in shared memory and takes row tiles in turn.  Its 16 warps split the columns (`wk` of them) and row
-// tiles (16 / wk) so that the longest warp has the fewest boxes; tokens that do not fit are split over the blocks of a cluster.  Shares
-// are added in the order of the columns.
+//   A block per SM keeps its tokens in shared memory and has a run of row tiles.  Of up to 16 of them at a turn, its 16 warps take equal
+// runs of boxes, so a warp works on one tile or two and ends each with its share of the sums; tokens that do not fit are split
+// over the blocks of a cluster.  Shares are added in the order of the columns.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -34,16 +34,19 @@ struct FewArgs {
     uint32_t* status;
     uint64_t rows, cols;
     uint32_t tokens, scaled, y_dtype, group;
-    uint32_t boxes;      // of 256 columns
-    uint32_t wk;         // warps that share a row tile
+    uint32_t rank_boxes, rank_more;         // boxes of 256 columns to a block of a cluster, and how many blocks have one more
+    uint32_t cluster_tiles, cluster_more;   // the same of row tiles to a cluster
+    uint32_t turns;
     uint32_t depth;      // boxes under way per warp
     uint32_t pitch;      // bytes of a token's values in shared memory
+    uint32_t most;       // row tiles of a turn
     uint32_t wide;       // tokens can be read 8 values at a time
 };
 
 inline uint32_t few_pitch(uint32_t boxes) { return boxes * BOX_COLS * 2 + 64; }  // neighbours in different banks
-inline uint32_t few_smem(uint32_t tokens, uint32_t boxes, uint32_t depth, uint32_t parts, uint32_t ranks, uint32_t wk) {
-    const uint32_t shares = 2 * (FEW_WARPS + (ranks > 1 ? FEW_WARPS / wk : 0)) * tokens * 64;
+// most: row tiles a block has at a turn.
+inline uint32_t few_smem(uint32_t tokens, uint32_t boxes, uint32_t depth, uint32_t parts, uint32_t ranks, uint32_t most) {
+    const uint32_t shares = (2 * FEW_WARPS + (ranks > 1 ? most : 0)) * tokens * 64;
     return 1024 + FEW_HEAD + FEW_WARPS * depth * (BOX_BYTES + BOX_SCALES) + shares + parts * tokens * few_pitch(boxes);
 }
 
@@ -210,10 +213,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
     constexpr int FLOOR = sizeof(T) == 4 || std::is_same<T, __half>::value ? -14 : sizeof(T) == 1 ? -21 : -17;
     extern __shared__ uint8_t dynamic[];
     uint8_t* base = dynamic + (1024 - (smem_u32(dynamic) & 1023)) % 1024;
-    // head: barriers of every warp and box, extremes, flag
-    uint32_t* const most = reinterpret_cast<uint32_t*>(base + 960);
-    uint32_t* const least = reinterpret_cast<uint32_t*>(base + 964);
-    volatile uint32_t* const failed = reinterpret_cast<uint32_t*>(base + 968);
+    // head: barriers of every warp and box, extremes of every warp, flag
+    uint32_t* const extremes = reinterpret_cast<uint32_t*>(base + 512);
+    volatile uint32_t* const failed = reinterpret_cast<uint32_t*>(base + 960);
     uint8_t* const ring = base + FEW_HEAD;
     float* const shares = reinterpret_cast<float*>(ring + FEW_WARPS * a.depth * (BOX_BYTES + BOX_SCALES));
     const uint32_t per = a.tokens * 16;                 // results of a row tile
@@ -221,104 +223,135 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
-    uint8_t* const xs = reinterpret_cast<uint8_t*>(sums + (ranks > 1 ? 2 * (FEW_WARPS / a.wk) * per : 0));
+    uint8_t* const xs = reinterpret_cast<uint8_t*>(sums + (ranks > 1 ? a.most * per : 0));
 
-    // this block's boxes, and this warp's among them
-    const uint32_t tiles = FEW_WARPS / a.wk, part = warp % a.wk;
-    const uint32_t block_lo = uint32_t(uint64_t(a.boxes) * rank / ranks), block_n = uint32_t(uint64_t(a.boxes) * (rank + 1) / ranks) - block_lo;
-    const uint32_t lo = block_lo + block_n * part / a.wk, n = block_lo + block_n * (part + 1) / a.wk - lo;
-    const uint32_t step = gridDim.x / ranks, groups = uint32_t((a.rows + 16 * tiles - 1) / (16 * tiles)), first_group = blockIdx.x / ranks;
-    const uint32_t turns = (groups - first_group + step - 1) / step;  // groups of row tiles for this block: first_group, + step, ...
+    // this block's columns (boxes block_lo, + block_n) and row tiles (tile_lo, + tile_n), up to a.most of them at a turn
+    const uint32_t block_lo = rank * a.rank_boxes + min(rank, a.rank_more), block_n = a.rank_boxes + (rank < a.rank_more);
+    const uint32_t cluster_at = blockIdx.x >> (31 - __clz(ranks));
+    const uint32_t tile_lo = cluster_at * a.cluster_tiles + min(cluster_at, a.cluster_more), tile_n = a.cluster_tiles + (cluster_at < a.cluster_more);
+    const uint32_t turns = a.turns;
+    // i / block_n of what fits shared memory (a few thousand boxes): exact, the half keeps it off the borders
+    const float per_n = __frcp_rn(float(block_n));
+    auto over_n = [&](uint32_t i) { return uint32_t((float(i) + 0.5f) * per_n); };
+    // a turn's boxes in the order of tiles and columns; a warp has an equal run of them, at most as many as a tile has
+    struct Run { uint32_t tile, lo, hi; };
+    auto run_of = [&](uint32_t turn, uint32_t w) {
+        const uint32_t first = turn * a.most, all = (first < tile_n ? min(tile_n - first, a.most) : 0) * block_n;
+        return Run{tile_lo + first, all * w / FEW_WARPS, all * (w + 1) / FEW_WARPS};
+    };
+
+    // The tokens are asked for first, HOLD pieces of 256 values to a warp at a time, and those of a block with few stay in registers.
+    constexpr int HOLD = sizeof(T) == 4 ? 2 : 4;
+    const uint32_t pieces = a.tokens * block_n;
+    Eight<T> held[HOLD];
+    auto fetch = [&](uint32_t from) {
+#pragma unroll
+        for (int j = 0; j < HOLD; ++j) {
+            const uint32_t i = from + j * FEW_WARPS, token = over_n(i);
+            const uint64_t k = uint64_t(block_lo + i - token * block_n) * BOX_COLS + lane * 8;
+            held[j] = Eight<T>{};
+            if (i < pieces && k < a.cols) held[j] = load8<T>(a, token, k);
+        }
+    };
+    fetch(warp);
 
     const uint32_t bars = smem_u32(base) + warp * a.depth * 8;
     const uint32_t boxes_at = smem_u32(ring) + warp * a.depth * BOX_BYTES, scales_at = smem_u32(ring) + FEW_WARPS * a.depth * BOX_BYTES + warp * a.depth * BOX_SCALES;
-    if (threadIdx.x == 0) { *most = 0; *least = 0xFFFFFFFFu; *failed = 0; }
+    if (threadIdx.x == 0) *failed = 0;
     if (lane == 0) {
         for (uint32_t i = 0; i < a.depth; ++i) mbar_init(bars + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
     }
-    __syncwarp();
-    // the next box of this warp: boxes of a row tile, as often as there are passes, then the next turn's
-    uint32_t next_box = 0, next_slot = 0, next_pass = 0, next_row = (first_group * tiles + warp / a.wk) * 16;
-    uint32_t left = turns * n;  // boxes to ask for, but for further passes
-    auto load = [&](uint32_t passes) {
-        const uint32_t bar = bars + 8 * next_slot, box = lo + next_box;
+    // what lane 0 asks for next: box `ask` of the run, in column box ask_col of row tile ask_tile
+    Run asked = run_of(0, warp);
+    uint32_t ask = asked.lo, ask_col = asked.lo - over_n(asked.lo) * block_n, ask_row = (asked.tile + over_n(asked.lo)) * 16, ask_slot = 0, ask_pass = 0, ask_turn = 0;
+    auto load = [&] {
+        const uint32_t bar = bars + 8 * ask_slot, box = block_lo + ask_col;
         mbar_expect(bar, BOX_BYTES + BOX_SCALES);
-        tma_load(boxes_at + next_slot * BOX_BYTES, &values, bar, int32_t(box * (BOX_COLS / 2)), int32_t(next_row));
+        tma_load(boxes_at + ask_slot * BOX_BYTES, &values, bar, int32_t(box * (BOX_COLS / 2)), int32_t(ask_row));
         // 16 bytes of scales: these 256 columns' (NVFP4), or theirs and a neighbour's (MXFP4, eight of them)
-        tma_load(scales_at + next_slot * BOX_SCALES, &scales, bar, int32_t(MX ? box / 2 * 16 : box * 16), int32_t(next_row));
-        if (++next_slot == a.depth) next_slot = 0;
-        if (++next_box == n) {
-            next_box = 0;
-            if (++next_pass == passes) { next_pass = 0; next_row += step * tiles * 16; }
-        }
-        --left;
+        tma_load(scales_at + ask_slot * BOX_SCALES, &scales, bar, int32_t(MX ? box / 2 * 16 : box * 16), int32_t(ask_row));
+        if (++ask_slot == a.depth) ask_slot = 0;
+        if (++ask_col == block_n) { ask_col = 0; ask_row += 16; }
+        ++ask;
     };
-    // Until the passes are known only the first row tile's first pass is asked for.
-    if (lane == 0)
-        for (uint32_t i = 0; i < n && i < a.depth; ++i) {
-            const uint32_t bar = bars + 8 * i;
-            mbar_expect(bar, BOX_BYTES + BOX_SCALES);
-            tma_load(boxes_at + i * BOX_BYTES, &values, bar, int32_t((lo + i) * (BOX_COLS / 2)), int32_t(next_row));
-            tma_load(scales_at + i * BOX_SCALES, &scales, bar, int32_t(MX ? (lo + i) / 2 * 16 : (lo + i) * 16), int32_t(next_row));
+    // to the next pass or turn where a run has been asked for; false behind the last
+    auto goes_on = [&](uint32_t passes) {
+        while (ask == asked.hi) {
+            if (++ask_pass == passes) {
+                ask_pass = 0;
+                if (++ask_turn >= turns) { ask_turn = turns; return false; }
+                asked = run_of(ask_turn, warp);
+            }
+            ask = asked.lo;
+            ask_col = asked.lo - over_n(asked.lo) * block_n;
+            ask_row = (asked.tile + over_n(asked.lo)) * 16;
         }
-    __syncthreads();
+        return true;
+    };
+    // until the passes are known only the first one of the first turn is asked for
+    uint32_t under_way = 0;
+    if (lane == 0)
+        for (; under_way < a.depth && ask < asked.hi; ++under_way) load();
+    __syncwarp();
 
     // the largest and the smallest magnitude of the block's share of the tokens
-    const uint32_t pieces = a.tokens * block_n;  // of 256 values: one for a warp at a time
+    uint32_t largest, smallest;
     {
         Extremes x;
-        for (uint32_t i = warp; i < pieces; i += FEW_WARPS) {
-            const uint32_t token = i / block_n;
-            const uint64_t k = uint64_t(block_lo + i % block_n) * BOX_COLS + lane * 8;
-            if (k < a.cols) extremes8<T>(load8<T>(a, token, k), block_of<T>(a, token, k), x);
+        for (uint32_t from = warp; from < pieces; from += FEW_WARPS * HOLD) {
+            if (from != warp) fetch(from);
+#pragma unroll
+            for (int j = 0; j < HOLD; ++j) {
+                const uint32_t i = from + j * FEW_WARPS, token = over_n(i);
+                const uint64_t k = uint64_t(block_lo + i - token * block_n) * BOX_COLS + lane * 8;
+                if (i < pieces && k < a.cols) extremes8<T>(held[j], block_of<T>(a, token, k), x);
+            }
         }
         x.most = __reduce_max_sync(0xFFFFFFFFu, x.most);
         x.least = __reduce_min_sync(0xFFFFFFFFu, x.least);
-        if (lane == 0 && x.most) { atomicMax(most, x.most); atomicMin(least, x.least); }
+        if (lane == 0) { extremes[warp] = x.most; extremes[FEW_WARPS + warp] = x.least; }
+        __syncthreads();
+        const uint32_t v = extremes[lane];
+        largest = __reduce_max_sync(0xFFFFFFFFu, lane < FEW_WARPS ? v : 0);
+        smallest = __reduce_min_sync(0xFFFFFFFFu, lane < FEW_WARPS ? 0xFFFFFFFFu : v);
     }
-    __syncthreads();
     // 2^up takes the largest to [2^14, 2^15); a part has the bits down to 2^-24
-    const int up0 = min(126, 141 - int(*most >> 23));
-    const int bottom = *most ? max(int(*least >> 23), 1) - 127 + up0 - (*least >> 23 ? 0 : 23) : 0;
+    const int up0 = min(126, 141 - int(largest >> 23));
+    const int bottom = largest ? max(int(smallest >> 23), 1) - 127 + up0 - (smallest >> 23 ? 0 : 23) : 0;
     const uint32_t passes = 1 + (bottom < FLOOR ? uint32_t(FLOOR - bottom + FINER * PARTS - 1) / (FINER * PARTS) : 0);
-    if (lane == 0) {
-        left *= passes;
-        // what has been asked for, and the rest of the ring
-        const uint32_t done = min(n, a.depth);
-        left -= done;
-        next_box = done; next_slot = done == a.depth ? 0 : done;
-        if (next_box == n && n) {
-            next_box = 0;
-            if (++next_pass == passes) { next_pass = 0; next_row += step * tiles * 16; }
-        }
-        for (uint32_t i = done; i < a.depth && left; ++i) load(passes);
-    }
+    if (lane == 0)
+        for (; under_way < a.depth && goes_on(passes); ++under_way) load();
 
     const uint32_t part_bytes = a.tokens * a.pitch;
     auto stage = [&](uint32_t pass) {  // the parts of a pass of the tokens to shared memory
         const float first = power_of_two(up0);
         constexpr float FINE = float(1ull << FINER);
-        for (uint32_t i = warp; i < pieces; i += FEW_WARPS) {
-            const uint32_t token = i / block_n, at = i % block_n * BOX_COLS + lane * 8;
-            const uint64_t k = uint64_t(block_lo) * BOX_COLS + at;
-            float v[8] = {};
-            if (k < a.cols) unpack8<T>(load8<T>(a, token, k), block_of<T>(a, token, k), v);
+        for (uint32_t from = warp; from < pieces; from += FEW_WARPS * HOLD) {
+            if (pieces > FEW_WARPS * HOLD || pass) fetch(from);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= first;
-            for (uint32_t p = 0; p < pass * PARTS; ++p)
+            for (int h = 0; h < HOLD; ++h) {
+                const uint32_t i = from + h * FEW_WARPS, token = over_n(i), at = (i - token * block_n) * BOX_COLS + lane * 8;
+                if (i >= pieces) break;
+                const uint64_t k = uint64_t(block_lo) * BOX_COLS + at;
+                float v[8];
+                unpack8<T>(held[h], k < a.cols ? block_of<T>(a, token, k) : 1.0f, v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = after_part(v[j], FINE);
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                uint32_t h[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) h[j] = pack_half(v[2 * j], v[2 * j + 1]);
-                *reinterpret_cast<uint4*>(xs + p * part_bytes + token * a.pitch + at * 2) = make_uint4(h[0], h[1], h[2], h[3]);
-                if (p + 1 < PARTS)
+                for (int j = 0; j < 8; ++j) v[j] *= first;
+                for (uint32_t p = 0; p < pass * PARTS; ++p)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] = after_part(v[j], FINE);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = pack_half(v[2 * j], v[2 * j + 1]);
+                    *reinterpret_cast<uint4*>(xs + p * part_bytes + token * a.pitch + at * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (p + 1 < PARTS)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = after_part(v[j], FINE);
+                }
             }
         }
         __syncthreads();
@@ -330,8 +363,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
     for (int m = 0; m < NT; ++m) tokens_at[m] = smem_u32(xs) + min(m * 8 + g, a.tokens - 1) * a.pitch + t * 16;
     uint32_t slot = 0, parity = 0;
     for (uint32_t turn = 0; turn < turns; ++turn) {
-        const uint32_t group = first_group + turn * step;
-        float total[NT][4] = {};
+        const Run run = run_of(turn, warp);
         for (uint32_t pass = 0; pass < passes; ++pass) {
             if (passes > 1) {
                 __syncthreads();  // before these parts take the place of the last
@@ -341,13 +373,33 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
             const int up = up0 + FINER * PARTS * int(pass);
             const float down = power_of_two(up > 0 ? -up : 0), rest = power_of_two(up < 0 ? -up : 0);
             float sum[NT][4] = {}, sum2[NT][4] = {};
-            for (uint32_t i = 0; i < n; ++i) {
+            uint32_t col = run.lo - over_n(run.lo) * block_n;
+            // this warp's share of the tile that it has ended with: [token][row], in the first of its two places for its first tile
+            float* my = shares + warp * 2 * per;
+            auto hand_in = [&] {
+#pragma unroll
+                for (int m = 0; m < NT; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float v = sum[m][j];
+                        if (PARTS == 2 && !MX) v += sum2[m][j] * (1.0f / float(1ull << FINER));
+                        v *= MX ? rest : down * rest;
+                        const uint32_t token = m * 8 + 2 * t + (j & 1);
+                        if (token < a.tokens) {
+                            float* const to = my + token * 16 + g + (j >> 1) * 8;
+                            *to = pass ? *to + v : v;
+                        }
+                        sum[m][j] = sum2[m][j] = 0;
+                    }
+                my += per;
+            };
+            for (uint32_t i = run.lo; i < run.hi; ++i) {
                 mbar_wait(bars + 8 * slot, parity, failed);
                 const uint32_t box = boxes_at + slot * BOX_BYTES + (g * 144 + t * 4);  // TMA has swizzled the 16-byte pieces of a line
                 const uint32_t sc = scales_at + slot * BOX_SCALES + g * 16;
                 uint32_t s0[4], s1[4];  // scales of rows g and g + 8
                 if (MX) {
-                    const uint32_t half = ((lo + i) & 1) * 8;
+                    const uint32_t half = ((block_lo + col) & 1) * 8;
                     const uint2 p = lds64(sc + half), q = lds64(sc + 128 + half);
                     s0[0] = p.x; s0[1] = p.y; s1[0] = q.x; s1[1] = q.y;
                 } else {
@@ -356,7 +408,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
                 }
                 uint32_t xt[NT];  // where there is no token, another's values make sums that nobody stores
 #pragma unroll
-                for (int m = 0; m < NT; ++m) xt[m] = tokens_at[m] + (lo + i - block_lo) * (BOX_COLS * 2);
+                for (int m = 0; m < NT; ++m) xt[m] = tokens_at[m] + col * (BOX_COLS * 2);
                 const uint32_t nib = t / 2;
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {  // 32 columns: 16 bytes of a row, four to a lane
@@ -408,54 +460,49 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
                     }
                 }
                 __syncwarp();
-                if (lane == 0 && left && !*failed) load(passes);
+                if (lane == 0 && !*failed && goes_on(passes)) load();
                 if (++slot == a.depth) { slot = 0; parity ^= 1; }
+                if (++col == block_n) { col = 0; hand_in(); }
             }
-#pragma unroll
-            for (int m = 0; m < NT; ++m)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float v = sum[m][j];
-                    if (PARTS == 2 && !MX) v += sum2[m][j] * (1.0f / float(1ull << FINER));
-                    total[m][j] += (MX ? v : v * down) * rest;
-                }
+            if (col && run.hi > run.lo) hand_in();
         }
-        // shares of the warps, [token][row], in one of two places: a warp comes back to it after the barrier of the next turn
-        float* const my = shares + ((turn & 1) * FEW_WARPS + warp) * per;
-#pragma unroll
-        for (int m = 0; m < NT; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t token = m * 8 + 2 * t + (j & 1);
-                if (token < a.tokens) my[token * 16 + g + (j >> 1) * 8] = total[m][j];
-            }
         __syncthreads();
-        auto finish = [&](uint32_t e, float v) {
-            const uint32_t token = e % per / 16;
-            const uint64_t row = uint64_t(group * tiles + e / per) * 16 + e % 16;
+        // A tile's boxes are [q block_n, (q + 1) block_n) of the turn's; the first warp that has one of them may have ended another tile before.
+        const uint32_t first = turn * a.most, count = first < tile_n ? min(tile_n - first, a.most) : 0, all = count * block_n;
+        auto finish = [&](uint32_t q, uint32_t token, float v) {
+            const uint64_t row = uint64_t(tile_lo + first + q) * 16 + (threadIdx.x & 15);
             if (row >= a.rows) return;
             if (a.global_scale) v *= *a.global_scale;
             if (a.scaled == SCALE_ROW) v *= static_cast<const float*>(a.x_scales)[token];
             store_as(a.y, a.y_dtype, token * a.rows + row, *failed ? __uint_as_float(0x7FC00000u) : v);
         };
-        const float* const all = shares + (turn & 1) * FEW_WARPS * per;
-        float* const mine = sums + (turn & 1) * tiles * per;
-        for (uint32_t e = threadIdx.x; e < tiles * per; e += FEW_WARPS * 32) {
+        // a thread has row threadIdx.x % 16 of every 32nd pair of tile and token
+        const float per_token = __frcp_rn(float(a.tokens));
+        for (uint32_t e = threadIdx.x; e < count * per; e += FEW_WARPS * 32) {
+            const uint32_t q = uint32_t((float(e / 16) + 0.5f) * per_token), lo = q * block_n, hi = lo + block_n;
+            uint32_t w = uint32_t((float(lo * FEW_WARPS) + 0.5f) * __frcp_rn(float(all)));
             float v = 0;
-            for (uint32_t p = 0; p < a.wk; ++p) v += all[(e / per * a.wk + p) * per + e % per];
-            if (ranks == 1) finish(e, v);
-            else mine[e] = v;
+            for (uint32_t from = all * w / FEW_WARPS; from < hi && w < FEW_WARPS; ++w) {
+                const uint32_t to = all * (w + 1) / FEW_WARPS;
+                if (to > lo && to > from) v += shares[(w * 2 + (from < lo)) * per + e - q * per];
+                from = to;
+            }
+            if (ranks == 1) finish(q, e / 16 - q * a.tokens, v);
+            else sums[e] = v;
         }
         if (ranks > 1) {
             cluster.sync();
-            for (uint32_t e = rank * FEW_WARPS * 32 + threadIdx.x; e < tiles * per; e += ranks * FEW_WARPS * 32) {
+            for (uint32_t e = rank * FEW_WARPS * 32 + threadIdx.x; e < count * per; e += ranks * FEW_WARPS * 32) {
                 float v = 0;
-                for (uint32_t r = 0; r < ranks; ++r) v += *cluster.map_shared_rank(mine + e, r);
-                finish(e, v);
+                for (uint32_t r = 0; r < ranks; ++r) v += *cluster.map_shared_rank(sums + e, r);
+                const uint32_t q = uint32_t((float(e / 16) + 0.5f) * per_token);
+                finish(q, e / 16 - q * a.tokens, v);
             }
+            cluster.sync();  // before the sums are written again, and nobody leaves while others read its own
+        } else if (turn + 1 < turns) {
+            __syncthreads();
         }
     }
-    if (ranks > 1) cluster.sync();  // nobody leaves while others read its sums
     if (*failed && lane == 0) let_copies_land();
     if (threadIdx.x == 0 && *failed) atomicExch(a.status, 1u);
 }

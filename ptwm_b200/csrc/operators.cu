@@ -40,27 +40,17 @@ int64_t matrix_of(const ptwm_b200_scaled_weight* w, ScaledMatrix* out) {
 
 constexpr uint32_t SMEM_MOST = 227 * 1024;
 
-// How a product with few tokens is split; depth 0: not at all, its tokens do not fit shared memory.
-struct FewSplit { uint32_t wk, ranks, depth, smem, blocks; };
+// How a product with few tokens is split: a block per SM, clusters of as few as let the tokens fit shared memory beside two boxes
+// per warp (four where there is room).  depth 0: they do not.
+struct FewSplit { uint32_t ranks, most, depth, smem, blocks; };
 FewSplit few_split(uint64_t rows, uint32_t boxes, uint32_t tokens, uint32_t parts) {
     constexpr uint32_t SMS = 148;
-    const uint64_t tiles = (rows + 15) / 16;
+    const uint32_t tiles = uint32_t((rows + 15) / 16);
     for (uint32_t ranks = 1; ranks <= 8 && ranks <= boxes; ranks *= 2) {
-        const uint32_t share = (boxes + ranks - 1) / ranks;
-        // warps to a row tile: the fewest boxes for the warp that has most, and of equals the fewest shares to add
-        FewSplit best{};
-        uint64_t least = ~0ull;
-        for (uint32_t wk = 1; wk <= FEW_WARPS; wk *= 2) {
-            const uint64_t groups = (tiles + FEW_WARPS / wk - 1) / (FEW_WARPS / wk), at_once = SMS / ranks;
-            const uint64_t cost = (groups + at_once - 1) / at_once * ((share + wk - 1) / wk);
-            if (cost < least) { least = cost; best = {wk, ranks, 0, 0, uint32_t(std::min(groups, at_once) * ranks)}; }
-        }
+        const uint32_t share = (boxes + ranks - 1) / ranks, clusters = std::min(tiles, SMS / ranks), run = (tiles + clusters - 1) / clusters;
+        const uint32_t turns = (run + FEW_WARPS - 1) / FEW_WARPS, most = (run + turns - 1) / turns;
         for (uint32_t depth = 4; depth >= 2; --depth)
-            if (few_smem(tokens, share, depth, parts, ranks, best.wk) <= SMEM_MOST) {
-                best.depth = depth;
-                best.smem = few_smem(tokens, share, depth, parts, ranks, best.wk);
-                return best;
-            }
+            if (const uint32_t smem = few_smem(tokens, share, depth, parts, ranks, most); smem <= SMEM_MOST) return {ranks, most, depth, smem, clusters * ranks};
     }
     return {};
 }
@@ -183,8 +173,9 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
 
 int64_t launch_few(const ScaledMatrix& w, const TokenArgs& x, const FewSplit& s, uint32_t x_dtype, uint32_t y_dtype, int device, const PerDevice& dev, cudaStream_t st) {
     const uint32_t boxes = uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), tokens = uint32_t(x.tokens);
-    const FewArgs a{x.x, x.scales, w.global_scale, x.y, dev.status, w.rows, w.cols, tokens, x.scaled, y_dtype, w.group, boxes, s.wk, s.depth, few_pitch((boxes + s.ranks - 1) / s.ranks),
-                    reinterpret_cast<uintptr_t>(x.x) % 16 == 0};
+    const uint32_t tiles = uint32_t((w.rows + 15) / 16), clusters = s.blocks / s.ranks;
+    const FewArgs a{x.x, x.scales, w.global_scale, x.y, dev.status, w.rows, w.cols, tokens, x.scaled, y_dtype, w.group, boxes / s.ranks, boxes % s.ranks, tiles / clusters, tiles % clusters,
+                    ((tiles + clusters - 1) / clusters + s.most - 1) / s.most, s.depth, few_pitch((boxes + s.ranks - 1) / s.ranks), s.most, reinterpret_cast<uintptr_t>(x.x) % 16 == 0};
     CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
     CUtensorMap values, scales;
     int64_t rc = tensor_map(&values, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.values, w.cols / 2, w.rows, w.value_pitch, BOX_COLS / 2, 16);
