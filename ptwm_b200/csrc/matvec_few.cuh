@@ -1,7 +1,7 @@
 // Products of a 4-bit matrix with up to 16 tokens.
 //
 // What bounds them is reading the matrix, so it goes through the SMs once, in boxes of 16 rows x 256 columns that every warp
-// asks TMA for by itself, four ahead, without a barrier between warps.  A warp turns a box into the first operand of
+// asks TMA for by itself, some ahead, without a barrier between warps; the scales of all of a block's rows come at once.  A warp turns a box into the first operand of
 // mma.m16n8k16 (16 rows of the matrix, 8 tokens): tcgen05 would want it written back to shared memory, or to tensor memory, in
 // tiles of 128 rows first, for products that fill a sixteenth of its width.
 //   Operands are fp16.  An E2M1 number fits it; so does its product with an E4M3 scale (six significant bits, 2^-10 to 2688), which
@@ -24,7 +24,7 @@
 namespace ptwm {
 
 constexpr uint32_t FEW_TOKENS = 16;
-constexpr uint32_t BOX_COLS = 256, BOX_BYTES = 16 * BOX_COLS / 2, BOX_SCALES = 16 * 16, FEW_WARPS = 16, FEW_HEAD = 1024;
+constexpr uint32_t BOX_COLS = 256, BOX_BYTES = 16 * BOX_COLS / 2, FEW_WARPS = 16, FEW_DEPTH = 5, FEW_HEAD = 1024;  // FEW_DEPTH: boxes under way per warp, at most
 
 struct FewArgs {
     const void* x;
@@ -40,14 +40,17 @@ struct FewArgs {
     uint32_t depth;      // boxes under way per warp
     uint32_t pitch;      // bytes of a token's values in shared memory
     uint32_t most;       // row tiles of a turn
+    uint32_t lines;      // 128-byte lines of scales to a row
     uint32_t wide;       // tokens can be read 8 values at a time
 };
 
 inline uint32_t few_pitch(uint32_t boxes) { return boxes * BOX_COLS * 2 + 64; }  // neighbours in different banks
+// 128-byte lines of scales that a block with so many boxes has to a row, from the 16-byte piece on in which they begin.
+inline uint32_t few_lines(uint32_t boxes, uint32_t group) { return (boxes * (BOX_COLS / group) + (group == 32 ? 8 : 0) + 127) / 128; }
 // most: row tiles a block has at a turn.
-inline uint32_t few_smem(uint32_t tokens, uint32_t boxes, uint32_t depth, uint32_t parts, uint32_t ranks, uint32_t most) {
+inline uint32_t few_smem(uint32_t tokens, uint32_t boxes, uint32_t depth, uint32_t parts, uint32_t ranks, uint32_t most, uint32_t lines) {
     const uint32_t shares = (2 * FEW_WARPS + (ranks > 1 ? most : 0)) * tokens * 64;
-    return 1024 + FEW_HEAD + FEW_WARPS * depth * (BOX_BYTES + BOX_SCALES) + shares + parts * tokens * few_pitch(boxes);
+    return 1024 + FEW_HEAD + FEW_WARPS * depth * BOX_BYTES + most * 16 * lines * 128 + shares + parts * tokens * few_pitch(boxes);
 }
 
 // Eight values of a token, as they lie.
@@ -213,11 +216,15 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
     constexpr int FLOOR = sizeof(T) == 4 || std::is_same<T, __half>::value ? -14 : sizeof(T) == 1 ? -21 : -17;
     extern __shared__ uint8_t dynamic[];
     uint8_t* base = dynamic + (1024 - (smem_u32(dynamic) & 1023)) % 1024;
-    // head: barriers of every warp and box, extremes of every warp, flag
-    uint32_t* const extremes = reinterpret_cast<uint32_t*>(base + 512);
+    // head: barriers of every warp and box and of the scales, extremes of every warp, flag
+    static_assert(FEW_WARPS * FEW_DEPTH * 8 <= 768 && 776 + 2 * FEW_WARPS * 4 <= 960, "the head of shared memory does not overlap");
+    const uint32_t scales_bar = smem_u32(base) + 768;
+    uint32_t* const extremes = reinterpret_cast<uint32_t*>(base + 776);
     volatile uint32_t* const failed = reinterpret_cast<uint32_t*>(base + 960);
     uint8_t* const ring = base + FEW_HEAD;
-    float* const shares = reinterpret_cast<float*>(ring + FEW_WARPS * a.depth * (BOX_BYTES + BOX_SCALES));
+    const uint32_t line_bytes = a.most * 16 * 128;      // a line of every row of a turn
+    uint8_t* const scale_lines = ring + FEW_WARPS * a.depth * BOX_BYTES;
+    float* const shares = reinterpret_cast<float*>(scale_lines + a.lines * line_bytes);
     const uint32_t per = a.tokens * 16;                 // results of a row tile
     float* const sums = shares + 2 * FEW_WARPS * per;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane & 3;
@@ -256,44 +263,52 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
     fetch(warp);
 
     const uint32_t bars = smem_u32(base) + warp * a.depth * 8;
-    const uint32_t boxes_at = smem_u32(ring) + warp * a.depth * BOX_BYTES, scales_at = smem_u32(ring) + FEW_WARPS * a.depth * BOX_BYTES + warp * a.depth * BOX_SCALES;
-    if (threadIdx.x == 0) *failed = 0;
-    if (lane == 0) {
-        for (uint32_t i = 0; i < a.depth; ++i) mbar_init(bars + 8 * i, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        fence_async_shared();
-    }
-    // what lane 0 asks for next: box `ask` of the run, in column box ask_col of row tile ask_tile
-    Run asked = run_of(0, warp);
-    uint32_t ask = asked.lo, ask_col = asked.lo - over_n(asked.lo) * block_n, ask_row = (asked.tile + over_n(asked.lo)) * 16, ask_slot = 0, ask_pass = 0, ask_turn = 0;
+    const uint32_t boxes_at = smem_u32(ring) + warp * a.depth * BOX_BYTES;
+    // scales of a turn's rows, 16-byte pieces swizzled as those of the boxes
+    const uint32_t scale_first = (MX ? block_lo / 2 : block_lo) * 16;
+    auto load_scales = [&](uint32_t turn) {
+        mbar_expect(scales_bar, a.lines * line_bytes);
+        for (uint32_t i = 0; i < a.lines; ++i)
+            tma_load(smem_u32(scale_lines) + i * line_bytes, &scales, scales_bar, int32_t(scale_first + i * 128), int32_t((tile_lo + turn * a.most) * 16));
+    };
+    // what lane 0 asks for next: ask_left boxes of the run, from column box ask_col of the row tile at ask_row on
+    uint32_t ask_left, ask_col, ask_row, ask_slot = 0, ask_pass = 0, ask_turn = 0;
+    auto ask = [&](const Run& r) {
+        const uint32_t q = over_n(r.lo);
+        ask_left = r.hi - r.lo;
+        ask_col = r.lo - q * block_n;
+        ask_row = (r.tile + q) * 16;
+    };
+    ask(run_of(0, warp));
     auto load = [&] {
-        const uint32_t bar = bars + 8 * ask_slot, box = block_lo + ask_col;
-        mbar_expect(bar, BOX_BYTES + BOX_SCALES);
-        tma_load(boxes_at + ask_slot * BOX_BYTES, &values, bar, int32_t(box * (BOX_COLS / 2)), int32_t(ask_row));
-        // 16 bytes of scales: these 256 columns' (NVFP4), or theirs and a neighbour's (MXFP4, eight of them)
-        tma_load(scales_at + ask_slot * BOX_SCALES, &scales, bar, int32_t(MX ? box / 2 * 16 : box * 16), int32_t(ask_row));
+        const uint32_t bar = bars + 8 * ask_slot;
+        mbar_expect(bar, BOX_BYTES);
+        tma_load(boxes_at + ask_slot * BOX_BYTES, &values, bar, int32_t((block_lo + ask_col) * (BOX_COLS / 2)), int32_t(ask_row));
         if (++ask_slot == a.depth) ask_slot = 0;
         if (++ask_col == block_n) { ask_col = 0; ask_row += 16; }
-        ++ask;
+        --ask_left;
     };
     // to the next pass or turn where a run has been asked for; false behind the last
     auto goes_on = [&](uint32_t passes) {
-        while (ask == asked.hi) {
-            if (++ask_pass == passes) {
+        while (!ask_left) {
+            if (++ask_pass >= passes) {
                 ask_pass = 0;
                 if (++ask_turn >= turns) { ask_turn = turns; return false; }
-                asked = run_of(ask_turn, warp);
             }
-            ask = asked.lo;
-            ask_col = asked.lo - over_n(asked.lo) * block_n;
-            ask_row = (asked.tile + over_n(asked.lo)) * 16;
+            ask(run_of(ask_turn, warp));
         }
         return true;
     };
     // until the passes are known only the first one of the first turn is asked for
     uint32_t under_way = 0;
-    if (lane == 0)
-        for (; under_way < a.depth && ask < asked.hi; ++under_way) load();
+    if (lane == 0) {
+        for (uint32_t i = 0; i < a.depth; ++i) mbar_init(bars + 8 * i, 1);
+        if (warp == 0) { *failed = 0; mbar_init(scales_bar, 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_shared();
+        if (warp == 0) load_scales(0);
+        for (; under_way < a.depth && ask_left; ++under_way) load();
+    }
     __syncwarp();
 
     // the largest and the smallest magnitude of the block's share of the tokens
@@ -364,6 +379,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
     uint32_t slot = 0, parity = 0;
     for (uint32_t turn = 0; turn < turns; ++turn) {
         const Run run = run_of(turn, warp);
+        mbar_wait(scales_bar, turn & 1, failed);
         for (uint32_t pass = 0; pass < passes; ++pass) {
             if (passes > 1) {
                 __syncthreads();  // before these parts take the place of the last
@@ -373,7 +389,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
             const int up = up0 + FINER * PARTS * int(pass);
             const float down = power_of_two(up > 0 ? -up : 0), rest = power_of_two(up < 0 ? -up : 0);
             float sum[NT][4] = {}, sum2[NT][4] = {};
-            uint32_t col = run.lo - over_n(run.lo) * block_n;
+            const uint32_t tile0 = over_n(run.lo);
+            uint32_t col = run.lo - tile0 * block_n, scales_of = smem_u32(scale_lines) + (tile0 * 16 + g) * 128;
             // this warp's share of the tile that it has ended with: [token][row], in the first of its two places for its first tile
             float* my = shares + warp * 2 * per;
             auto hand_in = [&] {
@@ -396,15 +413,17 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
             for (uint32_t i = run.lo; i < run.hi; ++i) {
                 mbar_wait(bars + 8 * slot, parity, failed);
                 const uint32_t box = boxes_at + slot * BOX_BYTES + (g * 144 + t * 4);  // TMA has swizzled the 16-byte pieces of a line
-                const uint32_t sc = scales_at + slot * BOX_SCALES + g * 16;
-                uint32_t s0[4], s1[4];  // scales of rows g and g + 8
-                if (MX) {
-                    const uint32_t half = ((block_lo + col) & 1) * 8;
-                    const uint2 p = lds64(sc + half), q = lds64(sc + 128 + half);
-                    s0[0] = p.x; s0[1] = p.y; s1[0] = q.x; s1[1] = q.y;
-                } else {
-                    const uint4 p = lds128(sc), q = lds128(sc + 128);
-                    s0[0] = p.x; s0[1] = p.y; s0[2] = p.z; s0[3] = p.w; s1[0] = q.x; s1[1] = q.y; s1[2] = q.z; s1[3] = q.w;
+                uint32_t s0[4], s1[4];  // scales of rows g and g + 8: 8 bytes for the box's columns (MXFP4) or 16
+                {
+                    const uint32_t byte = MX ? (col + (block_lo & 1)) * 8 : col * 16;
+                    const uint32_t sc = scales_of + byte / 128 * line_bytes + ((byte / 16 ^ g) & 7) * 16;
+                    if (MX) {
+                        const uint2 p = lds64(sc + byte % 16), q = lds64(sc + byte % 16 + 1024);
+                        s0[0] = p.x; s0[1] = p.y; s1[0] = q.x; s1[1] = q.y;
+                    } else {
+                        const uint4 p = lds128(sc), q = lds128(sc + 1024);
+                        s0[0] = p.x; s0[1] = p.y; s0[2] = p.z; s0[3] = p.w; s1[0] = q.x; s1[1] = q.y; s1[2] = q.z; s1[3] = q.w;
+                    }
                 }
                 uint32_t xt[NT];  // where there is no token, another's values make sums that nobody stores
 #pragma unroll
@@ -460,9 +479,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
                     }
                 }
                 __syncwarp();
-                if (lane == 0 && !*failed && goes_on(passes)) load();
+                if (lane == 0 && (ask_left || goes_on(passes)) && !*failed) load();
                 if (++slot == a.depth) { slot = 0; parity ^= 1; }
-                if (++col == block_n) { col = 0; hand_in(); }
+                if (++col == block_n) { col = 0; scales_of += 16 * 128; hand_in(); }
             }
             if (col && run.hi > run.lo) hand_in();
         }
@@ -501,6 +520,11 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
             cluster.sync();  // before the sums are written again, and nobody leaves while others read its own
         } else if (turn + 1 < turns) {
             __syncthreads();
+        }
+        // the next turn's scales, where all have read this one's
+        if (threadIdx.x == 0 && turn + 1 < turns) {
+            fence_async_shared();
+            load_scales(turn + 1);
         }
     }
     if (*failed && lane == 0) let_copies_land();

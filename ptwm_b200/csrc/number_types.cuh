@@ -11,6 +11,8 @@ namespace ptwm {
 enum : uint32_t { DT_FP32 = 1, DT_FP16 = 4, DT_BF16 = 6, DT_E4M3 = 29 };
 enum : uint32_t { SCALE_NONE = 0, SCALE_ROW = 1, SCALE_BLOCK = 2 };  // how 8-bit values are scaled: not, fp32 per row, E8M0 per 32
 
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }

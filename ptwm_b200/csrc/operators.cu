@@ -41,21 +41,25 @@ int64_t matrix_of(const ptwm_b200_scaled_weight* w, ScaledMatrix* out) {
 constexpr uint32_t SMEM_MOST = 227 * 1024;
 
 // How a product with few tokens is split: a block per SM, clusters of as few as let the tokens fit shared memory beside two boxes
-// per warp (four where there is room).  depth 0: they do not.
-struct FewSplit { uint32_t ranks, most, depth, smem, blocks; };
-FewSplit few_split(uint64_t rows, uint32_t boxes, uint32_t tokens, uint32_t parts) {
+// per warp (up to five where there is room).  depth 0: they do not.
+struct FewSplit { uint32_t ranks, most, depth, smem, blocks, lines; };
+FewSplit few_split(uint64_t rows, uint32_t boxes, uint32_t tokens, uint32_t parts, uint32_t group) {
     constexpr uint32_t SMS = 148;
     const uint32_t tiles = uint32_t((rows + 15) / 16);
     for (uint32_t ranks = 1; ranks <= 8 && ranks <= boxes; ranks *= 2) {
         const uint32_t share = (boxes + ranks - 1) / ranks, clusters = std::min(tiles, SMS / ranks), run = (tiles + clusters - 1) / clusters;
-        const uint32_t turns = (run + FEW_WARPS - 1) / FEW_WARPS, most = (run + turns - 1) / turns;
-        for (uint32_t depth = 4; depth >= 2; --depth)
-            if (const uint32_t smem = few_smem(tokens, share, depth, parts, ranks, most); smem <= SMEM_MOST) return {ranks, most, depth, smem, clusters * ranks};
+        const uint32_t lines = few_lines(share, group);
+        // row tiles to a turn: as many as warps, fewer where the scales of all do not fit beside the rest
+        for (uint32_t limit = FEW_WARPS; limit; limit /= 2) {
+            const uint32_t turns = (run + limit - 1) / limit, most = (run + turns - 1) / turns;
+            for (uint32_t depth = FEW_DEPTH; depth >= 2; --depth)
+                if (const uint32_t smem = few_smem(tokens, share, depth, parts, ranks, most, lines); smem <= SMEM_MOST) return {ranks, most, depth, smem, clusters * ranks, lines};
+        }
     }
     return {};
 }
 FewSplit few_split(const ScaledMatrix& w, uint64_t tokens, uint32_t x_dtype) {
-    return tokens > FEW_TOKENS ? FewSplit{} : few_split(w.rows, uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), uint32_t(tokens), x_dtype == DT_FP32 ? 2 : 1);
+    return tokens > FEW_TOKENS ? FewSplit{} : few_split(w.rows, uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), uint32_t(tokens), x_dtype == DT_FP32 ? 2 : 1, w.group);
 }
 
 template <class F> void with_few(uint32_t x_dtype, bool two, bool mx, F f) {
@@ -175,11 +179,11 @@ int64_t launch_few(const ScaledMatrix& w, const TokenArgs& x, const FewSplit& s,
     const uint32_t boxes = uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), tokens = uint32_t(x.tokens);
     const uint32_t tiles = uint32_t((w.rows + 15) / 16), clusters = s.blocks / s.ranks;
     const FewArgs a{x.x, x.scales, w.global_scale, x.y, dev.status, w.rows, w.cols, tokens, x.scaled, y_dtype, w.group, boxes / s.ranks, boxes % s.ranks, tiles / clusters, tiles % clusters,
-                    ((tiles + clusters - 1) / clusters + s.most - 1) / s.most, s.depth, few_pitch((boxes + s.ranks - 1) / s.ranks), s.most, reinterpret_cast<uintptr_t>(x.x) % 16 == 0};
+                    ((tiles + clusters - 1) / clusters + s.most - 1) / s.most, s.depth, few_pitch((boxes + s.ranks - 1) / s.ranks), s.most, s.lines, reinterpret_cast<uintptr_t>(x.x) % 16 == 0};
     CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
     CUtensorMap values, scales;
     int64_t rc = tensor_map(&values, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.values, w.cols / 2, w.rows, w.value_pitch, BOX_COLS / 2, 16);
-    if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 16, 16);
+    if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 128, s.most * 16);
     if (rc < 0) return rc;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute cluster;
