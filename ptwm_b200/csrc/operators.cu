@@ -79,6 +79,42 @@ cudaError_t allow_few() {
     return e;
 }
 
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+uint32_t warps_for(uint64_t threads) { return uint32_t((threads + 31) / 32 * 32); }
+
+// One piece of 16 bytes to a thread where rows are few and a call takes as long as one of them (one row of 4096 bf16: 512 threads), two
+// where there are many (4 blocks of 256 on an SM rather than 2 of 512), four for what 1024 threads do not reach otherwise.
+template <class T, class W> void launch_norm(const NormArgs& a, uint32_t scaled, cudaStream_t st) {
+    constexpr uint64_t V = 16 / sizeof(T);
+    const bool wide = a.cols % V == 0 && aligned(a.x) && aligned(a.residual) && aligned(a.weight) && aligned(a.h) && aligned(a.y);
+    const uint64_t pieces = a.cols / V;
+    const uint32_t rows = uint32_t(a.rows);
+    if (wide && pieces <= 128 && a.rows > 148) {  // a row to a warp
+        const uint32_t blocks = (rows + 7) / 8;
+        if (pieces <= 32) rms_norm_rows_kernel<T, W, 1, true><<<blocks, 256, 0, st>>>(a, scaled);
+        else if (pieces <= 64) rms_norm_rows_kernel<T, W, 2, true><<<blocks, 256, 0, st>>>(a, scaled);
+        else rms_norm_rows_kernel<T, W, 4, true><<<blocks, 256, 0, st>>>(a, scaled);
+    } else if (wide && pieces <= 1024 && a.rows <= 296) rms_norm_rows_kernel<T, W, 1, false><<<rows, warps_for(pieces), 0, st>>>(a, scaled);
+    else if (wide && pieces <= 2048) rms_norm_rows_kernel<T, W, 2, false><<<rows, warps_for((pieces + 1) / 2), 0, st>>>(a, scaled);
+    else if (wide && pieces <= 4096) rms_norm_rows_kernel<T, W, 4, false><<<rows, warps_for((pieces + 3) / 4), 0, st>>>(a, scaled);
+    else if (scaled != SCALE_BLOCK && a.cols <= 16 * 1024) rms_norm_odd_rows_kernel<T, W, 16><<<rows, warps_for((a.cols + 15) / 16), 0, st>>>(a, scaled);
+    else rms_norm_long_kernel<T, W><<<rows, 256, 0, st>>>(a, scaled);
+}
+
+// Blocks of a gradient: each writes its share of dweight, so no more than fill the GPU.
+uint32_t grad_blocks(uint64_t rows) { return uint32_t(std::min<uint64_t>(rows, 296)); }
+
+template <class T, class W> void launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
+    constexpr uint64_t V = 16 / sizeof(T);
+    const bool wide = a.cols % V == 0 && aligned(a.h) && aligned(a.weight) && aligned(a.dy) && aligned(a.dh) && aligned(a.dx) && aligned(a.partial);
+    const uint64_t pieces = a.cols / V;
+    if (wide && pieces <= 512) rms_norm_grad_rows_kernel<T, W, 1, 512><<<a.blocks, warps_for(pieces), 0, st>>>(a);
+    else if (wide && pieces <= 1024) rms_norm_grad_rows_kernel<T, W, 2, 512><<<a.blocks, warps_for((pieces + 1) / 2), 0, st>>>(a);
+    else if (wide && pieces <= 2048) rms_norm_grad_rows_kernel<T, W, 2, 1024><<<a.blocks, warps_for((pieces + 1) / 2), 0, st>>>(a);
+    else rms_norm_grad_long_kernel<T, W><<<a.blocks, 512, 0, st>>>(a);
+    if (a.dweight) rms_norm_grad_weight_kernel<W><<<uint32_t((a.cols + 31) / 32), 1024, 0, st>>>(a);
+}
+
 // Where a wait inside a kernel gave up, per device: read by ptwm_b200_operator_status.
 __device__ uint32_t g_operator_status;
 
@@ -222,14 +258,12 @@ extern "C" int64_t ptwm_b200_rms_norm(uint64_t x, uint64_t residual, uint64_t we
     DeviceGuard guard{int(device)};
     if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
     const NormArgs a{at<void>(x), at<void>(residual), at<void>(weight), at<void>(h), at<void>(y), at<void>(scales), rows, cols, eps};
-    with_type(dtype, [&](auto t) {
-        with_type(weight_dtype, [&](auto w) { rms_norm_kernel<decltype(t), decltype(w)><<<uint32_t(rows), 256, 0, stream_of(stream)>>>(a, scaled); });
-    });
+    with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { launch_norm<decltype(t), decltype(w)>(a, scaled, stream_of(stream)); }); });
     CUDA_TRY(cudaGetLastError());
     return 0;
 }
 
-extern "C" uint64_t ptwm_b200_rms_norm_grad_scratch_bytes(uint64_t rows, uint64_t cols) { return std::min<uint64_t>(rows, 296) * cols * 4; }
+extern "C" uint64_t ptwm_b200_rms_norm_grad_scratch_bytes(uint64_t rows, uint64_t cols) { return grad_blocks(rows) * cols * 4; }
 
 extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t dy, uint64_t dh, uint64_t dx, uint64_t dweight, uint64_t scratch, uint64_t scratch_bytes,
                                            uint64_t rows, uint64_t cols, uint32_t dtype, uint32_t weight_dtype, float eps, uint32_t device, uint64_t stream) {
@@ -243,14 +277,9 @@ extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t
         if (dweight) CUDA_TRY(cudaMemsetAsync(at<void>(dweight), 0, cols * (weight_dtype == DT_FP32 ? 4 : 2), stream_of(stream)));
         return 0;
     }
-    const uint32_t blocks = uint32_t(std::min<uint64_t>(rows, 296));
+    const uint32_t blocks = grad_blocks(rows);
     const NormGradArgs a{at<void>(h), at<void>(weight), at<void>(dy), at<void>(dh), at<void>(dx), dweight ? at<float>(scratch) : nullptr, at<void>(dweight), rows, cols, eps, blocks};
-    with_type(dtype, [&](auto t) {
-        with_type(weight_dtype, [&](auto w) {
-            rms_norm_grad_kernel<decltype(t), decltype(w)><<<blocks, 256, 0, stream_of(stream)>>>(a);
-            if (dweight) rms_norm_grad_weight_kernel<decltype(w)><<<uint32_t((cols + 255) / 256), 256, 0, stream_of(stream)>>>(a);
-        });
-    });
+    with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { launch_norm_grad<decltype(t), decltype(w)>(a, stream_of(stream)); }); });
     CUDA_TRY(cudaGetLastError());
     return 0;
 }

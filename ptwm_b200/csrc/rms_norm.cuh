@@ -8,6 +8,10 @@
 //            p - 8 + (m > 1.75): the bits say it, no logarithm is taken.
 // Sums are fp32; where a maximum is not finite its scale is NaN and so are its values.
 #pragma once
+#include <string.h>
+
+#include <type_traits>
+
 #include "number_types.cuh"
 
 namespace ptwm {
@@ -19,16 +23,6 @@ struct NormArgs {
     float eps;
 };
 
-template <class Op> __device__ __forceinline__ float block_reduce(float v, float* shared, Op op, float none) {
-    for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = threadIdx.x % 32 < (blockDim.x + 31) / 32 ? shared[threadIdx.x % 32] : none;
-    for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    return v;
-}
-struct Add { __device__ float operator()(float a, float b) const { return a + b; } };
 // Of two magnitudes: NaN, whose bits are above infinity's, wins.
 struct MaxMagnitude { __device__ float operator()(float a, float b) const { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); } };
 
@@ -49,46 +43,240 @@ __device__ __forceinline__ float block_inverse(uint32_t e) {  // 2^(127 - e), ex
     return e == 255 ? __uint_as_float(0x7FC00000u) : e == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254 - e) << 23);
 }
 
-// One block per row, three passes over it.
+// 16 bytes of a row, as numbers.
+template <class T> struct Piece {
+    static constexpr int V = 16 / sizeof(T);
+    float v[V];
+};
+template <class T> __device__ __forceinline__ Piece<T> numbers(const uint4& w) {
+    Piece<T> p;
+    T e[Piece<T>::V];
+    memcpy(e, &w, 16);
+#pragma unroll
+    for (int i = 0; i < Piece<T>::V; ++i) p.v[i] = to_f32(e[i]);
+    return p;
+}
+template <class T> __device__ __forceinline__ uint4 rounded(const float* v) {
+    T e[Piece<T>::V];
+#pragma unroll
+    for (int i = 0; i < Piece<T>::V; ++i) e[i] = from_f32<T>(v[i]);
+    uint4 w;
+    memcpy(&w, e, 16);
+    return w;
+}
+// The weights that belong to piece i of a row of T.
+template <class T, class W> __device__ __forceinline__ void weights(const void* weight, uint32_t i, float* v) {
+    constexpr int V = Piece<T>::V, PIECES = V * sizeof(W) / 16;
+    if constexpr (PIECES == 0) {  // fp32 rows, 16-bit weights: half a piece
+        const uint2 w = static_cast<const uint2*>(weight)[i];
+        W e[V];
+        memcpy(e, &w, 8);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = to_f32(e[k]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const Piece<W> p = numbers<W>(static_cast<const uint4*>(weight)[i * PIECES + j]);
+#pragma unroll
+            for (int k = 0; k < Piece<W>::V; ++k) v[j * Piece<W>::V + k] = p.v[k];
+        }
+    }
+}
+
+// Sum and largest magnitude, or two sums, over the warp and, where a row has several, over the block.
+template <bool SUMS> __device__ __forceinline__ void reduce_two(float& a, float& b, uint32_t warps, float (*shared)[32]) {
+    auto join = [](float x, float y) { return SUMS ? x + y : MaxMagnitude()(x, y); };
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+        b = join(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
+    }
+    if (warps == 1) return;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (lane == 0) { shared[0][warp] = a; shared[1][warp] = b; }
+    __syncthreads();
+    a = lane < warps ? shared[0][lane] : 0.0f;
+    b = lane < warps ? shared[1][lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+        b = join(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
+    }
+}
+
+// V E4M3 values, the first in the lowest byte.
+template <int V> __device__ __forceinline__ void pack_e4m3(const float* v, uint32_t (&out)[V / 4]) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        uint16_t lo, hi;  // the conversion puts its first operand in the upper byte
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v[i + 1]), "f"(v[i]));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(v[i + 3]), "f"(v[i + 2]));
+        out[i / 4] = uint32_t(lo) | uint32_t(hi) << 16;
+    }
+}
+
+// Rows that start at multiples of 16 bytes.  Bound by memory, so everything is read once and a row stays in registers: N pieces of 16
+// bytes to a thread, a row to a warp (WARP) or to a block.  One reduction is enough for any output: with t = h weight the
+// largest |y| is r times the largest |t| (rounding keeps the order), and q = t / (max|t| / 448) needs no r at all.
+template <class T, class W, int N, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_rows_kernel(NormArgs a, uint32_t quant) {
+    constexpr int V = Piece<T>::V;
+    __shared__ float shared[2][32];
+    const uint32_t lanes = WARP ? 32 : blockDim.x, at = WARP ? threadIdx.x & 31 : threadIdx.x, pieces = uint32_t(a.cols / V);
+    const uint64_t row = WARP ? uint64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+    if (WARP && row >= a.rows) return;
+    const uint4* x = static_cast<const uint4*>(a.x) + row * pieces;
+    const uint4* res = static_cast<const uint4*>(a.residual) + row * pieces;
+    uint4 in[N], more[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t i = at + j * lanes;
+        in[j] = more[j] = make_uint4(0, 0, 0, 0);
+        if (i < pieces) {
+            in[j] = __ldcs(x + i);
+            if (a.residual) more[j] = __ldcs(res + i);
+        }
+    }
+    float t[N][V], sum = 0, most = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t i = at + j * lanes;
+        float w[V] = {};
+        if (i < pieces) weights<T, W>(a.weight, i, w);
+        Piece<T> h = numbers<T>(in[j]);
+        if (a.residual) {
+            const Piece<T> r = numbers<T>(more[j]);
+#pragma unroll
+            for (int k = 0; k < V; ++k) h.v[k] += r.v[k];
+            const uint4 stored = rounded<T>(h.v);
+            if (i < pieces) static_cast<uint4*>(a.h)[row * pieces + i] = stored;
+            h = numbers<T>(stored);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            sum += h.v[k] * h.v[k];
+            t[j][k] = h.v[k] * w[k];
+            most = MaxMagnitude()(most, fabsf(t[j][k]));
+        }
+    }
+    reduce_two<false>(sum, most, WARP ? 1 : lanes / 32, shared);
+    const float r = __frsqrt_rn(sum / float(a.cols) + a.eps), nan = __uint_as_float(0x7FC00000u);
+    if (quant == SCALE_NONE) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = at + j * lanes;
+#pragma unroll
+            for (int k = 0; k < V; ++k) t[j][k] *= r;
+            if (i < pieces) static_cast<uint4*>(a.y)[row * pieces + i] = rounded<T>(t[j]);
+        }
+        return;
+    }
+    using Out = typename std::conditional<V == 8, uint2, uint32_t>::type;
+    Out* q = static_cast<Out*>(a.y) + row * pieces;
+    const float s = is_finite(most * r) ? most * r / 448.0f : nan, part = most / 448.0f;
+    if (quant == SCALE_ROW && at == 0) static_cast<float*>(a.scales)[row] = s;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t i = at + j * lanes;
+        if (quant == SCALE_ROW) {
+            // part is 0 only where s is, and not finite only where s is not
+#pragma unroll
+            for (int k = 0; k < V; ++k) t[j][k] = s == 0.0f ? 0.0f : s == s ? t[j][k] / part : nan;
+        } else {
+            float m = 0;
+#pragma unroll
+            for (int k = 0; k < V; ++k) m = MaxMagnitude()(m, fabsf(t[j][k]));
+#pragma unroll
+            for (int o = 1; o < 32 / V; o *= 2) m = MaxMagnitude()(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));  // the threads of a block of 32
+            const uint32_t e = block_scale(m * r);
+            const float down = block_inverse(e);
+#pragma unroll
+            for (int k = 0; k < V; ++k) t[j][k] = t[j][k] * r * down;
+            if (i < pieces && i % (32 / V) == 0) static_cast<uint8_t*>(a.scales)[row * (a.cols / 32) + i / (32 / V)] = uint8_t(e);
+        }
+        uint32_t o[V / 4];
+        pack_e4m3<V>(t[j], o);
+        Out out;
+        memcpy(&out, o, sizeof out);
+        if (i < pieces) q[i] = out;
+    }
+}
+
+// Rows that start anywhere, a value at a time: N values to a thread, a row to a block.
+template <class T, class W, int N>
+__global__ void __launch_bounds__(1024) rms_norm_odd_rows_kernel(NormArgs a, uint32_t quant) {
+    __shared__ float shared[2][32];
+    const uint32_t cols = uint32_t(a.cols), lanes = blockDim.x;
+    const uint64_t first = uint64_t(blockIdx.x) * cols;
+    const T *x = static_cast<const T*>(a.x) + first, *res = static_cast<const T*>(a.residual) + first;
+    const W* w = static_cast<const W*>(a.weight);
+    float t[N], sum = 0, most = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t k = threadIdx.x + j * lanes;
+        t[j] = k < cols ? to_f32(x[k]) : 0.0f;
+    }
+    if (a.residual)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t k = threadIdx.x + j * lanes;
+            if (k < cols) {
+                const T h = from_f32<T>(t[j] + to_f32(res[k]));
+                static_cast<T*>(a.h)[first + k] = h;
+                t[j] = to_f32(h);
+            }
+        }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t k = threadIdx.x + j * lanes;
+        sum += t[j] * t[j];
+        t[j] = k < cols ? t[j] * to_f32(w[k]) : 0.0f;
+        most = MaxMagnitude()(most, fabsf(t[j]));
+    }
+    reduce_two<false>(sum, most, lanes / 32, shared);
+    const float r = __frsqrt_rn(sum / float(cols) + a.eps), s = is_finite(most * r) ? most * r / 448.0f : __uint_as_float(0x7FC00000u), part = most / 448.0f;
+    if (quant == SCALE_ROW && threadIdx.x == 0) static_cast<float*>(a.scales)[blockIdx.x] = s;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t k = threadIdx.x + j * lanes;
+        if (k >= cols) continue;
+        if (quant == SCALE_ROW) static_cast<uint8_t*>(a.y)[first + k] = f32_e4m3(s == 0.0f ? 0.0f : s == s ? t[j] / part : s);
+        else static_cast<T*>(a.y)[first + k] = from_f32<T>(t[j] * r);
+    }
+}
+
+// Rows of any length and place: a block per row, three passes over it.
 template <class T, class W>
-__global__ void __launch_bounds__(256) rms_norm_kernel(NormArgs a, uint32_t quant) {
-    __shared__ float shared[32];
+__global__ void __launch_bounds__(256) rms_norm_long_kernel(NormArgs a, uint32_t quant) {
+    __shared__ float shared[2][32];
     const uint64_t row = blockIdx.x, cols = a.cols;
     const T* x = static_cast<const T*>(a.x) + row * cols;
     const T* res = a.residual ? static_cast<const T*>(a.residual) + row * cols : nullptr;
     T* h = a.residual ? static_cast<T*>(a.h) + row * cols : nullptr;
     const W* w = static_cast<const W*>(a.weight);
-    float sum = 0;
+    float sum = 0, most = 0;
     for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) {
         float v = to_f32(x[k]);
         if (res) { const T s = from_f32<T>(v + to_f32(res[k])); h[k] = s; v = to_f32(s); }
         sum += v * v;
+        most = MaxMagnitude()(most, fabsf(v * to_f32(w[k])));
     }
-    sum = block_reduce(sum, shared, Add(), 0.0f);
-    const float r = rsqrtf(sum / float(cols) + a.eps);
+    reduce_two<false>(sum, most, blockDim.x / 32, shared);
+    const float r = __frsqrt_rn(sum / float(cols) + a.eps), s = is_finite(most * r) ? most * r / 448.0f : __uint_as_float(0x7FC00000u), part = most / 448.0f;
     const T* in = res ? h : x;
-    auto normed = [&](uint64_t k) { return to_f32(in[k]) * r * to_f32(w[k]); };
-    if (quant == SCALE_NONE) {
-        for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) static_cast<T*>(a.y)[row * cols + k] = from_f32<T>(normed(k));
-        return;
-    }
     uint8_t* q = static_cast<uint8_t*>(a.y) + row * cols;
-    if (quant == SCALE_ROW) {
-        float most = 0;
-        for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) most = MaxMagnitude()(most, fabsf(normed(k)));
-        most = block_reduce(most, shared, MaxMagnitude(), 0.0f);
-        const float s = is_finite(most) ? most / 448.0f : __uint_as_float(0x7FC00000u);
-        for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) q[k] = s == 0.0f ? 0 : f32_e4m3(normed(k) / s);
-        if (threadIdx.x == 0) static_cast<float*>(a.scales)[row] = s;
-        return;
-    }
-    for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) {  // cols is a multiple of 32: a warp has a block of values
-        const float v = normed(k);
-        float most = fabsf(v);
-        for (int o = 16; o; o >>= 1) most = MaxMagnitude()(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-        const uint32_t e = block_scale(most);
-        q[k] = f32_e4m3(v * block_inverse(e));
-        if ((threadIdx.x & 31) == 0) static_cast<uint8_t*>(a.scales)[row * (cols / 32) + k / 32] = uint8_t(e);
+    if (quant == SCALE_ROW && threadIdx.x == 0) static_cast<float*>(a.scales)[row] = s;
+    for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) {  // a warp has a block of 32 values at a time, or less than one at the end
+        const float t = to_f32(in[k]) * to_f32(w[k]);
+        if (quant == SCALE_NONE) static_cast<T*>(a.y)[row * cols + k] = from_f32<T>(t * r);
+        else if (quant == SCALE_ROW) q[k] = f32_e4m3(s == 0.0f ? 0.0f : s == s ? t / part : s);
+        else {
+            float m = fabsf(t);
+            for (int o = 16; o; o >>= 1) m = MaxMagnitude()(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            const uint32_t e = block_scale(m * r);
+            q[k] = f32_e4m3(t * r * block_inverse(e));
+            if ((threadIdx.x & 31) == 0) static_cast<uint8_t*>(a.scales)[row * (cols / 32) + k / 32] = uint8_t(e);
+        }
     }
 }
 
@@ -103,17 +291,87 @@ struct NormGradArgs {
     uint32_t blocks;
 };
 
-// A block takes rows blockIdx.x, + blocks, ...; its sums for dweight live in `partial`, where each column belongs to one thread.
+// A block takes rows blockIdx.x, + blocks, ...  Its threads keep their columns, N pieces of 16 bytes, and with them their sums for
+// dweight in registers; with 512 of them the next row is asked for before this one's reduction, which 64 registers of 1024 do not hold.
+template <class T, class W, int N, int MOST>
+__global__ void __launch_bounds__(MOST) rms_norm_grad_rows_kernel(NormGradArgs a) {
+    constexpr int V = Piece<T>::V;
+    __shared__ float shared[2][2][32];
+    const uint32_t lanes = blockDim.x, at = threadIdx.x, pieces = uint32_t(a.cols / V);
+    const uint4 *hs = static_cast<const uint4*>(a.h), *dys = static_cast<const uint4*>(a.dy), *dhs = static_cast<const uint4*>(a.dh);
+    uint4 h[N], dy[N], dh[N];
+    auto ask = [&](uint64_t row) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = at + j * lanes;
+            h[j] = dy[j] = dh[j] = make_uint4(0, 0, 0, 0);
+            if (row < a.rows && i < pieces) {
+                h[j] = __ldcs(hs + row * pieces + i);
+                dy[j] = __ldcs(dys + row * pieces + i);
+                if (dhs) dh[j] = __ldcs(dhs + row * pieces + i);
+            }
+        }
+    };
+    float dw[N][V] = {};
+    auto weights_of = [&](int j, float (&w)[V]) {  // again for every use: they stay in the L1
+#pragma unroll
+        for (int k = 0; k < V; ++k) w[k] = 0;
+        if (at + j * lanes < pieces) weights<T, W>(a.weight, at + j * lanes, w);
+    };
+    if (MOST <= 512) ask(blockIdx.x);
+    uint32_t turn = 0;
+    for (uint64_t row = blockIdx.x; row < a.rows; row += a.blocks, turn ^= 1) {
+        if (MOST > 512) ask(row);
+        float sq = 0, dot = 0;
+        uint4 h0[N], d0[N], r0[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            h0[j] = h[j]; d0[j] = dy[j]; r0[j] = dh[j];
+            const Piece<T> v = numbers<T>(h0[j]), d = numbers<T>(d0[j]);
+            float w[V];
+            weights_of(j, w);
+#pragma unroll
+            for (int k = 0; k < V; ++k) { sq += v.v[k] * v.v[k]; dot += d.v[k] * w[k] * v.v[k]; }
+        }
+        if (MOST <= 512) ask(row + a.blocks);
+        reduce_two<true>(sq, dot, lanes / 32, shared[turn]);
+        const float r = __frsqrt_rn(sq / float(a.cols) + a.eps), c = r * r * r * dot / float(a.cols);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = at + j * lanes;
+            const Piece<T> v = numbers<T>(h0[j]), d = numbers<T>(d0[j]), e = numbers<T>(r0[j]);
+            float g[V], w[V];
+            weights_of(j, w);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                g[k] = r * d.v[k] * w[k] - v.v[k] * c + e.v[k];
+                dw[j][k] += d.v[k] * v.v[k] * r;
+            }
+            if (a.dx && i < pieces) static_cast<uint4*>(a.dx)[row * pieces + i] = rounded<T>(g);
+        }
+    }
+    if (a.partial)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = at + j * lanes;
+            if (i < pieces)
+#pragma unroll
+                for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(a.partial + blockIdx.x * a.cols + i * V + k) = make_float4(dw[j][k], dw[j][k + 1], dw[j][k + 2], dw[j][k + 3]);
+        }
+}
+
+// Rows of any length and place; a block's sums for dweight live in `partial`, where each column belongs to one thread.
 template <class T, class W>
-__global__ void __launch_bounds__(256) rms_norm_grad_kernel(NormGradArgs a) {
-    __shared__ float shared[32];
+__global__ void __launch_bounds__(512) rms_norm_grad_long_kernel(NormGradArgs a) {
+    __shared__ float shared[2][2][32];
     const uint64_t cols = a.cols;
     const W* w = static_cast<const W*>(a.weight);
     float* part = a.partial ? a.partial + blockIdx.x * cols : nullptr;
     if (part) for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) part[k] = 0;
-    for (uint64_t row = blockIdx.x; row < a.rows; row += a.blocks) {
+    uint32_t turn = 0;
+    for (uint64_t row = blockIdx.x; row < a.rows; row += a.blocks, turn ^= 1) {
         const T* h = static_cast<const T*>(a.h) + row * cols;
-        const T* dy = a.dy ? static_cast<const T*>(a.dy) + row * cols : nullptr;
+        const T* dy = static_cast<const T*>(a.dy) + row * cols;
         const T* dh = a.dh ? static_cast<const T*>(a.dh) + row * cols : nullptr;
         float sq = 0, dot = 0;
         for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) {
@@ -121,10 +379,8 @@ __global__ void __launch_bounds__(256) rms_norm_grad_kernel(NormGradArgs a) {
             sq += v * v;
             dot += to_f32(dy[k]) * to_f32(w[k]) * v;
         }
-        sq = block_reduce(sq, shared, Add(), 0.0f);
-        dot = block_reduce(dot, shared, Add(), 0.0f);
-        const float r = rsqrtf(sq / float(cols) + a.eps);
-        const float c = r * r * r * dot / float(cols);
+        reduce_two<true>(sq, dot, blockDim.x / 32, shared[turn]);
+        const float r = __frsqrt_rn(sq / float(cols) + a.eps), c = r * r * r * dot / float(cols);
         for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) {
             const float v = to_f32(h[k]), d = to_f32(dy[k]);
             float g = r * d * to_f32(w[k]) - v * c;
@@ -135,12 +391,20 @@ __global__ void __launch_bounds__(256) rms_norm_grad_kernel(NormGradArgs a) {
     }
 }
 
-// dweight from the blocks' shares, added in their order.
-template <class W> __global__ void __launch_bounds__(256) rms_norm_grad_weight_kernel(NormGradArgs a) {
-    const uint64_t k = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (k >= a.cols) return;
+// dweight from the blocks' shares: 32 columns to a block, 32 runs of shares to a column, added in their order.
+template <class W> __global__ void __launch_bounds__(1024) rms_norm_grad_weight_kernel(NormGradArgs a) {
+    __shared__ float runs[32][33];
+    const uint64_t k = uint64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
+    const uint32_t run = threadIdx.x / 32;
     float sum = 0;
-    for (uint32_t b = 0; b < a.blocks; ++b) sum += a.partial[b * a.cols + k];
+    if (k < a.cols)
+        for (uint32_t b = a.blocks * run / 32; b < a.blocks * (run + 1) / 32; ++b) sum += a.partial[b * a.cols + k];
+    runs[run][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (run || k >= a.cols) return;
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) sum += runs[i][threadIdx.x];
     static_cast<W*>(a.dweight)[k] = from_f32<W>(sum);
 }
 
