@@ -83,21 +83,26 @@ bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 uint32_t warps_for(uint64_t threads) { return uint32_t((threads + 31) / 32 * 32); }
 
 // One piece of 16 bytes to a thread where rows are few and a call takes as long as one of them (one row of 4096 bf16: 512 threads), two
-// where there are many (4 blocks of 256 on an SM rather than 2 of 512), four for what 1024 threads do not reach otherwise.
-template <class T, class W> void launch_norm(const NormArgs& a, uint32_t scaled, cudaStream_t st) {
+// where there are many.  False: the rows are not made for it.
+template <class T, class W, uint32_t QUANT> bool launch_norm_rows(const NormArgs& a, cudaStream_t st) {
     constexpr uint64_t V = 16 / sizeof(T);
-    const bool wide = a.cols % V == 0 && aligned(a.x) && aligned(a.residual) && aligned(a.weight) && aligned(a.h) && aligned(a.y);
+    if (a.cols % V || !aligned(a.x) || !aligned(a.residual) || !aligned(a.weight) || !aligned(a.h) || !aligned(a.y)) return false;
     const uint64_t pieces = a.cols / V;
     const uint32_t rows = uint32_t(a.rows);
-    if (wide && pieces <= 128 && a.rows > 148) {  // a row to a warp
+    if (pieces <= 128 && a.rows > 148) {  // a row to a warp
         const uint32_t blocks = (rows + 7) / 8;
-        if (pieces <= 32) rms_norm_rows_kernel<T, W, 1, true><<<blocks, 256, 0, st>>>(a, scaled);
-        else if (pieces <= 64) rms_norm_rows_kernel<T, W, 2, true><<<blocks, 256, 0, st>>>(a, scaled);
-        else rms_norm_rows_kernel<T, W, 4, true><<<blocks, 256, 0, st>>>(a, scaled);
-    } else if (wide && pieces <= 1024 && a.rows <= 296) rms_norm_rows_kernel<T, W, 1, false><<<rows, warps_for(pieces), 0, st>>>(a, scaled);
-    else if (wide && pieces <= 2048) rms_norm_rows_kernel<T, W, 2, false><<<rows, warps_for((pieces + 1) / 2), 0, st>>>(a, scaled);
-    else if (wide && pieces <= 4096) rms_norm_rows_kernel<T, W, 4, false><<<rows, warps_for((pieces + 3) / 4), 0, st>>>(a, scaled);
-    else if (scaled != SCALE_BLOCK && a.cols <= 16 * 1024) rms_norm_odd_rows_kernel<T, W, 16><<<rows, warps_for((a.cols + 15) / 16), 0, st>>>(a, scaled);
+        if (pieces <= 32) rms_norm_rows_kernel<T, W, 1, true, QUANT><<<blocks, 256, 0, st>>>(a);
+        else if (pieces <= 64) rms_norm_rows_kernel<T, W, 2, true, QUANT><<<blocks, 256, 0, st>>>(a);
+        else rms_norm_rows_kernel<T, W, 4, true, QUANT><<<blocks, 256, 0, st>>>(a);
+    } else if (pieces <= 1024 && a.rows <= 296) rms_norm_rows_kernel<T, W, 1, false, QUANT><<<rows, warps_for(pieces), 0, st>>>(a);
+    else if (pieces <= 2048) rms_norm_rows_kernel<T, W, 2, false, QUANT><<<rows, warps_for((pieces + 1) / 2), 0, st>>>(a);
+    else return false;
+    return true;
+}
+template <class T, class W> void launch_norm(const NormArgs& a, uint32_t scaled, cudaStream_t st) {
+    const uint32_t rows = uint32_t(a.rows);
+    if (scaled == SCALE_NONE ? launch_norm_rows<T, W, SCALE_NONE>(a, st) : scaled == SCALE_ROW ? launch_norm_rows<T, W, SCALE_ROW>(a, st) : launch_norm_rows<T, W, SCALE_BLOCK>(a, st)) return;
+    if (scaled != SCALE_BLOCK && a.cols <= 16 * 1024) rms_norm_odd_rows_kernel<T, W, 16><<<rows, warps_for((a.cols + 15) / 16), 0, st>>>(a, scaled);
     else rms_norm_long_kernel<T, W><<<rows, 256, 0, st>>>(a, scaled);
 }
 

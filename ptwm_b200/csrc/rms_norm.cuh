@@ -23,8 +23,12 @@ struct NormArgs {
     float eps;
 };
 
-// Of two magnitudes: NaN, whose bits are above infinity's, wins.
-struct MaxMagnitude { __device__ float operator()(float a, float b) const { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); } };
+// The larger magnitude; NaN wins.
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
 
 __device__ __forceinline__ bool is_finite(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
 
@@ -83,24 +87,30 @@ template <class T, class W> __device__ __forceinline__ void weights(const void* 
     }
 }
 
-// Sum and largest magnitude, or two sums, over the warp and, where a row has several, over the block.
-template <bool SUMS> __device__ __forceinline__ void reduce_two(float& a, float& b, uint32_t warps, float (*shared)[32]) {
-    auto join = [](float x, float y) { return SUMS ? x + y : MaxMagnitude()(x, y); };
+// A sum and (TWO) a second one or (MOST) a largest magnitude, over the warp and, where a row has several, over the block: the warps'
+// results are read back as they lie, four at a time, which is less work than another round of shuffles.
+template <bool TWO, bool MOST> __device__ __forceinline__ void reduce(float& a, float& b, uint32_t warps, float (*shared)[32]) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-        b = join(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
+        if (TWO) b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
     }
+    // magnitudes compare as whole numbers, and a NaN is above infinity
+    if (MOST) b = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(b)));
     if (warps == 1) return;
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    if (lane == 0) { shared[0][warp] = a; shared[1][warp] = b; }
+    const uint32_t warp = threadIdx.x / 32, up = (warps + 3) / 4 * 4;
+    if ((threadIdx.x & 31) == 0) { shared[0][warp] = a; if (TWO || MOST) shared[1][warp] = b; }
+    if (threadIdx.x >= warps && threadIdx.x < up) shared[0][threadIdx.x] = shared[1][threadIdx.x] = 0;  // (a warp has 32 threads: there are as many)
     __syncthreads();
-    a = lane < warps ? shared[0][lane] : 0.0f;
-    b = lane < warps ? shared[1][lane] : 0.0f;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-        b = join(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
+    a = 0; b = 0;
+    for (uint32_t i = 0; i < up; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(&shared[0][i]);
+        a += (v.x + v.y) + (v.z + v.w);
+        if (TWO || MOST) {
+            const float4 u = *reinterpret_cast<const float4*>(&shared[1][i]);
+            if (TWO) b += (u.x + u.y) + (u.z + u.w);
+            else b = max_magnitude(max_magnitude(b, max_magnitude(u.x, u.y)), max_magnitude(u.z, u.w));
+        }
     }
 }
 
@@ -118,10 +128,11 @@ template <int V> __device__ __forceinline__ void pack_e4m3(const float* v, uint3
 // Rows that start at multiples of 16 bytes.  Bound by memory, so everything is read once and a row stays in registers: N pieces of 16
 // bytes to a thread, a row to a warp (WARP) or to a block.  One reduction is enough for any output: with t = h weight the
 // largest |y| is r times the largest |t| (rounding keeps the order), and q = t / (max|t| / 448) needs no r at all.
-template <class T, class W, int N, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_rows_kernel(NormArgs a, uint32_t quant) {
+template <class T, class W, int N, bool WARP, uint32_t QUANT>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_rows_kernel(NormArgs a) {
+    constexpr uint32_t quant = QUANT;
     constexpr int V = Piece<T>::V;
-    __shared__ float shared[2][32];
+    __shared__ __align__(16) float shared[2][32];
     const uint32_t lanes = WARP ? 32 : blockDim.x, at = WARP ? threadIdx.x & 31 : threadIdx.x, pieces = uint32_t(a.cols / V);
     const uint64_t row = WARP ? uint64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
     if (WARP && row >= a.rows) return;
@@ -156,10 +167,10 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_rows_kernel(NormAr
         for (int k = 0; k < V; ++k) {
             sum += h.v[k] * h.v[k];
             t[j][k] = h.v[k] * w[k];
-            most = MaxMagnitude()(most, fabsf(t[j][k]));
+            if (QUANT == SCALE_ROW) most = max_magnitude(most, t[j][k]);
         }
     }
-    reduce_two<false>(sum, most, WARP ? 1 : lanes / 32, shared);
+    reduce<false, QUANT == SCALE_ROW>(sum, most, WARP ? 1 : lanes / 32, shared);
     const float r = __frsqrt_rn(sum / float(a.cols) + a.eps), nan = __uint_as_float(0x7FC00000u);
     if (quant == SCALE_NONE) {
 #pragma unroll
@@ -173,21 +184,27 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_rows_kernel(NormAr
     }
     using Out = typename std::conditional<V == 8, uint2, uint32_t>::type;
     Out* q = static_cast<Out*>(a.y) + row * pieces;
-    const float s = is_finite(most * r) ? most * r / 448.0f : nan, part = most / 448.0f;
+    const float s = is_finite(most * r) ? most * r / 448.0f : nan, part = most / 448.0f, inverse = 448.0f / most;
+    const bool plain = s > 0.0f && most > 0x1p-100f;  // nearly always: a product for a division
     if (quant == SCALE_ROW && at == 0) static_cast<float*>(a.scales)[row] = s;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         const uint32_t i = at + j * lanes;
         if (quant == SCALE_ROW) {
             // part is 0 only where s is, and not finite only where s is not
+            if (plain) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) t[j][k] = s == 0.0f ? 0.0f : s == s ? t[j][k] / part : nan;
+                for (int k = 0; k < V; ++k) t[j][k] *= inverse;
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; ++k) t[j][k] = s == 0.0f ? 0.0f : s == s ? t[j][k] / part : nan;
+            }
         } else {
             float m = 0;
 #pragma unroll
-            for (int k = 0; k < V; ++k) m = MaxMagnitude()(m, fabsf(t[j][k]));
+            for (int k = 0; k < V; ++k) m = max_magnitude(m, t[j][k]);
 #pragma unroll
-            for (int o = 1; o < 32 / V; o *= 2) m = MaxMagnitude()(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));  // the threads of a block of 32
+            for (int o = 1; o < 32 / V; o *= 2) m = max_magnitude(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));  // the threads of a block of 32
             const uint32_t e = block_scale(m * r);
             const float down = block_inverse(e);
 #pragma unroll
@@ -205,7 +222,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_rows_kernel(NormAr
 // Rows that start anywhere, a value at a time: N values to a thread, a row to a block.
 template <class T, class W, int N>
 __global__ void __launch_bounds__(1024) rms_norm_odd_rows_kernel(NormArgs a, uint32_t quant) {
-    __shared__ float shared[2][32];
+    __shared__ __align__(16) float shared[2][32];
     const uint32_t cols = uint32_t(a.cols), lanes = blockDim.x;
     const uint64_t first = uint64_t(blockIdx.x) * cols;
     const T *x = static_cast<const T*>(a.x) + first, *res = static_cast<const T*>(a.residual) + first;
@@ -231,9 +248,9 @@ __global__ void __launch_bounds__(1024) rms_norm_odd_rows_kernel(NormArgs a, uin
         const uint32_t k = threadIdx.x + j * lanes;
         sum += t[j] * t[j];
         t[j] = k < cols ? t[j] * to_f32(w[k]) : 0.0f;
-        most = MaxMagnitude()(most, fabsf(t[j]));
+        most = max_magnitude(most, fabsf(t[j]));
     }
-    reduce_two<false>(sum, most, lanes / 32, shared);
+    reduce<false, true>(sum, most, lanes / 32, shared);
     const float r = __frsqrt_rn(sum / float(cols) + a.eps), s = is_finite(most * r) ? most * r / 448.0f : __uint_as_float(0x7FC00000u), part = most / 448.0f;
     if (quant == SCALE_ROW && threadIdx.x == 0) static_cast<float*>(a.scales)[blockIdx.x] = s;
 #pragma unroll
@@ -248,7 +265,7 @@ __global__ void __launch_bounds__(1024) rms_norm_odd_rows_kernel(NormArgs a, uin
 // Rows of any length and place: a block per row, three passes over it.
 template <class T, class W>
 __global__ void __launch_bounds__(256) rms_norm_long_kernel(NormArgs a, uint32_t quant) {
-    __shared__ float shared[2][32];
+    __shared__ __align__(16) float shared[2][32];
     const uint64_t row = blockIdx.x, cols = a.cols;
     const T* x = static_cast<const T*>(a.x) + row * cols;
     const T* res = a.residual ? static_cast<const T*>(a.residual) + row * cols : nullptr;
@@ -259,9 +276,9 @@ __global__ void __launch_bounds__(256) rms_norm_long_kernel(NormArgs a, uint32_t
         float v = to_f32(x[k]);
         if (res) { const T s = from_f32<T>(v + to_f32(res[k])); h[k] = s; v = to_f32(s); }
         sum += v * v;
-        most = MaxMagnitude()(most, fabsf(v * to_f32(w[k])));
+        most = max_magnitude(most, fabsf(v * to_f32(w[k])));
     }
-    reduce_two<false>(sum, most, blockDim.x / 32, shared);
+    reduce<false, true>(sum, most, blockDim.x / 32, shared);
     const float r = __frsqrt_rn(sum / float(cols) + a.eps), s = is_finite(most * r) ? most * r / 448.0f : __uint_as_float(0x7FC00000u), part = most / 448.0f;
     const T* in = res ? h : x;
     uint8_t* q = static_cast<uint8_t*>(a.y) + row * cols;
@@ -272,7 +289,7 @@ __global__ void __launch_bounds__(256) rms_norm_long_kernel(NormArgs a, uint32_t
         else if (quant == SCALE_ROW) q[k] = f32_e4m3(s == 0.0f ? 0.0f : s == s ? t / part : s);
         else {
             float m = fabsf(t);
-            for (int o = 16; o; o >>= 1) m = MaxMagnitude()(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            for (int o = 16; o; o >>= 1) m = max_magnitude(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
             const uint32_t e = block_scale(m * r);
             q[k] = f32_e4m3(t * r * block_inverse(e));
             if ((threadIdx.x & 31) == 0) static_cast<uint8_t*>(a.scales)[row * (cols / 32) + k / 32] = uint8_t(e);
@@ -296,7 +313,7 @@ struct NormGradArgs {
 template <class T, class W, int N, int MOST>
 __global__ void __launch_bounds__(MOST) rms_norm_grad_rows_kernel(NormGradArgs a) {
     constexpr int V = Piece<T>::V;
-    __shared__ float shared[2][2][32];
+    __shared__ __align__(16) float shared[2][2][32];
     const uint32_t lanes = blockDim.x, at = threadIdx.x, pieces = uint32_t(a.cols / V);
     const uint4 *hs = static_cast<const uint4*>(a.h), *dys = static_cast<const uint4*>(a.dy), *dhs = static_cast<const uint4*>(a.dh);
     uint4 h[N], dy[N], dh[N];
@@ -312,40 +329,49 @@ __global__ void __launch_bounds__(MOST) rms_norm_grad_rows_kernel(NormGradArgs a
             }
         }
     };
-    float dw[N][V] = {};
-    auto weights_of = [&](int j, float (&w)[V]) {  // again for every use: they stay in the L1
+    float dw[N][V] = {}, kept[N][V];
+    // the weights: in registers where a thread has one piece, else again for every use (they stay in the L1)
+    auto weights_of = [&](int j, float (&w)[V]) {
 #pragma unroll
         for (int k = 0; k < V; ++k) w[k] = 0;
         if (at + j * lanes < pieces) weights<T, W>(a.weight, at + j * lanes, w);
     };
+    if (N == 1) weights_of(0, kept[0]);
     if (MOST <= 512) ask(blockIdx.x);
     uint32_t turn = 0;
     for (uint64_t row = blockIdx.x; row < a.rows; row += a.blocks, turn ^= 1) {
         if (MOST > 512) ask(row);
         float sq = 0, dot = 0;
-        uint4 h0[N], d0[N], r0[N];
+        Piece<T> v[N], d[N];
+        uint4 r0[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            h0[j] = h[j]; d0[j] = dy[j]; r0[j] = dh[j];
-            const Piece<T> v = numbers<T>(h0[j]), d = numbers<T>(d0[j]);
+            v[j] = numbers<T>(h[j]);
+            d[j] = numbers<T>(dy[j]);
+            r0[j] = dh[j];
             float w[V];
-            weights_of(j, w);
+            if (N > 1) weights_of(j, w);
 #pragma unroll
-            for (int k = 0; k < V; ++k) { sq += v.v[k] * v.v[k]; dot += d.v[k] * w[k] * v.v[k]; }
+            for (int k = 0; k < V; ++k) { sq += v[j].v[k] * v[j].v[k]; dot += d[j].v[k] * (N > 1 ? w[k] : kept[0][k]) * v[j].v[k]; }
         }
         if (MOST <= 512) ask(row + a.blocks);
-        reduce_two<true>(sq, dot, lanes / 32, shared[turn]);
+        reduce<true, false>(sq, dot, lanes / 32, shared[turn]);
         const float r = __frsqrt_rn(sq / float(a.cols) + a.eps), c = r * r * r * dot / float(a.cols);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const uint32_t i = at + j * lanes;
-            const Piece<T> v = numbers<T>(h0[j]), d = numbers<T>(d0[j]), e = numbers<T>(r0[j]);
             float g[V], w[V];
-            weights_of(j, w);
+            if (N > 1) weights_of(j, w);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                g[k] = r * d.v[k] * w[k] - v.v[k] * c + e.v[k];
-                dw[j][k] += d.v[k] * v.v[k] * r;
+                const float u = d[j].v[k] * r;
+                g[k] = u * (N > 1 ? w[k] : kept[0][k]) - v[j].v[k] * c;
+                dw[j][k] += u * v[j].v[k];
+            }
+            if (dhs) {
+                const Piece<T> e = numbers<T>(r0[j]);
+#pragma unroll
+                for (int k = 0; k < V; ++k) g[k] += e.v[k];
             }
             if (a.dx && i < pieces) static_cast<uint4*>(a.dx)[row * pieces + i] = rounded<T>(g);
         }
@@ -363,7 +389,7 @@ __global__ void __launch_bounds__(MOST) rms_norm_grad_rows_kernel(NormGradArgs a
 // Rows of any length and place; a block's sums for dweight live in `partial`, where each column belongs to one thread.
 template <class T, class W>
 __global__ void __launch_bounds__(512) rms_norm_grad_long_kernel(NormGradArgs a) {
-    __shared__ float shared[2][2][32];
+    __shared__ __align__(16) float shared[2][2][32];
     const uint64_t cols = a.cols;
     const W* w = static_cast<const W*>(a.weight);
     float* part = a.partial ? a.partial + blockIdx.x * cols : nullptr;
@@ -379,7 +405,7 @@ __global__ void __launch_bounds__(512) rms_norm_grad_long_kernel(NormGradArgs a)
             sq += v * v;
             dot += to_f32(dy[k]) * to_f32(w[k]) * v;
         }
-        reduce_two<true>(sq, dot, blockDim.x / 32, shared[turn]);
+        reduce<true, false>(sq, dot, blockDim.x / 32, shared[turn]);
         const float r = __frsqrt_rn(sq / float(cols) + a.eps), c = r * r * r * dot / float(cols);
         for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) {
             const float v = to_f32(h[k]), d = to_f32(dy[k]);
