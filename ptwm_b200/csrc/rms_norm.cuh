@@ -72,7 +72,7 @@ template <class T> __device__ __forceinline__ uint4 rounded(const float* v) {
 template <class T, class W> __device__ __forceinline__ void weights(const void* weight, uint32_t i, float* v) {
     constexpr int V = Piece<T>::V, PIECES = V * sizeof(W) / 16;
     if constexpr (PIECES == 0) {  // fp32 rows, 16-bit weights: half a piece
-        const uint2 w = static_cast<const uint2*>(weight)[i];
+        const uint2 w = __ldg(static_cast<const uint2*>(weight) + i);
         W e[V];
         memcpy(e, &w, 8);
 #pragma unroll
@@ -80,7 +80,7 @@ template <class T, class W> __device__ __forceinline__ void weights(const void* 
     } else {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-            const Piece<W> p = numbers<W>(static_cast<const uint4*>(weight)[i * PIECES + j]);
+            const Piece<W> p = numbers<W>(__ldg(static_cast<const uint4*>(weight) + i * PIECES + j));  // (as an intrinsic: a plain load becomes eight of two bytes)
 #pragma unroll
             for (int k = 0; k < Piece<W>::V; ++k) v[j * Piece<W>::V + k] = p.v[k];
         }
@@ -89,14 +89,15 @@ template <class T, class W> __device__ __forceinline__ void weights(const void* 
 
 // A sum and (TWO) a second one or (MOST) a largest magnitude, over the warp and, where a row has several, over the block: the warps'
 // results are read back as they lie, four at a time, which is less work than another round of shuffles.
-template <bool TWO, bool MOST> __device__ __forceinline__ void reduce(float& a, float& b, uint32_t warps, float (*shared)[32]) {
+// LANES: 32, or 16 where a warp has two rows.
+template <bool TWO, bool MOST, int LANES = 32> __device__ __forceinline__ void reduce(float& a, float& b, uint32_t warps, float (*shared)[32]) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
+    for (int o = LANES / 2; o; o >>= 1) {
         a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
         if (TWO) b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
     }
     // magnitudes compare as whole numbers, and a NaN is above infinity
-    if (MOST) b = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(b)));
+    if (MOST) b = __uint_as_float(__reduce_max_sync(LANES == 32 ? 0xFFFFFFFFu : 0xFFFFu << (threadIdx.x & 16), __float_as_uint(b)));
     if (warps == 1) return;
     const uint32_t warp = threadIdx.x / 32, up = (warps + 3) / 4 * 4;
     if ((threadIdx.x & 31) == 0) { shared[0][warp] = a; if (TWO || MOST) shared[1][warp] = b; }
@@ -126,96 +127,105 @@ template <int V> __device__ __forceinline__ void pack_e4m3(const float* v, uint3
 }
 
 // Rows that start at multiples of 16 bytes.  Bound by memory, so everything is read once and a row stays in registers: N pieces of 16
-// bytes to a thread, a row to a warp (WARP) or to a block.  One reduction is enough for any output: with t = h weight the
-// largest |y| is r times the largest |t| (rounding keeps the order), and q = t / (max|t| / 448) needs no r at all.
-template <class T, class W, int N, bool WARP, uint32_t QUANT>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_rows_kernel(NormArgs a) {
-    constexpr uint32_t quant = QUANT;
+// bytes to a thread, a row to 16 or 32 lanes (LANES) or to a block (0), which has the next row on its way while it reduces one.  One reduction is
+// enough for any output: with t = h weight the largest |y| is r times the largest |t| (rounding keeps the order), and
+// q = t / (max|t| / 448) needs no r at all.
+template <class T, class W, int N, int LANES, uint32_t QUANT>
+__global__ void __launch_bounds__(LANES ? 256 : 1024) rms_norm_rows_kernel(NormArgs a) {
     constexpr int V = Piece<T>::V;
-    __shared__ __align__(16) float shared[2][32];
-    const uint32_t lanes = WARP ? 32 : blockDim.x, at = WARP ? threadIdx.x & 31 : threadIdx.x, pieces = uint32_t(a.cols / V);
-    const uint64_t row = WARP ? uint64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
-    if (WARP && row >= a.rows) return;
-    const uint4* x = static_cast<const uint4*>(a.x) + row * pieces;
-    const uint4* res = static_cast<const uint4*>(a.residual) + row * pieces;
+    constexpr bool WARP = LANES != 0;
+    constexpr uint32_t PER = WARP ? LANES : 1;
+    __shared__ __align__(16) float shared[2][2][32];
+    const uint32_t lanes = WARP ? PER : blockDim.x, at = WARP ? threadIdx.x % PER : threadIdx.x, pieces = uint32_t(a.cols / V);
+    const uint64_t step = WARP ? uint64_t(gridDim.x) * (blockDim.x / PER) : gridDim.x;
+    uint64_t row = WARP ? uint64_t(blockIdx.x) * (blockDim.x / PER) + threadIdx.x / PER : blockIdx.x;
+    const uint4 *xs = static_cast<const uint4*>(a.x), *rs = static_cast<const uint4*>(a.residual);
     uint4 in[N], more[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const uint32_t i = at + j * lanes;
-        in[j] = more[j] = make_uint4(0, 0, 0, 0);
-        if (i < pieces) {
-            in[j] = __ldcs(x + i);
-            if (a.residual) more[j] = __ldcs(res + i);
-        }
-    }
-    float t[N][V], sum = 0, most = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const uint32_t i = at + j * lanes;
-        float w[V] = {};
-        if (i < pieces) weights<T, W>(a.weight, i, w);
-        Piece<T> h = numbers<T>(in[j]);
-        if (a.residual) {
-            const Piece<T> r = numbers<T>(more[j]);
-#pragma unroll
-            for (int k = 0; k < V; ++k) h.v[k] += r.v[k];
-            const uint4 stored = rounded<T>(h.v);
-            if (i < pieces) static_cast<uint4*>(a.h)[row * pieces + i] = stored;
-            h = numbers<T>(stored);
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            sum += h.v[k] * h.v[k];
-            t[j][k] = h.v[k] * w[k];
-            if (QUANT == SCALE_ROW) most = max_magnitude(most, t[j][k]);
-        }
-    }
-    reduce<false, QUANT == SCALE_ROW>(sum, most, WARP ? 1 : lanes / 32, shared);
-    const float r = __frsqrt_rn(sum / float(a.cols) + a.eps), nan = __uint_as_float(0x7FC00000u);
-    if (quant == SCALE_NONE) {
+    auto ask = [&](uint64_t r) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const uint32_t i = at + j * lanes;
-#pragma unroll
-            for (int k = 0; k < V; ++k) t[j][k] *= r;
-            if (i < pieces) static_cast<uint4*>(a.y)[row * pieces + i] = rounded<T>(t[j]);
+            in[j] = more[j] = make_uint4(0, 0, 0, 0);
+            if (r < a.rows && i < pieces) {
+                in[j] = __ldcs(xs + r * pieces + i);
+                if (rs) more[j] = __ldcs(rs + r * pieces + i);
+            }
         }
-        return;
-    }
-    using Out = typename std::conditional<V == 8, uint2, uint32_t>::type;
-    Out* q = static_cast<Out*>(a.y) + row * pieces;
-    const float s = is_finite(most * r) ? most * r / 448.0f : nan, part = most / 448.0f, inverse = 448.0f / most;
-    const bool plain = s > 0.0f && most > 0x1p-100f;  // nearly always: a product for a division
-    if (quant == SCALE_ROW && at == 0) static_cast<float*>(a.scales)[row] = s;
+    };
+    ask(row);
+    // (two rows of a warp go on together: the shuffles want both)
+    for (uint32_t turn = 0; LANES == 16 ? __any_sync(0xFFFFFFFFu, row < a.rows) : row < a.rows; row += step, turn ^= 1) {
+        const bool there = LANES != 16 || row < a.rows;
+        float t[N][V], sum = 0, most = 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const uint32_t i = at + j * lanes;
-        if (quant == SCALE_ROW) {
-            // part is 0 only where s is, and not finite only where s is not
-            if (plain) {
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = at + j * lanes;
+            float w[V] = {};
+            if (i < pieces) weights<T, W>(a.weight, i, w);
+            Piece<T> h = numbers<T>(in[j]);
+            if (rs) {
+                const Piece<T> r = numbers<T>(more[j]);
 #pragma unroll
-                for (int k = 0; k < V; ++k) t[j][k] *= inverse;
-            } else {
+                for (int k = 0; k < V; ++k) h.v[k] += r.v[k];
+                const uint4 stored = rounded<T>(h.v);
+                if (there && i < pieces) static_cast<uint4*>(a.h)[row * pieces + i] = stored;
+                h = numbers<T>(stored);
+            }
 #pragma unroll
-                for (int k = 0; k < V; ++k) t[j][k] = s == 0.0f ? 0.0f : s == s ? t[j][k] / part : nan;
+            for (int k = 0; k < V; ++k) {
+                sum += h.v[k] * h.v[k];
+                t[j][k] = h.v[k] * w[k];
+                if (QUANT == SCALE_ROW) most = max_magnitude(most, t[j][k]);
+            }
+        }
+        ask(row + step);
+        reduce<false, QUANT == SCALE_ROW, LANES == 16 ? 16 : 32>(sum, most, WARP ? 1 : lanes / 32, shared[turn]);
+        const float r = __frsqrt_rn(sum / float(a.cols) + a.eps), nan = __uint_as_float(0x7FC00000u);
+        if constexpr (QUANT == SCALE_NONE) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint32_t i = at + j * lanes;
+#pragma unroll
+                for (int k = 0; k < V; ++k) t[j][k] *= r;
+                if (there && i < pieces) static_cast<uint4*>(a.y)[row * pieces + i] = rounded<T>(t[j]);
             }
         } else {
-            float m = 0;
+            using Out = typename std::conditional<V == 8, uint2, uint32_t>::type;
+            Out* q = static_cast<Out*>(a.y) + row * pieces;
+            const float s = is_finite(most * r) ? most * r / 448.0f : nan, part = most / 448.0f, inverse = 448.0f / most;
+            const bool plain = s > 0.0f && most > 0x1p-100f;  // nearly always: a product for a division
+            if (QUANT == SCALE_ROW && there && at == 0) static_cast<float*>(a.scales)[row] = s;
 #pragma unroll
-            for (int k = 0; k < V; ++k) m = max_magnitude(m, t[j][k]);
+            for (int j = 0; j < N; ++j) {
+                const uint32_t i = at + j * lanes;
+                if (QUANT == SCALE_ROW) {
+                    // part is 0 only where s is, and not finite only where s is not
+                    if (plain) {
 #pragma unroll
-            for (int o = 1; o < 32 / V; o *= 2) m = max_magnitude(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));  // the threads of a block of 32
-            const uint32_t e = block_scale(m * r);
-            const float down = block_inverse(e);
+                        for (int k = 0; k < V; ++k) t[j][k] *= inverse;
+                    } else {
 #pragma unroll
-            for (int k = 0; k < V; ++k) t[j][k] = t[j][k] * r * down;
-            if (i < pieces && i % (32 / V) == 0) static_cast<uint8_t*>(a.scales)[row * (a.cols / 32) + i / (32 / V)] = uint8_t(e);
+                        for (int k = 0; k < V; ++k) t[j][k] = s == 0.0f ? 0.0f : s == s ? t[j][k] / part : nan;
+                    }
+                } else {
+                    float m = 0;
+#pragma unroll
+                    for (int k = 0; k < V; ++k) m = max_magnitude(m, t[j][k]);
+#pragma unroll
+                    for (int o = 1; o < 32 / V; o *= 2) m = max_magnitude(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));  // the threads of a block of 32
+                    const uint32_t e = block_scale(m * r);
+                    const float down = block_inverse(e);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) t[j][k] = t[j][k] * r * down;
+                    if (there && i < pieces && i % (32 / V) == 0) static_cast<uint8_t*>(a.scales)[row * (a.cols / 32) + i / (32 / V)] = uint8_t(e);
+                }
+                uint32_t o[V / 4];
+                pack_e4m3<V>(t[j], o);
+                Out out;
+                memcpy(&out, o, sizeof out);
+                if (there && i < pieces) q[i] = out;
+            }
         }
-        uint32_t o[V / 4];
-        pack_e4m3<V>(t[j], o);
-        Out out;
-        memcpy(&out, o, sizeof out);
-        if (i < pieces) q[i] = out;
     }
 }
 
@@ -251,13 +261,14 @@ __global__ void __launch_bounds__(1024) rms_norm_odd_rows_kernel(NormArgs a, uin
         most = max_magnitude(most, fabsf(t[j]));
     }
     reduce<false, true>(sum, most, lanes / 32, shared);
-    const float r = __frsqrt_rn(sum / float(cols) + a.eps), s = is_finite(most * r) ? most * r / 448.0f : __uint_as_float(0x7FC00000u), part = most / 448.0f;
+    const float r = __frsqrt_rn(sum / float(cols) + a.eps), s = is_finite(most * r) ? most * r / 448.0f : __uint_as_float(0x7FC00000u), part = most / 448.0f, inverse = 448.0f / most;
+    const bool plain = s > 0.0f && most > 0x1p-100f;
     if (quant == SCALE_ROW && threadIdx.x == 0) static_cast<float*>(a.scales)[blockIdx.x] = s;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         const uint32_t k = threadIdx.x + j * lanes;
         if (k >= cols) continue;
-        if (quant == SCALE_ROW) static_cast<uint8_t*>(a.y)[first + k] = f32_e4m3(s == 0.0f ? 0.0f : s == s ? t[j] / part : s);
+        if (quant == SCALE_ROW) static_cast<uint8_t*>(a.y)[first + k] = f32_e4m3(plain ? t[j] * inverse : s == 0.0f ? 0.0f : s == s ? t[j] / part : s);
         else static_cast<T*>(a.y)[first + k] = from_f32<T>(t[j] * r);
     }
 }
@@ -311,7 +322,7 @@ struct NormGradArgs {
 // A block takes rows blockIdx.x, + blocks, ...  Its threads keep their columns, N pieces of 16 bytes, and with them their sums for
 // dweight in registers; with 512 of them the next row is asked for before this one's reduction, which 64 registers of 1024 do not hold.
 template <class T, class W, int N, int MOST>
-__global__ void __launch_bounds__(MOST) rms_norm_grad_rows_kernel(NormGradArgs a) {
+__global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kernel(NormGradArgs a) {
     constexpr int V = Piece<T>::V;
     __shared__ __align__(16) float shared[2][2][32];
     const uint32_t lanes = blockDim.x, at = threadIdx.x, pieces = uint32_t(a.cols / V);

@@ -55,7 +55,7 @@ def _inputs(rows, cols, dtype, seed, residual=True, weight_dtype=None):
     return x, res, w
 
 
-ROWS_COLS = [(1, 1), (3, 7), (1, 32), (5, 96), (2, 1000), (17, 1024), (1, 4096), (333, 4095), (7, 8200), (2, 10501), (3, 16384), (2, 40000), (1200, 64)]
+ROWS_COLS = [(1, 1), (3, 7), (1, 32), (5, 96), (2, 1000), (17, 1024), (1, 4096), (333, 4095), (7, 8200), (2, 10501), (3, 16384), (2, 40000), (1200, 64), (1203, 128), (301, 32), (999, 256), (500, 1024)]
 
 
 @pytest.mark.parametrize("rows, cols", ROWS_COLS)
