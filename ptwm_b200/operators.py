@@ -16,13 +16,16 @@ from typing import Any, Callable, Mapping, Optional, Sequence
 
 import torch
 
+from torch._C import _cuda_getCurrentRawStream as _stream  # what torch.cuda.current_stream() wraps, a microsecond faster
+
 from . import _lib
-from .container import _check, stream_handle
+from .container import _check
 
 __all__ = ["Projection", "ScaledActivations", "ScaledWeight", "matvec", "rms_norm"]
 
 _PLAIN = {torch.float32: 1, torch.float16: 4, torch.bfloat16: 6}
 _E4M3 = 29
+_TOO_SMALL = -2
 _QUANT = {None: 0, "row": 1, "block": 2}
 _U8 = (torch.uint8,) + ((torch.float4_e2m1fn_x2,) if hasattr(torch, "float4_e2m1fn_x2") else ())
 _E8M0 = torch.float8_e8m0fnu
@@ -169,19 +172,31 @@ class ScaledWeight:
 def _norm(x, weight, residual, eps: float, quant: Optional[str]):
     """(y or ScaledActivations, h) of checked, contiguous tensors."""
     cols = x.shape[-1]
-    device = x.device.index
-    h = x if residual is None else torch.empty_like(x)
-    scales = None
+    device = x.get_device()
+    rows = x.numel() // cols
+    h, residual_at = (x, 0) if residual is None else (torch.empty_like(x), residual.data_ptr())
     if quant is None:
-        y = torch.empty_like(x)
+        y, out, scales_at = torch.empty_like(x), None, 0
+        y_at = y.data_ptr()
     else:
-        y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        scales = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quant == "row" else
-                  torch.empty((*x.shape[:-1], cols // 32), dtype=_E8M0, device=x.device))
-    _check(_lib.lib().ptwm_b200_rms_norm(x.data_ptr(), 0 if residual is None else residual.data_ptr(), weight.data_ptr(), h.data_ptr(), y.data_ptr(),
-                                         0 if scales is None else scales.data_ptr(), x.numel() // cols, cols, _PLAIN[x.dtype], _PLAIN[weight.dtype],
-                                         _QUANT[quant], eps, device, stream_handle(device)))
-    return (y if quant is None else ScaledActivations._of(y, scales, quant)), h
+        values = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+        if quant == "row":
+            scales = _new(x.shape[:-1], torch.float32, x.device)
+        else:
+            scales = _new((*x.shape[:-1], cols // 32), _E8M0, x.device)
+        out, y_at, scales_at = ScaledActivations._of(values, scales, quant), values.data_ptr(), scales.data_ptr()
+    _check(_lib.lib().ptwm_b200_rms_norm(x.data_ptr(), residual_at, weight.data_ptr(), h.data_ptr(), y_at, scales_at, rows, cols, _PLAIN[x.dtype], _PLAIN[weight.dtype],
+                                         _QUANT[quant], eps, device, _stream(device)))
+    return (y if out is None else out), h
+
+
+def _new(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """torch.empty; its quickest form for the usual two dimensions."""
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+    if len(shape) == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -204,7 +219,7 @@ class _RmsNorm(torch.autograd.Function):
         else:
             dy = dy.contiguous()
             dh = None if dh is None else dh.contiguous()
-            cols, device = h.shape[-1], h.device.index
+            cols, device = h.shape[-1], h.get_device()
             rows = h.numel() // cols
             dx = torch.empty_like(h) if need_x else None
             dw = torch.empty_like(weight) if need_w else None
@@ -213,7 +228,7 @@ class _RmsNorm(torch.autograd.Function):
             scratch = torch.empty(size, dtype=torch.uint8, device=h.device) if size else None
             _check(L.ptwm_b200_rms_norm_grad(h.data_ptr(), weight.data_ptr(), dy.data_ptr(), 0 if dh is None else dh.data_ptr(), 0 if dx is None else dx.data_ptr(),
                                              0 if dw is None else dw.data_ptr(), 0 if scratch is None else scratch.data_ptr(), size, rows, cols, _PLAIN[h.dtype],
-                                             _PLAIN[weight.dtype], ctx.eps, device, stream_handle(device)))
+                                             _PLAIN[weight.dtype], ctx.eps, device, _stream(device)))
         return (dx if ctx.needs_input_grad[0] else None), dw, (dx if ctx.has_residual and ctx.needs_input_grad[2] else None), None
 
 
@@ -235,14 +250,15 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residu
         raise TypeError(f"x and weight are float32, float16 or bfloat16, got {x.dtype} and {weight.dtype}")
     if quant not in _QUANT:
         raise ValueError(f"quant is None, 'row' or 'block', got {quant!r}")
-    if x.dim() < 1 or x.shape[-1] == 0 or weight.shape != x.shape[-1:]:
-        raise ValueError(f"weight of shape {tuple(weight.shape)} does not fit rows of x, shape {tuple(x.shape)}")
-    if quant == "block" and x.shape[-1] % 32:
-        raise ValueError(f"block scales need whole blocks of 32 values, got rows of {x.shape[-1]}")
+    shape = x.shape
+    if not shape or shape[-1] == 0 or weight.shape != shape[-1:]:
+        raise ValueError(f"weight of shape {tuple(weight.shape)} does not fit rows of x, shape {tuple(shape)}")
+    if quant == "block" and shape[-1] % 32:
+        raise ValueError(f"block scales need whole blocks of 32 values, got rows of {shape[-1]}")
     if residual is not None:
         _on_cuda("residual", residual, x.device)
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}, x {x.dtype} {tuple(x.shape)}; they have to be alike")
+        if residual.shape != shape or residual.dtype != x.dtype:
+            raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}, x {x.dtype} {tuple(shape)}; they have to be alike")
     grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))
     if grad and quant is not None:
         raise ValueError("an 8-bit output has no gradient: call under torch.no_grad() or detach the inputs")
@@ -256,17 +272,20 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residu
 
 # ---- matvec ---------------------------------------------------------------------------------------
 def _product(x, scales, quant, weight: ScaledWeight, out_dtype: torch.dtype) -> torch.Tensor:
-    device, tokens, code = weight._ordinal, x.numel() // weight.cols, _E4M3 if scales is not None else _PLAIN[x.dtype]
-    y = torch.empty((*x.shape[:-1], weight.rows), dtype=out_dtype, device=x.device)
-    scratch, size = _scratch(weight, x, tokens, code, 0)
-    _check(_lib.lib().ptwm_b200_matvec(weight._ref, x.data_ptr(), 0 if scales is None else scales.data_ptr(), y.data_ptr(), tokens, code, _QUANT[quant], _PLAIN[out_dtype],
-                                       0 if scratch is None else scratch.data_ptr(), size, device, stream_handle(device)))
+    device, tokens, code = weight._ordinal, x.numel() // weight.cols, _PLAIN[x.dtype] if scales is None else _E4M3
+    y = _new((*x.shape[:-1], weight.rows), out_dtype, weight.device)
+    # few tokens, and bf16 ones that lie well, need no scratch: it is asked for where the call says so
+    args = (weight._ref, x.data_ptr(), 0 if scales is None else scales.data_ptr(), y.data_ptr(), tokens, code, _QUANT[quant], _PLAIN[out_dtype])
+    rc = _lib.lib().ptwm_b200_matvec(*args, 0, 0, device, _stream(device))
+    if rc == _TOO_SMALL:
+        scratch = _scratch(weight, x, tokens, code, 0)
+        rc = _lib.lib().ptwm_b200_matvec(*args, scratch.data_ptr(), scratch.numel(), device, _stream(device))
+    _check(rc)
     return y
 
 
-def _scratch(weight: ScaledWeight, x: torch.Tensor, tokens: int, code: int, grad: int):
-    size = _lib.lib().ptwm_b200_matvec_scratch_bytes(weight._ref, x.data_ptr(), tokens, code, grad)
-    return (torch.empty(size, dtype=torch.uint8, device=x.device) if size else None), size
+def _scratch(weight: ScaledWeight, x: torch.Tensor, tokens: int, code: int, grad: int) -> torch.Tensor:
+    return torch.empty(_lib.lib().ptwm_b200_matvec_scratch_bytes(weight._ref, x.data_ptr(), tokens, code, grad), dtype=torch.uint8, device=x.device)
 
 
 class _Matvec(torch.autograd.Function):
@@ -281,10 +300,12 @@ class _Matvec(torch.autograd.Function):
         w = ctx.weight
         dy = dy.to(ctx.dtype).contiguous()
         dx = torch.empty((*dy.shape[:-1], w.cols), dtype=ctx.dtype, device=dy.device)
-        tokens, code = dy.numel() // w.rows, _PLAIN[ctx.dtype]
-        scratch, size = _scratch(w, dy, tokens, code, 1)
-        _check(_lib.lib().ptwm_b200_matvec_grad(w._ref, dy.data_ptr(), dx.data_ptr(), tokens, code, 0 if scratch is None else scratch.data_ptr(), size, w._ordinal,
-                                                stream_handle(w._ordinal)))
+        args = (w._ref, dy.data_ptr(), dx.data_ptr(), dy.numel() // w.rows, _PLAIN[ctx.dtype])
+        rc = _lib.lib().ptwm_b200_matvec_grad(*args, 0, 0, w._ordinal, _stream(w._ordinal))
+        if rc == _TOO_SMALL:
+            scratch = _scratch(w, dy, args[3], args[4], 1)
+            rc = _lib.lib().ptwm_b200_matvec_grad(*args, scratch.data_ptr(), scratch.numel(), w._ordinal, _stream(w._ordinal))
+        _check(rc)
         return dx, None, None
 
 
@@ -310,7 +331,7 @@ def matvec(x, weight: ScaledWeight, *, out_dtype: Optional[torch.dtype] = None) 
         raise TypeError(f"out_dtype is float32, float16 or bfloat16, got {out_dtype}")
     if x.device != weight.device:
         raise ValueError(f"x lives on {x.device}, the weight on {weight.device}")
-    if x.dim() < 1 or x.shape[-1] != weight.cols:
+    if not x.shape or x.shape[-1] != weight.cols:
         raise ValueError(f"x of shape {tuple(x.shape)} does not fit a matrix of {weight.rows} x {weight.cols}")
     if not x.is_contiguous():
         x = x.contiguous()
