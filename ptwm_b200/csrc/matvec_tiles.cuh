@@ -2,7 +2,7 @@
 //
 //   forward:   D[n][m] = sum_k W[n][k] x[m][k]       gradient: D[k][m] = sum_n W[n][k] dy[m][n]
 // A block makes a tile of 128 rows of D (n, or k) and up to 256 tokens.  The matrix stays packed until it is in shared memory:
-// TMA brings boxes of nibbles and scales, eight warps turn them into bf16 (exactly: a nibble times its scale has at most six
+// TMA brings boxes of nibbles and scales, sixteen warps turn them into bf16 (exactly: a nibble times its scale has at most six
 // significant bits) in the swizzled lines the tensor cores read, and one thread issues the MMAs.  Tokens come as bf16 by TMA.
 // Tokens of other types are bf16 parts that add up to them: E4M3 is one, fp16 two, fp32 three (token_parts_kernel); each part is
 // multiplied with the same converted tile, and all sums meet in the same fp32 accumulator.  In the gradient the contraction
@@ -16,7 +16,7 @@ namespace ptwm {
 constexpr uint32_t TILE_ROWS = 128;                 // rows of D to a block
 constexpr uint32_t STEP = 64;                       // contraction to a converted tile: one 128-byte line of bf16
 constexpr uint32_t RAW_STAGES = 6, RAW_BYTES = 8192, SCALES_BYTES = 8192, A_STAGES = 4, A_BYTES = TILE_ROWS * STEP * 2;
-constexpr uint32_t TILES_THREADS = 352;             // warp 0: TMA of the matrix, 1: MMA, 2: TMA of the tokens, 3 to 10: conversion, then the results
+constexpr uint32_t TILES_THREADS = 640;             // warp 0: TMA of the matrix, 1: MMA, 2: TMA of the tokens, 4 to 19: conversion, then the results
 constexpr uint32_t TILES_HEAD = 1024;               // barriers and the like, in front of the buffers
 
 struct TilesArgs {
@@ -70,11 +70,12 @@ constexpr float NV_REST = 1024.0f;
 template <bool GRAD> struct TilesShared {
     static constexpr uint32_t raw = TILES_HEAD, scales = raw + RAW_STAGES * RAW_BYTES, a = scales + SCALES_BYTES, b = a + A_STAGES * A_BYTES;
     static constexpr uint32_t raw_rows = GRAD ? STEP : TILE_ROWS, scale_bytes = raw_rows * 16, scale_slots = SCALES_BYTES / scale_bytes;
-    // barriers: raw full / empty, a full / empty, b full / empty, accumulator full
-    static constexpr uint32_t raw_full = 0, raw_empty = 64, a_full = 128, a_empty = 192, b_full = 256, b_empty = 320, done = 384, tmem = 392, failed = 396;
+    // barriers: raw full / empty, scales full (a slot is free once all raw stages before raw - RAW_STAGES are), a full / empty, b full / empty,
+    // accumulator full
+    static constexpr uint32_t raw_full = 0, raw_empty = 64, a_full = 128, a_empty = 192, b_full = 256, b_empty = 320, scales_full = 384, done = 448, tmem = 456, failed = 460;
 };
 
-// Nibbles of one thread (16 bytes: 32 values) -> four 16-byte pieces of bf16.
+// 16 bytes of nibbles (32 values) -> four 16-byte pieces of bf16.  s: the scale of all (MXFP4), or of the first and the second half.
 __device__ __forceinline__ void convert32(const uint4& v, uint32_t group, uint32_t s, uint4 (&out)[4]) {
     const uint32_t words[4] = {v.x, v.y, v.z, v.w};
     uint32_t more = 0x3F803F80u;
@@ -111,9 +112,10 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
 
     if (threadIdx.x == 0) {
         *failed = 0;
-        for (uint32_t i = 0; i < RAW_STAGES; ++i) { mbar_init(sb + S::raw_full + 8 * i, 1); mbar_init(sb + S::raw_empty + 8 * i, 8); }
-        for (uint32_t i = 0; i < A_STAGES; ++i) { mbar_init(sb + S::a_full + 8 * i, 8); mbar_init(sb + S::a_empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < RAW_STAGES; ++i) { mbar_init(sb + S::raw_full + 8 * i, 1); mbar_init(sb + S::raw_empty + 8 * i, GRAD ? 4 : 8); }  // four warps for each of its steps
+        for (uint32_t i = 0; i < A_STAGES; ++i) { mbar_init(sb + S::a_full + 8 * i, 4); mbar_init(sb + S::a_empty + 8 * i, 1); }
         for (uint32_t i = 0; i < t.b_stages; ++i) { mbar_init(sb + S::b_full + 8 * i, 1); mbar_init(sb + S::b_empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < S::scale_slots; ++i) mbar_init(sb + S::scales_full + 8 * i, 1);
         mbar_init(sb + S::done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -125,87 +127,103 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
 
     if (warp == 0) {
         if (elect_one()) {
-            for (uint32_t raw = 0; raw < raws && !*failed; ++raw) {
-                const uint32_t st = raw % RAW_STAGES, full = sb + S::raw_full + 8 * st;
-                if (raw >= RAW_STAGES) mbar_wait(sb + S::raw_empty + 8 * st, (raw / RAW_STAGES - 1) & 1, failed);
-                if (*failed) break;
-                const bool with_scales = raw % scale_raws == 0;
-                mbar_expect(full, S::raw_rows * (with_scales ? 80 : 64));
+            uint32_t st = 0, parity = 1, slot = 0, piece = 0, scale_x = GRAD ? row0 / t.group & ~15u : 0;
+            for (uint32_t raw = 0; raw < raws; ++raw) {
+                const uint32_t full = sb + S::raw_full + 8 * st;
+                if (raw >= RAW_STAGES && !mbar_wait(sb + S::raw_empty + 8 * st, parity, failed)) break;
+                mbar_expect(full, S::raw_rows * 64);
                 if (GRAD) tma_load(sb + S::raw + st * RAW_BYTES, &values, full, int32_t(row0 / 2), int32_t(raw * STEP));
                 else tma_load(sb + S::raw + st * RAW_BYTES, &values, full, int32_t(raw * 64), int32_t(row0));
-                if (with_scales) {
+                if (piece == 0) {
                     // its slot was last read for raw stages before raw - RAW_STAGES: there are enough slots for those in between
-                    const uint32_t dst = sb + S::scales + raw / scale_raws % S::scale_slots * S::scale_bytes;
-                    if (GRAD) tma_load(dst, &scales, full, int32_t(row0 / t.group & ~15u), int32_t(raw * STEP));
-                    else tma_load(dst, &scales, full, int32_t(raw / scale_raws * 16), int32_t(row0));
+                    const uint32_t bar = sb + S::scales_full + 8 * slot;
+                    mbar_expect(bar, S::scale_bytes);
+                    tma_load(sb + S::scales + slot * S::scale_bytes, &scales, bar, int32_t(scale_x), int32_t(GRAD ? raw * STEP : row0));
+                    if (!GRAD) scale_x += 16;
+                    if (++slot == S::scale_slots) slot = 0;
                 }
+                if (++piece == scale_raws) piece = 0;
+                if (++st == RAW_STAGES) { st = 0; parity ^= 1; }
             }
             // every load has been waited for by those who use it, unless something failed: then what is under way gets time to land
             if (*failed) let_copies_land();
         }
     } else if (warp == 2) {
         if (elect_one()) {
-            for (uint32_t b = 0; b < steps * t.parts && !*failed; ++b) {
-                const uint32_t st = b % t.b_stages, full = sb + S::b_full + 8 * st;
-                if (b >= t.b_stages) mbar_wait(sb + S::b_empty + 8 * st, (b / t.b_stages - 1) & 1, failed);
-                if (*failed) break;
+            // (counters instead of divisions: one thread's latency is what these two warps cost)
+            uint32_t st = 0, parity = 1, p = 0, step = 0;
+            for (uint32_t b = 0; b < steps * t.parts; ++b) {
+                const uint32_t full = sb + S::b_full + 8 * st;
+                if (b >= t.b_stages && !mbar_wait(sb + S::b_empty + 8 * st, parity, failed)) break;
                 mbar_expect(full, b_bytes);
-                tma_load(sb + S::b + st * b_bytes, &tokens, full, int32_t(b / t.parts * STEP), int32_t(b % t.parts * t.part_rows + token0));
+                tma_load(sb + S::b + st * b_bytes, &tokens, full, int32_t(step * STEP), int32_t(p * t.part_rows + token0));
+                if (++st == t.b_stages) { st = 0; parity ^= 1; }
+                if (++p == t.parts) { p = 0; ++step; }
             }
             if (*failed) let_copies_land();
         }
     } else if (warp == 1) {
         if (elect_one()) {
             const uint32_t idesc = instruction_desc(t.tile_tokens, GRAD);
-            for (uint32_t step = 0, b = 0; step < steps && !*failed; ++step) {
-                const uint32_t as = step % A_STAGES;
-                mbar_wait(sb + S::a_full + 8 * as, step / A_STAGES & 1, failed);
-                for (uint32_t p = 0; p < t.parts; ++p, ++b) {
-                    const uint32_t bs = b % t.b_stages;
-                    mbar_wait(sb + S::b_full + 8 * bs, b / t.b_stages & 1, failed);
-                    if (*failed) break;
+            const uint64_t a_desc = operand_desc(sb + S::a, GRAD ? 8192 : 16, 1024), b_desc = operand_desc(sb + S::b, 16, 1024);
+            uint32_t as = 0, a_parity = 0, bs = 0, b_parity = 0;
+            bool more = false, ok = true;
+            for (uint32_t step = 0; step < steps && ok; ++step) {
+                ok = mbar_wait(sb + S::a_full + 8 * as, a_parity, failed);
+                const uint64_t ad = a_desc + as * (A_BYTES / 16);
+                for (uint32_t p = 0; p < t.parts && ok; ++p) {
+                    ok = mbar_wait(sb + S::b_full + 8 * bs, b_parity, failed);
+                    if (!ok) break;
                     tc_fence_after();
+                    const uint64_t bd = b_desc + bs * (b_bytes / 16);
 #pragma unroll
                     for (uint32_t k = 0; k < STEP / 16; ++k) {
-                        const uint32_t a_addr = sb + S::a + as * A_BYTES + (GRAD ? k * 2048 : k * 32);
-                        const uint64_t ad = GRAD ? operand_desc(a_addr, 8192, 1024) : operand_desc(a_addr, 16, 1024);
-                        mma_f16(tmem, ad, operand_desc(sb + S::b + bs * b_bytes + k * 32, 16, 1024), idesc, (b | k) != 0);
+                        mma_f16(tmem, ad + k * (GRAD ? 2048 / 16 : 32 / 16), bd + k * 2, idesc, more);
+                        more = true;
                     }
                     tc_commit(sb + S::b_empty + 8 * bs);
+                    if (++bs == t.b_stages) { bs = 0; b_parity ^= 1; }
                 }
-                if (!*failed) tc_commit(sb + S::a_empty + 8 * as);
+                if (ok) tc_commit(sb + S::a_empty + 8 * as);
+                if (++as == A_STAGES) { as = 0; a_parity ^= 1; }
             }
             tc_commit(sb + S::done);
         }
-    } else {
-        const uint32_t c = threadIdx.x - 96;
-        // this thread's 16 bytes of a raw stage: forward row c / 2 and half c % 2 of either step's 32 bytes; in the gradient row (c % 128) / 2 and
-        // one quarter of its 64 bytes, so that eight neighbours store to eight different 16-byte banks
-        const uint32_t row = GRAD ? c % 128 / 2 : c / 2, quarter = GRAD ? c % 2 + c / 128 * 2 : c % 2;
+    } else if (warp >= 4) {
+        // Four groups of four warps take a step each in turn: a step is some 200 instructions of a thread in a row, and four of them are under way.
+        // A thread has 32 bytes of a row (64 values of it): forward the step's part of row c, in the gradient one half of row c % 64.  TMA has swizzled
+        // the 16-byte pieces of a raw stage's 64-byte rows, so that neighbouring rows lie in different banks, and they are stored swizzled.
+        const uint32_t team = (warp - 4) / 4, c = threadIdx.x % 128, row = GRAD ? c % 64 : c, half = c / 64;
         const uint32_t first_group = GRAD ? row0 / t.group & 15u : 0;
-        const uint32_t out = GRAD ? (quarter / 2) * 8192 + row / 8 * 1024 + row % 8 * 128 : row / 8 * 1024 + row % 8 * 128;
-        for (uint32_t step = 0; step < steps && !*failed; ++step) {
-            const uint32_t raw = GRAD ? step : step / 2, st = raw % RAW_STAGES, as = step % A_STAGES;
-            const uint32_t q = GRAD ? quarter : step % 2 * 2 + quarter;  // which 32 of the 128 k
+        const uint32_t out = (GRAD ? half * 8192 : 0) + row / 8 * 1024 + row % 8 * 128;
+        for (uint32_t step = team; step < steps && !*failed; step += 4) {
+            const uint32_t raw = GRAD ? step : step / 2, st = raw % RAW_STAGES;
+            const uint32_t pair = GRAD ? half : step % 2;  // which 64 of the 128 k
             mbar_wait(sb + S::raw_full + 8 * st, raw / RAW_STAGES & 1, failed);
-            const uint4 v = *reinterpret_cast<const uint4*>(base + S::raw + st * RAW_BYTES + row * 64 + q * 16);
-            const uint8_t* sp = base + S::scales + raw / scale_raws % S::scale_slots * S::scale_bytes + row * 16;
-            const uint32_t g = first_group + raw % scale_raws * (128 / t.group);
-            const uint32_t s = t.group == 32 ? sp[g + q] : *reinterpret_cast<const uint16_t*>(sp + g + 2 * q);
+            const uint8_t* line = base + S::raw + st * RAW_BYTES + row * 64;
+            const uint4 v0 = *reinterpret_cast<const uint4*>(line + ((pair * 2 ^ row / 2) & 3) * 16), v1 = *reinterpret_cast<const uint4*>(line + ((pair * 2 + 1 ^ row / 2) & 3) * 16);
+            const uint32_t scale_at = raw / scale_raws, slot = scale_at % S::scale_slots;
+            mbar_wait(sb + S::scales_full + 8 * slot, scale_at / S::scale_slots & 1, failed);
+            const uint8_t* sp = base + S::scales + slot * S::scale_bytes + row * 16;
+            const uint32_t g = first_group + raw % scale_raws * (128 / t.group) + pair * (64 / t.group);
+            const uint32_t s = t.group == 32 ? *reinterpret_cast<const uint16_t*>(sp + g) : *reinterpret_cast<const uint32_t*>(sp + g);
+            if (step >= 4) mbar_wait(sb + S::a_empty + 8 * team, (step / 4 - 1) & 1, failed);
+            uint8_t* dst = base + S::a + team * A_BYTES + out;
             uint4 o[4];
-            convert32(v, t.group, s, o);
-            if (step >= A_STAGES) mbar_wait(sb + S::a_empty + 8 * as, (step / A_STAGES - 1) & 1, failed);
-            uint8_t* dst = base + S::a + as * A_BYTES + out;
+            convert32(v0, t.group, s, o);
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + (((quarter % 2 * 4 + j) ^ (row % 8)) * 16)) = o[j];
+            for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + ((j ^ (row % 8)) * 16)) = o[j];
+            convert32(v1, t.group, t.group == 32 ? s >> 8 : s >> 16, o);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + ((4 + j ^ (row % 8)) * 16)) = o[j];
             fence_async_shared();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(sb + S::a_full + 8 * as);
-                if (GRAD || step % 2 || step + 1 == steps) mbar_arrive(sb + S::raw_empty + 8 * st);
+                mbar_arrive(sb + S::a_full + 8 * team);
+                mbar_arrive(sb + S::raw_empty + 8 * st);
             }
         }
-        // results: a warp reaches the 32 lanes (rows of D) that its number modulo 4 names; the two warps of a quarter share the tokens
+        // results: a warp reaches the 32 lanes (rows of D) that its number modulo 4 names; the four teams share the tokens
         mbar_wait(sb + S::done, 0, failed);
         tc_fence_after();
         const uint32_t lanes = warp % 4 * 32;
@@ -213,8 +231,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
         float factor = t.group == 32 ? 1.0f : NV_REST;
         if (t.global_scale) factor *= *t.global_scale;
         if (*failed) factor = __uint_as_float(0x7FC00000u);
-        const uint32_t half = (t.tile_tokens / 16 + 1) / 2 * 16, from = warp < 7 ? 0 : half, to = warp < 7 ? half : t.tile_tokens;
-        for (uint32_t m = from; m < to; m += 16) {
+        for (uint32_t m = team * 16; m < t.tile_tokens; m += 64) {
             uint32_t v[16];
             tmem_load16(tmem + (lanes << 16) + m, v);
             if (n < t.rows) {

@@ -27,14 +27,14 @@ __device__ __forceinline__ uint64_t nanoseconds() {
 // Waits are bounded: one that lasts for two seconds raises *failed (shared memory), after which every wait of the block returns at once.
 constexpr uint64_t WAIT_NS = 2000000000ull;
 constexpr uint32_t WAIT_TRIES = 1u << 24;  // in case that clock stands still
-__device__ __noinline__ void mbar_wait_long(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
+__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
     const uint64_t began = nanoseconds();
     for (uint32_t i = 0; !mbar_try(bar, parity); ++i)
-        if (*failed || i == WAIT_TRIES || nanoseconds() - began > WAIT_NS) { *failed = 1; return; }
+        if (*failed || i == WAIT_TRIES || nanoseconds() - began > WAIT_NS) { *failed = 1; return false; }
+    return true;
 }
-__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
-    if (!mbar_try(bar, parity)) mbar_wait_long(bar, parity, failed);
-}
+// False: given up.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) { return mbar_try(bar, parity) || mbar_wait_long(bar, parity, failed); }
 // For a thread that has issued copies and will not see them land: time for them to.
 __device__ __forceinline__ void let_copies_land() {
     for (uint32_t i = 0; i < 65536; ++i) __nanosleep(64);
@@ -80,6 +80,7 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&v)[16]) {
 // Shared-memory descriptor of an operand in 128-byte swizzled lines, eight lines (1024 bytes) to a repeating unit.
 //   K-major: a line holds 64 k of one row; `stride` is from one unit of eight rows to the next (the other offset is unused).
 //   MN-major: a line holds 64 rows of one k; `lead` is from one unit of 64 rows to the next, `stride` from eight k to the next eight.
+// 16 bytes further on is one more.
 __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
     return uint64_t((addr & 0x3FFFF) >> 4) | uint64_t(lead >> 4) << 16 | uint64_t(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
