@@ -37,4 +37,10 @@ template <> __device__ __forceinline__ float token_value<uint8_t>(const TokenArg
     return t.scaled == SCALE_ROW ? v : v * e8m0_f32(static_cast<const uint8_t*>(t.scales)[m * (cols / 32) + k / 32]);
 }
 
+__device__ __forceinline__ void store_as(void* y, uint32_t dtype, uint64_t i, float v) {
+    if (dtype == DT_BF16) static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+    else if (dtype == DT_FP16) static_cast<__half*>(y)[i] = __float2half_rn(v);
+    else static_cast<float*>(y)[i] = v;
+}
+
 }  // namespace ptwm

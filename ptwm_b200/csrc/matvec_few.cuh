@@ -178,12 +178,6 @@ __device__ __forceinline__ uint32_t half2_mul(uint32_t a, uint32_t b) {
     return r;
 }
 
-__device__ __forceinline__ void store_as(void* y, uint32_t dtype, uint64_t i, float v) {
-    if (dtype == DT_BF16) static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
-    else if (dtype == DT_FP16) static_cast<__half*>(y)[i] = __float2half_rn(v);
-    else static_cast<float*>(y)[i] = v;
-}
-
 __device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])

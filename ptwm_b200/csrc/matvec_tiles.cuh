@@ -7,7 +7,14 @@
 // Tokens of other types are bf16 parts that add up to them: E4M3 is one, fp16 two, fp32 three (token_parts_kernel); each part is
 // multiplied with the same converted tile, and all sums meet in the same fp32 accumulator.  In the gradient the contraction
 // runs down the rows of the matrix, so the converted tile is MN-major: the same lines, another descriptor.
+//   Where tiles are fewer than SMs, the blocks of a cluster share a tile's contraction and add their sums over distributed shared
+// memory, in the order of their ranks.
+//   What a step costs: 512 cycles of MMA with 256 tokens; some 200 cycles of ALU in conversion; and the issuing thread, to which a wait
+// for a barrier is 170 cycles, a commit 100 and four MMAs 100, ready or not.  So a stage has one barrier for all that arrives in it and is
+// two steps where tokens are few.
 #pragma once
+#include <cooperative_groups.h>
+
 #include "matvec.cuh"
 #include "tensor_core.cuh"
 
@@ -15,7 +22,7 @@ namespace ptwm {
 
 constexpr uint32_t TILE_ROWS = 128;                 // rows of D to a block
 constexpr uint32_t STEP = 64;                       // contraction to a converted tile: one 128-byte line of bf16
-constexpr uint32_t RAW_STAGES = 6, RAW_BYTES = 8192, SCALES_BYTES = 8192, A_STAGES = 4, A_BYTES = TILE_ROWS * STEP * 2;
+constexpr uint32_t RAW_STAGES = 6, RAW_BYTES = 8192, SCALES_BYTES = 8192, A_BYTES = TILE_ROWS * STEP * 2, MOST_STAGES = 6;
 constexpr uint32_t TILES_THREADS = 640;             // warp 0: TMA of the matrix, 1: MMA, 2: TMA of the tokens, 4 to 19: conversion, then the results
 constexpr uint32_t TILES_HEAD = 1024;               // barriers and the like, in front of the buffers
 
@@ -26,18 +33,20 @@ struct TilesArgs {
     uint64_t part_rows;        // rows from one part of the tokens to the next
     uint32_t parts;
     uint32_t tile_tokens;      // a multiple of 16, at most 256
-    uint32_t b_stages;
+    uint32_t stages;           // of `together` converted tiles and the tokens that belong to them
+    uint32_t together;         // 1 or 2 steps
+    uint32_t teams;            // of four warps that convert: 4, and no more than the steps of all stages
     uint32_t group;
+    uint32_t y_dtype;
     const float* global_scale;
     const float* token_scale;  // or null
     void* y;
     uint32_t* status;
 };
 
+__host__ __device__ constexpr uint32_t tiles_stage(uint32_t tile_tokens, uint32_t parts, uint32_t together) { return together * (A_BYTES + parts * tile_tokens * STEP * 2); }
 // Bytes of dynamic shared memory; 1024 more to align them.
-inline uint32_t tiles_smem(uint32_t tile_tokens, uint32_t b_stages) {
-    return 1024 + TILES_HEAD + RAW_STAGES * RAW_BYTES + SCALES_BYTES + A_STAGES * A_BYTES + b_stages * tile_tokens * STEP * 2;
-}
+inline uint32_t tiles_smem(uint32_t stage, uint32_t stages) { return 1024 + TILES_HEAD + RAW_STAGES * RAW_BYTES + SCALES_BYTES + stages * stage; }
 
 // Eight nibbles -> eight bf16 in their order, times `scale`.  A word takes the even nibble of a byte to its low half and the odd one
 // to its high half; a product puts their signs at bit 15 and the other three bits at 8..6, which reads as the number times 2^-126;
@@ -68,11 +77,11 @@ __device__ __forceinline__ uint32_t nv_scale(uint32_t s) {
 constexpr float NV_REST = 1024.0f;
 
 template <bool GRAD> struct TilesShared {
-    static constexpr uint32_t raw = TILES_HEAD, scales = raw + RAW_STAGES * RAW_BYTES, a = scales + SCALES_BYTES, b = a + A_STAGES * A_BYTES;
+    static constexpr uint32_t raw = TILES_HEAD, scales = raw + RAW_STAGES * RAW_BYTES, stages = scales + SCALES_BYTES;
     static constexpr uint32_t raw_rows = GRAD ? STEP : TILE_ROWS, scale_bytes = raw_rows * 16, scale_slots = SCALES_BYTES / scale_bytes;
-    // barriers: raw full / empty, scales full (a slot is free once all raw stages before raw - RAW_STAGES are), a full / empty, b full / empty,
-    // accumulator full
-    static constexpr uint32_t raw_full = 0, raw_empty = 64, a_full = 128, a_empty = 192, b_full = 256, b_empty = 320, scales_full = 384, done = 448, tmem = 456, failed = 460;
+    // barriers: raw full / empty, scales full (a slot is free once all raw stages before raw - RAW_STAGES are), stage full / empty, accumulator full
+    static constexpr uint32_t raw_full = 0, raw_empty = 64, full = 128, empty = 192, scales_full = 256, done = 320, tmem = 328, failed = 332;
+    static_assert(RAW_STAGES <= 8 && MOST_STAGES <= 8 && scale_slots <= 8, "barriers do not overlap");
 };
 
 // 16 bytes of nibbles (32 values) -> four 16-byte pieces of bf16.  s: the scale of all (MXFP4), or of the first and the second half.
@@ -92,29 +101,35 @@ __device__ __forceinline__ void convert32(const uint4& v, uint32_t group, uint32
     }
 }
 
-template <class Y, bool GRAD>
+template <bool GRAD>
 __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __grid_constant__ CUtensorMap values, const __grid_constant__ CUtensorMap scales,
                                                                         const __grid_constant__ CUtensorMap tokens, const TilesArgs t) {
+    namespace cg = cooperative_groups;
     using S = TilesShared<GRAD>;
     extern __shared__ uint8_t dynamic[];
     uint8_t* base = dynamic + (1024 - (smem_u32(dynamic) & 1023)) % 1024;
     const uint32_t sb = smem_u32(base);
     volatile uint32_t* failed = reinterpret_cast<uint32_t*>(base + S::failed);
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const uint32_t row0 = blockIdx.x * TILE_ROWS, token0 = blockIdx.y * t.tile_tokens;
-    const uint32_t steps = uint32_t((t.contraction + STEP - 1) / STEP);
-    // A raw stage is 128 k of 128 rows (two steps) forward, and 64 rows (one step) of the tile's 128 k in the gradient.
-    const uint32_t raws = GRAD ? steps : (steps + 1) / 2;
-    // A box of scales is 16 bytes of each row: 512 k (MXFP4) or 256 (NVFP4), so several raw stages forward, one in the gradient.
-    const uint32_t scale_raws = GRAD ? 1 : t.group == 32 ? 4 : 2;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t row0 = blockIdx.x / ranks * TILE_ROWS, token0 = blockIdx.y * t.tile_tokens;
+    // A raw stage is 128 k of 128 rows (two steps) forward, and 64 rows (one step) of the tile's 128 k in the gradient.  A box of scales is
+    // 16 bytes of each row: 512 k (MXFP4) or 256 (NVFP4), so several raw stages forward, one in the gradient.
+    const uint32_t scale_raws = GRAD ? 1 : t.group == 32 ? 4 : 2, unit = GRAD ? t.together : 2 * scale_raws;
+    // this block's steps: whole boxes of scales, and whole stages
+    const uint32_t units = uint32_t((t.contraction + unit * STEP - 1) / (unit * STEP));
+    const uint32_t step0 = units * rank / ranks * unit, all = uint32_t((t.contraction + STEP - 1) / STEP), end = min(units * (rank + 1) / ranks * unit, all);
+    const uint32_t steps = (end > step0 ? end - step0 + t.together - 1 : 0) / t.together * t.together;  // what is behind the contraction is zeros
+    const uint32_t raw0 = GRAD ? step0 : step0 / 2, raws = GRAD ? steps : (steps + 1) / 2;
     const uint32_t cols = t.tile_tokens <= 32 ? 32 : t.tile_tokens <= 64 ? 64 : t.tile_tokens <= 128 ? 128 : 256;
-    const uint32_t b_bytes = t.tile_tokens * STEP * 2;
+    const uint32_t b_bytes = t.tile_tokens * STEP * 2, stage_bytes = tiles_stage(t.tile_tokens, t.parts, t.together);
 
     if (threadIdx.x == 0) {
         *failed = 0;
-        for (uint32_t i = 0; i < RAW_STAGES; ++i) { mbar_init(sb + S::raw_full + 8 * i, 1); mbar_init(sb + S::raw_empty + 8 * i, GRAD ? 4 : 8); }  // four warps for each of its steps
-        for (uint32_t i = 0; i < A_STAGES; ++i) { mbar_init(sb + S::a_full + 8 * i, 4); mbar_init(sb + S::a_empty + 8 * i, 1); }
-        for (uint32_t i = 0; i < t.b_stages; ++i) { mbar_init(sb + S::b_full + 8 * i, 1); mbar_init(sb + S::b_empty + 8 * i, 1); }
+        // four warps convert a step
+        for (uint32_t i = 0; i < RAW_STAGES; ++i) { mbar_init(sb + S::raw_full + 8 * i, 1); mbar_init(sb + S::raw_empty + 8 * i, GRAD ? 4 : 8); }
+        for (uint32_t i = 0; i < t.stages; ++i) { mbar_init(sb + S::full + 8 * i, 4 * t.together + 1); mbar_init(sb + S::empty + 8 * i, 1); }
         for (uint32_t i = 0; i < S::scale_slots; ++i) mbar_init(sb + S::scales_full + 8 * i, 1);
         mbar_init(sb + S::done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -125,20 +140,21 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(base + S::tmem);
 
+    // (counters instead of divisions in the warps of one thread: its latency is what they cost)
     if (warp == 0) {
         if (elect_one()) {
-            uint32_t st = 0, parity = 1, slot = 0, piece = 0, scale_x = GRAD ? row0 / t.group & ~15u : 0;
+            uint32_t st = 0, parity = 1, slot = 0, piece = 0, scale_x = GRAD ? row0 / t.group & ~15u : raw0 / scale_raws * 16;
             for (uint32_t raw = 0; raw < raws; ++raw) {
-                const uint32_t full = sb + S::raw_full + 8 * st;
+                const uint32_t full = sb + S::raw_full + 8 * st, dst = sb + S::raw + st * RAW_BYTES;
                 if (raw >= RAW_STAGES && !mbar_wait(sb + S::raw_empty + 8 * st, parity, failed)) break;
                 mbar_expect(full, S::raw_rows * 64);
-                if (GRAD) tma_load(sb + S::raw + st * RAW_BYTES, &values, full, int32_t(row0 / 2), int32_t(raw * STEP));
-                else tma_load(sb + S::raw + st * RAW_BYTES, &values, full, int32_t(raw * 64), int32_t(row0));
+                if (GRAD) tma_load(dst, &values, full, int32_t(row0 / 2), int32_t((raw0 + raw) * STEP));
+                else tma_load(dst, &values, full, int32_t((raw0 + raw) * 64), int32_t(row0));
                 if (piece == 0) {
                     // its slot was last read for raw stages before raw - RAW_STAGES: there are enough slots for those in between
                     const uint32_t bar = sb + S::scales_full + 8 * slot;
                     mbar_expect(bar, S::scale_bytes);
-                    tma_load(sb + S::scales + slot * S::scale_bytes, &scales, bar, int32_t(scale_x), int32_t(GRAD ? raw * STEP : row0));
+                    tma_load(sb + S::scales + slot * S::scale_bytes, &scales, bar, int32_t(scale_x), int32_t(GRAD ? (raw0 + raw) * STEP : row0));
                     if (!GRAD) scale_x += 16;
                     if (++slot == S::scale_slots) slot = 0;
                 }
@@ -150,65 +166,65 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
         }
     } else if (warp == 2) {
         if (elect_one()) {
-            // (counters instead of divisions: one thread's latency is what these two warps cost)
-            uint32_t st = 0, parity = 1, p = 0, step = 0;
-            for (uint32_t b = 0; b < steps * t.parts; ++b) {
-                const uint32_t full = sb + S::b_full + 8 * st;
-                if (b >= t.b_stages && !mbar_wait(sb + S::b_empty + 8 * st, parity, failed)) break;
-                mbar_expect(full, b_bytes);
-                tma_load(sb + S::b + st * b_bytes, &tokens, full, int32_t(step * STEP), int32_t(p * t.part_rows + token0));
-                if (++st == t.b_stages) { st = 0; parity ^= 1; }
-                if (++p == t.parts) { p = 0; ++step; }
+            uint32_t st = 0, parity = 1, round = 0;
+            for (uint32_t step = 0; step < steps; step += t.together) {
+                const uint32_t full = sb + S::full + 8 * st;
+                uint32_t dst = sb + S::stages + st * stage_bytes + t.together * A_BYTES;
+                if (round && !mbar_wait(sb + S::empty + 8 * st, parity, failed)) break;
+                mbar_expect(full, t.together * t.parts * b_bytes);
+                for (uint32_t i = 0; i < t.together; ++i)
+                    for (uint32_t p = 0; p < t.parts; ++p, dst += b_bytes) tma_load(dst, &tokens, full, int32_t((step0 + step + i) * STEP), int32_t(p * t.part_rows + token0));
+                if (++st == t.stages) { st = 0; parity ^= 1; round = 1; }
             }
             if (*failed) let_copies_land();
         }
     } else if (warp == 1) {
         if (elect_one()) {
             const uint32_t idesc = instruction_desc(t.tile_tokens, GRAD);
-            const uint64_t a_desc = operand_desc(sb + S::a, GRAD ? 8192 : 16, 1024), b_desc = operand_desc(sb + S::b, 16, 1024);
-            uint32_t as = 0, a_parity = 0, bs = 0, b_parity = 0;
-            bool more = false, ok = true;
-            for (uint32_t step = 0; step < steps && ok; ++step) {
-                ok = mbar_wait(sb + S::a_full + 8 * as, a_parity, failed);
-                const uint64_t ad = a_desc + as * (A_BYTES / 16);
-                for (uint32_t p = 0; p < t.parts && ok; ++p) {
-                    ok = mbar_wait(sb + S::b_full + 8 * bs, b_parity, failed);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t bd = b_desc + bs * (b_bytes / 16);
+            const uint64_t a_desc = operand_desc(sb + S::stages, GRAD ? 8192 : 16, 1024), b_desc = operand_desc(sb + S::stages + t.together * A_BYTES, 16, 1024);
+            uint32_t st = 0, parity = 0;
+            bool more = false;
+            for (uint32_t step = 0; step < steps; step += t.together) {
+                if (!mbar_wait(sb + S::full + 8 * st, parity, failed)) break;
+                tc_fence_after();
+                uint64_t ad = a_desc + st * (stage_bytes / 16), bd = b_desc + st * (stage_bytes / 16);
+                for (uint32_t i = 0; i < t.together; ++i, ad += A_BYTES / 16)
+                    for (uint32_t p = 0; p < t.parts; ++p, bd += b_bytes / 16) {
 #pragma unroll
-                    for (uint32_t k = 0; k < STEP / 16; ++k) {
-                        mma_f16(tmem, ad + k * (GRAD ? 2048 / 16 : 32 / 16), bd + k * 2, idesc, more);
-                        more = true;
+                        for (uint32_t k = 0; k < STEP / 16; ++k) {
+                            mma_f16(tmem, ad + k * (GRAD ? 2048 / 16 : 32 / 16), bd + k * 2, idesc, more);
+                            more = true;
+                        }
                     }
-                    tc_commit(sb + S::b_empty + 8 * bs);
-                    if (++bs == t.b_stages) { bs = 0; b_parity ^= 1; }
-                }
-                if (ok) tc_commit(sb + S::a_empty + 8 * as);
-                if (++as == A_STAGES) { as = 0; a_parity ^= 1; }
+                tc_commit(sb + S::empty + 8 * st);
+                if (++st == t.stages) { st = 0; parity ^= 1; }
             }
             tc_commit(sb + S::done);
         }
     } else if (warp >= 4) {
-        // Four groups of four warps take a step each in turn: a step is some 200 instructions of a thread in a row, and four of them are under way.
+        // Teams of four warps take a step each in turn: a step is some 200 instructions of a thread in a row, and up to four of them are under way.
+        // With no more teams than steps in all stages a team that waits for a stage to be free waits for its last use but one at most: two back, the
+        // parity of its barrier would say that it is free.
         // A thread has 32 bytes of a row (64 values of it): forward the step's part of row c, in the gradient one half of row c % 64.  TMA has swizzled
         // the 16-byte pieces of a raw stage's 64-byte rows, so that neighbouring rows lie in different banks, and they are stored swizzled.
         const uint32_t team = (warp - 4) / 4, c = threadIdx.x % 128, row = GRAD ? c % 64 : c, half = c / 64;
         const uint32_t first_group = GRAD ? row0 / t.group & 15u : 0;
         const uint32_t out = (GRAD ? half * 8192 : 0) + row / 8 * 1024 + row % 8 * 128;
-        for (uint32_t step = team; step < steps && !*failed; step += 4) {
-            const uint32_t raw = GRAD ? step : step / 2, st = raw % RAW_STAGES;
+        uint32_t st = team / t.together, round = 0;  // stage of the step, and how often the stages have been gone through
+        while (st >= t.stages) { st -= t.stages; ++round; }
+        for (uint32_t step = team; step < steps && team < t.teams; step += t.teams) {
+            const uint32_t raw = GRAD ? step : step / 2, rs = raw % RAW_STAGES;
             const uint32_t pair = GRAD ? half : step % 2;  // which 64 of the 128 k
-            mbar_wait(sb + S::raw_full + 8 * st, raw / RAW_STAGES & 1, failed);
-            const uint8_t* line = base + S::raw + st * RAW_BYTES + row * 64;
+            if (!mbar_wait(sb + S::raw_full + 8 * rs, raw / RAW_STAGES & 1, failed)) break;
+            const uint8_t* line = base + S::raw + rs * RAW_BYTES + row * 64;
             const uint4 v0 = *reinterpret_cast<const uint4*>(line + ((pair * 2 ^ row / 2) & 3) * 16), v1 = *reinterpret_cast<const uint4*>(line + ((pair * 2 + 1 ^ row / 2) & 3) * 16);
             const uint32_t scale_at = raw / scale_raws, slot = scale_at % S::scale_slots;
-            mbar_wait(sb + S::scales_full + 8 * slot, scale_at / S::scale_slots & 1, failed);
+            if (!mbar_wait(sb + S::scales_full + 8 * slot, scale_at / S::scale_slots & 1, failed)) break;
             const uint8_t* sp = base + S::scales + slot * S::scale_bytes + row * 16;
             const uint32_t g = first_group + raw % scale_raws * (128 / t.group) + pair * (64 / t.group);
             const uint32_t s = t.group == 32 ? *reinterpret_cast<const uint16_t*>(sp + g) : *reinterpret_cast<const uint32_t*>(sp + g);
-            if (step >= 4) mbar_wait(sb + S::a_empty + 8 * team, (step / 4 - 1) & 1, failed);
-            uint8_t* dst = base + S::a + team * A_BYTES + out;
+            if (round && !mbar_wait(sb + S::empty + 8 * st, (round - 1) & 1, failed)) break;
+            uint8_t* dst = base + S::stages + st * stage_bytes + step % t.together * A_BYTES + out;
             uint4 o[4];
             convert32(v0, t.group, s, o);
 #pragma unroll
@@ -219,9 +235,11 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
             fence_async_shared();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(sb + S::a_full + 8 * team);
-                mbar_arrive(sb + S::raw_empty + 8 * st);
+                mbar_arrive(sb + S::full + 8 * st);
+                mbar_arrive(sb + S::raw_empty + 8 * rs);
             }
+            st += t.teams / t.together;
+            while (st >= t.stages) { st -= t.stages; ++round; }
         }
         // results: a warp reaches the 32 lanes (rows of D) that its number modulo 4 names; the four teams share the tokens
         mbar_wait(sb + S::done, 0, failed);
@@ -231,21 +249,40 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
         float factor = t.group == 32 ? 1.0f : NV_REST;
         if (t.global_scale) factor *= *t.global_scale;
         if (*failed) factor = __uint_as_float(0x7FC00000u);
+        if (!steps) factor = 0;
+        float* const sums = reinterpret_cast<float*>(base + TILES_HEAD);  // [token][row]: nothing reads or writes the buffers any more
         for (uint32_t m = team * 16; m < t.tile_tokens; m += 64) {
             uint32_t v[16];
             tmem_load16(tmem + (lanes << 16) + m, v);
-            if (n < t.rows) {
+            if (ranks > 1) {
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) sums[(m + j) * TILE_ROWS + lanes + lane] = steps ? __uint_as_float(v[j]) * factor : 0.0f;
+            } else if (n < t.rows) {
 #pragma unroll
                 for (uint32_t j = 0; j < 16; ++j) {
                     const uint64_t token = token0 + m + j;
                     if (token < t.tokens) {
                         const float f = __uint_as_float(v[j]) * factor;
-                        static_cast<Y*>(t.y)[token * t.rows + n] = from_f32<Y>(t.token_scale ? f * t.token_scale[token] : f);
+                        store_as(t.y, t.y_dtype, token * t.rows + n, t.token_scale ? f * t.token_scale[token] : f);
                     }
                 }
             }
         }
         tc_fence_before();
+    }
+    if (ranks > 1) {
+        __syncwarp();
+        cluster.sync();
+        float* const sums = reinterpret_cast<float*>(base + TILES_HEAD);
+        const uint32_t r = threadIdx.x % TILE_ROWS;
+        const uint64_t n = row0 + r;
+        for (uint32_t m = t.tile_tokens * rank / ranks + threadIdx.x / TILE_ROWS; m < t.tile_tokens * (rank + 1) / ranks; m += TILES_THREADS / TILE_ROWS) {
+            float v = 0;
+            for (uint32_t i = 0; i < ranks; ++i) v += *cluster.map_shared_rank(sums + m * TILE_ROWS + r, i);
+            const uint64_t token = token0 + m;
+            if (n < t.rows && token < t.tokens) store_as(t.y, t.y_dtype, token * t.rows + n, t.token_scale ? v * t.token_scale[token] : v);
+        }
+        cluster.sync();  // nobody leaves while others read its sums
     }
     __syncthreads();
     if (warp == 1) {

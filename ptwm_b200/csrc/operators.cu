@@ -130,10 +130,6 @@ struct PerDevice { uint32_t* status = nullptr; bool attributes = false; };
 std::mutex g_devices_mu;
 std::map<int, PerDevice> g_devices;
 
-template <class Y, bool GRAD> cudaError_t allow_tiles() {
-    return cudaFuncSetAttribute(matvec_tiles_kernel<Y, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(tiles_smem(256, 3)));
-}
-
 // Once per device, with that device current.
 int64_t device_of(int device, PerDevice* out) {
     std::lock_guard<std::mutex> g(g_devices_mu);
@@ -143,12 +139,8 @@ int64_t device_of(int device, PerDevice* out) {
         CUDA_TRY(cudaGetSymbolAddress(&p, g_operator_status));
         d.status = static_cast<uint32_t*>(p);
         CUDA_TRY(allow_few());
-        CUDA_TRY((allow_tiles<float, false>()));
-        CUDA_TRY((allow_tiles<__half, false>()));
-        CUDA_TRY((allow_tiles<__nv_bfloat16, false>()));
-        CUDA_TRY((allow_tiles<float, true>()));
-        CUDA_TRY((allow_tiles<__half, true>()));
-        CUDA_TRY((allow_tiles<__nv_bfloat16, true>()));
+        CUDA_TRY(cudaFuncSetAttribute(matvec_tiles_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_MOST)));
+        CUDA_TRY(cudaFuncSetAttribute(matvec_tiles_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_MOST)));
         d.attributes = true;
     }
     *out = d;
@@ -188,6 +180,29 @@ Parts parts_of(uint64_t x, uint64_t tokens, uint64_t contraction, uint32_t dtype
     return {parts, pitch, parts * tokens * pitch * 2};
 }
 
+// How a product is cut into tiles.
+struct TilesSplit { uint32_t tile_tokens, ranks, stages, together; };
+TilesSplit tiles_split(uint64_t rows, uint64_t contraction, uint64_t tokens, uint32_t parts, bool grad, uint32_t group) {
+    constexpr uint32_t SMS = 148;
+    // as few tiles of tokens as 256 columns (128 where a stage holds parts) allow, all of a size
+    const uint64_t most = parts == 1 ? 256 : 128, across = (tokens + most - 1) / most;
+    const uint32_t tile_tokens = uint32_t(((tokens + across - 1) / across + 15) / 16 * 16);
+    // two steps to a stage where that leaves room for three
+    const uint32_t room = SMEM_MOST - tiles_smem(0, 0), together = 3 * tiles_stage(tile_tokens, parts, 2) <= room ? 2 : 1;
+    const uint32_t stages = std::min<uint32_t>(MOST_STAGES, room / tiles_stage(tile_tokens, parts, together));
+    // blocks of a cluster for a tile's contraction: rounds of blocks x (steps of one, and what a block costs besides, in steps)
+    const uint64_t tiles = (rows + TILE_ROWS - 1) / TILE_ROWS * across, steps = (contraction + STEP - 1) / STEP, unit = grad ? together : group == 32 ? 8 : 4;
+    uint32_t ranks = 1;
+    uint64_t least = ~0ull;
+    for (uint32_t r = 1; r <= 8; r *= 2) {
+        const uint64_t units = (steps + unit - 1) / unit, rounds = (tiles * r + SMS - 1) / SMS;
+        if (r > units) break;
+        const uint64_t cost = rounds * ((units + r - 1) / r * unit + (r == 1 ? 8 : 12));
+        if (cost < least) { least = cost; ranks = r; }
+    }
+    return {tile_tokens, ranks, stages, together};
+}
+
 template <bool GRAD>
 int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, int device, const PerDevice& dev, cudaStream_t st) {
     const uint64_t rows = GRAD ? w.cols : w.rows, contraction = GRAD ? w.rows : w.cols;
@@ -202,20 +217,26 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
         CUDA_TRY(cudaGetLastError());
         tokens = out;
     }
-    const uint64_t tiles = (x.tokens + 255) / 256;
-    TilesArgs t{rows, contraction, x.tokens, x.tokens, p.parts, uint32_t(((x.tokens + tiles - 1) / tiles + 15) / 16 * 16), 0, w.group, w.global_scale,
+    const TilesSplit split = tiles_split(rows, contraction, x.tokens, p.parts, GRAD, w.group);
+    TilesArgs t{rows, contraction, x.tokens, x.tokens, p.parts, split.tile_tokens, split.stages, split.together, std::min<uint32_t>(4, split.stages * split.together), w.group, y_dtype, w.global_scale,
                 x.scaled == SCALE_ROW ? static_cast<const float*>(x.scales) : nullptr, x.y, dev.status};
-    const uint32_t b_bytes = t.tile_tokens * STEP * 2;
-    t.b_stages = std::min<uint32_t>(8, 3 * 256 * STEP * 2 / b_bytes);
     CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
     CUtensorMap values, scales, tmap;
     int64_t rc = tensor_map(&values, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B, w.values, w.cols / 2, w.rows, w.value_pitch, 64, GRAD ? STEP : TILE_ROWS);
     if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 16, GRAD ? STEP : TILE_ROWS);
     if (rc == 0) rc = tensor_map(&tmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, tokens, contraction, p.parts * x.tokens, p.pitch * 2, STEP, t.tile_tokens);
     if (rc < 0) return rc;
-    const dim3 grid(uint32_t((rows + TILE_ROWS - 1) / TILE_ROWS), uint32_t((x.tokens + t.tile_tokens - 1) / t.tile_tokens));
-    with_type(y_dtype, [&](auto o) { matvec_tiles_kernel<decltype(o), GRAD><<<grid, TILES_THREADS, tiles_smem(t.tile_tokens, t.b_stages), st>>>(values, scales, tmap, t); });
-    CUDA_TRY(cudaGetLastError());
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim = {split.ranks, 1, 1};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(uint32_t((rows + TILE_ROWS - 1) / TILE_ROWS) * split.ranks, uint32_t((x.tokens + t.tile_tokens - 1) / t.tile_tokens));
+    cfg.blockDim = dim3(TILES_THREADS);
+    cfg.dynamicSmemBytes = tiles_smem(tiles_stage(t.tile_tokens, t.parts, t.together), t.stages);
+    cfg.stream = st;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, matvec_tiles_kernel<GRAD>, values, scales, tmap, t));
     return 0;
 }
 
