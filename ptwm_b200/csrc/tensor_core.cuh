@@ -33,8 +33,13 @@ __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volat
         if (*failed || i == WAIT_TRIES || nanoseconds() - began > WAIT_NS) { *failed = 1; return false; }
     return true;
 }
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
 // False: given up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) { return mbar_try(bar, parity) || mbar_wait_long(bar, parity, failed); }
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) { return mbar_test(bar, parity) || mbar_wait_long(bar, parity, failed); }
 // For a thread that has issued copies and will not see them land: time for them to.
 __device__ __forceinline__ void let_copies_land() {
     for (uint32_t i = 0; i < 65536; ++i) __nanosleep(64);

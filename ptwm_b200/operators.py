@@ -171,23 +171,27 @@ class ScaledWeight:
 # ---- rms_norm -------------------------------------------------------------------------------------
 def _norm(x, weight, residual, eps: float, quant: Optional[str]):
     """(y or ScaledActivations, h) of checked, contiguous tensors."""
-    cols = x.shape[-1]
+    shape = x.shape
+    cols = shape[-1]
     device = x.get_device()
-    rows = x.numel() // cols
-    h, residual_at = (x, 0) if residual is None else (torch.empty_like(x), residual.data_ptr())
+    if residual is None:
+        h, h_at, residual_at = x, 0, 0
+    else:
+        h = torch.empty_like(x)
+        h_at, residual_at = h.data_ptr(), residual.data_ptr()
     if quant is None:
-        y, out, scales_at = torch.empty_like(x), None, 0
-        y_at = y.data_ptr()
+        out = torch.empty_like(x)
+        y_at, scales_at = out.data_ptr(), 0
     else:
         values = torch.empty_like(x, dtype=torch.float8_e4m3fn)
-        if quant == "row":
-            scales = _new(x.shape[:-1], torch.float32, x.device)
-        else:
-            scales = _new((*x.shape[:-1], cols // 32), _E8M0, x.device)
-        out, y_at, scales_at = ScaledActivations._of(values, scales, quant), values.data_ptr(), scales.data_ptr()
-    _check(_lib.lib().ptwm_b200_rms_norm(x.data_ptr(), residual_at, weight.data_ptr(), h.data_ptr(), y_at, scales_at, rows, cols, _PLAIN[x.dtype], _PLAIN[weight.dtype],
-                                         _QUANT[quant], eps, device, _stream(device)))
-    return (y if out is None else out), h
+        scales = _new(shape[:-1], torch.float32, x.device) if quant == "row" else _new((*shape[:-1], cols // 32), _E8M0, x.device)
+        out = ScaledActivations._of(values, scales, quant)
+        y_at, scales_at = values.data_ptr(), scales.data_ptr()
+    rc = _lib.lib().ptwm_b200_rms_norm(x.data_ptr(), residual_at, weight.data_ptr(), h_at, y_at, scales_at, x.numel() // cols, cols, _PLAIN[x.dtype], _PLAIN[weight.dtype],
+                                       _QUANT[quant], eps, device, _stream(device))
+    if rc < 0:
+        _check(rc)
+    return out, h
 
 
 def _new(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
@@ -199,20 +203,26 @@ def _new(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     return torch.empty(shape, dtype=dtype, device=device)
 
 
+def _once() -> None:
+    if torch.is_grad_enabled():  # as it is in a backward pass with create_graph
+        raise RuntimeError("rms_norm and matvec have first derivatives only: their backward passes cannot be differentiated")
+
+
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         y, h = _norm(x, weight, residual, eps, None)
         ctx.save_for_backward(h, weight)
-        ctx.eps, ctx.has_residual = eps, residual is not None
+        ctx.eps = eps
         ctx.set_materialize_grads(False)
         return (y, h) if residual is not None else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh=None):
+        _once()
         h, weight = ctx.saved_tensors
-        need_x, need_w = ctx.needs_input_grad[0] or ctx.needs_input_grad[2], ctx.needs_input_grad[1]
+        for_x, need_w, for_residual, _ = ctx.needs_input_grad
+        need_x = for_x or for_residual
         if dy is None:  # only the residual stream was used
             dx = dh
             dw = torch.zeros_like(weight) if need_w and dh is not None else None
@@ -225,11 +235,11 @@ class _RmsNorm(torch.autograd.Function):
             dw = torch.empty_like(weight) if need_w else None
             L = _lib.lib()
             size = L.ptwm_b200_rms_norm_grad_scratch_bytes(rows, cols) if need_w else 0
-            scratch = torch.empty(size, dtype=torch.uint8, device=h.device) if size else None
+            scratch = _new((size,), torch.uint8, h.device) if size else None
             _check(L.ptwm_b200_rms_norm_grad(h.data_ptr(), weight.data_ptr(), dy.data_ptr(), 0 if dh is None else dh.data_ptr(), 0 if dx is None else dx.data_ptr(),
                                              0 if dw is None else dw.data_ptr(), 0 if scratch is None else scratch.data_ptr(), size, rows, cols, _PLAIN[h.dtype],
                                              _PLAIN[weight.dtype], ctx.eps, device, _stream(device)))
-        return (dx if ctx.needs_input_grad[0] else None), dw, (dx if ctx.has_residual and ctx.needs_input_grad[2] else None), None
+        return (dx if for_x else None), dw, (dx if for_residual else None), None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residual: Optional[torch.Tensor] = None, quant: Optional[str] = None):
@@ -244,43 +254,57 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residu
     that is not finite has NaN for scale and values.
 
     Without ``quant`` there are gradients for x, residual and weight."""
+    try:
+        device, dtype, shape = x.get_device(), x.dtype, x.shape
+        fine = (device >= 0 and weight.get_device() == device and dtype in _PLAIN and weight.dtype in _PLAIN and weight.shape == shape[-1:] and shape[-1] > 0
+                and quant in _QUANT and (quant != "block" or shape[-1] % 32 == 0)
+                and (residual is None or (residual.get_device() == device and residual.dtype is dtype and residual.shape == shape)))
+    except (AttributeError, IndexError, TypeError):
+        fine = False
+    if not fine:
+        _refuse_norm(x, weight, residual, quant)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        if quant is not None:
+            raise ValueError("an 8-bit output has no gradient: call under torch.no_grad() or detach the inputs")
+        return _RmsNorm.apply(x.contiguous(), weight.contiguous(), None if residual is None else residual.contiguous(), float(eps))
+    y, h = _norm(x.contiguous(), weight.contiguous(), None if residual is None else residual.contiguous(), eps, quant)
+    return y if residual is None else (y, h)
+
+
+def _refuse_norm(x, weight, residual, quant) -> None:
+    """What is wrong with the arguments of ``rms_norm``."""
     _on_cuda("x", x)
     _on_cuda("weight", weight, x.device)
     if x.dtype not in _PLAIN or weight.dtype not in _PLAIN:
         raise TypeError(f"x and weight are float32, float16 or bfloat16, got {x.dtype} and {weight.dtype}")
     if quant not in _QUANT:
         raise ValueError(f"quant is None, 'row' or 'block', got {quant!r}")
-    shape = x.shape
-    if not shape or shape[-1] == 0 or weight.shape != shape[-1:]:
-        raise ValueError(f"weight of shape {tuple(weight.shape)} does not fit rows of x, shape {tuple(shape)}")
-    if quant == "block" and shape[-1] % 32:
-        raise ValueError(f"block scales need whole blocks of 32 values, got rows of {shape[-1]}")
+    if not x.shape or x.shape[-1] == 0 or weight.shape != x.shape[-1:]:
+        raise ValueError(f"weight of shape {tuple(weight.shape)} does not fit rows of x, shape {tuple(x.shape)}")
+    if quant == "block" and x.shape[-1] % 32:
+        raise ValueError(f"block scales need whole blocks of 32 values, got rows of {x.shape[-1]}")
     if residual is not None:
         _on_cuda("residual", residual, x.device)
-        if residual.shape != shape or residual.dtype != x.dtype:
-            raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}, x {x.dtype} {tuple(shape)}; they have to be alike")
-    grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))
-    if grad and quant is not None:
-        raise ValueError("an 8-bit output has no gradient: call under torch.no_grad() or detach the inputs")
-    x, weight = x.contiguous(), weight.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    if grad:
-        return _RmsNorm.apply(x, weight, residual, float(eps))
-    y, h = _norm(x, weight, residual, eps, quant)
-    return y if residual is None else (y, h)
+        raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}, x {x.dtype} {tuple(x.shape)}; they have to be alike")
+    raise TypeError("rms_norm: unsuitable arguments")
 
 
 # ---- matvec ---------------------------------------------------------------------------------------
 def _product(x, scales, quant, weight: ScaledWeight, out_dtype: torch.dtype) -> torch.Tensor:
-    device, tokens, code = weight._ordinal, x.numel() // weight.cols, _PLAIN[x.dtype] if scales is None else _E4M3
-    y = _new((*x.shape[:-1], weight.rows), out_dtype, weight.device)
+    device, tokens, shape = weight._ordinal, x.numel() // weight.cols, x.shape
+    if scales is None:
+        code, scales_at = _PLAIN[x.dtype], 0
+    else:
+        code, scales_at = _E4M3, scales.data_ptr()
+    y = _new((shape[0], weight.rows) if len(shape) == 2 else (*shape[:-1], weight.rows), out_dtype, weight.device)
     # few tokens, and bf16 ones that lie well, need no scratch: it is asked for where the call says so
-    args = (weight._ref, x.data_ptr(), 0 if scales is None else scales.data_ptr(), y.data_ptr(), tokens, code, _QUANT[quant], _PLAIN[out_dtype])
+    args = (weight._ref, x.data_ptr(), scales_at, y.data_ptr(), tokens, code, _QUANT[quant], _PLAIN[out_dtype])
     rc = _lib.lib().ptwm_b200_matvec(*args, 0, 0, device, _stream(device))
-    if rc == _TOO_SMALL:
-        scratch = _scratch(weight, x, tokens, code, 0)
-        rc = _lib.lib().ptwm_b200_matvec(*args, scratch.data_ptr(), scratch.numel(), device, _stream(device))
-    _check(rc)
+    if rc < 0:
+        if rc == _TOO_SMALL:
+            scratch = _scratch(weight, x, tokens, code, 0)
+            rc = _lib.lib().ptwm_b200_matvec(*args, scratch.data_ptr(), scratch.numel(), device, _stream(device))
+        _check(rc)
     return y
 
 
@@ -295,8 +319,8 @@ class _Matvec(torch.autograd.Function):
         return _product(x, None, None, weight, out_dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once()
         w = ctx.weight
         dy = dy.to(ctx.dtype).contiguous()
         dx = torch.empty((*dy.shape[:-1], w.cols), dtype=ctx.dtype, device=dy.device)
@@ -316,23 +340,24 @@ def matvec(x, weight: ScaledWeight, *, out_dtype: Optional[torch.dtype] = None) 
     (x's type; bf16 for ScaledActivations).  The gradient goes back to a plain x; the matrix has none."""
     if not isinstance(weight, ScaledWeight):
         raise TypeError(f"weight is a ScaledWeight, got {type(weight).__name__}")
-    scales = quant = None
-    if isinstance(x, ScaledActivations):
+    if type(x) is ScaledActivations:
         scales, quant, x = x.scales, x.quant, x.values
         out_dtype = out_dtype or torch.bfloat16
         if not scales.is_contiguous():
             scales = scales.contiguous()
     else:
+        scales = quant = None
         _on_cuda("x", x)
         if x.dtype not in _PLAIN:
             raise TypeError(f"x is float32, float16, bfloat16 or ScaledActivations, got {x.dtype}")
         out_dtype = out_dtype or x.dtype
     if out_dtype not in _PLAIN:
         raise TypeError(f"out_dtype is float32, float16 or bfloat16, got {out_dtype}")
-    if x.device != weight.device:
+    if x.get_device() != weight._ordinal:
         raise ValueError(f"x lives on {x.device}, the weight on {weight.device}")
-    if not x.shape or x.shape[-1] != weight.cols:
-        raise ValueError(f"x of shape {tuple(x.shape)} does not fit a matrix of {weight.rows} x {weight.cols}")
+    shape = x.shape
+    if not shape or shape[-1] != weight.cols:
+        raise ValueError(f"x of shape {tuple(shape)} does not fit a matrix of {weight.rows} x {weight.cols}")
     if not x.is_contiguous():
         x = x.contiguous()
     if scales is None and x.requires_grad and torch.is_grad_enabled():

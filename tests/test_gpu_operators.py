@@ -229,6 +229,16 @@ def test_norm_gradient_of_one_output_and_of_some_inputs():
         rms_norm(x, w, quant="row")
 
 
+def test_second_derivatives_are_refused():
+    x, res, w = _inputs(3, 64, torch.float32, 1)
+    x.requires_grad_()
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        torch.autograd.grad(rms_norm(x, w).square().sum(), x, create_graph=True)
+    m = ScaledWeight(*_matrix(32, 64, "mxfp4", 1))
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        torch.autograd.grad(matvec(x, m).square().sum(), x, create_graph=True)
+
+
 # ---- matvec ------------------------------------------------------------------------------------------
 def _weight64(values, scales, top):
     codes = torch.stack((values & 15, values >> 4), -1).reshape(values.shape[0], -1)
