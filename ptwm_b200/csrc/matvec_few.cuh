@@ -241,6 +241,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
         return Run{tile_lo + first, all * w / FEW_WARPS, all * (w + 1) / FEW_WARPS};
     };
 
+    others_may_start();
+    after_those_before();
     // The tokens are asked for first, HOLD pieces of 256 values to a warp at a time, and those of a block with few stay in registers.
     constexpr int HOLD = sizeof(T) == 4 ? 2 : 4;
     const uint32_t pieces = a.tokens * block_n;

@@ -139,6 +139,8 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(base + S::tmem);
+    others_may_start();
+    after_those_before();
 
     // (counters instead of divisions in the warps of one thread: its latency is what they cost)
     if (warp == 0) {
@@ -299,6 +301,8 @@ template <class T>
 __global__ void __launch_bounds__(256) token_parts_kernel(TokenArgs t, uint64_t cols, __nv_bfloat16* out, uint32_t pitch, uint64_t part_rows) {
     constexpr int PARTS = sizeof(T) == 4 ? 3 : sizeof(T) == 1 ? 1 : std::is_same<T, __half>::value ? 2 : 1;
     const uint64_t m = blockIdx.x;
+    others_may_start();
+    after_those_before();
     for (uint64_t k = uint64_t(blockIdx.y) * 256 + threadIdx.x; k < pitch; k += uint64_t(gridDim.y) * 256) {
         float rest = k < cols ? token_value<T>(t, m, k, cols) : 0.0f;
         const bool finite = (__float_as_uint(rest) & 0x7F800000u) != 0x7F800000u;

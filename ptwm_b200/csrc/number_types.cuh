@@ -21,6 +21,12 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Programmatic dependent launch.  A kernel of these operators may start while the one before it in the stream ends: it does nothing but
+// find its place and make its barriers until after_those_before(), where all that was enqueued before it is done and can be seen.
+// The one behind it may start from others_may_start() on.
+__device__ __forceinline__ void others_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void after_those_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // 2^(e - 127) of an E8M0 code; 255 is NaN.  Code 0 is the subnormal 2^-127.
 __device__ __forceinline__ float e8m0_f32(uint32_t e) { return e == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float(e ? e << 23 : 0x00400000u); }
 

@@ -26,6 +26,23 @@ template <class F> void with_type(uint32_t t, F f) {
     else f(__nv_bfloat16());
 }
 
+// Enqueues a kernel that may start while the one before it in the stream ends (see after_those_before).
+template <class... P, class... A> cudaError_t enqueue(void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t smem, uint32_t ranks, cudaStream_t st, const A&... args) {
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim = {ranks, 1, 1};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attrs;
+    cfg.numAttrs = ranks > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 int64_t matrix_of(const ptwm_b200_scaled_weight* w, ScaledMatrix* out) {
     if (!w || !w->values || !w->scales) return fail(PTWM_RC_INVALID_INPUT, "scaled weight: null pointer");
     if (w->group != 16 && w->group != 32) return fail(PTWM_RC_INVALID_INPUT, "scaled weight: groups are 16 (E4M3 scales) or 32 (E8M0 scales) values");
@@ -84,7 +101,7 @@ uint32_t warps_for(uint64_t threads) { return uint32_t((threads + 31) / 32 * 32)
 
 // One piece of 16 bytes to a thread where rows are few and a call takes as long as one of them (one row of 4096 bf16: 512 threads), two
 // where there are many.  False: the rows are not made for it.
-template <class T, class W, uint32_t QUANT> bool launch_norm_rows(const NormArgs& a, cudaStream_t st) {
+template <class T, class W, uint32_t QUANT> bool launch_norm_rows(const NormArgs& a, cudaStream_t st, cudaError_t& e) {
     constexpr uint64_t V = 16 / sizeof(T);
     if (a.cols % V || !aligned(a.x) || !aligned(a.residual) || !aligned(a.weight) || !aligned(a.h) || !aligned(a.y)) return false;
     const uint64_t pieces = a.cols / V;
@@ -93,34 +110,38 @@ template <class T, class W, uint32_t QUANT> bool launch_norm_rows(const NormArgs
     // next ones after it.  Rows of up to 128 pieces to half a warp or a warp, all at once (200,000 rows of 128 bf16: 46 us, 51 in turns).
     auto blocks = [&](uint32_t threads) { return std::min<uint32_t>(rows, 148 * std::max(1u, 1024 / threads)); };
     if (pieces <= 128 && a.rows > 148) {
-        if (pieces <= 16) rms_norm_rows_kernel<T, W, 1, 16, QUANT><<<(rows + 15) / 16, 256, 0, st>>>(a);
-        else if (pieces <= 32) rms_norm_rows_kernel<T, W, 1, 32, QUANT><<<(rows + 7) / 8, 256, 0, st>>>(a);
-        else if (pieces <= 64) rms_norm_rows_kernel<T, W, 2, 32, QUANT><<<(rows + 7) / 8, 256, 0, st>>>(a);
-        else rms_norm_rows_kernel<T, W, 4, 32, QUANT><<<(rows + 7) / 8, 256, 0, st>>>(a);
-    } else if (pieces <= 1024 && a.rows <= 296) rms_norm_rows_kernel<T, W, 1, 0, QUANT><<<rows, warps_for(pieces), 0, st>>>(a);
-    else if (pieces <= 2048) rms_norm_rows_kernel<T, W, 2, 0, QUANT><<<blocks(warps_for((pieces + 1) / 2)), warps_for((pieces + 1) / 2), 0, st>>>(a);
+        if (pieces <= 16) e = enqueue(rms_norm_rows_kernel<T, W, 1, 16, QUANT>, dim3((rows + 15) / 16), 256, 0, 1, st, a);
+        else if (pieces <= 32) e = enqueue(rms_norm_rows_kernel<T, W, 1, 32, QUANT>, dim3((rows + 7) / 8), 256, 0, 1, st, a);
+        else if (pieces <= 64) e = enqueue(rms_norm_rows_kernel<T, W, 2, 32, QUANT>, dim3((rows + 7) / 8), 256, 0, 1, st, a);
+        else e = enqueue(rms_norm_rows_kernel<T, W, 4, 32, QUANT>, dim3((rows + 7) / 8), 256, 0, 1, st, a);
+    } else if (pieces <= 1024 && a.rows <= 296) e = enqueue(rms_norm_rows_kernel<T, W, 1, 0, QUANT>, dim3(rows), warps_for(pieces), 0, 1, st, a);
+    else if (pieces <= 2048) e = enqueue(rms_norm_rows_kernel<T, W, 2, 0, QUANT>, dim3(blocks(warps_for((pieces + 1) / 2))), warps_for((pieces + 1) / 2), 0, 1, st, a);
     else return false;
     return true;
 }
-template <class T, class W> void launch_norm(const NormArgs& a, uint32_t scaled, cudaStream_t st) {
+template <class T, class W> cudaError_t launch_norm(const NormArgs& a, uint32_t scaled, cudaStream_t st) {
     const uint32_t rows = uint32_t(a.rows);
-    if (scaled == SCALE_NONE ? launch_norm_rows<T, W, SCALE_NONE>(a, st) : scaled == SCALE_ROW ? launch_norm_rows<T, W, SCALE_ROW>(a, st) : launch_norm_rows<T, W, SCALE_BLOCK>(a, st)) return;
-    if (scaled != SCALE_BLOCK && a.cols <= 16 * 1024) rms_norm_odd_rows_kernel<T, W, 16><<<rows, warps_for((a.cols + 15) / 16), 0, st>>>(a, scaled);
-    else rms_norm_long_kernel<T, W><<<rows, 256, 0, st>>>(a, scaled);
+    cudaError_t e = cudaSuccess;
+    if (scaled == SCALE_NONE ? launch_norm_rows<T, W, SCALE_NONE>(a, st, e) : scaled == SCALE_ROW ? launch_norm_rows<T, W, SCALE_ROW>(a, st, e) : launch_norm_rows<T, W, SCALE_BLOCK>(a, st, e)) return e;
+    if (scaled != SCALE_BLOCK && a.cols <= 16 * 1024) e = enqueue(rms_norm_odd_rows_kernel<T, W, 16>, dim3(rows), warps_for((a.cols + 15) / 16), 0, 1, st, a, scaled);
+    else e = enqueue(rms_norm_long_kernel<T, W>, dim3(rows), 256, 0, 1, st, a, scaled);
+    return e;
 }
 
 // Blocks of a gradient: each writes its share of dweight, so no more than fill the GPU.
 uint32_t grad_blocks(uint64_t rows) { return uint32_t(std::min<uint64_t>(rows, 296)); }
 
-template <class T, class W> void launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
+template <class T, class W> cudaError_t launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
+    cudaError_t e;
     constexpr uint64_t V = 16 / sizeof(T);
     const bool wide = a.cols % V == 0 && aligned(a.h) && aligned(a.weight) && aligned(a.dy) && aligned(a.dh) && aligned(a.dx) && aligned(a.partial);
     const uint64_t pieces = a.cols / V;
-    if (wide && pieces <= 512) rms_norm_grad_rows_kernel<T, W, 1, 512><<<a.blocks, warps_for(pieces), 0, st>>>(a);
-    else if (wide && pieces <= 1024) rms_norm_grad_rows_kernel<T, W, 2, 512><<<a.blocks, warps_for((pieces + 1) / 2), 0, st>>>(a);
-    else if (wide && pieces <= 2048) rms_norm_grad_rows_kernel<T, W, 2, 1024><<<a.blocks, warps_for((pieces + 1) / 2), 0, st>>>(a);
-    else rms_norm_grad_long_kernel<T, W><<<a.blocks, 512, 0, st>>>(a);
-    if (a.dweight) rms_norm_grad_weight_kernel<W><<<uint32_t((a.cols + 31) / 32), 1024, 0, st>>>(a);
+    if (wide && pieces <= 512) e = enqueue(rms_norm_grad_rows_kernel<T, W, 1, 512>, dim3(a.blocks), warps_for(pieces), 0, 1, st, a);
+    else if (wide && pieces <= 1024) e = enqueue(rms_norm_grad_rows_kernel<T, W, 2, 512>, dim3(a.blocks), warps_for((pieces + 1) / 2), 0, 1, st, a);
+    else if (wide && pieces <= 2048) e = enqueue(rms_norm_grad_rows_kernel<T, W, 2, 1024>, dim3(a.blocks), warps_for((pieces + 1) / 2), 0, 1, st, a);
+    else e = enqueue(rms_norm_grad_long_kernel<T, W>, dim3(a.blocks), 512, 0, 1, st, a);
+    if (a.dweight && e == cudaSuccess) e = enqueue(rms_norm_grad_weight_kernel<W>, dim3(uint32_t((a.cols + 31) / 32)), 1024, 0, 1, st, a);
+    return e;
 }
 
 // Where a wait inside a kernel gave up, per device: read by ptwm_b200_operator_status.
@@ -212,9 +233,10 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     if (p.bytes) {
         auto* out = at<__nv_bfloat16>(scratch);
         const dim3 grid(uint32_t(x.tokens), uint32_t(std::min<uint64_t>((p.pitch + 255) / 256, 64)));
-        if (x_dtype == DT_E4M3) token_parts_kernel<uint8_t><<<grid, 256, 0, st>>>(x, contraction, out, uint32_t(p.pitch), x.tokens);
-        else with_type(x_dtype, [&](auto v) { token_parts_kernel<decltype(v)><<<grid, 256, 0, st>>>(x, contraction, out, uint32_t(p.pitch), x.tokens); });
-        CUDA_TRY(cudaGetLastError());
+        cudaError_t e;
+        if (x_dtype == DT_E4M3) e = enqueue(token_parts_kernel<uint8_t>, grid, 256, 0, 1, st, x, contraction, out, uint32_t(p.pitch), x.tokens);
+        else with_type(x_dtype, [&](auto v) { e = enqueue(token_parts_kernel<decltype(v)>, grid, 256, 0, 1, st, x, contraction, out, uint32_t(p.pitch), x.tokens); });
+        CUDA_TRY(e);
         tokens = out;
     }
     const TilesSplit split = tiles_split(rows, contraction, x.tokens, p.parts, GRAD, w.group);
@@ -226,17 +248,8 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 16, GRAD ? STEP : TILE_ROWS);
     if (rc == 0) rc = tensor_map(&tmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, tokens, contraction, p.parts * x.tokens, p.pitch * 2, STEP, t.tile_tokens);
     if (rc < 0) return rc;
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim = {split.ranks, 1, 1};
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(uint32_t((rows + TILE_ROWS - 1) / TILE_ROWS) * split.ranks, uint32_t((x.tokens + t.tile_tokens - 1) / t.tile_tokens));
-    cfg.blockDim = dim3(TILES_THREADS);
-    cfg.dynamicSmemBytes = tiles_smem(tiles_stage(t.tile_tokens, t.parts, t.together), t.stages);
-    cfg.stream = st;
-    cfg.attrs = &cluster;
-    cfg.numAttrs = 1;
-    CUDA_TRY(cudaLaunchKernelEx(&cfg, matvec_tiles_kernel<GRAD>, values, scales, tmap, t));
+    const dim3 grid(uint32_t((rows + TILE_ROWS - 1) / TILE_ROWS) * split.ranks, uint32_t((x.tokens + t.tile_tokens - 1) / t.tile_tokens));
+    CUDA_TRY(enqueue(matvec_tiles_kernel<GRAD>, grid, TILES_THREADS, tiles_smem(tiles_stage(t.tile_tokens, t.parts, t.together), t.stages), split.ranks, st, values, scales, tmap, t));
     return 0;
 }
 
@@ -250,18 +263,8 @@ int64_t launch_few(const ScaledMatrix& w, const TokenArgs& x, const FewSplit& s,
     int64_t rc = tensor_map(&values, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.values, w.cols / 2, w.rows, w.value_pitch, BOX_COLS / 2, 16);
     if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 128, s.most * 16);
     if (rc < 0) return rc;
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim = {s.ranks, 1, 1};
-    cfg.gridDim = dim3(s.blocks);
-    cfg.blockDim = dim3(FEW_WARPS * 32);
-    cfg.dynamicSmemBytes = s.smem;
-    cfg.stream = st;
-    cfg.attrs = &cluster;
-    cfg.numAttrs = 1;
     cudaError_t e = cudaSuccess;
-    with_few(x_dtype, tokens > 8, w.group == 32, [&](auto f) { e = cudaLaunchKernelEx(&cfg, f, values, scales, a); });
+    with_few(x_dtype, tokens > 8, w.group == 32, [&](auto f) { e = enqueue(f, dim3(s.blocks), FEW_WARPS * 32, s.smem, s.ranks, st, values, scales, a); });
     CUDA_TRY(e);
     return 0;
 }
@@ -287,8 +290,9 @@ extern "C" int64_t ptwm_b200_rms_norm(uint64_t x, uint64_t residual, uint64_t we
     DeviceGuard guard{int(device)};
     if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
     const NormArgs a{at<void>(x), at<void>(residual), at<void>(weight), at<void>(h), at<void>(y), at<void>(scales), rows, cols, eps};
-    with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { launch_norm<decltype(t), decltype(w)>(a, scaled, stream_of(stream)); }); });
-    CUDA_TRY(cudaGetLastError());
+    cudaError_t e;
+    with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { e = launch_norm<decltype(t), decltype(w)>(a, scaled, stream_of(stream)); }); });
+    CUDA_TRY(e);
     return 0;
 }
 
@@ -308,8 +312,9 @@ extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t
     }
     const uint32_t blocks = grad_blocks(rows);
     const NormGradArgs a{at<void>(h), at<void>(weight), at<void>(dy), at<void>(dh), at<void>(dx), dweight ? at<float>(scratch) : nullptr, at<void>(dweight), rows, cols, eps, blocks};
-    with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { launch_norm_grad<decltype(t), decltype(w)>(a, stream_of(stream)); }); });
-    CUDA_TRY(cudaGetLastError());
+    cudaError_t e;
+    with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { e = launch_norm_grad<decltype(t), decltype(w)>(a, stream_of(stream)); }); });
+    CUDA_TRY(e);
     return 0;
 }
 

@@ -152,6 +152,8 @@ __global__ void __launch_bounds__(LANES ? 256 : 1024) rms_norm_rows_kernel(NormA
             }
         }
     };
+    others_may_start();
+    after_those_before();
     ask(row);
     // (two rows of a warp go on together: the shuffles want both)
     for (uint32_t turn = 0; LANES == 16 ? __any_sync(0xFFFFFFFFu, row < a.rows) : row < a.rows; row += step, turn ^= 1) {
@@ -237,6 +239,8 @@ __global__ void __launch_bounds__(1024) rms_norm_odd_rows_kernel(NormArgs a, uin
     const uint64_t first = uint64_t(blockIdx.x) * cols;
     const T *x = static_cast<const T*>(a.x) + first, *res = static_cast<const T*>(a.residual) + first;
     const W* w = static_cast<const W*>(a.weight);
+    others_may_start();
+    after_those_before();
     float t[N], sum = 0, most = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -282,6 +286,8 @@ __global__ void __launch_bounds__(256) rms_norm_long_kernel(NormArgs a, uint32_t
     const T* res = a.residual ? static_cast<const T*>(a.residual) + row * cols : nullptr;
     T* h = a.residual ? static_cast<T*>(a.h) + row * cols : nullptr;
     const W* w = static_cast<const W*>(a.weight);
+    others_may_start();
+    after_those_before();
     float sum = 0, most = 0;
     for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) {
         float v = to_f32(x[k]);
@@ -347,6 +353,8 @@ __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kerne
         for (int k = 0; k < V; ++k) w[k] = 0;
         if (at + j * lanes < pieces) weights<T, W>(a.weight, at + j * lanes, w);
     };
+    others_may_start();
+    after_those_before();
     if (N == 1) weights_of(0, kept[0]);
     if (MOST <= 512) ask(blockIdx.x);
     uint32_t turn = 0;
@@ -404,6 +412,8 @@ __global__ void __launch_bounds__(512) rms_norm_grad_long_kernel(NormGradArgs a)
     const uint64_t cols = a.cols;
     const W* w = static_cast<const W*>(a.weight);
     float* part = a.partial ? a.partial + blockIdx.x * cols : nullptr;
+    others_may_start();
+    after_those_before();
     if (part) for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) part[k] = 0;
     uint32_t turn = 0;
     for (uint64_t row = blockIdx.x; row < a.rows; row += a.blocks, turn ^= 1) {
@@ -433,6 +443,8 @@ template <class W> __global__ void __launch_bounds__(1024) rms_norm_grad_weight_
     __shared__ float runs[32][33];
     const uint64_t k = uint64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
     const uint32_t run = threadIdx.x / 32;
+    others_may_start();
+    after_those_before();
     float sum = 0;
     if (k < a.cols)
         for (uint32_t b = a.blocks * run / 32; b < a.blocks * (run + 1) / 32; ++b) sum += a.partial[b * a.cols + k];
