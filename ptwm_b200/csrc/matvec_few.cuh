@@ -241,23 +241,6 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
         return Run{tile_lo + first, all * w / FEW_WARPS, all * (w + 1) / FEW_WARPS};
     };
 
-    others_may_start();
-    after_those_before();
-    // The tokens are asked for first, HOLD pieces of 256 values to a warp at a time, and those of a block with few stay in registers.
-    constexpr int HOLD = sizeof(T) == 4 ? 2 : 4;
-    const uint32_t pieces = a.tokens * block_n;
-    Eight<T> held[HOLD];
-    auto fetch = [&](uint32_t from) {
-#pragma unroll
-        for (int j = 0; j < HOLD; ++j) {
-            const uint32_t i = from + j * FEW_WARPS, token = over_n(i);
-            const uint64_t k = uint64_t(block_lo + i - token * block_n) * BOX_COLS + lane * 8;
-            held[j] = Eight<T>{};
-            if (i < pieces && k < a.cols) held[j] = load8<T>(a, token, k);
-        }
-    };
-    fetch(warp);
-
     const uint32_t bars = smem_u32(base) + warp * a.depth * 8;
     const uint32_t boxes_at = smem_u32(ring) + warp * a.depth * BOX_BYTES;
     // scales of a turn's rows, 16-byte pieces swizzled as those of the boxes
@@ -295,15 +278,37 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
         }
         return true;
     };
-    // until the passes are known only the first one of the first turn is asked for
-    uint32_t under_way = 0;
+    // HOLD pieces of 256 values of the tokens to a warp at a time; those of a block with few stay in registers.
+    constexpr int HOLD = sizeof(T) == 4 ? 4 : 8;
+    const uint32_t pieces = a.tokens * block_n;
+    Eight<T> held[HOLD];
+    auto fetch = [&](uint32_t from) {
+#pragma unroll
+        for (int j = 0; j < HOLD; ++j) {
+            const uint32_t i = from + j * FEW_WARPS;
+            held[j] = Eight<T>{};
+            if (i >= pieces) continue;
+            const uint32_t token = over_n(i);
+            const uint64_t k = uint64_t(block_lo + i - token * block_n) * BOX_COLS + lane * 8;
+            if (k < a.cols) held[j] = load8<T>(a, token, k);
+        }
+    };
     if (lane == 0) {
         for (uint32_t i = 0; i < a.depth; ++i) mbar_init(bars + 8 * i, 1);
         if (warp == 0) { *failed = 0; mbar_init(scales_bar, 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
+    }
+    __syncwarp();
+    others_may_start();
+    after_those_before();
+    fetch(warp);
+    // Until the passes are known only the first one of the first turn is asked for, and before the tokens are staged two boxes of it: what a warp's
+    // requests wait for one another (24 cycles each, sixteen warps) the tokens would wait for too.
+    uint32_t under_way = 0;
+    if (lane == 0) {
         if (warp == 0) load_scales(0);
-        for (; under_way < a.depth && ask_left; ++under_way) load();
+        for (; under_way < 2 && ask_left; ++under_way) load();
     }
     __syncwarp();
 
@@ -315,9 +320,15 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
             if (from != warp) fetch(from);
 #pragma unroll
             for (int j = 0; j < HOLD; ++j) {
-                const uint32_t i = from + j * FEW_WARPS, token = over_n(i);
-                const uint64_t k = uint64_t(block_lo + i - token * block_n) * BOX_COLS + lane * 8;
-                if (i < pieces && k < a.cols) extremes8<T>(held[j], block_of<T>(a, token, k), x);
+                const uint32_t i = from + j * FEW_WARPS;
+                if (i >= pieces) break;
+                if (sizeof(T) == 1) {
+                    const uint32_t token = over_n(i);
+                    const uint64_t k = uint64_t(block_lo + i - token * block_n) * BOX_COLS + lane * 8;
+                    if (k < a.cols) extremes8<T>(held[j], block_of<T>(a, token, k), x);
+                } else {
+                    extremes8<T>(held[j], 1.0f, x);  // what is behind the columns is zeros
+                }
             }
         }
         x.most = __reduce_max_sync(0xFFFFFFFFu, x.most);
@@ -332,8 +343,6 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
     const int up0 = min(126, 141 - int(largest >> 23));
     const int bottom = largest ? max(int(smallest >> 23), 1) - 127 + up0 - (smallest >> 23 ? 0 : 23) : 0;
     const uint32_t passes = 1 + (bottom < FLOOR ? uint32_t(FLOOR - bottom + FINER * PARTS - 1) / (FINER * PARTS) : 0);
-    if (lane == 0)
-        for (; under_way < a.depth && goes_on(passes); ++under_way) load();
 
     const uint32_t part_bytes = a.tokens * a.pitch;
     auto stage = [&](uint32_t pass) {  // the parts of a pass of the tokens to shared memory
@@ -368,6 +377,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
         __syncthreads();
     };
     if (passes == 1) stage(0);
+    if (lane == 0)
+        for (; under_way < a.depth && goes_on(passes); ++under_way) load();
 
     uint32_t tokens_at[NT];
 #pragma unroll
