@@ -5,8 +5,10 @@
 // TMA brings boxes of nibbles and scales, sixteen warps turn them into bf16 (exactly: a nibble times its scale has at most six
 // significant bits) in the swizzled lines the tensor cores read, and one thread issues the MMAs.  Tokens come as bf16 by TMA.
 // Tokens of other types are bf16 parts that add up to them: E4M3 is one, fp16 two, fp32 three (token_parts_kernel); each part is
-// multiplied with the same converted tile, and all sums meet in the same fp32 accumulator.  In the gradient the contraction
-// runs down the rows of the matrix, so the converted tile is MN-major: the same lines, another descriptor.
+// multiplied with the same converted tile, and all sums meet in the same fp32 accumulator.
+//   Forward, a converted tile goes to tensor memory, whose lanes are the rows that the threads convert.  In shared memory it would be
+// written and read beside the tokens, 128 bytes a cycle for all: with 256 tokens that is 830 cycles for a step whose MMAs take 512.
+// In the gradient the contraction runs down the rows of the matrix, and the tile lies in shared memory as an MN-major operand.
 //   Where tiles are fewer than SMs, the blocks of a cluster share a tile's contraction and add their sums over distributed shared
 // memory, in the order of their ranks.
 //   What a step costs: 512 cycles of MMA with 256 tokens; some 200 cycles of ALU in conversion; and the issuing thread, to which a wait
@@ -44,9 +46,15 @@ struct TilesArgs {
     uint32_t* status;
 };
 
-__host__ __device__ constexpr uint32_t tiles_stage(uint32_t tile_tokens, uint32_t parts, uint32_t together) { return together * (A_BYTES + parts * tile_tokens * STEP * 2); }
+__host__ __device__ constexpr uint32_t tiles_stage(uint32_t tile_tokens, uint32_t parts, uint32_t together, bool grad) {
+    return together * ((grad ? A_BYTES : 0) + parts * tile_tokens * STEP * 2);
+}
 // Bytes of dynamic shared memory; 1024 more to align them.
 inline uint32_t tiles_smem(uint32_t stage, uint32_t stages) { return 1024 + TILES_HEAD + RAW_STAGES * RAW_BYTES + SCALES_BYTES + stages * stage; }
+// A block has an SM to itself: two that wait for tensor memory on each other's could wait for good.
+constexpr uint32_t TILES_LEAST_SMEM = 120 * 1024;
+constexpr uint32_t TMEM_COLS = 512, A_COLS = STEP / 2;   // columns of tensor memory; of a converted tile in it
+inline uint32_t tiles_tmem_stages(uint32_t tile_tokens, uint32_t together) { return (TMEM_COLS - (tile_tokens + 31) / 32 * 32) / (together * A_COLS); }
 
 // Eight nibbles -> eight bf16 in their order, times `scale`.  A word takes the even nibble of a byte to its low half and the odd one
 // to its high half; a product puts their signs at bit 15 and the other three bits at 8..6, which reads as the number times 2^-126;
@@ -122,8 +130,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
     const uint32_t step0 = units * rank / ranks * unit, all = uint32_t((t.contraction + STEP - 1) / STEP), end = min(units * (rank + 1) / ranks * unit, all);
     const uint32_t steps = (end > step0 ? end - step0 + t.together - 1 : 0) / t.together * t.together;  // what is behind the contraction is zeros
     const uint32_t raw0 = GRAD ? step0 : step0 / 2, raws = GRAD ? steps : (steps + 1) / 2;
-    const uint32_t cols = t.tile_tokens <= 32 ? 32 : t.tile_tokens <= 64 ? 64 : t.tile_tokens <= 128 ? 128 : 256;
-    const uint32_t b_bytes = t.tile_tokens * STEP * 2, stage_bytes = tiles_stage(t.tile_tokens, t.parts, t.together);
+    const uint32_t b_bytes = t.tile_tokens * STEP * 2, stage_bytes = tiles_stage(t.tile_tokens, t.parts, t.together, GRAD), b_first = GRAD ? t.together * A_BYTES : 0;
 
     if (threadIdx.x == 0) {
         *failed = 0;
@@ -134,11 +141,12 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
         mbar_init(sb + S::done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tmem_alloc(sb + S::tmem, cols);
+    if (warp == 1) tmem_alloc(sb + S::tmem, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(base + S::tmem);
+    const uint32_t a_tmem = tmem + (t.tile_tokens + 31) / 32 * 32;  // converted tiles behind the sums
     others_may_start();
     after_those_before();
 
@@ -171,7 +179,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
             uint32_t st = 0, parity = 1, round = 0;
             for (uint32_t step = 0; step < steps; step += t.together) {
                 const uint32_t full = sb + S::full + 8 * st;
-                uint32_t dst = sb + S::stages + st * stage_bytes + t.together * A_BYTES;
+                uint32_t dst = sb + S::stages + st * stage_bytes + b_first;
                 if (round && !mbar_wait(sb + S::empty + 8 * st, parity, failed)) break;
                 mbar_expect(full, t.together * t.parts * b_bytes);
                 for (uint32_t i = 0; i < t.together; ++i)
@@ -183,18 +191,20 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
     } else if (warp == 1) {
         if (elect_one()) {
             const uint32_t idesc = instruction_desc(t.tile_tokens, GRAD);
-            const uint64_t a_desc = operand_desc(sb + S::stages, GRAD ? 8192 : 16, 1024), b_desc = operand_desc(sb + S::stages + t.together * A_BYTES, 16, 1024);
+            const uint64_t a_desc = operand_desc(sb + S::stages, 8192, 1024), b_desc = operand_desc(sb + S::stages + b_first, 16, 1024);
             uint32_t st = 0, parity = 0;
             bool more = false;
             for (uint32_t step = 0; step < steps; step += t.together) {
                 if (!mbar_wait(sb + S::full + 8 * st, parity, failed)) break;
                 tc_fence_after();
                 uint64_t ad = a_desc + st * (stage_bytes / 16), bd = b_desc + st * (stage_bytes / 16);
-                for (uint32_t i = 0; i < t.together; ++i, ad += A_BYTES / 16)
+                uint32_t at = a_tmem + st * t.together * A_COLS;
+                for (uint32_t i = 0; i < t.together; ++i, ad += A_BYTES / 16, at += A_COLS)
                     for (uint32_t p = 0; p < t.parts; ++p, bd += b_bytes / 16) {
 #pragma unroll
                         for (uint32_t k = 0; k < STEP / 16; ++k) {
-                            mma_f16(tmem, ad + k * (GRAD ? 2048 / 16 : 32 / 16), bd + k * 2, idesc, more);
+                            if (GRAD) mma_f16(tmem, ad + k * (2048 / 16), bd + k * 2, idesc, more);
+                            else mma_f16_tmem(tmem, at + k * 8, bd + k * 2, idesc, more);
                             more = true;
                         }
                     }
@@ -208,10 +218,10 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
         // With no more teams than steps in all stages a team that waits for a stage to be free waits for its last use but one at most: two back, the
         // parity of its barrier would say that it is free.
         // A thread has 32 bytes of a row (64 values of it): forward the step's part of row c, in the gradient one half of row c % 64.  TMA has swizzled
-        // the 16-byte pieces of a raw stage's 64-byte rows, so that neighbouring rows lie in different banks, and they are stored swizzled.
+        // the 16-byte pieces of a raw stage's 64-byte rows, so that neighbouring rows lie in different banks, and in shared memory they are stored swizzled.
         const uint32_t team = (warp - 4) / 4, c = threadIdx.x % 128, row = GRAD ? c % 64 : c, half = c / 64;
         const uint32_t first_group = GRAD ? row0 / t.group & 15u : 0;
-        const uint32_t out = (GRAD ? half * 8192 : 0) + row / 8 * 1024 + row % 8 * 128;
+        const uint32_t out = half * 8192 + row / 8 * 1024 + row % 8 * 128;
         uint32_t st = team / t.together, round = 0;  // stage of the step, and how often the stages have been gone through
         while (st >= t.stages) { st -= t.stages; ++round; }
         for (uint32_t step = team; step < steps && team < t.teams; step += t.teams) {
@@ -226,15 +236,29 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
             const uint32_t g = first_group + raw % scale_raws * (128 / t.group) + pair * (64 / t.group);
             const uint32_t s = t.group == 32 ? *reinterpret_cast<const uint16_t*>(sp + g) : *reinterpret_cast<const uint32_t*>(sp + g);
             if (round && !mbar_wait(sb + S::empty + 8 * st, (round - 1) & 1, failed)) break;
-            uint8_t* dst = base + S::stages + st * stage_bytes + step % t.together * A_BYTES + out;
             uint4 o[4];
-            convert32(v0, t.group, s, o);
+            if constexpr (GRAD) {
+                uint8_t* dst = base + S::stages + st * stage_bytes + step % t.together * A_BYTES + out;
+                convert32(v0, t.group, s, o);
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + ((j ^ (row % 8)) * 16)) = o[j];
-            convert32(v1, t.group, t.group == 32 ? s >> 8 : s >> 16, o);
+                for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + ((j ^ (row % 8)) * 16)) = o[j];
+                convert32(v1, t.group, t.group == 32 ? s >> 8 : s >> 16, o);
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + ((4 + j ^ (row % 8)) * 16)) = o[j];
-            fence_async_shared();
+                for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + ((4 + j ^ (row % 8)) * 16)) = o[j];
+                fence_async_shared();
+            } else {
+                tc_fence_after();  // the MMAs that read what was here before are done
+                const uint32_t at = a_tmem + (warp % 4 * 32 << 16) + (st * t.together + step % t.together) * A_COLS;
+                uint32_t v[16];
+                convert32(v0, t.group, s, o);
+                memcpy(v, o, 64);
+                tmem_store16(at, v);
+                convert32(v1, t.group, t.group == 32 ? s >> 8 : s >> 16, o);
+                memcpy(v, o, 64);
+                tmem_store16(at + 16, v);
+                tmem_wait_stores();
+                tc_fence_before();
+            }
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(sb + S::full + 8 * st);
@@ -289,7 +313,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_free(tmem, cols);
+        tmem_free(tmem, TMEM_COLS);
     }
     if (threadIdx.x == 0 && *failed) atomicExch(t.status, 1u);
 }

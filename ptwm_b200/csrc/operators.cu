@@ -211,8 +211,9 @@ TilesSplit tiles_split(uint64_t rows, uint64_t contraction, uint64_t tokens, uin
     const uint64_t most = parts == 1 ? 256 : 128, across = (tokens + most - 1) / most;
     const uint32_t tile_tokens = uint32_t(((tokens + across - 1) / across + 15) / 16 * 16);
     // two steps to a stage where that leaves room for three
-    const uint32_t room = SMEM_MOST - tiles_smem(0, 0), together = 3 * tiles_stage(tile_tokens, parts, 2) <= room ? 2 : 1;
-    const uint32_t stages = std::min<uint32_t>(MOST_STAGES, room / tiles_stage(tile_tokens, parts, together));
+    const uint32_t room = SMEM_MOST - tiles_smem(0, 0), together = 3 * tiles_stage(tile_tokens, parts, 2, grad) <= room ? 2 : 1;
+    uint32_t stages = std::min<uint32_t>(MOST_STAGES, room / tiles_stage(tile_tokens, parts, together, grad));
+    if (!grad) stages = std::min(stages, tiles_tmem_stages(tile_tokens, together));
     // blocks of a cluster for a tile's contraction: rounds of blocks x (steps of one, and what a block costs besides, in steps)
     const uint64_t tiles = (rows + TILE_ROWS - 1) / TILE_ROWS * across, steps = (contraction + STEP - 1) / STEP, unit = grad ? together : group == 32 ? 8 : 4;
     uint32_t ranks = 1;
@@ -251,7 +252,7 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     if (rc == 0) rc = tensor_map(&tmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, tokens, contraction, p.parts * x.tokens, p.pitch * 2, STEP, t.tile_tokens);
     if (rc < 0) return rc;
     const dim3 grid(uint32_t((rows + TILE_ROWS - 1) / TILE_ROWS) * split.ranks, uint32_t((x.tokens + t.tile_tokens - 1) / t.tile_tokens));
-    CUDA_TRY(enqueue(matvec_tiles_kernel<GRAD>, grid, TILES_THREADS, tiles_smem(tiles_stage(t.tile_tokens, t.parts, t.together), t.stages), split.ranks, st, values, scales, tmap, t));
+    CUDA_TRY(enqueue(matvec_tiles_kernel<GRAD>, grid, TILES_THREADS, std::max(TILES_LEAST_SMEM, tiles_smem(tiles_stage(t.tile_tokens, t.parts, t.together, GRAD), t.stages)), split.ranks, st, values, scales, tmap, t));
     return 0;
 }
 
