@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(LANES ? 256 : 1024) rms_norm_rows_kernel(NormA
 
 // Rows that start anywhere, a value at a time: N values to a thread, a row to a block.
 template <class T, class W, int N>
-__global__ void __launch_bounds__(1024) rms_norm_odd_rows_kernel(NormArgs a, uint32_t quant) {
+__global__ void __launch_bounds__(1024, 2) rms_norm_odd_rows_kernel(NormArgs a, uint32_t quant) {
     __shared__ __align__(16) float shared[2][32];
     const uint32_t cols = uint32_t(a.cols), lanes = blockDim.x;
     const uint64_t first = uint64_t(blockIdx.x) * cols;

@@ -387,4 +387,6 @@ class Projection:
     def __call__(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> tuple[list[torch.Tensor], torch.Tensor]:
         got = rms_norm(x, self.norm, self.eps, residual=residual, quant=self.quant)
         y, h = (got, x) if residual is None else got
-        return [matvec(y, w, out_dtype=x.dtype) for w in self.weights], h
+        if self.quant is not None:  # checked, contiguous and without a gradient
+            return [_product(y.values, y.scales, self.quant, w, x.dtype) for w in self.weights], h
+        return [matvec(y, w) for w in self.weights], h
