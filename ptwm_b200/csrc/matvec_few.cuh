@@ -200,11 +200,40 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
     return v;
 }
 
-// NT: groups of eight tokens.  MX: E8M0 scales per 32 columns, else E4M3 per 16.
-template <class T, int NT, bool MX>
+__device__ __forceinline__ uint32_t lds16(uint32_t at) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+// Where a == b; v stays as it is elsewhere.
+__device__ __forceinline__ void lds128_where(uint4& v, uint32_t at, uint32_t a, uint32_t b) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.u32 p, %5, %6;\n\t@p ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "r"(at), "r"(a), "r"(b));
+}
+// Two scales, the first in the lower byte.
+template <bool MX> __device__ __forceinline__ float2 scale_pair(uint32_t two) {
+    if (!MX) return half2_floats(e4m3x2_half2(two));
+    uint32_t pair;
+    asm("{\n\t.reg .b16 e;\n\tcvt.u16.u32 e, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, e;\n\t}" : "=r"(pair) : "r"(two));
+    return make_float2(__uint_as_float(pair << 16), __uint_as_float(pair & 0xFFFF0000u));
+}
+
+// TOKENS: at most so many, 1, 2, 8 or 16.  MX: E8M0 scales per 32 columns, else E4M3 per 16.
+//   With one token or two the eight columns of an MMA are 8 / TOKENS groups of the matrix for each: a lane has the tokens' values only where
+// the group is its column's, and zeros elsewhere (E2M1 has no infinities to multiply them with).  So one MMA after the other adds to the
+// same sums, and their scales are wanted once for eight groups or four: 185 instructions to a box with one token, 280 with eight.
+template <class T, int TOKENS, bool MX>
 __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __grid_constant__ CUtensorMap values, const __grid_constant__ CUtensorMap scales, const FewArgs a) {
     namespace cg = cooperative_groups;
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;       // kept side by side
+    constexpr int NT = TOKENS > 8 ? 2 : 1, P = TOKENS < 8 ? TOKENS : 8;
+    constexpr bool SPREAD = P < 8;
+    static_assert(!SPREAD || PARTS == 1, "values in one part only are spread");
+    constexpr int GROUPS = 8 / P, PERIOD = SPREAD ? (MX ? GROUPS : GROUPS / 2) : 1;  // groups side by side, and the chunks of 32 columns that have them
     constexpr int FINER = sizeof(T) == 4 ? 12 : 39;     // powers of two from one part to the next
     // from which power on, after scaling, values of the type are exact in the parts of a pass (fp32: to 2^-23)
     constexpr int FLOOR = sizeof(T) == 4 || std::is_same<T, __half>::value ? -14 : sizeof(T) == 1 ? -21 : -17;
@@ -382,7 +411,12 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
 
     uint32_t tokens_at[NT];
 #pragma unroll
-    for (int m = 0; m < NT; ++m) tokens_at[m] = smem_u32(xs) + min(m * 8 + g, a.tokens - 1) * a.pitch + t * 16;
+    for (int m = 0; m < NT; ++m) tokens_at[m] = smem_u32(xs) + min(SPREAD ? g % P : m * 8 + g, a.tokens - 1) * a.pitch + t * 16;
+    // spread: the chunk of a period whose values this lane has (NVFP4: lanes 0 and 1 of four hold a chunk's first group, 2 and 3 its second)
+    const uint32_t mine = MX ? g / P : (g / P & 1) == t / 2 ? g / P / 2 : 99;
+    uint4 spread[PERIOD];
+#pragma unroll
+    for (int c = 0; c < PERIOD; ++c) spread[c] = make_uint4(0, 0, 0, 0);
     uint32_t slot = 0, parity = 0;
     for (uint32_t turn = 0; turn < turns; ++turn) {
         const Run run = run_of(turn, warp);
@@ -401,6 +435,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
             // this warp's share of the tile that it has ended with: [token][row], in the first of its two places for its first tile
             float* my = shares + warp * 2 * per;
             auto hand_in = [&] {
+                if constexpr (SPREAD) {  // a token's columns are those of its groups
+                    if (P == 1) { sum[0][0] += sum[0][1]; sum[0][2] += sum[0][3]; }
+#pragma unroll
+                    for (int j = 0; j < 4; j += P == 1 ? 2 : 1)
+#pragma unroll
+                        for (int o = 1; o < 4; o *= 2) sum[0][j] += __shfl_xor_sync(0xFFFFFFFFu, sum[0][j], o);
+                }
 #pragma unroll
                 for (int m = 0; m < NT; ++m)
 #pragma unroll
@@ -409,7 +450,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
                         if (PARTS == 2 && !MX) v += sum2[m][j] * (1.0f / float(1ull << FINER));
                         v *= MX ? rest : down * rest;
                         const uint32_t token = m * 8 + 2 * t + (j & 1);
-                        if (token < a.tokens) {
+                        if (token < a.tokens && (!SPREAD || token < P)) {
                             float* const to = my + token * 16 + g + (j >> 1) * 8;
                             *to = pass ? *to + v : v;
                         }
@@ -420,17 +461,42 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
             for (uint32_t i = run.lo; i < run.hi; ++i) {
                 mbar_wait(bars + 8 * slot, parity, failed);
                 const uint32_t box = boxes_at + slot * BOX_BYTES + (g * 144 + t * 4);  // TMA has swizzled the 16-byte pieces of a line
-                uint32_t s0[4], s1[4];  // scales of rows g and g + 8: 8 bytes for the box's columns (MXFP4) or 16
-                {
-                    const uint32_t byte = MX ? (col + (block_lo & 1)) * 8 : col * 16;
-                    const uint32_t sc = scales_of + byte / 128 * line_bytes + ((byte / 16 ^ g) & 7) * 16;
-                    if (MX) {
-                        const uint2 p = lds64(sc + byte % 16), q = lds64(sc + byte % 16 + 1024);
-                        s0[0] = p.x; s0[1] = p.y; s1[0] = q.x; s1[1] = q.y;
-                    } else {
-                        const uint4 p = lds128(sc), q = lds128(sc + 1024);
-                        s0[0] = p.x; s0[1] = p.y; s0[2] = p.z; s0[3] = p.w; s1[0] = q.x; s1[1] = q.y; s1[2] = q.z; s1[3] = q.w;
+                const uint32_t byte = MX ? (col + (block_lo & 1)) * 8 : col * 16;  // of a row's scales: 8 are the box's (MXFP4) or 16
+                const uint32_t sc = scales_of + byte / 128 * line_bytes + ((byte / 16 ^ g) & 7) * 16 + byte % 16;
+                if constexpr (SPREAD) {
+                    const uint32_t xt = tokens_at[0] + col * (BOX_COLS * 2);
+                    float d[4];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {  // 32 columns: 16 bytes of a row, four to a lane
+                        const uint32_t w = box ^ uint32_t(c << 4);
+                        uint32_t h0[4], h1[4];
+                        nibbles_to_half(lds32(w), h0);
+                        nibbles_to_half(lds32(w + 1024), h1);
+                        uint4& b = spread[c % PERIOD];
+                        lds128_where(b, xt + c * 64, mine, uint32_t(c % PERIOD));
+                        if (c % PERIOD == 0) mma16816_first(d, h0[0], h1[0], h0[1], h1[1], b.x, b.y);
+                        else mma16816(d, h0[0], h1[0], h0[1], h1[1], b.x, b.y);
+                        mma16816(d, h0[2], h1[2], h0[3], h1[3], b.z, b.w);  // (two chains of sums: no faster)
+                        if (c % PERIOD == PERIOD - 1) {
+                            // columns 2 t and 2 t + 1: two groups (P = 1), or one and both tokens
+                            const uint32_t at = sc + c / PERIOD * GROUPS + (P == 1 ? 2 * t : t);
+                            const uint32_t r0 = P == 1 ? lds16(at) : lds8(at), r1 = P == 1 ? lds16(at + 1024) : lds8(at + 1024);
+                            const float2 f0 = scale_pair<MX>(r0), f1 = scale_pair<MX>(r1);
+                            const float k = MX ? down : 1.0f;
+                            sum[0][0] += d[0] * (f0.x * k);
+                            sum[0][1] += d[1] * ((P == 1 ? f0.y : f0.x) * k);
+                            sum[0][2] += d[2] * (f1.x * k);
+                            sum[0][3] += d[3] * ((P == 1 ? f1.y : f1.x) * k);
+                        }
                     }
+                } else {
+                uint32_t s0[4], s1[4];  // scales of rows g and g + 8
+                if (MX) {
+                    const uint2 p = lds64(sc), q = lds64(sc + 1024);
+                    s0[0] = p.x; s0[1] = p.y; s1[0] = q.x; s1[1] = q.y;
+                } else {
+                    const uint4 p = lds128(sc), q = lds128(sc + 1024);
+                    s0[0] = p.x; s0[1] = p.y; s0[2] = p.z; s0[3] = p.w; s1[0] = q.x; s1[1] = q.y; s1[2] = q.z; s1[3] = q.w;
                 }
                 uint32_t xt[NT];  // where there is no token, another's values make sums that nobody stores
 #pragma unroll
@@ -444,10 +510,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
                     nibbles_to_half(lds32(w + 1024), h1);
                     float f0 = 0, f1 = 0;
                     if (MX) {
-                        uint32_t pair;
-                        asm("{\n\t.reg .b16 e;\n\tcvt.u16.u32 e, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, e;\n\t}" : "=r"(pair) : "r"(__byte_perm(s0[c / 4], s1[c / 4], (c & 3) | (4 + (c & 3)) << 4)));
-                        f0 = __uint_as_float(pair << 16) * down;
-                        f1 = __uint_as_float(pair & 0xFFFF0000u) * down;
+                        const float2 f = scale_pair<MX>(__byte_perm(s0[c / 4], s1[c / 4], (c & 3) | (4 + (c & 3)) << 4));
+                        f0 = f.x * down;
+                        f1 = f.y * down;
                     } else {
                         const uint32_t b = (c & 1) * 2 + nib;  // lanes 0 and 1 hold the first group of 16 columns, 2 and 3 the second
                         const uint32_t pair = e4m3x2_half2(__byte_perm(s0[c / 2], s1[c / 2], b | (4 + b) << 4));
@@ -484,6 +549,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
                             }
                         }
                     }
+                }
                 }
                 __syncwarp();
                 if (lane == 0 && (ask_left || goes_on(passes)) && !*failed) load();

@@ -81,20 +81,27 @@ FewSplit few_split(const ScaledMatrix& w, uint64_t tokens, uint32_t x_dtype) {
     return tokens > FEW_TOKENS ? FewSplit{} : few_split(w.rows, uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), uint32_t(tokens), x_dtype == DT_FP32 ? 2 : 1, w.group);
 }
 
-template <class F> void with_few(uint32_t x_dtype, bool two, bool mx, F f) {
-    auto pick = [&](auto v) {
+template <class F> void with_few(uint32_t x_dtype, uint32_t tokens, bool mx, F f) {
+    auto pick = [&](auto v, auto m) {
         using T = decltype(v);
-        if (mx) two ? f(matvec_few_kernel<T, 2, true>) : f(matvec_few_kernel<T, 1, true>);
-        else two ? f(matvec_few_kernel<T, 2, false>) : f(matvec_few_kernel<T, 1, false>);
+        constexpr bool MX = decltype(m)::value;
+        if (tokens > 8) return f(matvec_few_kernel<T, 16, MX>);
+        if constexpr (sizeof(T) < 4) {
+            if (tokens == 1) return f(matvec_few_kernel<T, 1, MX>);
+            if (tokens == 2) return f(matvec_few_kernel<T, 2, MX>);
+        }
+        f(matvec_few_kernel<T, 8, MX>);
     };
-    if (x_dtype == DT_E4M3) pick(uint8_t());
-    else with_type(x_dtype, pick);
+    auto either = [&](auto v) { mx ? pick(v, std::true_type()) : pick(v, std::false_type()); };
+    if (x_dtype == DT_E4M3) either(uint8_t());
+    else with_type(x_dtype, either);
 }
 cudaError_t allow_few() {
     cudaError_t e = cudaSuccess;
     for (uint32_t t : {DT_FP32, DT_FP16, DT_BF16, DT_E4M3})
-        for (int k = 0; k < 4 && e == cudaSuccess; ++k)
-            with_few(t, k & 1, k & 2, [&](auto f) { e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_MOST)); });
+        for (uint32_t tokens : {1u, 2u, 8u, 16u})
+            for (bool mx : {false, true})
+                if (e == cudaSuccess) with_few(t, tokens, mx, [&](auto f) { e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_MOST)); });
     return e;
 }
 
@@ -267,7 +274,7 @@ int64_t launch_few(const ScaledMatrix& w, const TokenArgs& x, const FewSplit& s,
     if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 128, s.most * 16);
     if (rc < 0) return rc;
     cudaError_t e = cudaSuccess;
-    with_few(x_dtype, tokens > 8, w.group == 32, [&](auto f) { e = enqueue(f, dim3(s.blocks), FEW_WARPS * 32, s.smem, s.ranks, st, values, scales, a); });
+    with_few(x_dtype, tokens, w.group == 32, [&](auto f) { e = enqueue(f, dim3(s.blocks), FEW_WARPS * 32, s.smem, s.ranks, st, values, scales, a); });
     CUDA_TRY(e);
     return 0;
 }
