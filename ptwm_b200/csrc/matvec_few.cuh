@@ -26,14 +26,21 @@ namespace ptwm {
 constexpr uint32_t FEW_TOKENS = 16;
 constexpr uint32_t BOX_COLS = 256, BOX_BYTES = 16 * BOX_COLS / 2, FEW_WARPS = 16, FEW_DEPTH = 5, FEW_HEAD = 1024;  // FEW_DEPTH: boxes under way per warp, at most
 
+// Up to so many matrices that read the same tokens, as one: their row tiles one after the other.
+constexpr uint32_t FEW_MATRICES = 4;
+struct FewMatrix {
+    const float* global_scale;
+    void* y;
+    uint32_t rows, first;   // and the number of row tiles before its own
+};
+struct FewMaps { CUtensorMap values[FEW_MATRICES], scales[FEW_MATRICES]; };
 struct FewArgs {
     const void* x;
     const void* x_scales;
-    const float* global_scale;
-    void* y;
+    FewMatrix m[FEW_MATRICES];
     uint32_t* status;
-    uint64_t rows, cols;
-    uint32_t tokens, scaled, y_dtype, group;
+    uint64_t cols;
+    uint32_t count, tokens, scaled, y_dtype;
     uint32_t rank_boxes, rank_more;         // boxes of 256 columns to a block of a cluster, and how many blocks have one more
     uint32_t cluster_tiles, cluster_more;   // the same of row tiles to a cluster
     uint32_t turns;
@@ -227,7 +234,7 @@ template <bool MX> __device__ __forceinline__ float2 scale_pair(uint32_t two) {
 // the group is its column's, and zeros elsewhere (E2M1 has no infinities to multiply them with).  So one MMA after the other adds to the
 // same sums, and their scales are wanted once for eight groups or four: 185 instructions to a box with one token, 280 with eight.
 template <class T, int TOKENS, bool MX>
-__global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __grid_constant__ CUtensorMap values, const __grid_constant__ CUtensorMap scales, const FewArgs a) {
+__global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __grid_constant__ FewMaps maps, const __grid_constant__ FewArgs a) {
     namespace cg = cooperative_groups;
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;       // kept side by side
     constexpr int NT = TOKENS > 8 ? 2 : 1, P = TOKENS < 8 ? TOKENS : 8;
@@ -274,26 +281,42 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
     const uint32_t boxes_at = smem_u32(ring) + warp * a.depth * BOX_BYTES;
     // scales of a turn's rows, 16-byte pieces swizzled as those of the boxes
     const uint32_t scale_first = (MX ? block_lo / 2 : block_lo) * 16;
-    auto load_scales = [&](uint32_t turn) {
-        mbar_expect(scales_bar, a.lines * line_bytes);
-        for (uint32_t i = 0; i < a.lines; ++i)
-            tma_load(smem_u32(scale_lines) + i * line_bytes, &scales, scales_bar, int32_t(scale_first + i * 128), int32_t((tile_lo + turn * a.most) * 16));
+    auto matrix_at = [&](uint32_t tile) {
+        uint32_t m = 0;
+        while (m + 1 < a.count && tile >= a.m[m + 1].first) ++m;
+        return m;
     };
-    // what lane 0 asks for next: ask_left boxes of the run, from column box ask_col of the row tile at ask_row on
-    uint32_t ask_left, ask_col, ask_row, ask_slot = 0, ask_pass = 0, ask_turn = 0;
+    auto load_scales = [&](uint32_t turn) {
+        // a box of all rows of the turn, or where they may be of several matrices one for each tile
+        const uint32_t first = tile_lo + turn * a.most, n = a.count == 1 ? 1 : min(tile_n - turn * a.most, a.most);
+        mbar_expect(scales_bar, a.lines * (a.count == 1 ? line_bytes : n * 2048));
+        for (uint32_t q = 0; q < n; ++q) {
+            const uint32_t m = matrix_at(first + q);
+            for (uint32_t i = 0; i < a.lines; ++i)
+                tma_load(smem_u32(scale_lines) + i * line_bytes + q * 2048, &maps.scales[m], scales_bar, int32_t(scale_first + i * 128), int32_t((first + q - a.m[m].first) * 16));
+        }
+    };
+    // what lane 0 asks for next: ask_left boxes of the run, from column box ask_col of row tile ask_tile on, which is at ask_row of its matrix
+    uint32_t ask_left, ask_col, ask_tile, ask_m, ask_row, ask_slot = 0, ask_pass = 0, ask_turn = 0;
     auto ask = [&](const Run& r) {
         const uint32_t q = over_n(r.lo);
         ask_left = r.hi - r.lo;
         ask_col = r.lo - q * block_n;
-        ask_row = (r.tile + q) * 16;
+        ask_tile = r.tile + q;
+        ask_m = matrix_at(ask_tile);
+        ask_row = (ask_tile - a.m[ask_m].first) * 16;
     };
     ask(run_of(0, warp));
     auto load = [&] {
         const uint32_t bar = bars + 8 * ask_slot;
         mbar_expect(bar, BOX_BYTES);
-        tma_load(boxes_at + ask_slot * BOX_BYTES, &values, bar, int32_t((block_lo + ask_col) * (BOX_COLS / 2)), int32_t(ask_row));
+        tma_load(boxes_at + ask_slot * BOX_BYTES, &maps.values[ask_m], bar, int32_t((block_lo + ask_col) * (BOX_COLS / 2)), int32_t(ask_row));
         if (++ask_slot == a.depth) ask_slot = 0;
-        if (++ask_col == block_n) { ask_col = 0; ask_row += 16; }
+        if (++ask_col == block_n) {
+            ask_col = 0;
+            ask_row += 16;
+            if (ask_m + 1 < a.count && ++ask_tile == a.m[ask_m + 1].first) { ++ask_m; ask_row = 0; }
+        }
         --ask_left;
     };
     // to the next pass or turn where a run has been asked for; false behind the last
@@ -562,11 +585,11 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
         // A tile's boxes are [q block_n, (q + 1) block_n) of the turn's; the first warp that has one of them may have ended another tile before.
         const uint32_t first = turn * a.most, count = first < tile_n ? min(tile_n - first, a.most) : 0, all = count * block_n;
         auto finish = [&](uint32_t q, uint32_t token, float v) {
-            const uint64_t row = uint64_t(tile_lo + first + q) * 16 + (threadIdx.x & 15);
-            if (row >= a.rows) return;
-            if (a.global_scale) v *= *a.global_scale;
+            const uint32_t m = matrix_at(tile_lo + first + q), row = (tile_lo + first + q - a.m[m].first) * 16 + (threadIdx.x & 15), rows = a.m[m].rows;
+            if (row >= rows) return;
+            if (a.m[m].global_scale) v *= *a.m[m].global_scale;
             if (a.scaled == SCALE_ROW) v *= static_cast<const float*>(a.x_scales)[token];
-            store_as(a.y, a.y_dtype, token * a.rows + row, *failed ? __uint_as_float(0x7FC00000u) : v);
+            store_as(a.m[m].y, a.y_dtype, uint64_t(token) * rows + row, *failed ? __uint_as_float(0x7FC00000u) : v);
         };
         // a thread has row threadIdx.x % 16 of every 32nd pair of tile and token
         const float per_token = __frcp_rn(float(a.tokens));

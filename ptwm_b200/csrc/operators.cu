@@ -60,9 +60,8 @@ constexpr uint32_t SMEM_MOST = 227 * 1024;
 // How a product with few tokens is split: a block per SM, clusters of as few as let the tokens fit shared memory beside two boxes
 // per warp (up to five where there is room).  depth 0: they do not.
 struct FewSplit { uint32_t ranks, most, depth, smem, blocks, lines; };
-FewSplit few_split(uint64_t rows, uint32_t boxes, uint32_t tokens, uint32_t parts, uint32_t group) {
+FewSplit few_split(uint32_t tiles, uint32_t boxes, uint32_t tokens, uint32_t parts, uint32_t group) {
     constexpr uint32_t SMS = 148;
-    const uint32_t tiles = uint32_t((rows + 15) / 16);
     // Where two blocks to a cluster, or for more than eight tokens one turn, are not enough, tiles are quicker: 8 tokens of 4096 x 14336 (NVFP4) take 22 us
     // in two blocks (25 in tiles), 9 of them 35 (25), 16 in four blocks 62 (25); 16 of 14336 x 4096 20 (25).
     for (uint32_t ranks = 1; ranks <= 2 && ranks <= boxes; ranks *= 2) {
@@ -77,8 +76,10 @@ FewSplit few_split(uint64_t rows, uint32_t boxes, uint32_t tokens, uint32_t part
     }
     return {};
 }
-FewSplit few_split(const ScaledMatrix& w, uint64_t tokens, uint32_t x_dtype) {
-    return tokens > FEW_TOKENS ? FewSplit{} : few_split(w.rows, uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), uint32_t(tokens), x_dtype == DT_FP32 ? 2 : 1, w.group);
+uint32_t few_boxes(const ScaledMatrix& w) { return uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS); }
+uint32_t few_tiles(const ScaledMatrix& w) { return uint32_t((w.rows + 15) / 16); }
+FewSplit few_split(const ScaledMatrix& w, uint32_t tiles, uint64_t tokens, uint32_t x_dtype) {
+    return tokens > FEW_TOKENS ? FewSplit{} : few_split(tiles, few_boxes(w), uint32_t(tokens), x_dtype == DT_FP32 ? 2 : 1, w.group);
 }
 
 template <class F> void with_few(uint32_t x_dtype, uint32_t tokens, bool mx, F f) {
@@ -263,18 +264,24 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     return 0;
 }
 
-int64_t launch_few(const ScaledMatrix& w, const TokenArgs& x, const FewSplit& s, uint32_t x_dtype, uint32_t y_dtype, int device, const PerDevice& dev, cudaStream_t st) {
-    const uint32_t boxes = uint32_t((w.cols + BOX_COLS - 1) / BOX_COLS), tokens = uint32_t(x.tokens);
-    const uint32_t tiles = uint32_t((w.rows + 15) / 16), clusters = s.blocks / s.ranks;
-    const FewArgs a{x.x, x.scales, w.global_scale, x.y, dev.status, w.rows, w.cols, tokens, x.scaled, y_dtype, w.group, boxes / s.ranks, boxes % s.ranks, tiles / clusters, tiles % clusters,
-                    ((tiles + clusters - 1) / clusters + s.most - 1) / s.most, s.depth, few_pitch((boxes + s.ranks - 1) / s.ranks), s.most, s.lines, reinterpret_cast<uintptr_t>(x.x) % 16 == 0};
+// `count` matrices of the same columns and kind of scales; x.y is not looked at.
+int64_t launch_few(const ScaledMatrix* w, const uint64_t* y, uint32_t count, uint32_t tiles, const TokenArgs& x, const FewSplit& s, uint32_t x_dtype, uint32_t y_dtype, int device,
+                   const PerDevice& dev, cudaStream_t st) {
+    const uint32_t boxes = few_boxes(*w), tokens = uint32_t(x.tokens), clusters = s.blocks / s.ranks;
+    FewArgs a{x.x, x.scales, {}, dev.status, w->cols, count, tokens, x.scaled, y_dtype, boxes / s.ranks, boxes % s.ranks, tiles / clusters, tiles % clusters,
+              ((tiles + clusters - 1) / clusters + s.most - 1) / s.most, s.depth, few_pitch((boxes + s.ranks - 1) / s.ranks), s.most, s.lines, reinterpret_cast<uintptr_t>(x.x) % 16 == 0};
     CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
-    CUtensorMap values, scales;
-    int64_t rc = tensor_map(&values, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.values, w.cols / 2, w.rows, w.value_pitch, BOX_COLS / 2, 16);
-    if (rc == 0) rc = tensor_map(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w.scales, w.cols / w.group, w.rows, w.scale_pitch, 128, s.most * 16);
-    if (rc < 0) return rc;
+    FewMaps maps;
+    uint32_t first = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        int64_t rc = tensor_map(&maps.values[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w[i].values, w[i].cols / 2, w[i].rows, w[i].value_pitch, BOX_COLS / 2, 16);
+        if (rc == 0) rc = tensor_map(&maps.scales[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, w[i].scales, w[i].cols / w[i].group, w[i].rows, w[i].scale_pitch, 128, count == 1 ? s.most * 16 : 16);
+        if (rc < 0) return rc;
+        a.m[i] = FewMatrix{w[i].global_scale, at<void>(y[i]), uint32_t(w[i].rows), first};
+        first += few_tiles(w[i]);
+    }
     cudaError_t e = cudaSuccess;
-    with_few(x_dtype, tokens, w.group == 32, [&](auto f) { e = enqueue(f, dim3(s.blocks), FEW_WARPS * 32, s.smem, s.ranks, st, values, scales, a); });
+    with_few(x_dtype, tokens, w->group == 32, [&](auto f) { e = enqueue(f, dim3(s.blocks), FEW_WARPS * 32, s.smem, s.ranks, st, maps, a); });
     CUDA_TRY(e);
     return 0;
 }
@@ -330,28 +337,53 @@ extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t
 
 extern "C" uint64_t ptwm_b200_matvec_scratch_bytes(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t tokens, uint32_t x_dtype, uint32_t grad) {
     ScaledMatrix m;
-    if (matrix_of(w, &m) < 0 || (!grad && few_split(m, tokens, x_dtype).depth)) return 0;
+    if (matrix_of(w, &m) < 0 || (!grad && few_split(m, few_tiles(m), tokens, x_dtype).depth)) return 0;
     return parts_of(x, tokens, grad ? m.rows : m.cols, x_dtype).bytes;
+}
+
+extern "C" int64_t ptwm_b200_matvec_group(const ptwm_b200_scaled_weight* const* weights, const uint64_t* y, uint32_t count, uint64_t x, uint64_t x_scales, uint64_t tokens,
+                                          uint32_t x_dtype, uint32_t x_scaled, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, uint32_t device, uint64_t stream) {
+    ScaledMatrix w[FEW_MATRICES];
+    if (!weights || !y || !count) return fail(PTWM_RC_INVALID_INPUT, "matvec: no matrix");
+    if (count > FEW_MATRICES) return fail(PTWM_RC_UNSUPPORTED, "matvec: more than 4 matrices in a call");
+    uint64_t tiles = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        if (const int64_t rc = matrix_of(weights[i], &w[i]); rc < 0) return rc;
+        if (w[i].cols != w[0].cols) return fail(PTWM_RC_INVALID_INPUT, "matvec: matrices of a call have the same columns");
+        tiles += few_tiles(w[i]);
+    }
+    if (!plain_type(y_dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec: the output is fp32, fp16 or bf16");
+    if (x_dtype == DT_E4M3 ? (x_scaled != SCALE_ROW && x_scaled != SCALE_BLOCK) || !x_scales : !plain_type(x_dtype) || x_scaled)
+        return fail(PTWM_RC_UNSUPPORTED, "matvec: tokens are fp32, fp16, bf16, or E4M3 with scales per row or block");
+    if (x_scaled == SCALE_BLOCK && w[0].cols % 32) return fail(PTWM_RC_INVALID_INPUT, "matvec: block scales need whole blocks of 32 columns");
+    if (tokens > (1u << 19)) return fail(PTWM_RC_UNSUPPORTED, "matvec: more than 2^19 tokens in a call");
+    if (!tokens) return 0;
+    if (!x) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
+    for (uint32_t i = 0; i < count; ++i)
+        if (!y[i]) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
+    DeviceGuard guard{int(device)};
+    if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
+    TokenArgs t{at<void>(x), at<void>(x_scales), tokens, x_scaled, nullptr};
+    PerDevice dev;
+    if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
+    bool alike = true;
+    for (uint32_t i = 1; i < count; ++i) alike &= w[i].group == w[0].group;
+    if (alike)
+        if (const FewSplit s = few_split(w[0], uint32_t(tiles), tokens, x_dtype); s.depth)
+            return launch_few(w, y, count, uint32_t(tiles), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream));
+    for (uint32_t i = 0; i < count; ++i) {
+        const FewSplit s = few_split(w[i], few_tiles(w[i]), tokens, x_dtype);
+        t.y = at<void>(y[i]);
+        const int64_t rc = s.depth ? launch_few(&w[i], y + i, 1, few_tiles(w[i]), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream))
+                                   : launch_tiles<false>(w[i], t, x_dtype, y_dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
+        if (rc < 0) return rc;
+    }
+    return 0;
 }
 
 extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint64_t x, uint64_t x_scales, uint64_t y, uint64_t tokens, uint32_t x_dtype, uint32_t x_scaled,
                                     uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, uint32_t device, uint64_t stream) {
-    ScaledMatrix w;
-    if (const int64_t rc = matrix_of(weight, &w); rc < 0) return rc;
-    if (!plain_type(y_dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec: the output is fp32, fp16 or bf16");
-    if (x_dtype == DT_E4M3 ? (x_scaled != SCALE_ROW && x_scaled != SCALE_BLOCK) || !x_scales : !plain_type(x_dtype) || x_scaled)
-        return fail(PTWM_RC_UNSUPPORTED, "matvec: tokens are fp32, fp16, bf16, or E4M3 with scales per row or block");
-    if (x_scaled == SCALE_BLOCK && w.cols % 32) return fail(PTWM_RC_INVALID_INPUT, "matvec: block scales need whole blocks of 32 columns");
-    if (tokens > (1u << 19)) return fail(PTWM_RC_UNSUPPORTED, "matvec: more than 2^19 tokens in a call");
-    if (!tokens) return 0;
-    if (!x || !y) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
-    DeviceGuard guard{int(device)};
-    if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
-    const TokenArgs t{at<void>(x), at<void>(x_scales), tokens, x_scaled, at<void>(y)};
-    PerDevice dev;
-    if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
-    if (const FewSplit s = few_split(w, tokens, x_dtype); s.depth) return launch_few(w, t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream));
-    return launch_tiles<false>(w, t, x_dtype, y_dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
+    return ptwm_b200_matvec_group(&weight, &y, 1, x, x_scales, tokens, x_dtype, x_scaled, y_dtype, scratch, scratch_bytes, device, stream);
 }
 
 extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dtype, uint64_t scratch, uint64_t scratch_bytes,

@@ -369,7 +369,7 @@ class Projection:
     """A norm and the matrices that read its output, such as the gate and up projections of a feed-forward block.
 
     ``projection(x, residual)`` returns ``([W x' for W in weights], h)`` with ``x', h = rms_norm(x, norm, eps,
-    residual=residual, quant=quant)``; ``h`` is x where there is no residual."""
+    residual=residual, quant=quant)``; ``h`` is x where there is no residual.  The matrices' products are one launch where tokens are few."""
 
     def __init__(self, norm: torch.Tensor, weights: Sequence[ScaledWeight], *, eps: float = 1e-6, quant: Optional[str] = None) -> None:
         self.norm, self.weights, self.eps, self.quant = norm, list(weights), eps, quant
@@ -383,10 +383,32 @@ class Projection:
                 raise TypeError(f"weights are ScaledWeights, got {type(w).__name__}")
             if w.cols != norm.shape[0] or w.device != norm.device:
                 raise ValueError(f"a norm of {norm.shape[0]} on {norm.device} does not fit {w!r}")
+        parts = [self.weights[i:i + 4] for i in range(0, len(self.weights), 4)]
+        self._calls = [((C.c_uint64 * len(p))(*[w._ref for w in p]), p) for p in parts]
 
     def __call__(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> tuple[list[torch.Tensor], torch.Tensor]:
         got = rms_norm(x, self.norm, self.eps, residual=residual, quant=self.quant)
         y, h = (got, x) if residual is None else got
         if self.quant is not None:  # checked, contiguous and without a gradient
-            return [_product(y.values, y.scales, self.quant, w, x.dtype) for w in self.weights], h
-        return [matvec(y, w) for w in self.weights], h
+            return self._products(y.values, y.scales, x.dtype), h
+        if y.requires_grad and torch.is_grad_enabled():
+            return [matvec(y, w) for w in self.weights], h
+        return self._products(y, None, x.dtype), h
+
+    def _products(self, x: torch.Tensor, scales: Optional[torch.Tensor], out_dtype: torch.dtype) -> list[torch.Tensor]:
+        """The products of all matrices, four to a call."""
+        out = []
+        device, tokens, head = x.get_device(), x.numel() // self.norm.shape[0], tuple(x.shape[:-1])
+        code, scales_at = (_PLAIN[x.dtype], 0) if scales is None else (_E4M3, scales.data_ptr())
+        for refs, weights in self._calls:
+            ys = [_new((*head, w.rows), out_dtype, x.device) for w in weights]
+            at = (C.c_uint64 * len(ys))(*[y.data_ptr() for y in ys])
+            args = (refs, at, len(ys), x.data_ptr(), scales_at, tokens, code, _QUANT[self.quant], _PLAIN[out_dtype])
+            rc = _lib.lib().ptwm_b200_matvec_group(*args, 0, 0, device, _stream(device))
+            if rc < 0:
+                if rc == _TOO_SMALL:
+                    scratch = max((_scratch(w, x, tokens, code, 0) for w in weights), key=torch.Tensor.numel)  # one of them may want some where another does not
+                    rc = _lib.lib().ptwm_b200_matvec_group(*args, scratch.data_ptr(), scratch.numel(), device, _stream(device))
+                _check(rc)
+            out += ys
+        return out

@@ -486,6 +486,23 @@ def test_matvec_layouts_of_matrix_and_tokens():
     assert torch.equal(matvec(ScaledActivations(q.t().contiguous().t(), both[:, 0]), ScaledWeight(values, scales)), want)
 
 
+@pytest.mark.parametrize("tokens", [1, 2, 5, 12, 40])
+@pytest.mark.parametrize("quant", [None, "row", "block"])
+@pytest.mark.parametrize("sizes", [[64], [16, 8], [300, 33, 7], [1, 2000, 16, 48], [20, 40, 60, 80, 100], [7000, 40]])
+def test_projections_of_several_matrices(tokens, quant, sizes):
+    """Whole numbers, so that every matrix of a projection gives what it gives alone."""
+    k = 1056
+    kinds = ["nvfp4", "mxfp4"] if len(sizes) in (3, 5) else ["mxfp4"]
+    weights = [ScaledWeight(*_matrix(n, k, kinds[i % len(kinds)], i + n)) for i, n in enumerate(sizes)]
+    x = torch.randint(0, 2, (tokens, k), generator=_gen(5), device="cuda").to(torch.bfloat16) * 2 - 1  # a root mean square of one
+    p = Projection(torch.ones(k, device="cuda", dtype=torch.bfloat16), weights, eps=0.0, quant=quant)
+    ys, h = p(x)
+    assert torch.equal(h, x) and len(ys) == len(sizes)
+    same = rms_norm(x, torch.ones(k, device="cuda", dtype=torch.bfloat16), 0.0, quant=quant)  # with row scales that is 448 times 1/448, as fp32 has it
+    for y, w, n in zip(ys, weights, sizes):
+        assert y.shape == (tokens, n) and torch.equal(y, matvec(same, w, out_dtype=torch.bfloat16))
+
+
 def test_a_token_does_not_depend_on_its_neighbours():
     """The same token gives the same bits beside others that hold infinities, as long as as many are asked for."""
     w = ScaledWeight(*_matrix(200, 2048, "nvfp4", 3))

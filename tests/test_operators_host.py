@@ -44,6 +44,12 @@ def test_tokens_that_are_none(L):
                      ((p, A, A, A, 1, 29, 0, 6), UNSUPPORTED), ((p, A, A, A, 1, 29, 3, 6), UNSUPPORTED), ((p, 0, 0, A, 1, 6, 0, 6), INVALID), ((p, A, 0, 0, 1, 6, 0, 6), INVALID),
                      ((p, A, 0, A, (1 << 19) + 1, 6, 0, 6), UNSUPPORTED), ((C.addressof(nv), A, A, A, 1, 29, 2, 6), INVALID), ((None, A, 0, A, 1, 6, 0, 6), INVALID)]:
         assert L.ptwm_b200_matvec(*args, 0, 0, 0, 1) == rc, args
+    other = _weight(cols=96, value_pitch=48)
+    refs, ys = (C.c_uint64 * 5)(p, C.addressof(other), p, p, p), (C.c_uint64 * 5)(A, A, 0, A, A)
+    for count, at, rc in [(0, ys, INVALID), (2, ys, INVALID), (5, ys, UNSUPPORTED), (1, None, INVALID)]:
+        assert L.ptwm_b200_matvec_group(refs, at, count, A, 0, 1, 6, 0, 6, 0, 0, 0, 1) == rc, count
+    refs[1] = p
+    assert L.ptwm_b200_matvec_group(refs, ys, 3, A, 0, 1, 6, 0, 6, 0, 0, 0, 1) == INVALID
     assert L.ptwm_b200_matvec(p, 0, 0, 0, 0, 6, 0, 6, 0, 0, 0, 1) == 0  # no tokens: nothing to do, on any machine
     for args, rc in [((p, A, A, 1, 29), UNSUPPORTED), ((p, 0, A, 1, 6), INVALID), ((p, A, 0, 1, 6), INVALID)]:
         assert L.ptwm_b200_matvec_grad(*args, 0, 0, 0, 1) == rc, args
