@@ -9,6 +9,9 @@
 //   Forward, a converted tile goes to tensor memory, whose lanes are the rows that the threads convert.  In shared memory it would be
 // written and read beside the tokens, 128 bytes a cycle for all: with 256 tokens that is 830 cycles for a step whose MMAs take 512.
 // In the gradient the contraction runs down the rows of the matrix, and the tile lies in shared memory as an MN-major operand.
+//   The tensor cores cut what an fp32 sum cannot hold where others round: over 14336 values of fp32 tokens, three parts of them, that is
+// 5e-6 of the result.  Where the results are fp32 (FLUSH), the sums of every 256 of the contraction are added up in registers: 8e-7
+// (512: 1.5e-6, and 2 to 6 % less time; 128: 5e-7, 6 to 20 % more).  Results of 16 bits are rounded by a thousand times as much.
 //   Where tiles are fewer than SMs, the blocks of a cluster share a tile's contraction and add their sums over distributed shared
 // memory, in the order of their ranks.
 //   What a step costs: 512 cycles of MMA with 256 tokens; some 200 cycles of ALU in conversion; and the issuing thread, to which a wait
@@ -54,7 +57,9 @@ inline uint32_t tiles_smem(uint32_t stage, uint32_t stages) { return 1024 + TILE
 // A block has an SM to itself: two that wait for tensor memory on each other's could wait for good.
 constexpr uint32_t TILES_LEAST_SMEM = 120 * 1024;
 constexpr uint32_t TMEM_COLS = 512, A_COLS = STEP / 2;   // columns of tensor memory; of a converted tile in it
-inline uint32_t tiles_tmem_stages(uint32_t tile_tokens, uint32_t together) { return (TMEM_COLS - (tile_tokens + 31) / 32 * 32) / (together * A_COLS); }
+constexpr uint32_t FLUSH_STEPS = 4, FLUSH_TOKENS = 128;  // tokens: what a thread has registers for
+__host__ __device__ constexpr uint32_t tiles_sums(uint32_t tile_tokens, bool flush) { return (tile_tokens + 31) / 32 * 32 * (flush ? 2 : 1); }
+inline uint32_t tiles_tmem_stages(uint32_t tile_tokens, uint32_t together, bool flush) { return (TMEM_COLS - tiles_sums(tile_tokens, flush)) / (together * A_COLS); }
 
 // Eight nibbles -> eight bf16 in their order, times `scale`.  A word takes the even nibble of a byte to its low half and the odd one
 // to its high half; a product puts their signs at bit 15 and the other three bits at 8..6, which reads as the number times 2^-126;
@@ -87,8 +92,9 @@ constexpr float NV_REST = 1024.0f;
 template <bool GRAD> struct TilesShared {
     static constexpr uint32_t raw = TILES_HEAD, scales = raw + RAW_STAGES * RAW_BYTES, stages = scales + SCALES_BYTES;
     static constexpr uint32_t raw_rows = GRAD ? STEP : TILE_ROWS, scale_bytes = raw_rows * 16, scale_slots = SCALES_BYTES / scale_bytes;
-    // barriers: raw full / empty, scales full (a slot is free once all raw stages before raw - RAW_STAGES are), stage full / empty, accumulator full
-    static constexpr uint32_t raw_full = 0, raw_empty = 64, full = 128, empty = 192, scales_full = 256, done = 320, tmem = 328, failed = 332;
+    // barriers: raw full / empty, scales full (a slot is free once all raw stages before raw - RAW_STAGES are), stage full / empty, two of sums done and
+    // flushed
+    static constexpr uint32_t raw_full = 0, raw_empty = 64, full = 128, empty = 192, scales_full = 256, done = 320, flushed = 336, tmem = 352, failed = 356;
     static_assert(RAW_STAGES <= 8 && MOST_STAGES <= 8 && scale_slots <= 8, "barriers do not overlap");
 };
 
@@ -109,7 +115,7 @@ __device__ __forceinline__ void convert32(const uint4& v, uint32_t group, uint32
     }
 }
 
-template <bool GRAD>
+template <bool GRAD, bool FLUSH>
 __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __grid_constant__ CUtensorMap values, const __grid_constant__ CUtensorMap scales,
                                                                         const __grid_constant__ CUtensorMap tokens, const TilesArgs t) {
     namespace cg = cooperative_groups;
@@ -138,7 +144,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
         for (uint32_t i = 0; i < RAW_STAGES; ++i) { mbar_init(sb + S::raw_full + 8 * i, 1); mbar_init(sb + S::raw_empty + 8 * i, GRAD ? 4 : 8); }
         for (uint32_t i = 0; i < t.stages; ++i) { mbar_init(sb + S::full + 8 * i, 4 * t.together + 1); mbar_init(sb + S::empty + 8 * i, 1); }
         for (uint32_t i = 0; i < S::scale_slots; ++i) mbar_init(sb + S::scales_full + 8 * i, 1);
-        mbar_init(sb + S::done, 1);
+        for (uint32_t i = 0; i < 2; ++i) { mbar_init(sb + S::done + 8 * i, 1); mbar_init(sb + S::flushed + 8 * i, 16); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc(sb + S::tmem, TMEM_COLS);
@@ -146,7 +152,8 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(base + S::tmem);
-    const uint32_t a_tmem = tmem + (t.tile_tokens + 31) / 32 * 32;  // converted tiles behind the sums
+    const uint32_t sums_cols = tiles_sums(t.tile_tokens, false), a_tmem = tmem + tiles_sums(t.tile_tokens, FLUSH);  // converted tiles behind the sums
+    const uint32_t segments = FLUSH ? (steps + FLUSH_STEPS - 1) / FLUSH_STEPS : 1;
     others_may_start();
     after_those_before();
 
@@ -194,7 +201,15 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
             const uint64_t a_desc = operand_desc(sb + S::stages, 8192, 1024), b_desc = operand_desc(sb + S::stages + b_first, 16, 1024);
             uint32_t st = 0, parity = 0;
             bool more = false;
+            uint32_t d = tmem, segment = 0;
             for (uint32_t step = 0; step < steps; step += t.together) {
+                if (FLUSH && step && step % FLUSH_STEPS == 0) {  // the other sums, once what was in them has been taken
+                    tc_commit(sb + S::done + 8 * (segment & 1));
+                    ++segment;
+                    if (segment > 1 && !mbar_wait(sb + S::flushed + 8 * (segment & 1), (segment / 2 - 1) & 1, failed)) break;
+                    d = tmem + (segment & 1) * sums_cols;
+                    more = false;
+                }
                 if (!mbar_wait(sb + S::full + 8 * st, parity, failed)) break;
                 tc_fence_after();
                 uint64_t ad = a_desc + st * (stage_bytes / 16), bd = b_desc + st * (stage_bytes / 16);
@@ -203,15 +218,15 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
                     for (uint32_t p = 0; p < t.parts; ++p, bd += b_bytes / 16) {
 #pragma unroll
                         for (uint32_t k = 0; k < STEP / 16; ++k) {
-                            if (GRAD) mma_f16(tmem, ad + k * (2048 / 16), bd + k * 2, idesc, more);
-                            else mma_f16_tmem(tmem, at + k * 8, bd + k * 2, idesc, more);
+                            if (GRAD) mma_f16(d, ad + k * (2048 / 16), bd + k * 2, idesc, more);
+                            else mma_f16_tmem(d, at + k * 8, bd + k * 2, idesc, more);
                             more = true;
                         }
                     }
                 tc_commit(sb + S::empty + 8 * st);
                 if (++st == t.stages) { st = 0; parity ^= 1; }
             }
-            tc_commit(sb + S::done);
+            tc_commit(sb + S::done + 8 * (segment & 1));
         }
     } else if (warp >= 4) {
         // Teams of four warps take a step each in turn: a step is some 200 instructions of a thread in a row, and up to four of them are under way.
@@ -224,7 +239,32 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
         const uint32_t out = half * 8192 + row / 8 * 1024 + row % 8 * 128;
         uint32_t st = team / t.together, round = 0;  // stage of the step, and how often the stages have been gone through
         while (st >= t.stages) { st -= t.stages; ++round; }
+        const uint32_t lanes = warp % 4 * 32;
+        float total[FLUSH ? FLUSH_TOKENS / 4 : 1];
+        uint32_t next = 0;
+        if (FLUSH)
+#pragma unroll
+            for (uint32_t i = 0; i < FLUSH_TOKENS / 4; ++i) total[i] = 0;
+        auto flush = [&] {  // the sums of segment `next`: this team's columns of them
+            const uint32_t which = next & 1;
+            mbar_wait(sb + S::done + 8 * which, next / 2 & 1, failed);
+            tc_fence_after();
+#pragma unroll
+            for (uint32_t i = 0; i < FLUSH_TOKENS / 64; ++i)
+                if (team * 16 + i * 64 < t.tile_tokens) {
+                    uint32_t v[16];
+                    tmem_load16(tmem + which * sums_cols + (lanes << 16) + team * 16 + i * 64, v);
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; ++j) total[i * 16 + j] += __uint_as_float(v[j]);
+                }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sb + S::flushed + 8 * which);
+            ++next;
+        };
         for (uint32_t step = team; step < steps && team < t.teams; step += t.teams) {
+            if constexpr (FLUSH)
+                while (next + 2 <= step / FLUSH_STEPS) flush();
             const uint32_t raw = GRAD ? step : step / 2, rs = raw % RAW_STAGES;
             const uint32_t pair = GRAD ? half : step % 2;  // which 64 of the 128 k
             if (!mbar_wait(sb + S::raw_full + 8 * rs, raw / RAW_STAGES & 1, failed)) break;
@@ -268,21 +308,31 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
             while (st >= t.stages) { st -= t.stages; ++round; }
         }
         // results: a warp reaches the 32 lanes (rows of D) that its number modulo 4 names; the four teams share the tokens
-        mbar_wait(sb + S::done, 0, failed);
-        tc_fence_after();
-        const uint32_t lanes = warp % 4 * 32;
+        if constexpr (FLUSH) {
+            while (next < segments) flush();
+        } else {
+            mbar_wait(sb + S::done, 0, failed);
+            tc_fence_after();
+        }
         const uint64_t n = row0 + lanes + lane;
         float factor = t.group == 32 ? 1.0f : NV_REST;
         if (t.global_scale) factor *= *t.global_scale;
         if (*failed) factor = __uint_as_float(0x7FC00000u);
-        if (!steps) factor = 0;
         float* const sums = reinterpret_cast<float*>(base + TILES_HEAD);  // [token][row]: nothing reads or writes the buffers any more
-        for (uint32_t m = team * 16; m < t.tile_tokens; m += 64) {
+#pragma unroll 1
+        for (uint32_t i = 0; i < (FLUSH ? FLUSH_TOKENS / 64 : 4); ++i) {
+            const uint32_t m = team * 16 + i * 64;
+            if (m >= t.tile_tokens) break;
             uint32_t v[16];
-            tmem_load16(tmem + (lanes << 16) + m, v);
+            if constexpr (FLUSH) {
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) v[j] = __float_as_uint(i == 0 ? total[j] : total[16 + j]);
+            } else {
+                tmem_load16(tmem + (lanes << 16) + m, v);
+            }
             if (ranks > 1) {
 #pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) sums[(m + j) * TILE_ROWS + lanes + lane] = steps ? __uint_as_float(v[j]) * factor : 0.0f;
+                for (uint32_t j = 0; j < 16; ++j) sums[(m + j) * TILE_ROWS + lanes + lane] = __uint_as_float(v[j]) * factor;
             } else if (n < t.rows) {
 #pragma unroll
                 for (uint32_t j = 0; j < 16; ++j) {

@@ -170,8 +170,8 @@ int64_t device_of(int device, PerDevice* out) {
         CUDA_TRY(cudaGetSymbolAddress(&p, g_operator_status));
         d.status = static_cast<uint32_t*>(p);
         CUDA_TRY(allow_few());
-        CUDA_TRY(cudaFuncSetAttribute(matvec_tiles_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_MOST)));
-        CUDA_TRY(cudaFuncSetAttribute(matvec_tiles_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_MOST)));
+        for (const auto f : {matvec_tiles_kernel<false, false>, matvec_tiles_kernel<false, true>, matvec_tiles_kernel<true, false>, matvec_tiles_kernel<true, true>})
+            CUDA_TRY(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_MOST)));
         d.attributes = true;
     }
     *out = d;
@@ -213,15 +213,16 @@ Parts parts_of(uint64_t x, uint64_t tokens, uint64_t contraction, uint32_t dtype
 
 // How a product is cut into tiles.
 struct TilesSplit { uint32_t tile_tokens, ranks, stages, together; };
-TilesSplit tiles_split(uint64_t rows, uint64_t contraction, uint64_t tokens, uint32_t parts, bool grad, uint32_t group) {
+TilesSplit tiles_split(uint64_t rows, uint64_t contraction, uint64_t tokens, uint32_t parts, bool grad, bool flush, uint32_t group) {
     constexpr uint32_t SMS = 148;
-    // as few tiles of tokens as 256 columns (128 where a stage holds parts) allow, all of a size
-    const uint64_t most = parts == 1 ? 256 : 128, across = (tokens + most - 1) / most;
+    // as few tiles of tokens as 256 columns (128 where a stage holds parts, or results are flushed) allow, all of a size
+    static_assert(FLUSH_TOKENS == 128, "");
+    const uint64_t most = parts == 1 && !flush ? 256 : 128, across = (tokens + most - 1) / most;
     const uint32_t tile_tokens = uint32_t(((tokens + across - 1) / across + 15) / 16 * 16);
     // two steps to a stage where that leaves room for three
     const uint32_t room = SMEM_MOST - tiles_smem(0, 0), together = 3 * tiles_stage(tile_tokens, parts, 2, grad) <= room ? 2 : 1;
     uint32_t stages = std::min<uint32_t>(MOST_STAGES, room / tiles_stage(tile_tokens, parts, together, grad));
-    if (!grad) stages = std::min(stages, tiles_tmem_stages(tile_tokens, together));
+    if (!grad) stages = std::min(stages, tiles_tmem_stages(tile_tokens, together, flush));
     // blocks of a cluster for a tile's contraction: rounds of blocks x (steps of one, and what a block costs besides, in steps)
     const uint64_t tiles = (rows + TILE_ROWS - 1) / TILE_ROWS * across, steps = (contraction + STEP - 1) / STEP, unit = grad ? together : group == 32 ? 8 : 4;
     uint32_t ranks = 1;
@@ -250,7 +251,8 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
         CUDA_TRY(e);
         tokens = out;
     }
-    const TilesSplit split = tiles_split(rows, contraction, x.tokens, p.parts, GRAD, w.group);
+    const bool flush = y_dtype == DT_FP32;
+    const TilesSplit split = tiles_split(rows, contraction, x.tokens, p.parts, GRAD, flush, w.group);
     TilesArgs t{rows, contraction, x.tokens, x.tokens, p.parts, split.tile_tokens, split.stages, split.together, std::min<uint32_t>(4, split.stages * split.together), w.group, y_dtype, w.global_scale,
                 x.scaled == SCALE_ROW ? static_cast<const float*>(x.scales) : nullptr, x.y, dev.status};
     CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
@@ -260,7 +262,8 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     if (rc == 0) rc = tensor_map(&tmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, tokens, contraction, p.parts * x.tokens, p.pitch * 2, STEP, t.tile_tokens);
     if (rc < 0) return rc;
     const dim3 grid(uint32_t((rows + TILE_ROWS - 1) / TILE_ROWS) * split.ranks, uint32_t((x.tokens + t.tile_tokens - 1) / t.tile_tokens));
-    CUDA_TRY(enqueue(matvec_tiles_kernel<GRAD>, grid, TILES_THREADS, std::max(TILES_LEAST_SMEM, tiles_smem(tiles_stage(t.tile_tokens, t.parts, t.together, GRAD), t.stages)), split.ranks, st, values, scales, tmap, t));
+    const uint32_t smem = std::max(TILES_LEAST_SMEM, tiles_smem(tiles_stage(t.tile_tokens, t.parts, t.together, GRAD), t.stages));
+    CUDA_TRY(enqueue(flush ? matvec_tiles_kernel<GRAD, true> : matvec_tiles_kernel<GRAD, false>, grid, TILES_THREADS, smem, split.ranks, st, values, scales, tmap, t));
     return 0;
 }
 
