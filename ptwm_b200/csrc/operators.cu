@@ -1,6 +1,7 @@
 // Host side of the operators that apply decoded weights: rms_norm and matvec with 4-bit weights.  A translation unit of its
 // own; every call enqueues its kernels on the caller's stream and returns.
 #include <algorithm>
+#include <exception>
 #include <map>
 #include <mutex>
 #include <type_traits>
@@ -14,6 +15,11 @@
 using namespace ptwm;
 
 namespace {
+
+// The body of an entry point: no exception leaves it.
+template <class F> int64_t guarded(F f) {
+    try { return f(); } catch (const std::exception& e) { return fail(PTWM_RC_INTERNAL, e.what()); }
+}
 
 template <class T> T* at(uint64_t p) { return reinterpret_cast<T*>(uintptr_t(p)); }
 cudaStream_t stream_of(uint64_t s) { return reinterpret_cast<cudaStream_t>(uintptr_t(s)); }
@@ -292,50 +298,56 @@ int64_t launch_few(const ScaledMatrix* w, const uint64_t* y, uint32_t count, uin
 }  // namespace
 
 extern "C" int64_t ptwm_b200_operator_status(uint32_t device) {
-    DeviceGuard guard{int(device)};
-    if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
-    uint32_t v = 0;
-    CUDA_TRY(cudaMemcpyFromSymbol(&v, g_operator_status, 4));
-    return v;
+    return guarded([&]() -> int64_t {
+        DeviceGuard guard{int(device)};
+        if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
+        uint32_t v = 0;
+        CUDA_TRY(cudaMemcpyFromSymbol(&v, g_operator_status, 4));
+        return v;
+    });
 }
 
 extern "C" int64_t ptwm_b200_rms_norm(uint64_t x, uint64_t residual, uint64_t weight, uint64_t h, uint64_t y, uint64_t scales, uint64_t rows, uint64_t cols,
                                       uint32_t dtype, uint32_t weight_dtype, uint32_t scaled, float eps, uint32_t device, uint64_t stream) {
-    if (!plain_type(dtype) || !plain_type(weight_dtype)) return fail(PTWM_RC_UNSUPPORTED, "rms_norm: x and weight are fp32, fp16 or bf16");
-    if (scaled > SCALE_BLOCK) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: unknown output scaling");
-    if (!cols || (scaled == SCALE_BLOCK && cols % 32)) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: rows must not be empty, and hold whole blocks of 32 for block scales");
-    if (rows > 0x7FFFFFFFull || cols > 0x7FFFFFFFull) return fail(PTWM_RC_UNSUPPORTED, "rms_norm: more than 2^31 - 1 rows or columns");
-    if (!rows) return 0;
-    if (!x || !weight || !y || (residual && !h) || (scaled && !scales)) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: null device pointer");
-    DeviceGuard guard{int(device)};
-    if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
-    const NormArgs a{at<void>(x), at<void>(residual), at<void>(weight), at<void>(h), at<void>(y), at<void>(scales), rows, cols, eps};
-    cudaError_t e;
-    with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { e = launch_norm<decltype(t), decltype(w)>(a, scaled, stream_of(stream)); }); });
-    CUDA_TRY(e);
-    return 0;
+    return guarded([&]() -> int64_t {
+        if (!plain_type(dtype) || !plain_type(weight_dtype)) return fail(PTWM_RC_UNSUPPORTED, "rms_norm: x and weight are fp32, fp16 or bf16");
+        if (scaled > SCALE_BLOCK) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: unknown output scaling");
+        if (!cols || (scaled == SCALE_BLOCK && cols % 32)) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: rows must not be empty, and hold whole blocks of 32 for block scales");
+        if (rows > 0x7FFFFFFFull || cols > 0x7FFFFFFFull) return fail(PTWM_RC_UNSUPPORTED, "rms_norm: more than 2^31 - 1 rows or columns");
+        if (!rows) return 0;
+        if (!x || !weight || !y || (residual && !h) || (scaled && !scales)) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: null device pointer");
+        DeviceGuard guard{int(device)};
+        if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
+        const NormArgs a{at<void>(x), at<void>(residual), at<void>(weight), at<void>(h), at<void>(y), at<void>(scales), rows, cols, eps};
+        cudaError_t e;
+        with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { e = launch_norm<decltype(t), decltype(w)>(a, scaled, stream_of(stream)); }); });
+        CUDA_TRY(e);
+        return 0;
+    });
 }
 
 extern "C" uint64_t ptwm_b200_rms_norm_grad_scratch_bytes(uint64_t rows, uint64_t cols) { return grad_blocks(rows) * cols * 4; }
 
 extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t dy, uint64_t dh, uint64_t dx, uint64_t dweight, uint64_t scratch, uint64_t scratch_bytes,
                                            uint64_t rows, uint64_t cols, uint32_t dtype, uint32_t weight_dtype, float eps, uint32_t device, uint64_t stream) {
-    if (!plain_type(dtype) || !plain_type(weight_dtype)) return fail(PTWM_RC_UNSUPPORTED, "rms_norm_grad: tensors are fp32, fp16 or bf16");
-    if (!cols || rows > 0x7FFFFFFFull || cols > 0x7FFFFFFFull) return fail(PTWM_RC_UNSUPPORTED, "rms_norm_grad: rows of 1 to 2^31 - 1 values, at most as many of them");
-    if (rows && (!h || !weight || !dy || (!dx && !dweight))) return fail(PTWM_RC_INVALID_INPUT, "rms_norm_grad: null device pointer");
-    if (rows && dweight && (!scratch || scratch_bytes < ptwm_b200_rms_norm_grad_scratch_bytes(rows, cols))) return fail(PTWM_RC_BUFFER_TOO_SMALL, "rms_norm_grad: scratch too small");
-    DeviceGuard guard{int(device)};
-    if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
-    if (!rows) {
-        if (dweight) CUDA_TRY(cudaMemsetAsync(at<void>(dweight), 0, cols * (weight_dtype == DT_FP32 ? 4 : 2), stream_of(stream)));
+    return guarded([&]() -> int64_t {
+        if (!plain_type(dtype) || !plain_type(weight_dtype)) return fail(PTWM_RC_UNSUPPORTED, "rms_norm_grad: tensors are fp32, fp16 or bf16");
+        if (!cols || rows > 0x7FFFFFFFull || cols > 0x7FFFFFFFull) return fail(PTWM_RC_UNSUPPORTED, "rms_norm_grad: rows of 1 to 2^31 - 1 values, at most as many of them");
+        if (rows && (!h || !weight || !dy || (!dx && !dweight))) return fail(PTWM_RC_INVALID_INPUT, "rms_norm_grad: null device pointer");
+        if (rows && dweight && (!scratch || scratch_bytes < ptwm_b200_rms_norm_grad_scratch_bytes(rows, cols))) return fail(PTWM_RC_BUFFER_TOO_SMALL, "rms_norm_grad: scratch too small");
+        DeviceGuard guard{int(device)};
+        if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
+        if (!rows) {
+            if (dweight) CUDA_TRY(cudaMemsetAsync(at<void>(dweight), 0, cols * (weight_dtype == DT_FP32 ? 4 : 2), stream_of(stream)));
+            return 0;
+        }
+        const uint32_t blocks = grad_blocks(rows);
+        const NormGradArgs a{at<void>(h), at<void>(weight), at<void>(dy), at<void>(dh), at<void>(dx), dweight ? at<float>(scratch) : nullptr, at<void>(dweight), rows, cols, eps, blocks};
+        cudaError_t e;
+        with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { e = launch_norm_grad<decltype(t), decltype(w)>(a, stream_of(stream)); }); });
+        CUDA_TRY(e);
         return 0;
-    }
-    const uint32_t blocks = grad_blocks(rows);
-    const NormGradArgs a{at<void>(h), at<void>(weight), at<void>(dy), at<void>(dh), at<void>(dx), dweight ? at<float>(scratch) : nullptr, at<void>(dweight), rows, cols, eps, blocks};
-    cudaError_t e;
-    with_type(dtype, [&](auto t) { with_type(weight_dtype, [&](auto w) { e = launch_norm_grad<decltype(t), decltype(w)>(a, stream_of(stream)); }); });
-    CUDA_TRY(e);
-    return 0;
+    });
 }
 
 extern "C" uint64_t ptwm_b200_matvec_scratch_bytes(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t tokens, uint32_t x_dtype, uint32_t grad) {
@@ -346,42 +358,44 @@ extern "C" uint64_t ptwm_b200_matvec_scratch_bytes(const ptwm_b200_scaled_weight
 
 extern "C" int64_t ptwm_b200_matvec_group(const ptwm_b200_scaled_weight* const* weights, const uint64_t* y, uint32_t count, uint64_t x, uint64_t x_scales, uint64_t tokens,
                                           uint32_t x_dtype, uint32_t x_scaled, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, uint32_t device, uint64_t stream) {
-    ScaledMatrix w[FEW_MATRICES];
-    if (!weights || !y || !count) return fail(PTWM_RC_INVALID_INPUT, "matvec: no matrix");
-    if (count > FEW_MATRICES) return fail(PTWM_RC_UNSUPPORTED, "matvec: more than 4 matrices in a call");
-    uint64_t tiles = 0;
-    for (uint32_t i = 0; i < count; ++i) {
-        if (const int64_t rc = matrix_of(weights[i], &w[i]); rc < 0) return rc;
-        if (w[i].cols != w[0].cols) return fail(PTWM_RC_INVALID_INPUT, "matvec: matrices of a call have the same columns");
-        tiles += few_tiles(w[i]);
-    }
-    if (!plain_type(y_dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec: the output is fp32, fp16 or bf16");
-    if (x_dtype == DT_E4M3 ? (x_scaled != SCALE_ROW && x_scaled != SCALE_BLOCK) || !x_scales : !plain_type(x_dtype) || x_scaled)
-        return fail(PTWM_RC_UNSUPPORTED, "matvec: tokens are fp32, fp16, bf16, or E4M3 with scales per row or block");
-    if (x_scaled == SCALE_BLOCK && w[0].cols % 32) return fail(PTWM_RC_INVALID_INPUT, "matvec: block scales need whole blocks of 32 columns");
-    if (tokens > (1u << 19)) return fail(PTWM_RC_UNSUPPORTED, "matvec: more than 2^19 tokens in a call");
-    if (!tokens) return 0;
-    if (!x) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
-    for (uint32_t i = 0; i < count; ++i)
-        if (!y[i]) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
-    DeviceGuard guard{int(device)};
-    if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
-    TokenArgs t{at<void>(x), at<void>(x_scales), tokens, x_scaled, nullptr};
-    PerDevice dev;
-    if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
-    bool alike = true;
-    for (uint32_t i = 1; i < count; ++i) alike &= w[i].group == w[0].group;
-    if (alike)
-        if (const FewSplit s = few_split(w[0], uint32_t(tiles), tokens, x_dtype); s.depth)
-            return launch_few(w, y, count, uint32_t(tiles), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream));
-    for (uint32_t i = 0; i < count; ++i) {
-        const FewSplit s = few_split(w[i], few_tiles(w[i]), tokens, x_dtype);
-        t.y = at<void>(y[i]);
-        const int64_t rc = s.depth ? launch_few(&w[i], y + i, 1, few_tiles(w[i]), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream))
-                                   : launch_tiles<false>(w[i], t, x_dtype, y_dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
-        if (rc < 0) return rc;
-    }
-    return 0;
+    return guarded([&]() -> int64_t {
+        ScaledMatrix w[FEW_MATRICES];
+        if (!weights || !y || !count) return fail(PTWM_RC_INVALID_INPUT, "matvec: no matrix");
+        if (count > FEW_MATRICES) return fail(PTWM_RC_UNSUPPORTED, "matvec: more than 4 matrices in a call");
+        uint64_t tiles = 0;
+        for (uint32_t i = 0; i < count; ++i) {
+            if (const int64_t rc = matrix_of(weights[i], &w[i]); rc < 0) return rc;
+            if (w[i].cols != w[0].cols) return fail(PTWM_RC_INVALID_INPUT, "matvec: matrices of a call have the same columns");
+            tiles += few_tiles(w[i]);
+        }
+        if (!plain_type(y_dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec: the output is fp32, fp16 or bf16");
+        if (x_dtype == DT_E4M3 ? x_scaled != SCALE_ROW && x_scaled != SCALE_BLOCK : !plain_type(x_dtype) || x_scaled)
+            return fail(PTWM_RC_UNSUPPORTED, "matvec: tokens are fp32, fp16, bf16, or E4M3 with scales per row or block");
+        if (x_scaled == SCALE_BLOCK && w[0].cols % 32) return fail(PTWM_RC_INVALID_INPUT, "matvec: block scales need whole blocks of 32 columns");
+        if (tokens > (1u << 19)) return fail(PTWM_RC_UNSUPPORTED, "matvec: more than 2^19 tokens in a call");
+        if (!tokens) return 0;
+        if (!x || (x_scaled && !x_scales)) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
+        for (uint32_t i = 0; i < count; ++i)
+            if (!y[i]) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
+        DeviceGuard guard{int(device)};
+        if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
+        TokenArgs t{at<void>(x), at<void>(x_scales), tokens, x_scaled, nullptr};
+        PerDevice dev;
+        if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
+        bool alike = true;
+        for (uint32_t i = 1; i < count; ++i) alike &= w[i].group == w[0].group;
+        if (alike)
+            if (const FewSplit s = few_split(w[0], uint32_t(tiles), tokens, x_dtype); s.depth)
+                return launch_few(w, y, count, uint32_t(tiles), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream));
+        for (uint32_t i = 0; i < count; ++i) {
+            const FewSplit s = few_split(w[i], few_tiles(w[i]), tokens, x_dtype);
+            t.y = at<void>(y[i]);
+            const int64_t rc = s.depth ? launch_few(&w[i], y + i, 1, few_tiles(w[i]), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream))
+                                       : launch_tiles<false>(w[i], t, x_dtype, y_dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
+            if (rc < 0) return rc;
+        }
+        return 0;
+    });
 }
 
 extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint64_t x, uint64_t x_scales, uint64_t y, uint64_t tokens, uint32_t x_dtype, uint32_t x_scaled,
@@ -391,16 +405,18 @@ extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint6
 
 extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dtype, uint64_t scratch, uint64_t scratch_bytes,
                                          uint32_t device, uint64_t stream) {
-    ScaledMatrix w;
-    if (const int64_t rc = matrix_of(weight, &w); rc < 0) return rc;
-    if (!plain_type(dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec_grad: gradients are fp32, fp16 or bf16");
-    if (tokens > (1u << 19)) return fail(PTWM_RC_UNSUPPORTED, "matvec_grad: more than 2^19 tokens in a call");
-    if (!tokens) return 0;
-    if (!dy || !dx) return fail(PTWM_RC_INVALID_INPUT, "matvec_grad: null device pointer");
-    DeviceGuard guard{int(device)};
-    if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
-    const TokenArgs t{at<void>(dy), nullptr, tokens, SCALE_NONE, at<void>(dx)};
-    PerDevice dev;
-    if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
-    return launch_tiles<true>(w, t, dtype, dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
+    return guarded([&]() -> int64_t {
+        ScaledMatrix w;
+        if (const int64_t rc = matrix_of(weight, &w); rc < 0) return rc;
+        if (!plain_type(dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec_grad: gradients are fp32, fp16 or bf16");
+        if (tokens > (1u << 19)) return fail(PTWM_RC_UNSUPPORTED, "matvec_grad: more than 2^19 tokens in a call");
+        if (!tokens) return 0;
+        if (!dy || !dx) return fail(PTWM_RC_INVALID_INPUT, "matvec_grad: null device pointer");
+        DeviceGuard guard{int(device)};
+        if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
+        const TokenArgs t{at<void>(dy), nullptr, tokens, SCALE_NONE, at<void>(dx)};
+        PerDevice dev;
+        if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
+        return launch_tiles<true>(w, t, dtype, dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
+    });
 }

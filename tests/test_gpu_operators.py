@@ -503,6 +503,18 @@ def test_projections_of_several_matrices(tokens, quant, sizes):
         assert y.shape == (tokens, n) and torch.equal(y, matvec(same, w, out_dtype=torch.bfloat16))
 
 
+@pytest.mark.parametrize("quant", [None, "row", "block"])
+@pytest.mark.parametrize("shape", [(512,), (3, 512), (2, 3, 512), (0, 512), (2, 0, 512)])
+def test_projections_of_any_number_of_dimensions(shape, quant):
+    w = ScaledWeight(*_matrix(256, 512, "mxfp4", 3))
+    norm = torch.ones(512, device="cuda", dtype=torch.bfloat16)
+    x = torch.randn(*shape, generator=_gen(3), device="cuda").to(torch.bfloat16)
+    (y,), h = Projection(norm, [w], quant=quant)(x, x)
+    q, k = rms_norm(x, norm, residual=x, quant=quant)
+    assert y.shape == (*shape[:-1], 256) and h.shape == x.shape and torch.equal(h, k)
+    assert torch.equal(y, matvec(q, w))
+
+
 def test_a_token_does_not_depend_on_its_neighbours():
     """The same token gives the same bits beside others that hold infinities, as long as as many are asked for."""
     w = ScaledWeight(*_matrix(200, 2048, "nvfp4", 3))

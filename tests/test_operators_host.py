@@ -40,7 +40,7 @@ def test_tokens_that_are_none(L):
     w = _weight()
     p = C.addressof(w)
     nv = _weight(cols=48, group=16, value_pitch=32)
-    for args, rc in [((p, A, 0, A, 1, 6, 0, 13), UNSUPPORTED), ((p, A, 0, A, 1, 13, 0, 6), UNSUPPORTED), ((p, A, A, A, 1, 6, 1, 6), UNSUPPORTED), ((p, A, 0, A, 1, 29, 1, 6), UNSUPPORTED),
+    for args, rc in [((p, A, 0, A, 1, 6, 0, 13), UNSUPPORTED), ((p, A, 0, A, 1, 13, 0, 6), UNSUPPORTED), ((p, A, A, A, 1, 6, 1, 6), UNSUPPORTED), ((p, A, 0, A, 1, 29, 1, 6), INVALID),
                      ((p, A, A, A, 1, 29, 0, 6), UNSUPPORTED), ((p, A, A, A, 1, 29, 3, 6), UNSUPPORTED), ((p, 0, 0, A, 1, 6, 0, 6), INVALID), ((p, A, 0, 0, 1, 6, 0, 6), INVALID),
                      ((p, A, 0, A, (1 << 19) + 1, 6, 0, 6), UNSUPPORTED), ((C.addressof(nv), A, A, A, 1, 29, 2, 6), INVALID), ((None, A, 0, A, 1, 6, 0, 6), INVALID)]:
         assert L.ptwm_b200_matvec(*args, 0, 0, 0, 1) == rc, args
@@ -51,6 +51,7 @@ def test_tokens_that_are_none(L):
     refs[1] = p
     assert L.ptwm_b200_matvec_group(refs, ys, 3, A, 0, 1, 6, 0, 6, 0, 0, 0, 1) == INVALID
     assert L.ptwm_b200_matvec(p, 0, 0, 0, 0, 6, 0, 6, 0, 0, 0, 1) == 0  # no tokens: nothing to do, on any machine
+    assert L.ptwm_b200_matvec(p, 0, 0, 0, 0, 29, 2, 6, 0, 0, 0, 1) == 0
     for args, rc in [((p, A, A, 1, 29), UNSUPPORTED), ((p, 0, A, 1, 6), INVALID), ((p, A, 0, 1, 6), INVALID)]:
         assert L.ptwm_b200_matvec_grad(*args, 0, 0, 0, 1) == rc, args
 
