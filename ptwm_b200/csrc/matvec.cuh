@@ -24,11 +24,6 @@ struct TokenArgs {
     void* y;
 };
 
-__device__ __forceinline__ float group_scale(const ScaledMatrix& w, uint64_t row, uint64_t k) {
-    const uint8_t s = w.scales[row * w.scale_pitch + k / w.group];
-    return w.group == 32 ? e8m0_f32(s) : e4m3_f32(s);
-}
-
 template <class T> __device__ __forceinline__ float token_value(const TokenArgs& t, uint64_t m, uint64_t k, uint64_t cols) {
     return to_f32(static_cast<const T*>(t.x)[m * cols + k]);
 }

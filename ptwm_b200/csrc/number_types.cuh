@@ -1,4 +1,4 @@
-// The number types of the operators: fp32, fp16, bf16 (public dtype codes 1, 4, 6), E4M3 with scales, and E2M1 nibbles.
+// The number types of the operators: fp32, fp16 and bf16 (public dtype codes 1, 4, 6), and E4M3 with scales.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -21,6 +21,14 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two 16-bit values of a word, the first in its lower half.
+template <class T> __device__ __forceinline__ float2 two_f32(uint32_t w);
+template <> __device__ __forceinline__ float2 two_f32<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <> __device__ __forceinline__ float2 two_f32<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+template <class T> __device__ __forceinline__ uint32_t two_rounded(float2 v);
+template <> __device__ __forceinline__ uint32_t two_rounded<__half>(float2 v) { const __half2 h = __float22half2_rn(v); return *reinterpret_cast<const uint32_t*>(&h); }
+template <> __device__ __forceinline__ uint32_t two_rounded<__nv_bfloat16>(float2 v) { const __nv_bfloat162 h = __float22bfloat162_rn(v); return *reinterpret_cast<const uint32_t*>(&h); }
+
 // Programmatic dependent launch.  A kernel of these operators may start while the one before it in the stream ends: it does nothing but
 // find its place and make its barriers until after_those_before(), where all that was enqueued before it is done and can be seen.
 // The one behind it may start from others_may_start() on.
@@ -33,12 +41,5 @@ __device__ __forceinline__ float e8m0_f32(uint32_t e) { return e == 255 ? __uint
 __device__ __forceinline__ float e4m3_f32(uint8_t v) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3))); }
 // Nearest E4M3 value, ties to even; beyond 448 it is 448, NaN stays NaN.
 __device__ __forceinline__ uint8_t f32_e4m3(float v) { return uint8_t(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3)); }
-
-// E2M1: a sign, two bits of exponent with bias 1, one of mantissa; 0 and 0.5 are its subnormals.
-__device__ __forceinline__ float e2m1_f32(uint32_t c) {
-    const uint32_t e = (c >> 1) & 3, m = c & 1;
-    const float v = e ? __uint_as_float(((126 + e) << 23) | (m << 22)) : 0.5f * float(m);
-    return (c & 8) ? -v : v;
-}
 
 }  // namespace ptwm
