@@ -139,22 +139,33 @@ template <class T, class W> cudaError_t launch_norm(const NormArgs& a, uint32_t 
     const uint32_t rows = uint32_t(a.rows);
     cudaError_t e = cudaSuccess;
     if (scaled == SCALE_NONE ? launch_norm_rows<T, W, SCALE_NONE>(a, st, e) : scaled == SCALE_ROW ? launch_norm_rows<T, W, SCALE_ROW>(a, st, e) : launch_norm_rows<T, W, SCALE_BLOCK>(a, st, e)) return e;
-    if (scaled != SCALE_BLOCK && a.cols <= 16 * 1024) e = enqueue(rms_norm_odd_rows_kernel<T, W, 16>, dim3(rows), warps_for((a.cols + 15) / 16), 0, 1, st, a, scaled);
+    constexpr uint64_t V = 16 / sizeof(T);
+    const uint64_t pieces = a.cols / V + 2;   // of the whole tensor that a row has a share of, at most
+    if (scaled != SCALE_BLOCK && pieces <= 2048 && aligned(a.x) && aligned(a.residual) && aligned(a.weight) && aligned(a.h) && aligned(a.y)) {
+        const uint32_t threads = warps_for((pieces + 1) / 2);
+        e = enqueue(rms_norm_between_kernel<T, W>, dim3(std::min<uint32_t>(rows, 148 * std::max(1u, 1024 / threads))), threads, 0, 1, st, a, scaled);
+    } else if (scaled != SCALE_BLOCK && a.cols <= 16 * 1024) e = enqueue(rms_norm_odd_rows_kernel<T, W, 16>, dim3(rows), warps_for((a.cols + 15) / 16), 0, 1, st, a, scaled);
     else e = enqueue(rms_norm_long_kernel<T, W>, dim3(rows), 256, 0, 1, st, a, scaled);
     return e;
 }
 
-// Blocks of a gradient: each writes its share of dweight, so no more than fill the GPU.
-uint32_t grad_blocks(uint64_t rows) { return uint32_t(std::min<uint64_t>(rows, 296)); }
+// Blocks of a gradient: each writes its share of dweight, so no more than fill the GPU.  296 rows on, a row begins at the same place of 16 bytes.
+constexpr uint32_t GRAD_BLOCKS = 296;
+static_assert(GRAD_BLOCKS % 8 == 0, "");
+uint32_t grad_blocks(uint64_t rows) { return uint32_t(std::min<uint64_t>(rows, GRAD_BLOCKS)); }
 
+template <class T, class W, bool BETWEEN> bool launch_norm_grad_rows(const NormGradArgs& a, uint64_t pieces, cudaStream_t st, cudaError_t& e) {
+    if (pieces <= 512) e = enqueue(rms_norm_grad_rows_kernel<T, W, 1, 512, BETWEEN>, dim3(a.blocks), warps_for(pieces), 0, 1, st, a);
+    else if (pieces <= 1024) e = enqueue(rms_norm_grad_rows_kernel<T, W, 2, 512, BETWEEN>, dim3(a.blocks), warps_for((pieces + 1) / 2), 0, 1, st, a);
+    else if (pieces <= 2048) e = enqueue(rms_norm_grad_rows_kernel<T, W, 2, 1024, BETWEEN>, dim3(a.blocks), warps_for((pieces + 1) / 2), 0, 1, st, a);
+    else return false;
+    return true;
+}
 template <class T, class W> cudaError_t launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
     cudaError_t e;
     constexpr uint64_t V = 16 / sizeof(T);
-    const bool wide = a.cols % V == 0 && aligned(a.h) && aligned(a.weight) && aligned(a.dy) && aligned(a.dh) && aligned(a.dx) && aligned(a.partial);
-    const uint64_t pieces = a.cols / V;
-    if (wide && pieces <= 512) e = enqueue(rms_norm_grad_rows_kernel<T, W, 1, 512>, dim3(a.blocks), warps_for(pieces), 0, 1, st, a);
-    else if (wide && pieces <= 1024) e = enqueue(rms_norm_grad_rows_kernel<T, W, 2, 512>, dim3(a.blocks), warps_for((pieces + 1) / 2), 0, 1, st, a);
-    else if (wide && pieces <= 2048) e = enqueue(rms_norm_grad_rows_kernel<T, W, 2, 1024>, dim3(a.blocks), warps_for((pieces + 1) / 2), 0, 1, st, a);
+    const bool wide = aligned(a.h) && aligned(a.weight) && aligned(a.dy) && aligned(a.dh) && aligned(a.dx) && aligned(a.partial);
+    if (wide && (a.cols % V ? launch_norm_grad_rows<T, W, true>(a, a.cols / V + 2, st, e) : launch_norm_grad_rows<T, W, false>(a, a.cols / V, st, e))) {}
     else e = enqueue(rms_norm_grad_long_kernel<T, W>, dim3(a.blocks), 512, 0, 1, st, a);
     if (a.dweight && e == cudaSuccess) e = enqueue(rms_norm_grad_weight_kernel<W>, dim3(uint32_t((a.cols + 31) / 32)), 1024, 0, 1, st, a);
     return e;

@@ -128,6 +128,34 @@ template <class T> __device__ __forceinline__ typename std::conditional<Piece<T>
 }
 __device__ __forceinline__ float max_magnitude(float a, float2 b) { return max_magnitude(max_magnitude(a, b.x), b.y); }
 
+template <class T> __device__ __forceinline__ void times(Piece<T>& p, float f) {
+#pragma unroll
+    for (int k = 0; k < Piece<T>::P; ++k) p.v[k] = __fmul2_rn(p.v[k], make_float2(f, f));
+}
+
+// A row's way into E4M3, from its largest |h weight| and r.
+struct RowScale {
+    float most, r, top, inverse;
+    __device__ __forceinline__ RowScale(float most, float r) : most(most), r(r), top(most * r), inverse(0) {
+        if (is_finite(top) && top > 0x1p-100f && most > 0x1p-100f) inverse = 448.0f / most;  // nearly always: a product for a division
+    }
+    __device__ __forceinline__ float scale() const { return is_finite(top) ? top / 448.0f : __uint_as_float(0x7FC00000u); }
+    template <class T, int N> __device__ __forceinline__ void apply(Piece<T> (&t)[N]) const {
+        if (inverse != 0.0f) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) times(t[j], inverse);
+            return;
+        }
+        // part is 0 only where s is, and not finite only where s is not
+        const float s = scale(), part = most / 448.0f;
+        auto divided = [&](float v) { return s == 0.0f ? 0.0f : s == s ? v / part : s; };
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int k = 0; k < Piece<T>::P; ++k) t[j].v[k] = make_float2(divided(t[j].v[k].x), divided(t[j].v[k].y));
+    }
+};
+
 // Rows that start at multiples of 16 bytes.  Bound by memory, so everything is read once and a row stays in registers: N pieces of 16
 // bytes to a thread, a row to 16 or 32 lanes (LANES) or to a block (0), which has the next row on its way while it reduces one.  One reduction is
 // enough for any output: with t = h weight the largest |y| is r times the largest |t| (rounding keeps the order), and
@@ -189,11 +217,7 @@ __global__ void __launch_bounds__(LANES ? 256 : 1024) rms_norm_rows_kernel(NormA
         float sum = sums.x + sums.y;
         ask(row + step);
         reduce<false, QUANT == SCALE_ROW, LANES == 16 ? 16 : 32>(sum, most, WARP ? 1 : lanes / 32, shared[turn]);
-        const float r = __frsqrt_rn(sum / float(a.cols) + a.eps), nan = __uint_as_float(0x7FC00000u);
-        auto times = [](Piece<T>& p, float f) {
-#pragma unroll
-            for (int k = 0; k < P; ++k) p.v[k] = __fmul2_rn(p.v[k], make_float2(f, f));
-        };
+        const float r = __frsqrt_rn(sum / float(a.cols) + a.eps);
         if constexpr (QUANT == SCALE_NONE) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
@@ -204,22 +228,9 @@ __global__ void __launch_bounds__(LANES ? 256 : 1024) rms_norm_rows_kernel(NormA
         } else {
             auto* q = static_cast<decltype(pack_e4m3(t[0]))*>(a.y) + row * pieces;
             if constexpr (QUANT == SCALE_ROW) {
-                const float top = most * r;
-                auto scale = [&] { return is_finite(top) ? top / 448.0f : nan; };
-                if (there && at == 0) static_cast<float*>(a.scales)[row] = scale();
-                if (is_finite(top) && top > 0x1p-100f && most > 0x1p-100f) {  // nearly always: a product for a division
-                    const float inverse = 448.0f / most;
-#pragma unroll
-                    for (int j = 0; j < N; ++j) times(t[j], inverse);
-                } else {
-                    // part is 0 only where s is, and not finite only where s is not
-                    const float s = scale(), part = most / 448.0f;
-                    auto divided = [&](float v) { return s == 0.0f ? 0.0f : s == s ? v / part : nan; };
-#pragma unroll
-                    for (int j = 0; j < N; ++j)
-#pragma unroll
-                        for (int k = 0; k < P; ++k) t[j].v[k] = make_float2(divided(t[j].v[k].x), divided(t[j].v[k].y));
-                }
+                const RowScale scale(most, r);
+                if (there && at == 0) static_cast<float*>(a.scales)[row] = scale.scale();
+                scale.apply(t);
             }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
@@ -241,7 +252,174 @@ __global__ void __launch_bounds__(LANES ? 256 : 1024) rms_norm_rows_kernel(NormA
     }
 }
 
-// Rows that start anywhere, a value at a time: N values to a thread, a row to a block.
+// The weights from number `o` on, which may begin before the first and end behind the last of them: zeros there.  Pieces that cover them are
+// put in place by whole words and then by half of one; the block's threads have the same way to go.
+template <class T, class W> __device__ __forceinline__ Piece<T> weights_from(const void* weight, int o, int cols) {
+    constexpr int V = Piece<T>::V, G = sizeof(W) == 2 ? V : 4, WORDS = G * int(sizeof(W)) / 4, PIECES = V / G + 1, HALF = 4 / int(sizeof(W));
+    Piece<T> p;
+    const int first = (o >= 0 ? o : o - G + 1) / G, s = o - first * G;
+    if (first >= 0 && (first + PIECES) * G <= cols) {
+        uint32_t w[WORDS * PIECES];
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j)
+            if constexpr (WORDS == 4) {
+                const uint4 v = __ldg(static_cast<const uint4*>(weight) + first + j);
+                w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+            } else {
+                const uint2 v = __ldg(static_cast<const uint2*>(weight) + first + j);
+                w[2 * j] = v.x; w[2 * j + 1] = v.y;
+            }
+#pragma unroll
+        for (int b = WORDS / 2; b; b /= 2)
+            if (s & (b * HALF)) {
+#pragma unroll
+                for (int j = 0; j + b < WORDS * PIECES; ++j) w[j] = w[j + b];
+            }
+        if constexpr (HALF == 2) {
+            if (s & 1) {
+#pragma unroll
+                for (int j = 0; j + 1 < WORDS * PIECES; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
+            }
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) p.v[k] = two_f32<W>(w[k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) p.v[k] = make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+        }
+    } else {
+        auto one = [&](int k) { return k >= 0 && k < cols ? to_f32(static_cast<const W*>(weight)[k]) : 0.0f; };
+#pragma unroll
+        for (int k = 0; k < V / 2; ++k) p.v[k] = make_float2(one(o + 2 * k), one(o + 2 * k + 1));
+    }
+    return p;
+}
+
+// A piece of a tensor of so many values, whose last one may be cut short.
+template <class T> __device__ __forceinline__ uint4 load_piece(const T* p, uint64_t piece, uint64_t values) {
+    constexpr int V = Piece<T>::V;
+    if ((piece + 1) * V <= values) return __ldcs(reinterpret_cast<const uint4*>(p) + piece);
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (piece * V + k < values) {
+            if constexpr (V == 4) w[k] = __float_as_uint(p[piece * V + k]);
+            else w[k / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(p)[piece * V + k]) << (k % 2 * 16);
+        }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Of a piece whose first value has place `o` in a row (which may be before it): what is the row's, to memory, or with zeros for the rest.
+template <class T> __device__ __forceinline__ void store_piece(T* to, int o, int cols, const uint4& w) {
+    constexpr int V = Piece<T>::V;
+    if (o >= 0 && o + V <= cols) {
+        *reinterpret_cast<uint4*>(to) = w;
+        return;
+    }
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (o + k >= 0 && o + k < cols) {
+            if constexpr (V == 4) to[k] = __uint_as_float(words[k]);
+            else reinterpret_cast<uint16_t*>(to)[k] = uint16_t(words[k / 2] >> (k % 2 * 16));
+        }
+}
+template <class T> __device__ __forceinline__ void keep_own(Piece<T>& p, int o, int cols) {
+    if (o >= 0 && o + Piece<T>::V <= cols) return;
+    auto own = [&](int k) { return o + k >= 0 && o + k < cols; };
+#pragma unroll
+    for (int k = 0; k < Piece<T>::P; ++k) p.v[k] = make_float2(own(2 * k) ? p.v[k].x : 0.0f, own(2 * k + 1) ? p.v[k].y : 0.0f);
+}
+
+// Rows of a length that no piece divides, in tensors that start at multiples of 16 bytes: the pieces are those of the whole tensor, so that
+// everything but the weights still moves 16 bytes at a time; of the two at a row's ends, which belong to its neighbours as well, a
+// block takes what is its own.  Two pieces to a thread, a row to a block, with the next one on its way.
+//   8192 rows of 4097 bf16 with a residual into E4M3: 56.5 us, 4.2 TB/s (131.7 with a value to a load); 333 of 10501 fp16: 8.7 us (12.4), of
+// which a row from memory to memory by itself takes 3.7.  Bound by instructions, two a value of them to put the weights in place.
+template <class T, class W>
+__global__ void __launch_bounds__(1024) rms_norm_between_kernel(NormArgs a, uint32_t quant) {
+    constexpr int V = Piece<T>::V, P = Piece<T>::P, N = 2;
+    __shared__ __align__(16) float shared[2][2][32];
+    const uint32_t at = threadIdx.x, lanes = blockDim.x;
+    const int cols = int(a.cols);
+    const uint64_t values = a.rows * a.cols;
+    const T *xs = static_cast<const T*>(a.x), *rs = static_cast<const T*>(a.residual);
+    uint4 in[N], more[N];
+    auto ask = [&](uint64_t row) {
+        const uint64_t first = row * a.cols / V, end = (row + 1) * a.cols;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint64_t piece = first + at + j * lanes;
+            in[j] = more[j] = make_uint4(0, 0, 0, 0);
+            if (row < a.rows && piece * V < end) {
+                in[j] = load_piece(xs, piece, values);
+                if (rs) more[j] = load_piece(rs, piece, values);
+            }
+        }
+    };
+    others_may_start();
+    after_those_before();
+    ask(blockIdx.x);
+    uint32_t turn = 0;
+    for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const uint64_t first = row * a.cols / V;
+        const int before = int(row * a.cols % V);   // values of the first piece that are the row's before
+        Piece<T> t[N];
+        float2 sums = {};
+        float most = 0;
+        auto place = [&](int j) { return int(at + j * lanes) * V - before; };  // of a piece in its row
+        auto number = [&](int j) { return (first + at + j * lanes) * V; };            // of its first value in the tensor
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int o = place(j);
+            Piece<T> h = numbers<T>(in[j]);
+            if (rs) {
+                const Piece<T> r = numbers<T>(more[j]);
+#pragma unroll
+                for (int k = 0; k < P; ++k) h.v[k] = __fadd2_rn(h.v[k], r.v[k]);
+                const uint4 stored = rounded<T>(h);
+                store_piece(static_cast<T*>(a.h) + number(j), o, cols, stored);
+                h = numbers<T>(stored);
+            }
+            keep_own(h, o, cols);
+            const Piece<T> w = weights_from<T, W>(a.weight, o, cols);
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                sums = __ffma2_rn(h.v[k], h.v[k], sums);
+                t[j].v[k] = __fmul2_rn(h.v[k], w.v[k]);
+                most = max_magnitude(most, t[j].v[k]);
+            }
+        }
+        ask(row + gridDim.x);
+        float sum = sums.x + sums.y;
+        reduce<false, true>(sum, most, lanes / 32, shared[turn]);
+        const RowScale scale(most, __frsqrt_rn(sum / float(a.cols) + a.eps));
+        if (quant == SCALE_ROW) {
+            if (at == 0) static_cast<float*>(a.scales)[row] = scale.scale();
+            scale.apply(t);
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (quant == SCALE_NONE) {
+                times(t[j], scale.r);
+                store_piece(static_cast<T*>(a.y) + number(j), place(j), cols, rounded<T>(t[j]));
+                continue;
+            }
+            const int o = place(j);
+            const auto q = pack_e4m3(t[j]);
+            uint8_t* to = static_cast<uint8_t*>(a.y) + number(j);
+            if (o >= 0 && o + V <= cols) *reinterpret_cast<decltype(pack_e4m3(t[j]))*>(to) = q;
+            else {
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    if (o + k >= 0 && o + k < cols) {
+                        if constexpr (V == 4) to[k] = uint8_t(q >> (k * 8));
+                        else to[k] = uint8_t((k < 4 ? q.x : q.y) >> (k % 4 * 8));
+                    }
+            }
+        }
+    }
+}
+
+// Rows that start anywhere (8192 of 4097 bf16 with a residual: 131.7 us), a value at a time: N values to a thread, a row to a block.
 template <class T, class W, int N>
 __global__ void __launch_bounds__(1024, 2) rms_norm_odd_rows_kernel(NormArgs a, uint32_t quant) {
     __shared__ __align__(16) float shared[2][32];
@@ -339,11 +517,17 @@ struct NormGradArgs {
 // dweight in registers; with 512 of them the next row is asked for before this one's reduction, which 64 registers of 1024 do not hold.
 // Bound by memory and, at half its rate, by what a row waits for its reduction: 4096 rows of 4096 with the residual's gradient take 29.4 us
 // in bf16 (4.6 TB/s; 31.3 with a value at a time), 47.9 in fp32 (5.6 TB/s), the weights' sum with it.
-template <class T, class W, int N, int MOST>
+// BETWEEN: rows of a length that no piece divides, with the pieces of the whole tensor.  The blocks are as many as makes each one's rows
+// begin at the same place of a piece, so a thread has the same columns in all of them (4096 rows of 4097: 64 us, 170 a value at a time).
+template <class T, class W, int N, int MOST, bool BETWEEN>
 __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kernel(NormGradArgs a) {
     constexpr int V = Piece<T>::V, P = Piece<T>::P;
     __shared__ __align__(16) float shared[2][2][32];
-    const uint32_t lanes = blockDim.x, at = threadIdx.x, pieces = uint32_t(a.cols / V);
+    const uint32_t lanes = blockDim.x, at = threadIdx.x;
+    const int cols = int(a.cols), before = BETWEEN ? int(blockIdx.x * a.cols % V) : 0;
+    const uint32_t pieces = uint32_t(cols + before + (BETWEEN ? V - 1 : 0)) / V;
+    const uint64_t values = a.rows * a.cols;
+    auto place = [&](int j) { return int(at + j * lanes) * V - before; };
     const uint4 *hs = static_cast<const uint4*>(a.h), *dys = static_cast<const uint4*>(a.dy), *dhs = static_cast<const uint4*>(a.dh);
     uint4 h[N], dy[N], dh[N];
     auto ask = [&](uint64_t row) {
@@ -352,15 +536,25 @@ __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kerne
             const uint32_t i = at + j * lanes;
             h[j] = dy[j] = dh[j] = make_uint4(0, 0, 0, 0);
             if (row < a.rows && i < pieces) {
-                h[j] = __ldcs(hs + row * pieces + i);
-                dy[j] = __ldcs(dys + row * pieces + i);
-                if (dhs) dh[j] = __ldcs(dhs + row * pieces + i);
+                if constexpr (BETWEEN) {
+                    const uint64_t piece = row * a.cols / V + i;
+                    h[j] = load_piece(static_cast<const T*>(a.h), piece, values);
+                    dy[j] = load_piece(static_cast<const T*>(a.dy), piece, values);
+                    if (dhs) dh[j] = load_piece(static_cast<const T*>(a.dh), piece, values);
+                } else {
+                    h[j] = __ldcs(hs + row * pieces + i);
+                    dy[j] = __ldcs(dys + row * pieces + i);
+                    if (dhs) dh[j] = __ldcs(dhs + row * pieces + i);
+                }
             }
         }
     };
     Piece<T> dw[N] = {}, kept;
     // the weights: in registers where a thread has one piece, else again for every use (they stay in the L1)
-    auto weights_of = [&](int j) { return at + j * lanes < pieces ? weights<T, W>(a.weight, at + j * lanes) : zeros<T>(); };
+    auto weights_of = [&](int j) {
+        if constexpr (BETWEEN) return weights_from<T, W>(a.weight, place(j), cols);
+        else return at + j * lanes < pieces ? weights<T, W>(a.weight, at + j * lanes) : zeros<T>();
+    };
     others_may_start();
     after_those_before();
     if (N == 1) kept = weights_of(0);
@@ -375,6 +569,10 @@ __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kerne
         for (int j = 0; j < N; ++j) {
             v[j] = numbers<T>(h[j]);
             d[j] = numbers<T>(dy[j]);
+            if (BETWEEN) {
+                keep_own(v[j], place(j), cols);
+                keep_own(d[j], place(j), cols);
+            }
             r0[j] = dh[j];
             const Piece<T> w = N > 1 ? weights_of(j) : kept;
 #pragma unroll
@@ -403,14 +601,25 @@ __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kerne
 #pragma unroll
                 for (int k = 0; k < P; ++k) g.v[k] = __fadd2_rn(g.v[k], e.v[k]);
             }
-            if (a.dx && i < pieces) static_cast<uint4*>(a.dx)[row * pieces + i] = rounded<T>(g);
+            if (a.dx && i < pieces) {
+                if constexpr (BETWEEN) store_piece(static_cast<T*>(a.dx) + (row * a.cols / V + i) * V, place(j), cols, rounded<T>(g));
+                else static_cast<uint4*>(a.dx)[row * pieces + i] = rounded<T>(g);
+            }
         }
     }
     if (a.partial)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const uint32_t i = at + j * lanes;
-            if (i < pieces)
+            if (BETWEEN) {
+                float* to = a.partial + blockIdx.x * a.cols + place(j);
+                auto own = [&](int k) { return place(j) + k >= 0 && place(j) + k < cols; };
+#pragma unroll
+                for (int k = 0; k < P; ++k) {
+                    if (own(2 * k)) to[2 * k] = dw[j].v[k].x;
+                    if (own(2 * k + 1)) to[2 * k + 1] = dw[j].v[k].y;
+                }
+            } else if (i < pieces)
 #pragma unroll
                 for (int k = 0; k < P; k += 2) *reinterpret_cast<float4*>(a.partial + blockIdx.x * a.cols + i * V + k * 2) = make_float4(dw[j].v[k].x, dw[j].v[k].y, dw[j].v[k + 1].x, dw[j].v[k + 1].y);
         }

@@ -140,6 +140,40 @@ def test_norm_of_zeros_infinities_and_nan(quant):
         assert torch.equal(plain.values.view(torch.uint8)[0], again.values.view(torch.uint8)[5])
 
 
+@pytest.mark.parametrize("rows, cols", [(1, 5), (40, 1), (37, 9), (21, 17), (9, 513), (700, 333), (5, 4095), (3, 8190), (2, 8191), (5, 16367), (2, 16383)])
+@pytest.mark.parametrize("dtype, weight_dtype", [("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "fp32"), ("fp32", "fp32"), ("fp32", "fp16")])
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("quant", [None, "row"])
+def test_norm_rows_that_share_pieces_with_their_neighbours(rows, cols, dtype, weight_dtype, residual, quant):
+    """Rows of a length that no 16 bytes divide; every second one, and all that lies around them, is NaN."""
+    dt = DT[dtype]
+    x, res, w = _inputs(rows, cols, dt, rows * 7 + cols, residual, DT[weight_dtype])
+    front = 48  # values, whole pieces
+    held = []
+    for t in (x, res):
+        if t is None:
+            held.append(None)
+            continue
+        wide = torch.full((front + 2 * rows * cols + 64,), math.nan, dtype=dt, device="cuda")
+        inside = wide[front:front + 2 * rows * cols].view(2 * rows, cols)
+        inside[::2] = t
+        held.append(inside)
+    got = rms_norm(held[0], w, 1e-5, residual=held[1], quant=quant)
+    y, h = got if residual else (got, None)
+    want_h, want = _norm64(x, w, 1e-5, res)
+    if residual:
+        assert torch.equal(h[::2], want_h) and bool(torch.isnan(h[1::2]).all())
+    if quant is None:
+        assert bool(torch.isnan(y[1::2]).all())
+        tol = (_half_step(dt) + _norm_slack(cols)) * want.abs() + _floor(dt)
+        assert bool(((y[::2].double() - want).abs() <= tol).all())
+    else:
+        assert bool(torch.isnan(y.scales[1::2]).all()) and bool(torch.isnan(y.values[1::2].float()).all())
+        s = want.abs().amax(-1) / 448
+        assert bool(((y.scales[::2].double() - s).abs() <= (_norm_slack(cols) + 2 * F32) * s).all())
+        _check_8(y.values[::2], y.scales[::2].double()[:, None], want, 2 * _norm_slack(cols), None)
+
+
 def test_norm_strides_offsets_and_empty_rows():
     base = torch.randn(9, 517, generator=_gen(2), device="cuda").to(torch.bfloat16)
     w = torch.randn(1030, generator=_gen(3), device="cuda").to(torch.bfloat16)
@@ -153,7 +187,7 @@ def test_norm_strides_offsets_and_empty_rows():
         assert y.shape == (0, 512) and h.shape == (0, 512)
 
 
-@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 7), (5, 96), (1, 4096), (700, 1000), (333, 4095), (2, 10501), (3, 16384), (2, 40000)])
+@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 7), (5, 96), (1, 4096), (700, 1000), (333, 4095), (2, 10501), (3, 16384), (2, 40000), (1000, 333), (600, 4097), (297, 8191), (299, 16367), (900, 5)])
 @pytest.mark.parametrize("dtype, weight_dtype", [("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp32")])
 @pytest.mark.parametrize("residual", [True, False])
 def test_norm_gradient(rows, cols, dtype, weight_dtype, residual):
