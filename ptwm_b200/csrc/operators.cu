@@ -141,7 +141,10 @@ template <class T, class W> cudaError_t launch_norm(const NormArgs& a, uint32_t 
     if (scaled == SCALE_NONE ? launch_norm_rows<T, W, SCALE_NONE>(a, st, e) : scaled == SCALE_ROW ? launch_norm_rows<T, W, SCALE_ROW>(a, st, e) : launch_norm_rows<T, W, SCALE_BLOCK>(a, st, e)) return e;
     constexpr uint64_t V = 16 / sizeof(T);
     const uint64_t pieces = a.cols / V + 2;   // of the whole tensor that a row has a share of, at most
-    if (scaled != SCALE_BLOCK && pieces <= 2048 && aligned(a.x) && aligned(a.residual) && aligned(a.weight) && aligned(a.h) && aligned(a.y)) {
+    const bool wide = aligned(a.x) && aligned(a.residual) && aligned(a.weight) && aligned(a.h) && aligned(a.y);
+    if (wide && a.cols % V == 0) e = enqueue(rms_norm_wide_kernel<T, W, false>, dim3(rows), 512, 0, 1, st, a, scaled);
+    else if (wide && pieces > 2048) e = enqueue(rms_norm_wide_kernel<T, W, true>, dim3(rows), 512, 0, 1, st, a, scaled);
+    else if (wide) {
         const uint32_t threads = warps_for((pieces + 1) / 2);
         e = enqueue(rms_norm_between_kernel<T, W>, dim3(std::min<uint32_t>(rows, 148 * std::max(1u, 1024 / threads))), threads, 0, 1, st, a, scaled);
     } else if (scaled != SCALE_BLOCK && a.cols <= 16 * 1024) e = enqueue(rms_norm_odd_rows_kernel<T, W, 16>, dim3(rows), warps_for((a.cols + 15) / 16), 0, 1, st, a, scaled);
@@ -165,7 +168,10 @@ template <class T, class W> cudaError_t launch_norm_grad(const NormGradArgs& a, 
     cudaError_t e;
     constexpr uint64_t V = 16 / sizeof(T);
     const bool wide = aligned(a.h) && aligned(a.weight) && aligned(a.dy) && aligned(a.dh) && aligned(a.dx) && aligned(a.partial);
-    if (wide && (a.cols % V ? launch_norm_grad_rows<T, W, true>(a, a.cols / V + 2, st, e) : launch_norm_grad_rows<T, W, false>(a, a.cols / V, st, e))) {}
+    const bool between = a.cols % V != 0;
+    const uint64_t pieces = a.cols / V + (between ? 2 : 0);
+    if (wide && (between ? launch_norm_grad_rows<T, W, true>(a, pieces, st, e) : launch_norm_grad_rows<T, W, false>(a, pieces, st, e))) {}
+    else if (wide && pieces <= 512 * 32 / V) e = enqueue(between ? rms_norm_grad_wide_kernel<T, W, true> : rms_norm_grad_wide_kernel<T, W, false>, dim3(a.blocks), 512, 0, 1, st, a);
     else e = enqueue(rms_norm_grad_long_kernel<T, W>, dim3(a.blocks), 512, 0, 1, st, a);
     if (a.dweight && e == cudaSuccess) e = enqueue(rms_norm_grad_weight_kernel<W>, dim3(uint32_t((a.cols + 31) / 32)), 1024, 0, 1, st, a);
     return e;

@@ -322,6 +322,20 @@ template <class T> __device__ __forceinline__ void store_piece(T* to, int o, int
             else reinterpret_cast<uint16_t*>(to)[k] = uint16_t(words[k / 2] >> (k % 2 * 16));
         }
 }
+template <bool BETWEEN, class T> __device__ __forceinline__ void store_e4m3(uint8_t* to, int o, int cols, const Piece<T>& p) {
+    auto q = pack_e4m3(p);
+    if constexpr (BETWEEN)
+        if (o < 0 || o + Piece<T>::V > cols) {
+#pragma unroll
+            for (int k = 0; k < Piece<T>::V; ++k)
+                if (o + k >= 0 && o + k < cols) {
+                    if constexpr (Piece<T>::V == 4) to[k] = uint8_t(q >> (k * 8));
+                    else to[k] = uint8_t((k < 4 ? q.x : q.y) >> (k % 4 * 8));
+                }
+            return;
+        }
+    *reinterpret_cast<decltype(q)*>(to) = q;
+}
 template <class T> __device__ __forceinline__ void keep_own(Piece<T>& p, int o, int cols) {
     if (o >= 0 && o + Piece<T>::V <= cols) return;
     auto own = [&](int k) { return o + k >= 0 && o + k < cols; };
@@ -403,19 +417,92 @@ __global__ void __launch_bounds__(1024) rms_norm_between_kernel(NormArgs a, uint
                 store_piece(static_cast<T*>(a.y) + number(j), place(j), cols, rounded<T>(t[j]));
                 continue;
             }
-            const int o = place(j);
-            const auto q = pack_e4m3(t[j]);
-            uint8_t* to = static_cast<uint8_t*>(a.y) + number(j);
-            if (o >= 0 && o + V <= cols) *reinterpret_cast<decltype(pack_e4m3(t[j]))*>(to) = q;
-            else {
-#pragma unroll
-                for (int k = 0; k < V; ++k)
-                    if (o + k >= 0 && o + k < cols) {
-                        if constexpr (V == 4) to[k] = uint8_t(q >> (k * 8));
-                        else to[k] = uint8_t((k < 4 ? q.x : q.y) >> (k % 4 * 8));
-                    }
-            }
+            store_e4m3<true, T>(static_cast<uint8_t*>(a.y) + number(j), place(j), cols, t[j]);
         }
+    }
+}
+
+// Rows that registers do not hold: twice over them, the second time from the caches, where what the rows of all blocks take has room.  BETWEEN:
+// pieces of the whole tensor, as above.  2048 rows of 14336 fp32 with a residual: 92 us, 5.1 TB/s (a value to a load 122), into E4M3 with row or
+// block scales 80 and 93 (124, 174); 1024 of 28672 bf16 62 (147).  Bound by memory and the second pass' trips to the L2.
+template <class T, class W, bool BETWEEN>
+__global__ void __launch_bounds__(512, 2) rms_norm_wide_kernel(NormArgs a, uint32_t quant) {
+    constexpr int V = Piece<T>::V, P = Piece<T>::P;
+    __shared__ __align__(16) float shared[2][32];
+    const uint64_t row = blockIdx.x, begin = row * a.cols, first = begin / V, values = a.rows * a.cols;
+    const int cols = int(a.cols), before = int(begin % V);
+    const uint32_t pieces = (uint32_t(cols) + before + V - 1) / V, lanes = blockDim.x;
+    const T *x = static_cast<const T*>(a.x), *res = static_cast<const T*>(a.residual);
+    T* const h_out = static_cast<T*>(a.h);
+    others_may_start();
+    after_those_before();
+    auto load = [&](const T* p, uint32_t i) {
+        if constexpr (BETWEEN) return load_piece(p, first + i, values);
+        else return __ldcg(reinterpret_cast<const uint4*>(p) + first + i);
+    };
+    auto store = [&](T* p, uint32_t i, const uint4& w) {
+        if constexpr (BETWEEN) store_piece(p + (first + i) * V, int(i * V) - before, cols, w);
+        else reinterpret_cast<uint4*>(p)[first + i] = w;
+    };
+    auto weight_of = [&](uint32_t i) {
+        if constexpr (BETWEEN) return weights_from<T, W>(a.weight, int(i * V) - before, cols);
+        else return weights<T, W>(a.weight, i);
+    };
+    float2 sums = {};
+    float most = 0;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < pieces; i += lanes) {
+        Piece<T> h = numbers<T>(load(x, i));
+        if (res) {
+            const Piece<T> r = numbers<T>(load(res, i));
+#pragma unroll
+            for (int k = 0; k < P; ++k) h.v[k] = __fadd2_rn(h.v[k], r.v[k]);
+            const uint4 stored = rounded<T>(h);
+            store(h_out, i, stored);
+            h = numbers<T>(stored);
+        }
+        if (BETWEEN) keep_own(h, int(i * V) - before, cols);
+#pragma unroll
+        for (int k = 0; k < P; ++k) sums = __ffma2_rn(h.v[k], h.v[k], sums);
+        if (quant == SCALE_ROW) {
+            const Piece<T> w = weight_of(i);
+#pragma unroll
+            for (int k = 0; k < P; ++k) most = max_magnitude(most, __fmul2_rn(h.v[k], w.v[k]));
+        }
+    }
+    float sum = sums.x + sums.y;
+    reduce<false, true>(sum, most, lanes / 32, shared);
+    const float r = __frsqrt_rn(sum / float(a.cols) + a.eps);
+    const RowScale scale(most, r);
+    if (quant == SCALE_ROW && threadIdx.x == 0) static_cast<float*>(a.scales)[row] = scale.scale();
+    for (uint32_t base = 0; base < pieces; base += lanes) {   // (a warp stays together: blocks of 32 values are several threads')
+        const uint32_t i = base + threadIdx.x;
+        Piece<T> t[1] = {};
+        if (i < pieces) {
+            // what this thread stored; of a piece that another row shares, what is not this row's does not matter
+            t[0] = numbers<T>(load(res ? h_out : x, i));
+            const Piece<T> w = weight_of(i);
+#pragma unroll
+            for (int k = 0; k < P; ++k) t[0].v[k] = __fmul2_rn(t[0].v[k], w.v[k]);
+        }
+        if (quant == SCALE_NONE) {
+            times(t[0], r);
+            if (i < pieces) store(static_cast<T*>(a.y), i, rounded<T>(t[0]));
+            continue;
+        }
+        if (quant == SCALE_ROW) scale.apply(t);
+        else {
+            float m = 0;
+#pragma unroll
+            for (int k = 0; k < P; ++k) m = max_magnitude(m, t[0].v[k]);
+#pragma unroll
+            for (int o = 1; o < 32 / V; o *= 2) m = max_magnitude(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            const uint32_t e = block_scale(m * r);
+            times(t[0], r);
+            times(t[0], block_inverse(e));
+            if (i < pieces && i % (32 / V) == 0) static_cast<uint8_t*>(a.scales)[row * (a.cols / 32) + i / (32 / V)] = uint8_t(e);
+        }
+        if (i < pieces) store_e4m3<BETWEEN, T>(static_cast<uint8_t*>(a.y) + (first + i) * V, int(i * V) - before, cols, t[0]);
     }
 }
 
@@ -623,6 +710,83 @@ __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kerne
 #pragma unroll
                 for (int k = 0; k < P; k += 2) *reinterpret_cast<float4*>(a.partial + blockIdx.x * a.cols + i * V + k * 2) = make_float4(dw[j].v[k].x, dw[j].v[k].y, dw[j].v[k + 1].x, dw[j].v[k + 1].y);
         }
+}
+
+// Rows that registers do not hold, up to 32 values for each of 512 threads: twice over them, the second time from the caches.  Columns and their
+// sums stay with a thread, as above.  2048 rows of 14336 fp32 with the residual's gradient: 120 us, 3.9 TB/s (320 a value to a load, sums in memory); of
+// 10001 139 (211).  Wider rows have the kernel below.
+template <class T, class W, bool BETWEEN>
+__global__ void __launch_bounds__(512, 2) rms_norm_grad_wide_kernel(NormGradArgs a) {
+    constexpr int V = Piece<T>::V, P = Piece<T>::P, N = 32 / V;
+    __shared__ __align__(16) float shared[2][2][32];
+    const uint32_t lanes = blockDim.x;
+    const int cols = int(a.cols), before = BETWEEN ? int(blockIdx.x * a.cols % V) : 0;
+    const uint32_t pieces = (uint32_t(cols) + before + V - 1) / V;
+    const uint64_t values = a.rows * a.cols;
+    const T *hs = static_cast<const T*>(a.h), *dys = static_cast<const T*>(a.dy), *dhs = static_cast<const T*>(a.dh);
+    auto place = [&](uint32_t i) { return int(i * V) - before; };
+    auto load = [&](const T* p, uint64_t first, uint32_t i) {
+        Piece<T> v;
+        if constexpr (BETWEEN) {
+            v = numbers<T>(load_piece(p, first + i, values));
+            keep_own(v, place(i), cols);
+        } else v = numbers<T>(__ldcg(reinterpret_cast<const uint4*>(p) + first + i));
+        return v;
+    };
+    auto weight_of = [&](uint32_t i) {
+        if constexpr (BETWEEN) return weights_from<T, W>(a.weight, place(i), cols);
+        else return weights<T, W>(a.weight, i);
+    };
+    Piece<T> dw[N] = {};
+    others_may_start();
+    after_those_before();
+    uint32_t turn = 0;
+    for (uint64_t row = blockIdx.x; row < a.rows; row += a.blocks, turn ^= 1) {
+        const uint64_t first = row * a.cols / V;
+        float2 sqs = {}, dots = {};
+#pragma unroll 2
+        for (uint32_t i = threadIdx.x; i < pieces; i += lanes) {
+            const Piece<T> v = load(hs, first, i), d = load(dys, first, i), w = weight_of(i);
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                sqs = __ffma2_rn(v.v[k], v.v[k], sqs);
+                dots = __ffma2_rn(__fmul2_rn(d.v[k], w.v[k]), v.v[k], dots);
+            }
+        }
+        float sq = sqs.x + sqs.y, dot = dots.x + dots.y;
+        reduce<true, false>(sq, dot, lanes / 32, shared[turn]);
+        const float r = __frsqrt_rn(sq / float(a.cols) + a.eps), c = r * r * r * dot / float(a.cols);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = threadIdx.x + j * lanes;
+            if (i >= pieces) continue;
+            const Piece<T> v = load(hs, first, i), d = load(dys, first, i), w = weight_of(i);
+            Piece<T> g;
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const float2 u = __fmul2_rn(d.v[k], make_float2(r, r));
+                g.v[k] = __ffma2_rn(u, w.v[k], __fmul2_rn(v.v[k], make_float2(-c, -c)));
+                dw[j].v[k] = __ffma2_rn(u, v.v[k], dw[j].v[k]);
+            }
+            if (!a.dx) continue;
+            if (dhs) {
+                const Piece<T> e = load(dhs, first, i);
+#pragma unroll
+                for (int k = 0; k < P; ++k) g.v[k] = __fadd2_rn(g.v[k], e.v[k]);
+            }
+            if constexpr (BETWEEN) store_piece(static_cast<T*>(a.dx) + (first + i) * V, place(i), cols, rounded<T>(g));
+            else static_cast<uint4*>(a.dx)[first + i] = rounded<T>(g);
+        }
+    }
+    if (!a.partial) return;
+    float* const to = a.partial + blockIdx.x * a.cols;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int o = place(threadIdx.x + j * lanes);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (o + k >= 0 && o + k < cols) to[o + k] = k % 2 ? dw[j].v[k / 2].y : dw[j].v[k / 2].x;
+    }
 }
 
 // Rows of any length and place; a block's sums for dweight live in `partial`, where each column belongs to one thread.

@@ -55,7 +55,7 @@ def _inputs(rows, cols, dtype, seed, residual=True, weight_dtype=None):
     return x, res, w
 
 
-ROWS_COLS = [(1, 1), (3, 7), (1, 32), (5, 96), (2, 1000), (17, 1024), (1, 4096), (333, 4095), (7, 8200), (2, 10501), (3, 16384), (2, 40000), (1200, 64), (1203, 128), (301, 32), (999, 256), (500, 1024)]
+ROWS_COLS = [(1, 1), (3, 7), (1, 32), (5, 96), (2, 1000), (17, 1024), (1, 4096), (333, 4095), (7, 8200), (2, 10501), (3, 16384), (2, 40000), (1200, 64), (1203, 128), (301, 32), (999, 256), (500, 1024), (4, 8224), (3, 16416), (2, 24992)]
 
 
 @pytest.mark.parametrize("rows, cols", ROWS_COLS)
@@ -140,7 +140,7 @@ def test_norm_of_zeros_infinities_and_nan(quant):
         assert torch.equal(plain.values.view(torch.uint8)[0], again.values.view(torch.uint8)[5])
 
 
-@pytest.mark.parametrize("rows, cols", [(1, 5), (40, 1), (37, 9), (21, 17), (9, 513), (700, 333), (5, 4095), (3, 8190), (2, 8191), (5, 16367), (2, 16383)])
+@pytest.mark.parametrize("rows, cols", [(1, 5), (40, 1), (37, 9), (21, 17), (9, 513), (700, 333), (5, 4095), (3, 8190), (2, 8191), (5, 16367), (2, 16383), (3, 20003)])
 @pytest.mark.parametrize("dtype, weight_dtype", [("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "fp32"), ("fp32", "fp32"), ("fp32", "fp16")])
 @pytest.mark.parametrize("residual", [True, False])
 @pytest.mark.parametrize("quant", [None, "row"])
@@ -187,7 +187,7 @@ def test_norm_strides_offsets_and_empty_rows():
         assert y.shape == (0, 512) and h.shape == (0, 512)
 
 
-@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 7), (5, 96), (1, 4096), (700, 1000), (333, 4095), (2, 10501), (3, 16384), (2, 40000), (1000, 333), (600, 4097), (297, 8191), (299, 16367), (900, 5)])
+@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 7), (5, 96), (1, 4096), (700, 1000), (333, 4095), (2, 10501), (3, 16384), (2, 40000), (1000, 333), (600, 4097), (297, 8191), (299, 16367), (900, 5), (310, 8200), (3, 16384), (300, 10001), (299, 12289)])
 @pytest.mark.parametrize("dtype, weight_dtype", [("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp32")])
 @pytest.mark.parametrize("residual", [True, False])
 def test_norm_gradient(rows, cols, dtype, weight_dtype, residual):
