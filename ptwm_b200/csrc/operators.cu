@@ -259,8 +259,9 @@ TilesSplit tiles_split(uint64_t rows, uint64_t contraction, uint64_t tokens, uin
     return {tile_tokens, ranks, stages, together};
 }
 
+// there: a call before this one has left the parts of the same tokens in the scratch.
 template <bool GRAD>
-int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, int device, const PerDevice& dev, cudaStream_t st) {
+int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, bool there, int device, const PerDevice& dev, cudaStream_t st) {
     const uint64_t rows = GRAD ? w.cols : w.rows, contraction = GRAD ? w.rows : w.cols;
     const Parts p = parts_of(reinterpret_cast<uintptr_t>(x.x), x.tokens, contraction, x_dtype);
     if (p.bytes > scratch_bytes || (p.bytes && !scratch)) return fail(PTWM_RC_BUFFER_TOO_SMALL, "matvec: scratch too small");
@@ -268,8 +269,9 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     if (p.bytes) {
         auto* out = at<__nv_bfloat16>(scratch);
         const dim3 grid(uint32_t(x.tokens), uint32_t(std::min<uint64_t>((p.pitch + 255) / 256, 64)));
-        cudaError_t e;
-        if (x_dtype == DT_E4M3) e = enqueue(token_parts_kernel<uint8_t>, grid, 256, 0, 1, st, x, contraction, out, uint32_t(p.pitch), x.tokens);
+        cudaError_t e = cudaSuccess;
+        if (there) {}
+        else if (x_dtype == DT_E4M3) e = enqueue(token_parts_kernel<uint8_t>, grid, 256, 0, 1, st, x, contraction, out, uint32_t(p.pitch), x.tokens);
         else with_type(x_dtype, [&](auto v) { e = enqueue(token_parts_kernel<decltype(v)>, grid, 256, 0, 1, st, x, contraction, out, uint32_t(p.pitch), x.tokens); });
         CUDA_TRY(e);
         tokens = out;
@@ -404,12 +406,14 @@ extern "C" int64_t ptwm_b200_matvec_group(const ptwm_b200_scaled_weight* const* 
         if (alike)
             if (const FewSplit s = few_split(w[0], uint32_t(tiles), tokens, x_dtype); s.depth)
                 return launch_few(w, y, count, uint32_t(tiles), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream));
+        bool there = false;
         for (uint32_t i = 0; i < count; ++i) {
             const FewSplit s = few_split(w[i], few_tiles(w[i]), tokens, x_dtype);
             t.y = at<void>(y[i]);
             const int64_t rc = s.depth ? launch_few(&w[i], y + i, 1, few_tiles(w[i]), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream))
-                                       : launch_tiles<false>(w[i], t, x_dtype, y_dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
+                                       : launch_tiles<false>(w[i], t, x_dtype, y_dtype, scratch, scratch_bytes, there, int(device), dev, stream_of(stream));
             if (rc < 0) return rc;
+            there |= !s.depth;
         }
         return 0;
     });
@@ -434,6 +438,6 @@ extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, 
         const TokenArgs t{at<void>(dy), nullptr, tokens, SCALE_NONE, at<void>(dx)};
         PerDevice dev;
         if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
-        return launch_tiles<true>(w, t, dtype, dtype, scratch, scratch_bytes, int(device), dev, stream_of(stream));
+        return launch_tiles<true>(w, t, dtype, dtype, scratch, scratch_bytes, false, int(device), dev, stream_of(stream));
     });
 }

@@ -24,7 +24,7 @@ from .container import _check
 __all__ = ["Projection", "ScaledActivations", "ScaledWeight", "matvec", "rms_norm"]
 
 _PLAIN = {torch.float32: 1, torch.float16: 4, torch.bfloat16: 6}
-_E4M3 = 29
+_E4M3, _BF16 = 29, 6
 _TOO_SMALL = -2
 _QUANT = {None: 0, "row": 1, "block": 2}
 _U8 = (torch.uint8,) + ((torch.float4_e2m1fn_x2,) if hasattr(torch, "float4_e2m1fn_x2") else ())
@@ -297,19 +297,21 @@ def _product(x, scales, quant, weight: ScaledWeight, out_dtype: torch.dtype) -> 
     else:
         code, scales_at = _E4M3, scales.data_ptr()
     y = _new((shape[0], weight.rows) if len(shape) == 2 else (*shape[:-1], weight.rows), out_dtype, weight.device)
-    # few tokens, and bf16 ones that lie well, need no scratch: it is asked for where the call says so
-    args = (weight._ref, x.data_ptr(), scales_at, y.data_ptr(), tokens, code, _QUANT[quant], _PLAIN[out_dtype])
-    rc = _lib.lib().ptwm_b200_matvec(*args, 0, 0, device, _stream(device))
-    if rc < 0:
-        if rc == _TOO_SMALL:
-            scratch = _scratch(weight, x, tokens, code, 0)
-            rc = _lib.lib().ptwm_b200_matvec(*args, scratch.data_ptr(), scratch.numel(), device, _stream(device))
-        _check(rc)
+    _with_scratch(_lib.lib().ptwm_b200_matvec, (weight._ref, x.data_ptr(), scales_at, y.data_ptr(), tokens, code, _QUANT[quant], _PLAIN[out_dtype]), (weight,), x, tokens, code, 0)
     return y
 
 
-def _scratch(weight: ScaledWeight, x: torch.Tensor, tokens: int, code: int, grad: int) -> torch.Tensor:
-    return torch.empty(_lib.lib().ptwm_b200_matvec_scratch_bytes(weight._ref, x.data_ptr(), tokens, code, grad), dtype=torch.uint8, device=x.device)
+def _with_scratch(call, args: tuple, weights: Sequence[ScaledWeight], x: torch.Tensor, tokens: int, code: int, grad: int) -> None:
+    """A product's call.  Few tokens, and bf16 ones that lie well, need no scratch: it is not asked for unless the call says so."""
+    device = weights[0]._ordinal
+    rc = _TOO_SMALL if code != _BF16 and (grad or tokens > 16) else call(*args, 0, 0, device, _stream(device))
+    if rc == _TOO_SMALL:
+        # (one of several matrices may want some where another does not)
+        size = max(_lib.lib().ptwm_b200_matvec_scratch_bytes(w._ref, x.data_ptr(), tokens, code, grad) for w in weights)
+        scratch = _new((size,), torch.uint8, x.device)
+        rc = call(*args, scratch.data_ptr(), size, device, _stream(device))
+    if rc < 0:
+        _check(rc)
 
 
 class _Matvec(torch.autograd.Function):
@@ -324,12 +326,8 @@ class _Matvec(torch.autograd.Function):
         w = ctx.weight
         dy = dy.to(ctx.dtype).contiguous()
         dx = torch.empty((*dy.shape[:-1], w.cols), dtype=ctx.dtype, device=dy.device)
-        args = (w._ref, dy.data_ptr(), dx.data_ptr(), dy.numel() // w.rows, _PLAIN[ctx.dtype])
-        rc = _lib.lib().ptwm_b200_matvec_grad(*args, 0, 0, w._ordinal, _stream(w._ordinal))
-        if rc == _TOO_SMALL:
-            scratch = _scratch(w, dy, args[3], args[4], 1)
-            rc = _lib.lib().ptwm_b200_matvec_grad(*args, scratch.data_ptr(), scratch.numel(), w._ordinal, _stream(w._ordinal))
-        _check(rc)
+        tokens, code = dy.numel() // w.rows, _PLAIN[ctx.dtype]
+        _with_scratch(_lib.lib().ptwm_b200_matvec_grad, (w._ref, dy.data_ptr(), dx.data_ptr(), tokens, code), (w,), dy, tokens, code, 1)
         return dx, None, None
 
 
@@ -398,17 +396,11 @@ class Projection:
     def _products(self, x: torch.Tensor, scales: Optional[torch.Tensor], out_dtype: torch.dtype) -> list[torch.Tensor]:
         """The products of all matrices, four to a call."""
         out = []
-        device, tokens, head = x.get_device(), x.numel() // self.norm.shape[0], tuple(x.shape[:-1])
+        tokens, head = x.numel() // self.norm.shape[0], tuple(x.shape[:-1])
         code, scales_at = (_PLAIN[x.dtype], 0) if scales is None else (_E4M3, scales.data_ptr())
         for refs, weights in self._calls:
             ys = [_new((*head, w.rows), out_dtype, x.device) for w in weights]
             at = (C.c_uint64 * len(ys))(*[y.data_ptr() for y in ys])
-            args = (refs, at, len(ys), x.data_ptr(), scales_at, tokens, code, _QUANT[self.quant], _PLAIN[out_dtype])
-            rc = _lib.lib().ptwm_b200_matvec_group(*args, 0, 0, device, _stream(device))
-            if rc < 0:
-                if rc == _TOO_SMALL:
-                    scratch = max((_scratch(w, x, tokens, code, 0) for w in weights), key=torch.Tensor.numel)  # one of them may want some where another does not
-                    rc = _lib.lib().ptwm_b200_matvec_group(*args, scratch.data_ptr(), scratch.numel(), device, _stream(device))
-                _check(rc)
+            _with_scratch(_lib.lib().ptwm_b200_matvec_group, (refs, at, len(ys), x.data_ptr(), scales_at, tokens, code, _QUANT[self.quant], _PLAIN[out_dtype]), weights, x, tokens, code, 0)
             out += ys
         return out
