@@ -7,7 +7,8 @@ output in 8 bits with scales (``ScaledActivations``) that ``matvec`` reads.  ``P
 read it.
 
 Every call runs on the current stream of its tensors' device, allocates its results with torch, waits for nothing and can be
-captured into a CUDA graph.
+captured into a CUDA graph; a backward pass (of any operator) only while no graph of the same leaves that was recorded
+outside the capture is still alive, since torch adds to their gradients on the stream that had them first.
 """
 from __future__ import annotations
 

@@ -654,6 +654,22 @@ def test_gradients_captured_and_replayed():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("rows, cols", [(5, 4096), (40, 517), (700, 9), (3, 16416), (3, 20003), (2, 10008)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("place", ["x", "residual"])
+def test_the_sum_may_be_written_over_an_input(rows, cols, dtype, place):
+    x, res, w = _inputs(rows, cols, DT[dtype], rows + cols)
+    y, h = rms_norm(x, w, 1e-5, residual=res)
+    torch.cuda.synchronize()
+    into, out = {"x": x, "residual": res}[place].clone(), torch.empty_like(x)
+    ins = {"x": x, "residual": res, place: into}
+    code = {"bf16": 6, "fp32": 1}[dtype]
+    torch.cuda.synchronize()
+    assert ptwm_b200._lib.lib().ptwm_b200_rms_norm(ins["x"].data_ptr(), ins["residual"].data_ptr(), w.data_ptr(), into.data_ptr(), out.data_ptr(), 0, rows, cols, code, code, 0, 1e-5, 0, 1) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(into, h) and torch.equal(out, y)
+
+
 def test_nothing_is_written_outside_the_results():
     w = ScaledWeight(*_matrix(100, 512, "mxfp4", 3))
     room = torch.full((1 << 22,), 7, dtype=torch.uint8, device="cuda")
