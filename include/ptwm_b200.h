@@ -342,7 +342,7 @@ typedef struct ptwm_b200_scaled_weight {
 } ptwm_b200_scaled_weight;
 
 /* Device memory that a product (grad = 0) or its gradient (1) of `tokens` rows at x (dy) needs as scratch: tokens that do not
- * reach the tensor cores as they lie are laid out there. */
+ * reach the tensor cores as they lie are laid out there.  It starts at a multiple of 16 bytes. */
 uint64_t ptwm_b200_matvec_scratch_bytes(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t tokens, uint32_t x_dtype, uint32_t grad);
 /* y[m][n] = sum over k of x[m][k] W[n][k] for `tokens` rows x of w->cols values, sums in fp32, rounded once to y_dtype. */
 int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t x_scales, uint64_t y, uint64_t tokens, uint32_t x_dtype, uint32_t x_scaled,

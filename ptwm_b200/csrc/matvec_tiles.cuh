@@ -14,6 +14,8 @@
 // (512: 1.5e-6, and 2 to 6 % less time; 128: 5e-7, 6 to 20 % more).  Results of 16 bits are rounded by a thousand times as much.
 //   Where tiles are fewer than SMs, the blocks of a cluster share a tile's contraction and add their sums over distributed shared
 // memory, in the order of their ranks.
+//   512 tokens of 14336 x 4096 MXFP4 take 61 us, 980 TFLOP/s (1.51 rounds of tiles cost two), 256 of them 32, their gradient 39.7; 1024 of 4096 x 14336
+// NVFP4 93, 1300 TFLOP/s.  Bound by shared memory (tokens in and out, 512 cycles a step, nibbles 80) beside the tensor cores (512).
 //   What a step costs: 512 cycles of MMA with 256 tokens; some 200 cycles of ALU in conversion; and the issuing thread, to which a wait
 // for a barrier is 170 cycles, a commit 100 and four MMAs 100, ready or not.  So a stage has one barrier for all that arrives in it and is
 // two steps where tokens are few.
@@ -368,24 +370,67 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
     if (threadIdx.x == 0 && *failed) atomicExch(t.status, 1u);
 }
 
+// Eight values of a token from k on, where they lie at a multiple of their size.
+__device__ __forceinline__ void eight_values(const float* p, float (&v)[8]) {
+    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <class T> __device__ __forceinline__ void eight_values(const T* p, float (&v)[8]) {
+    uint32_t w[4];
+    if constexpr (sizeof(T) == 2) {
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    } else {
+        const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p));
+        w[0] = a.x & 0xFFFF; w[1] = a.x >> 16; w[2] = a.y & 0xFFFF; w[3] = a.y >> 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float2 f;
+        if constexpr (sizeof(T) == 2) f = two_f32<T>(w[i]);
+        else f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w[i]), __NV_E4M3)));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
 // Tokens as bf16 parts whose sum they are: part p of token m is row p * part_rows + m of `out`, `pitch` values long, with zeros behind
 // `cols`.  E4M3 (times its block's scale) fits one bf16, fp16 two, fp32 three (each takes the next eight bits).  What is not finite is
-// its first part alone.
+// its first part alone.  Bound by memory: eight values to a thread, which are one load where the rows lie so (`wide`) and one
+// store.  4096 tokens of 4096 E4M3 10 us, 5 TB/s (a value to a thread 70), 512 of them 1.9 (9.5).
 template <class T>
-__global__ void __launch_bounds__(256) token_parts_kernel(TokenArgs t, uint64_t cols, __nv_bfloat16* out, uint32_t pitch, uint64_t part_rows) {
+__global__ void __launch_bounds__(256) token_parts_kernel(TokenArgs t, uint64_t cols, __nv_bfloat16* out, uint32_t pitch, uint64_t part_rows, bool wide) {
     constexpr int PARTS = sizeof(T) == 4 ? 3 : sizeof(T) == 1 ? 1 : std::is_same<T, __half>::value ? 2 : 1;
     const uint64_t m = blockIdx.x;
     others_may_start();
     after_those_before();
-    for (uint64_t k = uint64_t(blockIdx.y) * 256 + threadIdx.x; k < pitch; k += uint64_t(gridDim.y) * 256) {
-        float rest = k < cols ? token_value<T>(t, m, k, cols) : 0.0f;
-        const bool finite = (__float_as_uint(rest) & 0x7F800000u) != 0x7F800000u;
+    for (uint64_t k = (uint64_t(blockIdx.y) * 256 + threadIdx.x) * 8; k < pitch; k += uint64_t(gridDim.y) * 2048) {
+        float rest[8];
+        if (wide) {
+            eight_values(static_cast<const T*>(t.x) + m * cols + k, rest);
+            if (sizeof(T) == 1 && t.scaled == SCALE_BLOCK) {
+                const float s = e8m0_f32(static_cast<const uint8_t*>(t.scales)[m * (cols / 32) + k / 32]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) rest[i] *= s;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rest[i] = k + i < cols ? token_value<T>(t, m, k + i, cols) : 0.0f;
+        }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            // cut, not rounded: a value near the largest stays finite
-            const __nv_bfloat16 b = finite ? __float2bfloat16_rz(rest) : __float2bfloat16_rn(rest);
-            out[(p * part_rows + m) * pitch + k] = b;
-            rest = finite ? rest - __bfloat162float(b) : 0.0f;
+            uint32_t top[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                // cut, not rounded: a value near the largest stays finite
+                const uint32_t bits = __float_as_uint(rest[i]);
+                const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
+                top[i] = rest[i] == rest[i] ? bits & 0xFFFF0000u : 0x7FC00000u;
+                rest[i] = finite ? rest[i] - __uint_as_float(top[i]) : 0.0f;
+            }
+            *reinterpret_cast<uint4*>(out + (p * part_rows + m) * pitch + k) =
+                make_uint4(top[0] >> 16 | top[1], top[2] >> 16 | top[3], top[4] >> 16 | top[5], top[6] >> 16 | top[7]);
         }
     }
 }

@@ -265,14 +265,16 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     const uint64_t rows = GRAD ? w.cols : w.rows, contraction = GRAD ? w.rows : w.cols;
     const Parts p = parts_of(reinterpret_cast<uintptr_t>(x.x), x.tokens, contraction, x_dtype);
     if (p.bytes > scratch_bytes || (p.bytes && !scratch)) return fail(PTWM_RC_BUFFER_TOO_SMALL, "matvec: scratch too small");
+    if (p.bytes && scratch % 16) return fail(PTWM_RC_INVALID_INPUT, "matvec: scratch starts at a multiple of 16 bytes");
     const void* tokens = x.x;
     if (p.bytes) {
         auto* out = at<__nv_bfloat16>(scratch);
-        const dim3 grid(uint32_t(x.tokens), uint32_t(std::min<uint64_t>((p.pitch + 255) / 256, 64)));
+        const dim3 grid(uint32_t(x.tokens), uint32_t(std::min<uint64_t>((p.pitch + 2047) / 2048, 64)));
+        const bool wide = contraction % 8 == 0 && aligned(x.x);
         cudaError_t e = cudaSuccess;
         if (there) {}
-        else if (x_dtype == DT_E4M3) e = enqueue(token_parts_kernel<uint8_t>, grid, 256, 0, 1, st, x, contraction, out, uint32_t(p.pitch), x.tokens);
-        else with_type(x_dtype, [&](auto v) { e = enqueue(token_parts_kernel<decltype(v)>, grid, 256, 0, 1, st, x, contraction, out, uint32_t(p.pitch), x.tokens); });
+        else if (x_dtype == DT_E4M3) e = enqueue(token_parts_kernel<uint8_t>, grid, 256, 0, 1, st, x, contraction, out, uint32_t(p.pitch), x.tokens, wide);
+        else with_type(x_dtype, [&](auto v) { e = enqueue(token_parts_kernel<decltype(v)>, grid, 256, 0, 1, st, x, contraction, out, uint32_t(p.pitch), x.tokens, wide); });
         CUDA_TRY(e);
         tokens = out;
     }

@@ -549,6 +549,30 @@ def test_projections_of_any_number_of_dimensions(shape, quant):
     assert torch.equal(y, matvec(q, w))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_values_that_are_not_finite_stay_in_their_token(dtype, offset):
+    """Tokens that are laid out anew: the largest numbers, infinities and NaN, from a 16-byte boundary and from beside one."""
+    values, scales, _ = _matrix(48, 256, "mxfp4", 5)
+    values = values & 0x77 | 0x11   # no zero, no sign: an infinity stays one
+    w = ScaledWeight(values, scales)
+    dt = DT[dtype]
+    flat = torch.zeros(40 * 256 + 1, dtype=dt, device="cuda")
+    x = flat[offset:offset + 40 * 256].view(40, 256)
+    x.copy_(torch.randn(40, 256, generator=_gen(6), device="cuda"))
+    want = matvec(x, w, out_dtype=torch.float32)
+    x[3, 7], x[4, 250], x[5, 0], x[6] = math.inf, math.nan, -math.inf, 0
+    x[6, 9] = torch.finfo(dt).max
+    got = matvec(x, w, out_dtype=torch.float32)
+    keep = [i for i in range(40) if i not in (3, 4, 5, 6)]
+    assert torch.equal(got[keep], want[keep])
+    assert bool((got[3] == math.inf).all()) and bool(torch.isnan(got[4]).all()) and bool((got[5] == -math.inf).all())
+    w64 = _weight64(values, scales, None)
+    top = torch.finfo(dt).max * w64[:, 9]
+    fits = top < torch.finfo(torch.float32).max   # one product, of parts whose sums are exact
+    assert bool(((got[6].double() - top).abs() <= 2.0 ** -20 * top)[fits].all())
+
+
 def test_a_token_does_not_depend_on_its_neighbours():
     """The same token gives the same bits beside others that hold infinities, as long as as many are asked for."""
     w = ScaledWeight(*_matrix(200, 2048, "nvfp4", 3))
@@ -690,6 +714,7 @@ def test_nothing_is_written_outside_the_results():
         types = (1,) if grad else (1, 0, 1)
         torch.cuda.synchronize()
         assert call(w._ref, x.data_ptr(), *more, at, tokens, *types, there, size - 1, 0, stream) == -2
+        assert call(w._ref, x.data_ptr(), *more, at, tokens, *types, there + 8, size, 0, stream) == -1
         assert call(w._ref, x.data_ptr(), *more, at, tokens, *types, there, size, 0, stream) == 0
         torch.cuda.synchronize()
         end = 4096 + tokens * cols * 4
