@@ -2,6 +2,7 @@
 // own; every call enqueues its kernels on the caller's stream and returns.
 #include <algorithm>
 #include <exception>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <type_traits>
@@ -54,8 +55,8 @@ int64_t matrix_of(const ptwm_b200_scaled_weight* w, ScaledMatrix* out) {
     if (w->group != 16 && w->group != 32) return fail(PTWM_RC_INVALID_INPUT, "scaled weight: groups are 16 (E4M3 scales) or 32 (E8M0 scales) values");
     if (!w->rows || !w->cols || w->cols % w->group) return fail(PTWM_RC_INVALID_INPUT, "scaled weight: cols must be a positive multiple of the group");
     if (w->rows > (1u << 30) || w->cols > (1u << 30)) return fail(PTWM_RC_UNSUPPORTED, "scaled weight: more than 2^30 rows or columns");
-    if (w->value_pitch % 16 || w->scale_pitch % 16 || w->values % 16 || w->scales % 16)
-        return fail(PTWM_RC_INVALID_INPUT, "scaled weight: rows of values and scales start at multiples of 16 bytes");
+    if (w->value_pitch % 16 || w->scale_pitch % 16 || w->values % 16 || w->scales % 16 || w->global_scale % 4)
+        return fail(PTWM_RC_INVALID_INPUT, "scaled weight: rows of values and scales start at multiples of 16 bytes, the global scale at one of 4");
     if (w->value_pitch < w->cols / 2 || w->scale_pitch < w->cols / w->group) return fail(PTWM_RC_INVALID_INPUT, "scaled weight: pitch shorter than a row");
     *out = ScaledMatrix{at<const uint8_t>(w->values), at<const uint8_t>(w->scales), at<const float>(w->global_scale), w->rows, w->cols, w->value_pitch, w->scale_pitch, w->group};
     return 0;
@@ -225,6 +226,12 @@ int64_t tensor_map(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzl
     return 0;
 }
 
+// Whether one of these addresses is none for values of the type.
+bool beside(uint32_t dtype, std::initializer_list<uint64_t> pointers) {
+    const uint64_t size = dtype == DT_FP32 ? 4 : dtype == DT_E4M3 ? 1 : 2;
+    return std::any_of(pointers.begin(), pointers.end(), [&](uint64_t p) { return p % size != 0; });
+}
+
 // How the tokens of a product reach the tensor cores: as they are, or as parts in scratch.
 struct Parts { uint32_t parts; uint64_t pitch; uint64_t bytes; };
 Parts parts_of(uint64_t x, uint64_t tokens, uint64_t contraction, uint32_t dtype) {
@@ -337,6 +344,7 @@ extern "C" int64_t ptwm_b200_rms_norm(uint64_t x, uint64_t residual, uint64_t we
         if (rows > 0x7FFFFFFFull || cols > 0x7FFFFFFFull) return fail(PTWM_RC_UNSUPPORTED, "rms_norm: more than 2^31 - 1 rows or columns");
         if (!rows) return 0;
         if (!x || !weight || !y || (residual && !h) || (scaled && !scales)) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: null device pointer");
+        if (beside(dtype, {x, residual, h, scaled ? 0 : y}) || beside(weight_dtype, {weight}) || (scaled == SCALE_ROW && scales % 4)) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: a tensor lies beside its type's alignment");
         DeviceGuard guard{int(device)};
         if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
         const NormArgs a{at<void>(x), at<void>(residual), at<void>(weight), at<void>(h), at<void>(y), at<void>(scales), rows, cols, eps};
@@ -356,6 +364,7 @@ extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t
         if (!cols || rows > 0x7FFFFFFFull || cols > 0x7FFFFFFFull) return fail(PTWM_RC_UNSUPPORTED, "rms_norm_grad: rows of 1 to 2^31 - 1 values, at most as many of them");
         if (rows && (!h || !weight || !dy || (!dx && !dweight))) return fail(PTWM_RC_INVALID_INPUT, "rms_norm_grad: null device pointer");
         if (rows && dweight && (!scratch || scratch_bytes < ptwm_b200_rms_norm_grad_scratch_bytes(rows, cols))) return fail(PTWM_RC_BUFFER_TOO_SMALL, "rms_norm_grad: scratch too small");
+        if (beside(dtype, {h, dy, dh, dx}) || beside(weight_dtype, {weight, dweight}) || beside(DT_FP32, {scratch})) return fail(PTWM_RC_INVALID_INPUT, "rms_norm_grad: a tensor lies beside its type's alignment");
         DeviceGuard guard{int(device)};
         if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
         if (!rows) {
@@ -398,6 +407,8 @@ extern "C" int64_t ptwm_b200_matvec_group(const ptwm_b200_scaled_weight* const* 
         if (!x || (x_scaled && !x_scales)) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
         for (uint32_t i = 0; i < count; ++i)
             if (!y[i]) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
+            else if (beside(y_dtype, {y[i]})) return fail(PTWM_RC_INVALID_INPUT, "matvec: a tensor lies beside its type's alignment");
+        if (beside(x_dtype, {x}) || (x_scaled == SCALE_ROW && x_scales % 4)) return fail(PTWM_RC_INVALID_INPUT, "matvec: a tensor lies beside its type's alignment");
         DeviceGuard guard{int(device)};
         if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
         TokenArgs t{at<void>(x), at<void>(x_scales), tokens, x_scaled, nullptr};
@@ -435,6 +446,7 @@ extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, 
         if (tokens > (1u << 19)) return fail(PTWM_RC_UNSUPPORTED, "matvec_grad: more than 2^19 tokens in a call");
         if (!tokens) return 0;
         if (!dy || !dx) return fail(PTWM_RC_INVALID_INPUT, "matvec_grad: null device pointer");
+        if (beside(dtype, {dy, dx})) return fail(PTWM_RC_INVALID_INPUT, "matvec_grad: a tensor lies beside its type's alignment");
         DeviceGuard guard{int(device)};
         if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
         const TokenArgs t{at<void>(dy), nullptr, tokens, SCALE_NONE, at<void>(dx)};

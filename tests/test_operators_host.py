@@ -70,6 +70,21 @@ def test_norms_that_are_none(L):
         assert L.ptwm_b200_rms_norm_grad(*args, 1e-6, 0, 1) == rc, args
 
 
+def test_addresses_that_no_value_of_the_type_has(L):
+    w = _weight()
+    p = C.addressof(w)
+    for args in [(A + 1, 0, A, 0, A, 0, 4, 64, 6, 6, 0), (A + 2, 0, A, 0, A, 0, 4, 64, 1, 6, 0), (A, A + 1, A, A, A, 0, 4, 64, 6, 6, 0), (A, A, A, A + 1, A, 0, 4, 64, 6, 6, 0),
+                 (A, 0, A + 2, 0, A, 0, 4, 64, 6, 1, 0), (A, 0, A, 0, A + 1, 0, 4, 64, 4, 6, 0), (A, 0, A, 0, A, A + 2, 4, 64, 6, 6, 1)]:
+        assert L.ptwm_b200_rms_norm(*args, 1e-6, 0, 1) == INVALID, args
+    need = L.ptwm_b200_rms_norm_grad_scratch_bytes(4, 64)
+    for args in [(A, A, A + 1, 0, A, 0, 0, 0, 4, 64, 6, 6), (A, A, A, A + 1, A, 0, 0, 0, 4, 64, 6, 6), (A, A, A, 0, A, A + 2, A, need, 4, 64, 6, 1), (A, A, A, 0, A, A, A + 2, need, 4, 64, 6, 6)]:
+        assert L.ptwm_b200_rms_norm_grad(*args, 1e-6, 0, 1) == INVALID, args
+    for args in [(p, A + 1, 0, A, 1, 6, 0, 6), (p, A, 0, A + 2, 1, 6, 0, 1), (p, A, A + 2, A, 1, 29, 1, 6)]:
+        assert L.ptwm_b200_matvec(*args, 0, 0, 0, 1) == INVALID, args
+    for args in [(p, A + 1, A, 1, 6), (p, A, A + 2, 1, 1)]:
+        assert L.ptwm_b200_matvec_grad(*args, 0, 0, 0, 1) == INVALID, args
+
+
 def test_tensors_in_host_memory_are_refused():
     x = torch.zeros(2, 64)
     with pytest.raises(ValueError, match="host memory"):
