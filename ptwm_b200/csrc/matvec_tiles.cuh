@@ -14,8 +14,9 @@
 // (512: 1.5e-6, and 2 to 6 % less time; 128: 5e-7, 6 to 20 % more).  Results of 16 bits are rounded by a thousand times as much.
 //   Where tiles are fewer than SMs, the blocks of a cluster share a tile's contraction and add their sums over distributed shared
 // memory, in the order of their ranks.
-//   512 tokens of 14336 x 4096 MXFP4 take 61 us, 980 TFLOP/s (1.51 rounds of tiles cost two), 256 of them 32, their gradient 39.7; 1024 of 4096 x 14336
-// NVFP4 93, 1300 TFLOP/s.  Bound by shared memory (tokens in and out, 512 cycles a step, nibbles 80) beside the tensor cores (512).
+//   512 tokens of 14336 x 4096 MXFP4 take 59.5 us, 1010 TFLOP/s (1.51 rounds of tiles cost two), 256 of them 31.7, their gradient 39.3, 32 of them 21.  Bound by shared memory
+// (tokens in and out, 512 cycles a step, nibbles 80) beside the tensor cores (512); with up to 128 tokens by the instructions of conversion, which has
+// a kernel for either kind of scales: one for both took 25.4 us for 32 tokens.
 //   What a step costs: 512 cycles of MMA with 256 tokens; some 200 cycles of ALU in conversion; and the issuing thread, to which a wait
 // for a barrier is 170 cycles, a commit 100 and four MMAs 100, ready or not.  So a stage has one barrier for all that arrives in it and is
 // two steps where tokens are few.
@@ -43,7 +44,6 @@ struct TilesArgs {
     uint32_t stages;           // of `together` converted tiles and the tokens that belong to them
     uint32_t together;         // 1 or 2 steps
     uint32_t teams;            // of four warps that convert: 4, and no more than the steps of all stages
-    uint32_t group;
     uint32_t y_dtype;
     const float* global_scale;
     const float* token_scale;  // or null
@@ -67,10 +67,11 @@ inline uint32_t tiles_tmem_stages(uint32_t tile_tokens, uint32_t together, bool 
 // to its high half; a product puts their signs at bit 15 and the other three bits at 8..6, which reads as the number times 2^-126;
 // `scale` is the group's times 2^126.  Every step is exact.
 __device__ __forceinline__ void nibbles_to_bf16(uint32_t w, uint32_t scale, uint32_t (&out)[4]) {
-    const uint32_t odd = w >> 4;
+    const uint32_t even = w & 0x0F0F0F0Fu, odd = w >> 4 & 0x0F0F0F0Fu;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t v = __byte_perm(w, odd, i | i << 4 | (4 + i) << 8 | (4 + i) << 12) & 0x000F000Fu;
+        uint32_t v;   // (a byte's highest bit, in all of a byte, is 0: what __byte_perm does not offer)
+        asm("prmt.b32 %0, %1, %2, %3;" : "=r"(v) : "r"(even), "r"(odd), "r"(i | (8 | i) << 4 | (4 + i) << 8 | (12 + i) << 12));
         const uint32_t bits = (v * 0x1040u) & 0x81C081C0u;
         asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(out[i]) : "r"(bits), "r"(scale));
     }
@@ -101,15 +102,15 @@ template <bool GRAD> struct TilesShared {
 };
 
 // 16 bytes of nibbles (32 values) -> four 16-byte pieces of bf16.  s: the scale of all (MXFP4), or of the first and the second half.
-__device__ __forceinline__ void convert32(const uint4& v, uint32_t group, uint32_t s, uint4 (&out)[4]) {
+template <bool MX> __device__ __forceinline__ void convert32(const uint4& v, uint32_t s, uint4 (&out)[4]) {
     const uint32_t words[4] = {v.x, v.y, v.z, v.w};
     uint32_t more = 0x3F803F80u;
-    const uint32_t s0 = group == 32 ? mx_scale(s & 255, &more) : nv_scale(s & 255), s1 = group == 32 ? s0 : nv_scale(s >> 8 & 255);
+    const uint32_t s0 = MX ? mx_scale(s & 255, &more) : nv_scale(s & 255), s1 = MX ? s0 : nv_scale(s >> 8 & 255);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint32_t o[4];
         nibbles_to_bf16(words[i], i < 2 ? s0 : s1, o);
-        if (more != 0x3F803F80u) {
+        if (MX && more != 0x3F803F80u) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[j]) : "r"(more));
         }
@@ -117,11 +118,12 @@ __device__ __forceinline__ void convert32(const uint4& v, uint32_t group, uint32
     }
 }
 
-template <bool GRAD, bool FLUSH>
+template <bool GRAD, bool FLUSH, bool MX>
 __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __grid_constant__ CUtensorMap values, const __grid_constant__ CUtensorMap scales,
                                                                         const __grid_constant__ CUtensorMap tokens, const TilesArgs t) {
     namespace cg = cooperative_groups;
     using S = TilesShared<GRAD>;
+    constexpr uint32_t GROUP = MX ? 32 : 16;
     extern __shared__ uint8_t dynamic[];
     uint8_t* base = dynamic + (1024 - (smem_u32(dynamic) & 1023)) % 1024;
     const uint32_t sb = smem_u32(base);
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
     const uint32_t row0 = blockIdx.x / ranks * TILE_ROWS, token0 = blockIdx.y * t.tile_tokens;
     // A raw stage is 128 k of 128 rows (two steps) forward, and 64 rows (one step) of the tile's 128 k in the gradient.  A box of scales is
     // 16 bytes of each row: 512 k (MXFP4) or 256 (NVFP4), so several raw stages forward, one in the gradient.
-    const uint32_t scale_raws = GRAD ? 1 : t.group == 32 ? 4 : 2, unit = GRAD ? t.together : 2 * scale_raws;
+    const uint32_t scale_raws = GRAD ? 1 : MX ? 4 : 2, unit = GRAD ? t.together : 2 * scale_raws;
     // this block's steps: whole boxes of scales, and whole stages
     const uint32_t units = uint32_t((t.contraction + unit * STEP - 1) / (unit * STEP));
     const uint32_t step0 = units * rank / ranks * unit, all = uint32_t((t.contraction + STEP - 1) / STEP), end = min(units * (rank + 1) / ranks * unit, all);
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
     // (counters instead of divisions in the warps of one thread: its latency is what they cost)
     if (warp == 0) {
         if (elect_one()) {
-            uint32_t st = 0, parity = 1, slot = 0, piece = 0, scale_x = GRAD ? row0 / t.group & ~15u : raw0 / scale_raws * 16;
+            uint32_t st = 0, parity = 1, slot = 0, piece = 0, scale_x = GRAD ? row0 / GROUP & ~15u : raw0 / scale_raws * 16;
             for (uint32_t raw = 0; raw < raws; ++raw) {
                 const uint32_t full = sb + S::raw_full + 8 * st, dst = sb + S::raw + st * RAW_BYTES;
                 if (raw >= RAW_STAGES && !mbar_wait(sb + S::raw_empty + 8 * st, parity, failed)) break;
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
         // A thread has 32 bytes of a row (64 values of it): forward the step's part of row c, in the gradient one half of row c % 64.  TMA has swizzled
         // the 16-byte pieces of a raw stage's 64-byte rows, so that neighbouring rows lie in different banks, and in shared memory they are stored swizzled.
         const uint32_t team = (warp - 4) / 4, c = threadIdx.x % 128, row = GRAD ? c % 64 : c, half = c / 64;
-        const uint32_t first_group = GRAD ? row0 / t.group & 15u : 0;
+        const uint32_t first_group = GRAD ? row0 / GROUP & 15u : 0;
         const uint32_t out = half * 8192 + row / 8 * 1024 + row % 8 * 128;
         uint32_t st = team / t.together, round = 0;  // stage of the step, and how often the stages have been gone through
         while (st >= t.stages) { st -= t.stages; ++round; }
@@ -275,16 +277,16 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
             const uint32_t scale_at = raw / scale_raws, slot = scale_at % S::scale_slots;
             if (!mbar_wait(sb + S::scales_full + 8 * slot, scale_at / S::scale_slots & 1, failed)) break;
             const uint8_t* sp = base + S::scales + slot * S::scale_bytes + row * 16;
-            const uint32_t g = first_group + raw % scale_raws * (128 / t.group) + pair * (64 / t.group);
-            const uint32_t s = t.group == 32 ? *reinterpret_cast<const uint16_t*>(sp + g) : *reinterpret_cast<const uint32_t*>(sp + g);
+            const uint32_t g = first_group + raw % scale_raws * (128 / GROUP) + pair * (64 / GROUP);
+            const uint32_t s = MX ? *reinterpret_cast<const uint16_t*>(sp + g) : *reinterpret_cast<const uint32_t*>(sp + g);
             if (round && !mbar_wait(sb + S::empty + 8 * st, (round - 1) & 1, failed)) break;
             uint4 o[4];
             if constexpr (GRAD) {
                 uint8_t* dst = base + S::stages + st * stage_bytes + step % t.together * A_BYTES + out;
-                convert32(v0, t.group, s, o);
+                convert32<MX>(v0, s, o);
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + ((j ^ (row % 8)) * 16)) = o[j];
-                convert32(v1, t.group, t.group == 32 ? s >> 8 : s >> 16, o);
+                convert32<MX>(v1, MX ? s >> 8 : s >> 16, o);
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + ((4 + j ^ (row % 8)) * 16)) = o[j];
                 fence_async_shared();
@@ -292,10 +294,10 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
                 tc_fence_after();  // the MMAs that read what was here before are done
                 const uint32_t at = a_tmem + (warp % 4 * 32 << 16) + (st * t.together + step % t.together) * A_COLS;
                 uint32_t v[16];
-                convert32(v0, t.group, s, o);
+                convert32<MX>(v0, s, o);
                 memcpy(v, o, 64);
                 tmem_store16(at, v);
-                convert32(v1, t.group, t.group == 32 ? s >> 8 : s >> 16, o);
+                convert32<MX>(v1, MX ? s >> 8 : s >> 16, o);
                 memcpy(v, o, 64);
                 tmem_store16(at + 16, v);
                 tmem_wait_stores();
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 1) matvec_tiles_kernel(const __
             tc_fence_after();
         }
         const uint64_t n = row0 + lanes + lane;
-        float factor = t.group == 32 ? 1.0f : NV_REST;
+        float factor = MX ? 1.0f : NV_REST;
         if (t.global_scale) factor *= *t.global_scale;
         if (*failed) factor = __uint_as_float(0x7FC00000u);
         float* const sums = reinterpret_cast<float*>(base + TILES_HEAD);  // [token][row]: nothing reads or writes the buffers any more

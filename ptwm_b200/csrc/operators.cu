@@ -70,7 +70,7 @@ struct FewSplit { uint32_t ranks, most, depth, smem, blocks, lines; };
 FewSplit few_split(uint32_t tiles, uint32_t boxes, uint32_t tokens, uint32_t parts, uint32_t group) {
     constexpr uint32_t SMS = 148;
     // Where two blocks to a cluster, or for more than eight tokens one turn, are not enough, tiles are quicker: 8 tokens of 4096 x 14336 (NVFP4) take 22 us
-    // in two blocks (25 in tiles), 9 of them 35 (25), 16 in four blocks 62 (25); 16 of 14336 x 4096 20 (25).
+    // in two blocks (21 in tiles), 9 of them 35 (21), 16 in four blocks 62 (21); 16 of 14336 x 4096 20 (21), one of 4096 x 14336 11.7.
     for (uint32_t ranks = 1; ranks <= 2 && ranks <= boxes; ranks *= 2) {
         const uint32_t share = (boxes + ranks - 1) / ranks, clusters = std::min(tiles, SMS / ranks), run = (tiles + clusters - 1) / clusters;
         const uint32_t lines = few_lines(share, group);
@@ -194,7 +194,8 @@ int64_t device_of(int device, PerDevice* out) {
         CUDA_TRY(cudaGetSymbolAddress(&p, g_operator_status));
         d.status = static_cast<uint32_t*>(p);
         CUDA_TRY(allow_few());
-        for (const auto f : {matvec_tiles_kernel<false, false>, matvec_tiles_kernel<false, true>, matvec_tiles_kernel<true, false>, matvec_tiles_kernel<true, true>})
+        for (const auto f : {matvec_tiles_kernel<false, false, false>, matvec_tiles_kernel<false, false, true>, matvec_tiles_kernel<false, true, false>, matvec_tiles_kernel<false, true, true>,
+                             matvec_tiles_kernel<true, false, false>, matvec_tiles_kernel<true, false, true>, matvec_tiles_kernel<true, true, false>, matvec_tiles_kernel<true, true, true>})
             CUDA_TRY(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_MOST)));
         d.attributes = true;
     }
@@ -287,7 +288,7 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     }
     const bool flush = y_dtype == DT_FP32;
     const TilesSplit split = tiles_split(rows, contraction, x.tokens, p.parts, GRAD, flush, w.group);
-    TilesArgs t{rows, contraction, x.tokens, x.tokens, p.parts, split.tile_tokens, split.stages, split.together, std::min<uint32_t>(4, split.stages * split.together), w.group, y_dtype, w.global_scale,
+    TilesArgs t{rows, contraction, x.tokens, x.tokens, p.parts, split.tile_tokens, split.stages, split.together, std::min<uint32_t>(4, split.stages * split.together), y_dtype, w.global_scale,
                 x.scaled == SCALE_ROW ? static_cast<const float*>(x.scales) : nullptr, x.y, dev.status};
     CUDA_TRY(cudaSetDevice(device));  // a thread that has launched nothing yet (autograd's) has no context, which the tensor maps want
     CUtensorMap values, scales, tmap;
@@ -297,7 +298,9 @@ int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype
     if (rc < 0) return rc;
     const dim3 grid(uint32_t((rows + TILE_ROWS - 1) / TILE_ROWS) * split.ranks, uint32_t((x.tokens + t.tile_tokens - 1) / t.tile_tokens));
     const uint32_t smem = std::max(TILES_LEAST_SMEM, tiles_smem(tiles_stage(t.tile_tokens, t.parts, t.together, GRAD), t.stages));
-    CUDA_TRY(enqueue(flush ? matvec_tiles_kernel<GRAD, true> : matvec_tiles_kernel<GRAD, false>, grid, TILES_THREADS, smem, split.ranks, st, values, scales, tmap, t));
+    const auto kernel = w.group == 32 ? flush ? matvec_tiles_kernel<GRAD, true, true> : matvec_tiles_kernel<GRAD, false, true>
+                                      : flush ? matvec_tiles_kernel<GRAD, true, false> : matvec_tiles_kernel<GRAD, false, false>;
+    CUDA_TRY(enqueue(kernel, grid, TILES_THREADS, smem, split.ranks, st, values, scales, tmap, t));
     return 0;
 }
 
