@@ -17,7 +17,7 @@
 //   512 tokens of 14336 x 4096 MXFP4 take 59.5 us, 1010 TFLOP/s (1.51 rounds of tiles cost two), 256 of them 31.7, their gradient 39.3, 32 of them 21.  Bound by shared memory
 // (tokens in and out, 512 cycles a step, nibbles 80) beside the tensor cores (512); with up to 128 tokens by the instructions of conversion, which has
 // a kernel for either kind of scales: one for both took 25.4 us for 32 tokens.
-//   What a step costs: 512 cycles of MMA with 256 tokens; some 200 cycles of ALU in conversion; and the issuing thread, to which a wait
+//   What a step costs: 512 cycles of MMA with 256 tokens; some 300 issue slots of conversion; and the issuing thread, to which a wait
 // for a barrier is 170 cycles, a commit 100 and four MMAs 100, ready or not.  So a stage has one barrier for all that arrives in it and is
 // two steps where tokens are few.
 #pragma once
