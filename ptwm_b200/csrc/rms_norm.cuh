@@ -589,7 +589,9 @@ __global__ void __launch_bounds__(256) rms_norm_long_kernel(NormArgs a, uint32_t
     }
 }
 
-// Gradient.  With g = dy weight:  dx = dh + r g - h r^3 / K sum(g h)  (the residual's is the same),  dweight = sum over rows of dy h r.
+// Gradient.  With g = dy weight:  dx = dh + r g - (h r) (sum(g h) r / K r)  (the residual's is the same),  dweight = sum over rows of dy (h r).
+// In this order every number in between has the size of g, of r g or of a normed value.  r^3, with which the second term may also be written, leaves fp32's range from a
+// root mean square of 10^13 on, and below 10^-13 without eps.
 struct NormGradArgs {
     const void *h, *weight, *dy, *dh;
     void* dx;
@@ -602,10 +604,10 @@ struct NormGradArgs {
 
 // A block takes rows blockIdx.x, + blocks, ...  Its threads keep their columns, N pieces of 16 bytes, and with them their sums for
 // dweight in registers; with 512 of them the next row is asked for before this one's reduction, which 64 registers of 1024 do not hold.
-// Bound by memory and, at half its rate, by what a row waits for its reduction: 4096 rows of 4096 with the residual's gradient take 29.4 us
-// in bf16 (4.6 TB/s; 31.3 with a value at a time), 47.9 in fp32 (5.6 TB/s), the weights' sum with it.
+// Bound by memory and, at half its rate, by what a row waits for its reduction: 4096 rows of 4096 with the residual's gradient take 30.7 us
+// in bf16 (4.4 TB/s; a value at a time took 6 % more), 49.9 in fp32 (5.4 TB/s), the weights' sum with it.
 // BETWEEN: rows of a length that no piece divides, with the pieces of the whole tensor.  The blocks are as many as makes each one's rows
-// begin at the same place of a piece, so a thread has the same columns in all of them (4096 rows of 4097: 64 us, 170 a value at a time).
+// begin at the same place of a piece, so a thread has the same columns in all of them (4096 rows of 4097: 66 us, 170 a value at a time).
 template <class T, class W, int N, int MOST, bool BETWEEN>
 __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kernel(NormGradArgs a) {
     constexpr int V = Piece<T>::V, P = Piece<T>::P;
@@ -671,7 +673,7 @@ __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kerne
         float sq = sqs.x + sqs.y, dot = dots.x + dots.y;
         if (MOST <= 512) ask(row + a.blocks);
         reduce<true, false>(sq, dot, lanes / 32, shared[turn]);
-        const float r = __frsqrt_rn(sq / float(a.cols) + a.eps), c = r * r * r * dot / float(a.cols);
+        const float r = __frsqrt_rn(sq / float(a.cols) + a.eps), c = dot * r / float(a.cols) * r;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const uint32_t i = at + j * lanes;
@@ -679,9 +681,9 @@ __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kerne
             const Piece<T> w = N > 1 ? weights_of(j) : kept;
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                const float2 u = __fmul2_rn(d[j].v[k], make_float2(r, r));
-                g.v[k] = __ffma2_rn(u, w.v[k], __fmul2_rn(v[j].v[k], make_float2(-c, -c)));
-                dw[j].v[k] = __ffma2_rn(u, v[j].v[k], dw[j].v[k]);
+                const float2 n = __fmul2_rn(v[j].v[k], make_float2(r, r));
+                g.v[k] = __ffma2_rn(__fmul2_rn(d[j].v[k], make_float2(r, r)), w.v[k], __fmul2_rn(n, make_float2(-c, -c)));
+                dw[j].v[k] = __ffma2_rn(d[j].v[k], n, dw[j].v[k]);
             }
             if (dhs) {
                 const Piece<T> e = numbers<T>(r0[j]);
@@ -713,8 +715,8 @@ __global__ void __launch_bounds__(MOST, N == 1 ? 2 : 1) rms_norm_grad_rows_kerne
 }
 
 // Rows that registers do not hold, up to 32 values for each of 512 threads: twice over them, the second time from the caches.  Columns and their
-// sums stay with a thread, as above.  2048 rows of 14336 fp32 with the residual's gradient: 120 us, 3.9 TB/s (320 a value to a load, sums in memory); of
-// 10001 139 (211).  Wider rows have the kernel below.
+// sums stay with a thread, as above.  2048 rows of 14336 fp32 with the residual's gradient: 110 us, 4.3 TB/s (320 a value to a load, sums in memory); of
+// 10001 137 (211).  Wider rows have the kernel below.
 template <class T, class W, bool BETWEEN>
 __global__ void __launch_bounds__(512, 2) rms_norm_grad_wide_kernel(NormGradArgs a) {
     constexpr int V = Piece<T>::V, P = Piece<T>::P, N = 32 / V;
@@ -755,25 +757,20 @@ __global__ void __launch_bounds__(512, 2) rms_norm_grad_wide_kernel(NormGradArgs
         }
         float sq = sqs.x + sqs.y, dot = dots.x + dots.y;
         reduce<true, false>(sq, dot, lanes / 32, shared[turn]);
-        const float r = __frsqrt_rn(sq / float(a.cols) + a.eps), c = r * r * r * dot / float(a.cols);
+        const float r = __frsqrt_rn(sq / float(a.cols) + a.eps), c = dot * r / float(a.cols);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const uint32_t i = threadIdx.x + j * lanes;
             if (i >= pieces) continue;
             const Piece<T> v = load(hs, first, i), d = load(dys, first, i), w = weight_of(i);
-            Piece<T> g;
+            Piece<T> g = dhs && a.dx ? load(dhs, first, i) : zeros<T>();
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                const float2 u = __fmul2_rn(d.v[k], make_float2(r, r));
-                g.v[k] = __ffma2_rn(u, w.v[k], __fmul2_rn(v.v[k], make_float2(-c, -c)));
-                dw[j].v[k] = __ffma2_rn(u, v.v[k], dw[j].v[k]);
+                const float2 n = __fmul2_rn(v.v[k], make_float2(r, r));
+                g.v[k] = __ffma2_rn(__ffma2_rn(n, make_float2(-c, -c), __fmul2_rn(d.v[k], w.v[k])), make_float2(r, r), g.v[k]);
+                dw[j].v[k] = __ffma2_rn(d.v[k], n, dw[j].v[k]);
             }
             if (!a.dx) continue;
-            if (dhs) {
-                const Piece<T> e = load(dhs, first, i);
-#pragma unroll
-                for (int k = 0; k < P; ++k) g.v[k] = __fadd2_rn(g.v[k], e.v[k]);
-            }
             if constexpr (BETWEEN) store_piece(static_cast<T*>(a.dx) + (first + i) * V, place(i), cols, rounded<T>(g));
             else static_cast<uint4*>(a.dx)[first + i] = rounded<T>(g);
         }
@@ -811,13 +808,12 @@ __global__ void __launch_bounds__(512) rms_norm_grad_long_kernel(NormGradArgs a)
             dot += to_f32(dy[k]) * to_f32(w[k]) * v;
         }
         reduce<true, false>(sq, dot, blockDim.x / 32, shared[turn]);
-        const float r = __frsqrt_rn(sq / float(cols) + a.eps), c = r * r * r * dot / float(cols);
+        const float r = __frsqrt_rn(sq / float(cols) + a.eps), c = dot * r / float(cols);
         for (uint64_t k = threadIdx.x; k < cols; k += blockDim.x) {
-            const float v = to_f32(h[k]), d = to_f32(dy[k]);
-            float g = r * d * to_f32(w[k]) - v * c;
-            if (dh) g += to_f32(dh[k]);
+            const float n = to_f32(h[k]) * r, d = to_f32(dy[k]);
+            const float g = (d * to_f32(w[k]) - n * c) * r + (dh ? to_f32(dh[k]) : 0.0f);
             if (a.dx) static_cast<T*>(a.dx)[row * cols + k] = from_f32<T>(g);
-            if (part) part[k] += d * v * r;
+            if (part) part[k] += d * n;
         }
     }
 }

@@ -782,3 +782,35 @@ def test_tensor_sizes_beyond_32_bits():
     assert bool((got[:-200] == 0).all())
     want = matvec(one, m, out_dtype=torch.float32).double()
     assert bool(((got[-1].double() - want[0]).abs() <= 2.0 ** -7 * want[0].abs() + 1e-3 * want.abs().max()).all())
+
+
+@pytest.mark.parametrize("rows, cols", [(5, 4096), (700, 256), (40, 8192), (3, 16384), (300, 4097), (9, 513), (3, 10001), (3, 16384 + 8), (2, 40000)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("power, eps", [(45, 1e-5), (55, 1e-5), (-45, 0.0), (-55, 0.0)])
+@pytest.mark.parametrize("place", [0, 1])
+def test_norm_gradient_of_very_large_and_small_rows(rows, cols, dtype, power, eps, place):
+    """Rows whose squares fit fp32 where the third power of their root mean square, or of its inverse, does not.  place: in values, from
+    a boundary of 16 bytes."""
+    dt = DT[dtype]
+    g = _gen(rows + cols + power)
+
+    def placed(t):
+        flat = torch.zeros(t.numel() + place, dtype=dt, device="cuda")
+        flat[place:] = t.to(dt).flatten()
+        return flat[place:].view(t.shape)
+
+    x = placed(torch.randn(rows, cols, generator=g, device="cuda") * 2.0 ** power).requires_grad_()
+    w = placed(1 + 0.1 * torch.randn(cols, generator=g, device="cuda")).requires_grad_()
+    dy = placed(torch.randn(rows, cols, generator=g, device="cuda") + x.detach().float() * 2.0 ** -power)  # (a part along x: the second term counts)
+    dx, dw = torch.autograd.grad(rms_norm(x, w, eps), (x, w), dy)
+    h = x.detach().double()
+    r = (h.square().mean(-1, keepdim=True) + eps).rsqrt()
+    gw = dy.double() * w.detach().double()
+    mean = (gw * h).mean(-1, keepdim=True)
+    want = r * gw - h * r ** 3 * mean
+    size = r * gw.abs() + (h * r ** 3).abs() * (gw * h).abs().mean(-1, keepdim=True)
+    tol = _half_step(dt) * want.abs() + 4 * _norm_slack(cols) * size + _floor(dt)
+    assert bool(((dx.double() - want).abs() <= tol).all())
+    terms = dy.double() * h * r
+    tol = _half_step(dt) * terms.sum(0).abs() + ((rows + 16) * F32 + 2 * _norm_slack(cols)) * terms.abs().sum(0) + _floor(dt)
+    assert bool(((dw.double() - terms.sum(0)).abs() <= tol).all())
