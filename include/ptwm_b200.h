@@ -342,7 +342,7 @@ typedef struct ptwm_b200_scaled_weight {
 } ptwm_b200_scaled_weight;
 
 /* Device memory that a product (grad = 0) or its gradient (1) of `tokens` rows at x (dy) needs as scratch: tokens that do not
- * reach the tensor cores as they lie are laid out there.  It starts at a multiple of 16 bytes. */
+ * reach the tensor cores as they lie are laid out there; x_dtype is x's (dy's).  It starts at a multiple of 16 bytes. */
 uint64_t ptwm_b200_matvec_scratch_bytes(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t tokens, uint32_t x_dtype, uint32_t grad);
 /* y[m][n] = sum over k of x[m][k] W[n][k] for `tokens` rows x of w->cols values, sums in fp32, rounded once to y_dtype. */
 int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t x_scales, uint64_t y, uint64_t tokens, uint32_t x_dtype, uint32_t x_scaled,
@@ -351,7 +351,10 @@ int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t 
  * one launch, where all have scales of one kind.  Scratch: as for one of them. */
 int64_t ptwm_b200_matvec_group(const ptwm_b200_scaled_weight* const* weights, const uint64_t* y, uint32_t count, uint64_t x, uint64_t x_scales, uint64_t tokens,
                                uint32_t x_dtype, uint32_t x_scaled, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, uint32_t device_ordinal, uint64_t stream);
-/* dx[m][k] = sum over n of dy[m][n] W[n][k]: the gradient that goes back to the tokens. */
+/* dx[m][k] = sum over n of dy[m][n] W[n][k]: the gradient that goes back to the tokens, from dy of its own type, rounded once to dx_dtype. */
+int64_t ptwm_b200_matvec_grad_of(const ptwm_b200_scaled_weight* w, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dy_dtype, uint32_t dx_dtype, uint64_t scratch,
+                                 uint64_t scratch_bytes, uint32_t device_ordinal, uint64_t stream);
+/* The same where both have one type. */
 int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* w, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dtype, uint64_t scratch, uint64_t scratch_bytes,
                               uint32_t device_ordinal, uint64_t stream);
 /* 0, or 1 after a wait inside a kernel of these operators gave up on this device (its results are NaN): the waits are bounded, and

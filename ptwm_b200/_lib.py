@@ -104,6 +104,7 @@ _SIGNATURES = {
     "ptwm_b200_matvec_scratch_bytes": (C.c_uint64, [C.c_void_p] + [C.c_uint64] * 2 + [C.c_uint32] * 2),
     "ptwm_b200_matvec": (C.c_int64, [C.c_void_p] + [C.c_uint64] * 4 + [C.c_uint32] * 3 + [C.c_uint64] * 2 + [C.c_uint32, C.c_uint64]),
     "ptwm_b200_matvec_group": (C.c_int64, [C.c_void_p, C.c_void_p, C.c_uint32] + [C.c_uint64] * 3 + [C.c_uint32] * 3 + [C.c_uint64] * 2 + [C.c_uint32, C.c_uint64]),
+    "ptwm_b200_matvec_grad_of": (C.c_int64, [C.c_void_p] + [C.c_uint64] * 3 + [C.c_uint32] * 2 + [C.c_uint64] * 2 + [C.c_uint32, C.c_uint64]),
     "ptwm_b200_matvec_grad": (C.c_int64, [C.c_void_p] + [C.c_uint64] * 3 + [C.c_uint32] + [C.c_uint64] * 2 + [C.c_uint32, C.c_uint64]),
     "ptwm_b200_operator_status": (C.c_int64, [C.c_uint32]),
     "ptwm_hardware_backend_v1_cuda_stream_handle": (C.c_uint64, [C.c_uint32]),

@@ -440,21 +440,26 @@ extern "C" int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* weight, uint6
     return ptwm_b200_matvec_group(&weight, &y, 1, x, x_scales, tokens, x_dtype, x_scaled, y_dtype, scratch, scratch_bytes, device, stream);
 }
 
-extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dtype, uint64_t scratch, uint64_t scratch_bytes,
-                                         uint32_t device, uint64_t stream) {
+extern "C" int64_t ptwm_b200_matvec_grad_of(const ptwm_b200_scaled_weight* weight, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dy_dtype, uint32_t dx_dtype, uint64_t scratch,
+                                            uint64_t scratch_bytes, uint32_t device, uint64_t stream) {
     return guarded([&]() -> int64_t {
         ScaledMatrix w;
         if (const int64_t rc = matrix_of(weight, &w); rc < 0) return rc;
-        if (!plain_type(dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec_grad: gradients are fp32, fp16 or bf16");
+        if (!plain_type(dy_dtype) || !plain_type(dx_dtype)) return fail(PTWM_RC_UNSUPPORTED, "matvec_grad: gradients are fp32, fp16 or bf16");
         if (tokens > (1u << 19)) return fail(PTWM_RC_UNSUPPORTED, "matvec_grad: more than 2^19 tokens in a call");
         if (!tokens) return 0;
         if (!dy || !dx) return fail(PTWM_RC_INVALID_INPUT, "matvec_grad: null device pointer");
-        if (beside(dtype, {dy, dx})) return fail(PTWM_RC_INVALID_INPUT, "matvec_grad: a tensor lies beside its type's alignment");
+        if (beside(dy_dtype, {dy}) || beside(dx_dtype, {dx})) return fail(PTWM_RC_INVALID_INPUT, "matvec_grad: a tensor lies beside its type's alignment");
         DeviceGuard guard{int(device)};
         if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
         const TokenArgs t{at<void>(dy), nullptr, tokens, SCALE_NONE, at<void>(dx)};
         PerDevice dev;
         if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
-        return launch_tiles<true>(w, t, dtype, dtype, scratch, scratch_bytes, false, int(device), dev, stream_of(stream));
+        return launch_tiles<true>(w, t, dy_dtype, dx_dtype, scratch, scratch_bytes, false, int(device), dev, stream_of(stream));
     });
+}
+
+extern "C" int64_t ptwm_b200_matvec_grad(const ptwm_b200_scaled_weight* weight, uint64_t dy, uint64_t dx, uint64_t tokens, uint32_t dtype, uint64_t scratch, uint64_t scratch_bytes,
+                                         uint32_t device, uint64_t stream) {
+    return ptwm_b200_matvec_grad_of(weight, dy, dx, tokens, dtype, dtype, scratch, scratch_bytes, device, stream);
 }

@@ -325,10 +325,10 @@ class _Matvec(torch.autograd.Function):
     def backward(ctx, dy):
         _once()
         w = ctx.weight
-        dy = dy.to(ctx.dtype).contiguous()
+        dy = dy.contiguous()
         dx = torch.empty((*dy.shape[:-1], w.cols), dtype=ctx.dtype, device=dy.device)
-        tokens, code = dy.numel() // w.rows, _PLAIN[ctx.dtype]
-        _with_scratch(_lib.lib().ptwm_b200_matvec_grad, (w._ref, dy.data_ptr(), dx.data_ptr(), tokens, code), (w,), dy, tokens, code, 1)
+        tokens, code = dy.numel() // w.rows, _PLAIN[dy.dtype]  # the output's type
+        _with_scratch(_lib.lib().ptwm_b200_matvec_grad_of, (w._ref, dy.data_ptr(), dx.data_ptr(), tokens, code, _PLAIN[ctx.dtype]), (w,), dy, tokens, code, 1)
         return dx, None, None
 
 
@@ -336,7 +336,8 @@ def matvec(x, weight: ScaledWeight, *, out_dtype: Optional[torch.dtype] = None) 
     """``y[..., n] = sum_k x[..., k] W[n, k]`` with a 4-bit matrix, for one token or many.
 
     x is fp32, fp16 or bf16 of shape [..., cols], or ``ScaledActivations``.  Sums are fp32, rounded once to ``out_dtype``
-    (x's type; bf16 for ScaledActivations).  The gradient goes back to a plain x; the matrix has none."""
+    (x's type; bf16 for ScaledActivations).  The gradient goes back to a plain x, from the output's type and rounded once to x's; the
+    matrix has none."""
     if not isinstance(weight, ScaledWeight):
         raise TypeError(f"weight is a ScaledWeight, got {type(weight).__name__}")
     if type(x) is ScaledActivations:

@@ -814,3 +814,38 @@ def test_norm_gradient_of_very_large_and_small_rows(rows, cols, dtype, power, ep
     terms = dy.double() * h * r
     tol = _half_step(dt) * terms.sum(0).abs() + ((rows + 16) * F32 + 2 * _norm_slack(cols)) * terms.abs().sum(0) + _floor(dt)
     assert bool(((dw.double() - terms.sum(0)).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("tokens", [1, 6, 40, 200])
+@pytest.mark.parametrize("dtype, out", [("bf16", "fp32"), ("fp16", "fp32"), ("bf16", "fp16"), ("fp16", "bf16"), ("fp32", "bf16"), ("fp32", "fp16")])
+def test_matvec_gradient_from_an_output_of_another_type(kind, tokens, dtype, out):
+    """The gradient of an output is used as it comes: one rounding, into x's type, behind the sum."""
+    n, k = 160, 96
+    w = _matrix(n, k, kind, 21)
+    x = torch.randn(tokens, k, generator=_gen(1), device="cuda").to(DT[dtype]).requires_grad_()
+    dy = torch.randn(tokens, n, generator=_gen(2), device="cuda").to(DT[out])
+    dx, = torch.autograd.grad(matvec(x, ScaledWeight(*w), out_dtype=DT[out]), x, dy)
+    assert dx.dtype == x.dtype
+    _check_product(dx, dy.double(), _weight64(*w).T.contiguous(), x.dtype)
+
+
+@pytest.mark.parametrize("tokens", [1, 30, 150])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_matvec_gradient_of_fp32_outputs_keeps_small_differences_and_large_values(tokens, dtype):
+    # one nonzero to a column, or two that nearly cancel: the products and their sums are exact, and fit x's type where dy would not
+    n, k = 64, 64
+    codes = torch.zeros(n, k, dtype=torch.uint8, device="cuda")
+    codes[0, 0], codes[1, 0], codes[2, 33], codes[3, 32 + 31] = 2, 10, 2, 2  # 1, -1, 1, 1
+    scales = torch.full((n, 2), 127, dtype=torch.uint8, device="cuda")
+    scales[2, 1], scales[3, 1] = 117, 157  # 2^-10, 2^30
+    w = ScaledWeight(codes[:, 0::2] | codes[:, 1::2] << 4, scales)
+    x = torch.zeros(tokens, k, device="cuda", dtype=DT[dtype], requires_grad=True)
+    dy = torch.zeros(tokens, n, device="cuda")
+    dy[:, 0], dy[:, 1] = 1 + 2.0 ** -20, 1.0
+    dy[:, 2] = 100352.0     # past fp16: 98 in dx
+    dy[:, 3] = 5 * 2.0 ** -33  # below half its smallest step
+    dx, = torch.autograd.grad(matvec(x, w, out_dtype=torch.float32), x, dy)
+    want = torch.zeros(tokens, k, device="cuda")
+    want[:, 0], want[:, 33], want[:, 63] = 2.0 ** -20, 98.0, 0.625
+    assert torch.equal(dx.float(), want.to(DT[dtype]).float())

@@ -108,3 +108,11 @@ def test_names_of_a_microscaled_matrix():
     assert scaled_names("a", of("a", "a_scale", "a_scale_2")) == ("a", "a_scale", "a_scale_2")
     with pytest.raises(KeyError):
         scaled_names("a", of("a", "a_blocks", "b_scale"))
+
+
+def test_gradients_of_two_types_that_are_none(L):
+    p = C.addressof(_weight())
+    for args, rc in [((p, A, A, 1, 29, 6), UNSUPPORTED), ((p, A, A, 1, 6, 29), UNSUPPORTED), ((p, A + 2, A, 1, 1, 6), INVALID), ((p, A, A + 2, 1, 6, 1), INVALID), ((p, 0, A, 1, 1, 6), INVALID),
+                     ((p, A, 0, 1, 1, 6), INVALID), ((p, A, A, (1 << 19) + 1, 1, 6), UNSUPPORTED), ((None, A, A, 1, 1, 6), INVALID)]:
+        assert L.ptwm_b200_matvec_grad_of(*args, 0, 0, 0, 1) == rc, args
+    assert L.ptwm_b200_matvec_grad_of(p, 0, 0, 0, 1, 6, 0, 0, 0, 1) == 0
