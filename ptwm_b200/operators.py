@@ -161,6 +161,14 @@ class ScaledWeight:
         values, scales, top = scaled_names(name, state.__contains__)
         return cls(state[values], state[scales], None if top is None else state[top], expert=expert)
 
+    # Copies and pickles are made of the tensors: the addresses kept beside them are this object's own.
+    def __getstate__(self) -> tuple:
+        return self._values, self._scales, self._global, self.kind  # (bytes: plain pickle does not take float8 storages)
+
+    def __setstate__(self, state: tuple) -> None:
+        values, scales, top, kind = state
+        self.__init__(values, scales if kind == "mxfp4" else scales.view(torch.float8_e4m3fn), top)
+
     @property
     def shape(self) -> tuple[int, int]:
         return self.rows, self.cols
@@ -385,6 +393,13 @@ class Projection:
                 raise ValueError(f"a norm of {norm.shape[0]} on {norm.device} does not fit {w!r}")
         parts = [self.weights[i:i + 4] for i in range(0, len(self.weights), 4)]
         self._calls = [((C.c_uint64 * len(p))(*[w._ref for w in p]), p) for p in parts]
+
+    def __getstate__(self) -> tuple:  # a copy refers to its own matrices
+        return self.norm, self.weights, self.eps, self.quant
+
+    def __setstate__(self, state: tuple) -> None:
+        norm, weights, eps, quant = state
+        self.__init__(norm, weights, eps=eps, quant=quant)
 
     def __call__(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> tuple[list[torch.Tensor], torch.Tensor]:
         got = rms_norm(x, self.norm, self.eps, residual=residual, quant=self.quant)

@@ -1,5 +1,7 @@
 """rms_norm and matvec against their definitions in 64 bits."""
+import copy
 import math
+import pickle
 
 import numpy as np
 import pytest
@@ -849,3 +851,22 @@ def test_matvec_gradient_of_fp32_outputs_keeps_small_differences_and_large_value
     want = torch.zeros(tokens, k, device="cuda")
     want[:, 0], want[:, 33], want[:, 63] = 2.0 ** -20, 98.0, 0.625
     assert torch.equal(dx.float(), want.to(DT[dtype]).float())
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_copies_of_handles_multiply_by_their_own_matrix(kind, how):
+    values, scales, top = _matrix(80, 544, kind, 13)
+    room = torch.zeros(80, 640, dtype=torch.uint8, device="cuda")
+    room[:, :272] = values
+    x = _integers(5, 544, torch.bfloat16, 2)
+    w = ScaledWeight(room[:, :272], scales, top)
+    p = Projection(torch.ones(544, device="cuda", dtype=torch.bfloat16), [w, w], quant="block" if kind == "mxfp4" else None)
+    want, pair = matvec(x, w), p(x)[0]
+    c, q = how(w), how(p)
+    if how is not copy.copy:
+        room.fill_(0x11)
+        assert not torch.equal(matvec(x, w), want)
+    assert torch.equal(matvec(x, c), want)
+    for y, z in zip(q(x)[0], pair):
+        assert torch.equal(y, z)

@@ -1,12 +1,14 @@
 """Refusals of the operators that apply decoded weights, without a GPU: the C ABI looks at its arguments before it touches a
 device, and the Python side before it calls."""
+import copy
 import ctypes as C
+import pickle
 
 import pytest
 import torch
 
 import ptwm_b200
-from ptwm_b200 import _lib
+from ptwm_b200 import _lib, operators
 from ptwm_b200.operators import scaled_names
 
 INVALID, SMALL, UNSUPPORTED = -1, -2, -5
@@ -116,3 +118,39 @@ def test_gradients_of_two_types_that_are_none(L):
                      ((p, A, 0, 1, 1, 6), INVALID), ((p, A, A, (1 << 19) + 1, 1, 6), UNSUPPORTED), ((None, A, A, 1, 1, 6), INVALID)]:
         assert L.ptwm_b200_matvec_grad_of(*args, 0, 0, 0, 1) == rc, args
     assert L.ptwm_b200_matvec_grad_of(p, 0, 0, 0, 1, 6, 0, 0, 0, 1) == 0
+
+
+def _host_tensors(monkeypatch):
+    """Handles on host memory, which nothing may be launched with."""
+    monkeypatch.setattr(operators, "_on_cuda", lambda what, t, device=None: None)
+
+
+def _own_addresses(w):
+    assert w._ref == C.addressof(w._args)
+    assert w._args.values == w._values.data_ptr() and w._args.scales == w._scales.data_ptr() and w._args.global_scale == (0 if w._global is None else w._global.data_ptr())
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_copies_of_handles_have_addresses_of_their_own(monkeypatch, kind, how):
+    _host_tensors(monkeypatch)
+    values = torch.arange(64 * 128, dtype=torch.int32).to(torch.uint8).reshape(64, 128)
+    if kind == "mxfp4":
+        w = ptwm_b200.ScaledWeight(values, torch.full((64, 16), 127, dtype=torch.uint8)[:, :8])
+    else:
+        w = ptwm_b200.ScaledWeight(values, torch.ones(64, 16).to(torch.float8_e4m3fn), torch.tensor([0.5]))
+    _own_addresses(w)
+    c = how(w)
+    _own_addresses(c)
+    assert c._ref != w._ref and (how is copy.copy or c._values.data_ptr() != w._values.data_ptr())
+    assert c.kind == kind and c.shape == w.shape and torch.equal(c._values, w._values) and torch.equal(c._scales, w._scales)
+    for field in ("rows", "cols", "value_pitch", "scale_pitch", "group"):
+        assert getattr(c._args, field) == getattr(w._args, field)
+    p = ptwm_b200.Projection(torch.ones(256), [w, w, c, w, c], eps=1e-3, quant="row")
+    q = how(p)
+    assert (q.eps, q.quant, len(q.weights)) == (1e-3, "row", 5) and torch.equal(q.norm, p.norm)
+    refs = [r for call, _ in q._calls for r in call]
+    assert refs == [m._ref for m in q.weights] and [len(ws) for _, ws in q._calls] == [4, 1]
+    for m in q.weights:
+        _own_addresses(m)
+    assert how is copy.copy or not set(refs) & {w._ref, c._ref}
