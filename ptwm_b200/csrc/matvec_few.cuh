@@ -451,9 +451,10 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
                 __syncthreads();  // before these parts take the place of the last
                 stage(pass);
             }
-            // what undoes the scaling: powers below one with the scales of a group, so that nothing overflows, the others at the end
-            const int up = up0 + FINER * PARTS * int(pass);
-            const float down = power_of_two(up > 0 ? -up : 0), rest = power_of_two(up < 0 ? -up : 0);
+            // What undoes the scaling: powers below one with the scales of a group, so that nothing overflows, the others at the end; so is what
+            // of a power below one is no normal number, since a group's scale may bring the product back.
+            const int up = up0 + FINER * PARTS * int(pass), with_scales = min(max(up, 0), 126);
+            const float down = power_of_two(-with_scales), rest = power_of_two(with_scales - up);
             float sum[NT][4] = {}, sum2[NT][4] = {};
             const uint32_t tile0 = over_n(run.lo);
             uint32_t col = run.lo - tile0 * block_n, scales_of = smem_u32(scale_lines) + (tile0 * 16 + g) * 128;
@@ -473,7 +474,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
                     for (int j = 0; j < 4; ++j) {
                         float v = sum[m][j];
                         if (PARTS == 2 && !MX) v += sum2[m][j] * (1.0f / float(1ull << FINER));
-                        v *= MX ? rest : down * rest;
+                        v = (MX ? v : v * down) * rest;
                         const uint32_t token = m * 8 + 2 * t + (j & 1);
                         if (token < a.tokens && (!SPREAD || token < P)) {
                             float* const to = my + token * 16 + g + (j >> 1) * 8;

@@ -870,3 +870,49 @@ def test_copies_of_handles_multiply_by_their_own_matrix(kind, how):
     assert torch.equal(matvec(x, c), want)
     for y, z in zip(q(x)[0], pair):
         assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 16])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_matvec_tiny_tokens_far_below_others_against_large_scales(kind, tokens, dtype):
+    """Tokens at the low end of their type whose smallest values are a part of their own: it is undone by a power of two that fp32 does not hold."""
+    n, k = 32, 512
+    codes = torch.zeros(n, k, dtype=torch.uint8, device="cuda")
+    codes[:, 40], codes[1::2, 300] = 2, 2  # ones; the even rows do not see the large value
+    packed = codes[:, 0::2] | codes[:, 1::2] << 4
+    if kind == "mxfp4":
+        scales, top, factor = torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda"), None, 2.0 ** 120
+        scales[0::2, 1] = 247
+    else:
+        scales, top, factor = torch.ones(n, k // 16, device="cuda").to(torch.float8_e4m3fn), torch.tensor([2.0 ** 100], device="cuda"), 2.0 ** 108
+        scales[0::2, 2] = 256.0
+    x = torch.zeros(tokens, k, device="cuda")
+    for large, small in ((-104, -133), (-100, -126), (-88, -120), (-60, -118)):
+        x[:, 300], x[:, 40] = 2.0 ** large, 2.0 ** small
+        y = matvec(x.to(DT[dtype]), ScaledWeight(packed, scales, top), out_dtype=torch.float32)
+        # one product in a row, by powers of two: exact unless it, before NVFP4's global scale, is below the normal numbers
+        assert bool((y[:, 0::2] == 2.0 ** small * factor).all()), (large, small)
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 16])
+def test_matvec_smallest_8_bit_tokens_against_large_scales(kind, tokens):
+    """E4M3's smallest number on the smallest block scale, 2^-136, beside values that leave it to a second part: 2^-25 once the largest is 2^14."""
+    n, k = 32, 512
+    codes = torch.zeros(n, k, dtype=torch.uint8, device="cuda")
+    codes[:, 40], codes[1::2, 300] = 2, 2
+    packed = codes[:, 0::2] | codes[:, 1::2] << 4
+    if kind == "mxfp4":
+        scales, top, factor = torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda"), None, 2.0 ** 120
+        scales[0::2, 1] = 247
+    else:
+        scales, top, factor = torch.ones(n, k // 16, device="cuda").to(torch.float8_e4m3fn), torch.tensor([2.0 ** 100], device="cuda"), 2.0 ** 108
+        scales[0::2, 2] = 256.0
+    x = torch.zeros(tokens, k, device="cuda")
+    x[:, 300], x[:, 40] = 1.0, 2.0 ** -9
+    for large in range(-110, -84):
+        blocks = torch.full((tokens, k // 32), 127 + large, dtype=torch.uint8, device="cuda")
+        blocks[:, 1] = 0
+        y = matvec(ScaledActivations(x.to(torch.float8_e4m3fn), blocks), ScaledWeight(packed, scales, top), out_dtype=torch.float32)
+        assert bool((y[:, 0::2] == 2.0 ** -136 * factor).all()), large
