@@ -18,6 +18,7 @@ from typing import Any, Callable, Mapping, Optional, Sequence
 import torch
 
 from torch._C import _cuda_getCurrentRawStream as _stream  # what torch.cuda.current_stream() wraps, a microsecond faster
+from torch.autograd import forward_ad
 
 from . import _lib
 from .container import _check
@@ -212,9 +213,18 @@ def _new(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _once() -> None:
+def _refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """A dual tensor does not require a gradient, so nothing else would notice it."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("rms_norm and matvec have no forward-mode derivatives; unpack their dual tensors first")
+
+
+def _once(*grads: Optional[torch.Tensor]) -> None:
     if torch.is_grad_enabled():  # as it is in a backward pass with create_graph
         raise RuntimeError("rms_norm and matvec have first derivatives only: their backward passes cannot be differentiated")
+    _refuse_tangents(*grads)
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -228,7 +238,7 @@ class _RmsNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dh=None):
-        _once()
+        _once(dy, dh)
         h, weight = ctx.saved_tensors
         for_x, need_w, for_residual, _ = ctx.needs_input_grad
         need_x = for_x or for_residual
@@ -262,7 +272,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residu
     (max|y| / 448) or an E8M0 scale per 32 values (the smallest power of two that keeps them within 448).  A row or block
     that is not finite has NaN for scale and values.
 
-    Without ``quant`` there are gradients for x, residual and weight."""
+    Without ``quant`` there are gradients for x, residual and weight: first ones, backwards."""
     try:
         device, dtype, shape = x.get_device(), x.dtype, x.shape
         fine = (device >= 0 and weight.get_device() == device and dtype in _PLAIN and weight.dtype in _PLAIN and weight.shape == shape[-1:] and shape[-1] > 0
@@ -272,6 +282,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residu
         fine = False
     if not fine:
         _refuse_norm(x, weight, residual, quant)
+    _refuse_tangents(x, weight, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         if quant is not None:
             raise ValueError("an 8-bit output has no gradient: call under torch.no_grad() or detach the inputs")
@@ -331,7 +342,7 @@ class _Matvec(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _once()
+        _once(dy)
         w = ctx.weight
         dy = dy.contiguous()
         dx = torch.empty((*dy.shape[:-1], w.cols), dtype=ctx.dtype, device=dy.device)
@@ -344,8 +355,8 @@ def matvec(x, weight: ScaledWeight, *, out_dtype: Optional[torch.dtype] = None) 
     """``y[..., n] = sum_k x[..., k] W[n, k]`` with a 4-bit matrix, for one token or many.
 
     x is fp32, fp16 or bf16 of shape [..., cols], or ``ScaledActivations``.  Sums are fp32, rounded once to ``out_dtype``
-    (x's type; bf16 for ScaledActivations).  The gradient goes back to a plain x, from the output's type and rounded once to x's; the
-    matrix has none."""
+    (x's type; bf16 for ScaledActivations).  The gradient goes back to a plain x, from the output's type and rounded once to x's: the
+    first one, backwards.  The matrix has none."""
     if not isinstance(weight, ScaledWeight):
         raise TypeError(f"weight is a ScaledWeight, got {type(weight).__name__}")
     if type(x) is ScaledActivations:
@@ -366,6 +377,7 @@ def matvec(x, weight: ScaledWeight, *, out_dtype: Optional[torch.dtype] = None) 
     shape = x.shape
     if not shape or shape[-1] != weight.cols:
         raise ValueError(f"x of shape {tuple(shape)} does not fit a matrix of {weight.rows} x {weight.cols}")
+    _refuse_tangents(x, scales)
     if not x.is_contiguous():
         x = x.contiguous()
     if scales is None and x.requires_grad and torch.is_grad_enabled():

@@ -916,3 +916,29 @@ def test_matvec_smallest_8_bit_tokens_against_large_scales(kind, tokens):
         blocks[:, 1] = 0
         y = matvec(ScaledActivations(x.to(torch.float8_e4m3fn), blocks), ScaledWeight(packed, scales, top), out_dtype=torch.float32)
         assert bool((y[:, 0::2] == 2.0 ** -136 * factor).all()), large
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")  # torch.func's own
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor has no requires_grad; its tangent is not dropped."""
+    from torch.autograd import forward_ad
+    x, res, w = _inputs(3, 64, torch.float32, 1)
+    m = ScaledWeight(*_matrix(32, 64, "mxfp4", 1))
+    plain, product = rms_norm(x, w), matvec(x, m)
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, res, w)]
+        for call in (lambda: rms_norm(dual[0], w), lambda: rms_norm(x, dual[2]), lambda: rms_norm(x, w, residual=dual[1]), lambda: rms_norm(dual[0], w, quant="row"), lambda: matvec(dual[0], m),
+                     lambda: Projection(w, [m])(dual[0]), lambda: Projection(dual[2], [m])(x), lambda: matvec(ScaledActivations(x.to(torch.float8_e4m3fn), dual[0][:, 0]), m)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            matvec(dual[0], m)
+        assert torch.equal(rms_norm(x, w), plain) and torch.equal(matvec(x, m), product)
+        leaf = x.clone().requires_grad_()
+        for y in (rms_norm(leaf, w), matvec(leaf, m)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: rms_norm(t, w), (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: matvec(t, m), (x,), (torch.ones_like(x),))
