@@ -356,11 +356,13 @@ def matvec(x, weight: ScaledWeight, *, out_dtype: Optional[torch.dtype] = None) 
 
     x is fp32, fp16 or bf16 of shape [..., cols], or ``ScaledActivations``.  Sums are fp32, rounded once to ``out_dtype``
     (x's type; bf16 for ScaledActivations).  The gradient goes back to a plain x, from the output's type and rounded once to x's: the
-    first one, backwards.  The matrix has none."""
+    first one, backwards.  ScaledActivations and the matrix have none."""
     if not isinstance(weight, ScaledWeight):
         raise TypeError(f"weight is a ScaledWeight, got {type(weight).__name__}")
     if type(x) is ScaledActivations:
         scales, quant, x = x.scales, x.quant, x.values
+        if (scales.requires_grad or x.requires_grad) and torch.is_grad_enabled():
+            raise ValueError("8-bit tokens have no gradient: call under torch.no_grad() or detach their values and scales")
         out_dtype = out_dtype or torch.bfloat16
         if not scales.is_contiguous():
             scales = scales.contiguous()

@@ -942,3 +942,16 @@ def test_forward_mode_derivatives_are_refused():
         torch.func.jvp(lambda t: rms_norm(t, w), (x,), (torch.ones_like(x),))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: matvec(t, m), (x,), (torch.ones_like(x),))
+
+
+def test_8_bit_tokens_whose_gradient_would_be_lost_are_refused():
+    m = ScaledWeight(*_matrix(32, 64, "mxfp4", 1))
+    x = torch.randn(3, 64, generator=_gen(1), device="cuda", requires_grad=True)
+    scales = x.abs().amax(-1) / 448
+    values = (x / scales[:, None]).to(torch.float8_e4m3fn)
+    for tokens in (ScaledActivations(values.detach(), scales), ScaledActivations(values, scales.detach())):
+        with pytest.raises(ValueError, match="no gradient"):
+            matvec(tokens, m)
+        with torch.no_grad():
+            y = matvec(tokens, m)
+        assert torch.equal(y, matvec(ScaledActivations(values.detach(), scales.detach()), m))
