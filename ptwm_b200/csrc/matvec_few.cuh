@@ -57,9 +57,9 @@ inline uint32_t few_pitch(uint32_t boxes) { return boxes * BOX_COLS * 2 + 64; } 
 // 128-byte lines of scales that a block with so many boxes has to a row, from the 16-byte piece on in which they begin.
 inline uint32_t few_lines(uint32_t boxes, uint32_t group) { return (boxes * (BOX_COLS / group) + (group == 32 ? 8 : 0) + 127) / 128; }
 // most: row tiles a block has at a turn.
-inline uint32_t few_smem(uint32_t tokens, uint32_t boxes, uint32_t depth, uint32_t parts, uint32_t ranks, uint32_t most, uint32_t lines) {
-    const uint32_t shares = (2 * FEW_WARPS + (ranks > 1 ? most : 0)) * tokens * 64;
-    return 1024 + FEW_HEAD + FEW_WARPS * depth * BOX_BYTES + most * 16 * lines * 128 + shares + parts * tokens * few_pitch(boxes);
+inline uint64_t few_smem(uint32_t tokens, uint32_t boxes, uint32_t depth, uint32_t parts, uint32_t ranks, uint32_t most, uint32_t lines) {  // 64 bits: boxes are any matrix'
+    const uint64_t shares = (2 * FEW_WARPS + (ranks > 1 ? most : 0)) * tokens * 64;
+    return 1024 + FEW_HEAD + FEW_WARPS * depth * BOX_BYTES + uint64_t(most * 16) * lines * 128 + shares + uint64_t(parts * tokens) * few_pitch(boxes);
 }
 
 // Eight values of a token, as they lie.

@@ -78,7 +78,7 @@ FewSplit few_split(uint32_t tiles, uint32_t boxes, uint32_t tokens, uint32_t par
         for (uint32_t limit = FEW_WARPS; limit >= (tokens > 8 ? FEW_WARPS : 1); limit /= 2) {
             const uint32_t turns = (run + limit - 1) / limit, most = (run + turns - 1) / turns;
             for (uint32_t depth = FEW_DEPTH; depth >= 2; --depth)
-                if (const uint32_t smem = few_smem(tokens, share, depth, parts, ranks, most, lines); smem <= SMEM_MOST) return {ranks, most, depth, smem, clusters * ranks, lines};
+                if (const uint64_t smem = few_smem(tokens, share, depth, parts, ranks, most, lines); smem <= SMEM_MOST) return {ranks, most, depth, uint32_t(smem), clusters * ranks, lines};
         }
     }
     return {};

@@ -154,3 +154,11 @@ def test_copies_of_handles_have_addresses_of_their_own(monkeypatch, kind, how):
     for m in q.weights:
         _own_addresses(m)
     assert how is copy.copy or not set(refs) & {w._ref, c._ref}
+
+
+@pytest.mark.parametrize("cols, group, tokens, dtype, parts", [(954436352, 32, 2, 4, 2), (613565952, 16, 3, 4, 2), (858992640, 16, 1, 1, 3), (66587648, 32, 16, 1, 3)])
+def test_rows_far_too_long_for_shared_memory_go_to_tiles(L, cols, group, tokens, dtype, parts):
+    """What few tokens of such rows would want passes 2^32 bytes by a little: they are laid out for the kernel of many tokens instead."""
+    pitch = (cols // group + 15) // 16 * 16
+    w = _weight(rows=1, cols=cols, value_pitch=cols // 2, scale_pitch=pitch, group=group)
+    assert L.ptwm_b200_matvec_scratch_bytes(C.addressof(w), A, tokens, dtype, 0) == parts * tokens * cols * 2
