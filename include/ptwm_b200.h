@@ -321,7 +321,7 @@ int64_t ptwm_b200_fit_shared_states_host(const uint8_t* const* planes, const uin
  *   y = h / sqrt(mean(h^2) + eps) * weight, sums in fp32, rounded once
  * in the rows' type, or (scaled != SCALE_NONE) as E4M3 values with scales: per row max|y| / 448, per block the smallest
  * power of two that keeps the block within 448.  A maximum that is not finite makes its scale and values NaN; zeros have scale 0
- * (row) or 2^-127 (block).  All rows lie back to back; h may be x or residual. */
+ * (row) or 2^-127 (block).  All rows lie back to back, at most 2^30 columns and 2^31 - 1 of them; h may be x or residual. */
 int64_t ptwm_b200_rms_norm(uint64_t x, uint64_t residual, uint64_t weight, uint64_t h, uint64_t y, uint64_t scales, uint64_t rows, uint64_t cols,
                            uint32_t dtype, uint32_t weight_dtype, uint32_t scaled, float eps, uint32_t device_ordinal, uint64_t stream);
 /* Its gradient, for an output in the rows' type: dx (the residual's as well) and dweight from h, the gradient dy of y and

@@ -113,6 +113,8 @@ cudaError_t allow_few() {
     return e;
 }
 
+// Columns of a norm: the kernels have places in a row, and what is a few pieces behind its end, in signed 32 bits.
+constexpr uint64_t NORM_COLS = 1ull << 30;
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 uint32_t warps_for(uint64_t threads) { return uint32_t((threads + 31) / 32 * 32); }
 
@@ -344,7 +346,7 @@ extern "C" int64_t ptwm_b200_rms_norm(uint64_t x, uint64_t residual, uint64_t we
         if (!plain_type(dtype) || !plain_type(weight_dtype)) return fail(PTWM_RC_UNSUPPORTED, "rms_norm: x and weight are fp32, fp16 or bf16");
         if (scaled > SCALE_BLOCK) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: unknown output scaling");
         if (!cols || (scaled == SCALE_BLOCK && cols % 32)) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: rows must not be empty, and hold whole blocks of 32 for block scales");
-        if (rows > 0x7FFFFFFFull || cols > 0x7FFFFFFFull) return fail(PTWM_RC_UNSUPPORTED, "rms_norm: more than 2^31 - 1 rows or columns");
+        if (rows > 0x7FFFFFFFull || cols > NORM_COLS) return fail(PTWM_RC_UNSUPPORTED, "rms_norm: more than 2^31 - 1 rows or 2^30 columns");
         if (!rows) return 0;
         if (!x || !weight || !y || (residual && !h) || (scaled && !scales)) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: null device pointer");
         if (beside(dtype, {x, residual, h, scaled ? 0 : y}) || beside(weight_dtype, {weight}) || (scaled == SCALE_ROW && scales % 4)) return fail(PTWM_RC_INVALID_INPUT, "rms_norm: a tensor lies beside its type's alignment");
@@ -364,7 +366,7 @@ extern "C" int64_t ptwm_b200_rms_norm_grad(uint64_t h, uint64_t weight, uint64_t
                                            uint64_t rows, uint64_t cols, uint32_t dtype, uint32_t weight_dtype, float eps, uint32_t device, uint64_t stream) {
     return guarded([&]() -> int64_t {
         if (!plain_type(dtype) || !plain_type(weight_dtype)) return fail(PTWM_RC_UNSUPPORTED, "rms_norm_grad: tensors are fp32, fp16 or bf16");
-        if (!cols || rows > 0x7FFFFFFFull || cols > 0x7FFFFFFFull) return fail(PTWM_RC_UNSUPPORTED, "rms_norm_grad: rows of 1 to 2^31 - 1 values, at most as many of them");
+        if (!cols || rows > 0x7FFFFFFFull || cols > NORM_COLS) return fail(PTWM_RC_UNSUPPORTED, "rms_norm_grad: rows of 1 to 2^30 values, at most 2^31 - 1 of them");
         if (rows && (!h || !weight || !dy || (!dx && !dweight))) return fail(PTWM_RC_INVALID_INPUT, "rms_norm_grad: null device pointer");
         if (rows && dweight && (!scratch || scratch_bytes < ptwm_b200_rms_norm_grad_scratch_bytes(rows, cols))) return fail(PTWM_RC_BUFFER_TOO_SMALL, "rms_norm_grad: scratch too small");
         if (beside(dtype, {h, dy, dh, dx}) || beside(weight_dtype, {weight, dweight}) || beside(DT_FP32, {scratch})) return fail(PTWM_RC_INVALID_INPUT, "rms_norm_grad: a tensor lies beside its type's alignment");

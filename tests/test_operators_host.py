@@ -162,3 +162,10 @@ def test_rows_far_too_long_for_shared_memory_go_to_tiles(L, cols, group, tokens,
     pitch = (cols // group + 15) // 16 * 16
     w = _weight(rows=1, cols=cols, value_pitch=cols // 2, scale_pitch=pitch, group=group)
     assert L.ptwm_b200_matvec_scratch_bytes(C.addressof(w), A, tokens, dtype, 0) == parts * tokens * cols * 2
+
+
+@pytest.mark.parametrize("cols", [(1 << 30) + 1, (1 << 31) - 8, (1 << 31) - 1])
+def test_norms_of_rows_that_32_bits_do_not_count(L, cols):
+    for quant in (0, 1):
+        assert L.ptwm_b200_rms_norm(A, 0, A, 0, A, A, 1, cols, 6, 6, quant, 1e-6, 0, 1) == UNSUPPORTED
+    assert L.ptwm_b200_rms_norm_grad(A, A, A, 0, A, 0, 0, 0, 1, cols, 6, 6, 1e-6, 0, 1) == UNSUPPORTED
