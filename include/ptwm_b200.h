@@ -348,7 +348,7 @@ uint64_t ptwm_b200_matvec_scratch_bytes(const ptwm_b200_scaled_weight* w, uint64
 int64_t ptwm_b200_matvec(const ptwm_b200_scaled_weight* w, uint64_t x, uint64_t x_scales, uint64_t y, uint64_t tokens, uint32_t x_dtype, uint32_t x_scaled,
                          uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, uint32_t device_ordinal, uint64_t stream);
 /* The same for up to four matrices of the same columns that read the same tokens, y[i] for weights[i]: few tokens are read once, in
- * one launch, where all have scales of one kind.  Scratch: as for one of them. */
+ * one launch, where all have scales of one kind.  Scratch: the most that one of them wants; with less nothing is launched. */
 int64_t ptwm_b200_matvec_group(const ptwm_b200_scaled_weight* const* weights, const uint64_t* y, uint32_t count, uint64_t x, uint64_t x_scales, uint64_t tokens,
                                uint32_t x_dtype, uint32_t x_scaled, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, uint32_t device_ordinal, uint64_t stream);
 /* dx[m][k] = sum over n of dy[m][n] W[n][k]: the gradient that goes back to the tokens, from dy of its own type, rounded once to dx_dtype. */

@@ -244,6 +244,12 @@ Parts parts_of(uint64_t x, uint64_t tokens, uint64_t contraction, uint32_t dtype
     return {parts, pitch, parts * tokens * pitch * 2};
 }
 
+int64_t scratch_fits(const Parts& p, uint64_t scratch, uint64_t scratch_bytes) {
+    if (p.bytes > scratch_bytes || (p.bytes && !scratch)) return fail(PTWM_RC_BUFFER_TOO_SMALL, "matvec: scratch too small");
+    if (p.bytes && scratch % 16) return fail(PTWM_RC_INVALID_INPUT, "matvec: scratch starts at a multiple of 16 bytes");
+    return 0;
+}
+
 // How a product is cut into tiles.
 struct TilesSplit { uint32_t tile_tokens, ranks, stages, together; };
 TilesSplit tiles_split(uint64_t rows, uint64_t contraction, uint64_t tokens, uint32_t parts, bool grad, bool flush, uint32_t group) {
@@ -274,8 +280,7 @@ template <bool GRAD>
 int64_t launch_tiles(const ScaledMatrix& w, const TokenArgs& x, uint32_t x_dtype, uint32_t y_dtype, uint64_t scratch, uint64_t scratch_bytes, bool there, int device, const PerDevice& dev, cudaStream_t st) {
     const uint64_t rows = GRAD ? w.cols : w.rows, contraction = GRAD ? w.rows : w.cols;
     const Parts p = parts_of(reinterpret_cast<uintptr_t>(x.x), x.tokens, contraction, x_dtype);
-    if (p.bytes > scratch_bytes || (p.bytes && !scratch)) return fail(PTWM_RC_BUFFER_TOO_SMALL, "matvec: scratch too small");
-    if (p.bytes && scratch % 16) return fail(PTWM_RC_INVALID_INPUT, "matvec: scratch starts at a multiple of 16 bytes");
+    if (const int64_t rc = scratch_fits(p, scratch, scratch_bytes); rc < 0) return rc;
     const void* tokens = x.x;
     if (p.bytes) {
         auto* out = at<__nv_bfloat16>(scratch);
@@ -414,19 +419,30 @@ extern "C" int64_t ptwm_b200_matvec_group(const ptwm_b200_scaled_weight* const* 
             if (!y[i]) return fail(PTWM_RC_INVALID_INPUT, "matvec: null device pointer");
             else if (beside(y_dtype, {y[i]})) return fail(PTWM_RC_INVALID_INPUT, "matvec: a tensor lies beside its type's alignment");
         if (beside(x_dtype, {x}) || (x_scaled == SCALE_ROW && x_scales % 4)) return fail(PTWM_RC_INVALID_INPUT, "matvec: a tensor lies beside its type's alignment");
+        // one split for all, or one for each; what scratch they want is looked at before anything is launched
+        bool alike = true;
+        for (uint32_t i = 1; i < count; ++i) alike &= w[i].group == w[0].group;
+        const FewSplit all = alike ? few_split(w[0], uint32_t(tiles), tokens, x_dtype) : FewSplit{};
+        FewSplit each[FEW_MATRICES] = {};
+        if (!all.depth) {
+            bool in_tiles = count == 1;
+            if (count > 1)
+                for (uint32_t i = 0; i < count; ++i) {
+                    each[i] = few_split(w[i], few_tiles(w[i]), tokens, x_dtype);
+                    in_tiles |= !each[i].depth;
+                }
+            if (in_tiles)
+                if (const int64_t rc = scratch_fits(parts_of(x, tokens, w[0].cols, x_dtype), scratch, scratch_bytes); rc < 0) return rc;
+        }
         DeviceGuard guard{int(device)};
         if (guard.err != cudaSuccess) return fail(PTWM_RC_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(guard.err));
         TokenArgs t{at<void>(x), at<void>(x_scales), tokens, x_scaled, nullptr};
         PerDevice dev;
         if (const int64_t rc = device_of(int(device), &dev); rc < 0) return rc;
-        bool alike = true;
-        for (uint32_t i = 1; i < count; ++i) alike &= w[i].group == w[0].group;
-        if (alike)
-            if (const FewSplit s = few_split(w[0], uint32_t(tiles), tokens, x_dtype); s.depth)
-                return launch_few(w, y, count, uint32_t(tiles), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream));
+        if (all.depth) return launch_few(w, y, count, uint32_t(tiles), t, all, x_dtype, y_dtype, int(device), dev, stream_of(stream));
         bool there = false;
         for (uint32_t i = 0; i < count; ++i) {
-            const FewSplit s = few_split(w[i], few_tiles(w[i]), tokens, x_dtype);
+            const FewSplit& s = each[i];
             t.y = at<void>(y[i]);
             const int64_t rc = s.depth ? launch_few(&w[i], y + i, 1, few_tiles(w[i]), t, s, x_dtype, y_dtype, int(device), dev, stream_of(stream))
                                        : launch_tiles<false>(w[i], t, x_dtype, y_dtype, scratch, scratch_bytes, there, int(device), dev, stream_of(stream));
