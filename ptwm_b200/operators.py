@@ -391,10 +391,11 @@ class Projection:
     """A norm and the matrices that read its output, such as the gate and up projections of a feed-forward block.
 
     ``projection(x, residual)`` returns ``([W x' for W in weights], h)`` with ``x', h = rms_norm(x, norm, eps,
-    residual=residual, quant=quant)``; ``h`` is x where there is no residual.  The matrices' products are one launch where tokens are few."""
+    residual=residual, quant=quant)``; ``h`` is x where there is no residual.  The matrices' products are one launch where tokens are few.
+    ``norm`` and ``weights`` are checked against one another once, here, and stay as they are; others want another ``Projection``."""
 
     def __init__(self, norm: torch.Tensor, weights: Sequence[ScaledWeight], *, eps: float = 1e-6, quant: Optional[str] = None) -> None:
-        self.norm, self.weights, self.eps, self.quant = norm, list(weights), eps, quant
+        self._norm, self._weights, self.eps, self.quant = norm, tuple(weights), eps, quant
         _on_cuda("norm", norm)
         if quant not in _QUANT:
             raise ValueError(f"quant is None, 'row' or 'block', got {quant!r}")
@@ -407,6 +408,14 @@ class Projection:
                 raise ValueError(f"a norm of {norm.shape[0]} on {norm.device} does not fit {w!r}")
         parts = [self.weights[i:i + 4] for i in range(0, len(self.weights), 4)]
         self._calls = [((C.c_uint64 * len(p))(*[w._ref for w in p]), p) for p in parts]
+
+    @property
+    def norm(self) -> torch.Tensor:
+        return self._norm
+
+    @property
+    def weights(self) -> tuple[ScaledWeight, ...]:
+        return self._weights
 
     def __getstate__(self) -> tuple:  # a copy refers to its own matrices
         return self.norm, self.weights, self.eps, self.quant

@@ -181,3 +181,16 @@ def test_scratch_is_looked_at_before_any_launch(L):
     for scratch, size, rc in [(0, 0, SMALL), (0, need, SMALL), (A, need - 1, SMALL), (A + 8, need, INVALID)]:
         assert L.ptwm_b200_matvec_group(refs, ys, 2, A, 0, 16, 4, 0, 4, scratch, size, 0, 1) == rc
     assert L.ptwm_b200_matvec(C.addressof(many), A, 0, A, 16, 4, 0, 4, 0, 0, 0, 1) == SMALL
+
+
+def test_a_projection_keeps_its_norm_and_matrices(monkeypatch):
+    _host_tensors(monkeypatch)
+    given = [ptwm_b200.ScaledWeight(torch.zeros(n, 128, dtype=torch.uint8), torch.zeros(n, 16, dtype=torch.uint8)[:, :8]) for n in (16, 32)]
+    p = ptwm_b200.Projection(torch.ones(256), given)
+    kept = list(given)
+    given.append(given[0])
+    assert list(p.weights) == kept and not hasattr(p.weights, "append")
+    for name, value in (("weights", given), ("norm", torch.ones(512))):
+        with pytest.raises(AttributeError):
+            setattr(p, name, value)
+    assert [r for call, _ in p._calls for r in call] == [w._ref for w in p.weights]
