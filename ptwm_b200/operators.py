@@ -9,11 +9,13 @@ read it.
 Every call runs on the current stream of its tensors' device, allocates its results with torch, waits for nothing and can be
 captured into a CUDA graph; a backward pass (of any operator) only while no graph of the same leaves that was recorded
 outside the capture is still alive, since torch adds to their gradients on the stream that had them first.
+
+The waits inside the kernels are bounded.  None is expected to run out; a kernel in which one did writes NaN, and ``operator_status`` says so.
 """
 from __future__ import annotations
 
 import ctypes as C
-from typing import Any, Callable, Mapping, Optional, Sequence
+from typing import Any, Callable, Mapping, Optional, Sequence, Union
 
 import torch
 
@@ -23,7 +25,7 @@ from torch.autograd import forward_ad
 from . import _lib
 from .container import _check
 
-__all__ = ["Projection", "ScaledActivations", "ScaledWeight", "matvec", "rms_norm"]
+__all__ = ["Projection", "ScaledActivations", "ScaledWeight", "matvec", "operator_status", "rms_norm"]
 
 _PLAIN = {torch.float32: 1, torch.float16: 4, torch.bfloat16: 6}
 _E4M3, _BF16 = 29, 6
@@ -40,6 +42,13 @@ def _on_cuda(what: str, t: Any, device: Optional[torch.device] = None) -> None:
         raise ValueError(f"{what} lives in host memory; move it to CUDA first")
     if device is not None and t.device != device:
         raise ValueError(f"{what} lives on {t.device}, the others on {device}")
+
+
+def operator_status(device: Union[None, int, str, torch.device] = None) -> int:
+    """0, or 1 from when on a wait inside a kernel of these operators has given up on the device (the current one where it is None).
+    Waits for the device."""
+    index = device if isinstance(device, int) or device is None else torch.device(device).index
+    return _check(_lib.lib().ptwm_b200_operator_status(torch.cuda.current_device() if index is None else index))
 
 
 class ScaledActivations:

@@ -970,3 +970,10 @@ def test_a_call_with_too_little_scratch_writes_nothing():
     norm = torch.ones(6144, device="cuda", dtype=torch.float16)
     for y, w in zip(Projection(norm, [few, many])(x)[0], (few, many)):
         assert torch.equal(y, matvec(rms_norm(x, norm), w))
+
+
+def test_the_status_from_python():
+    for device in (None, 0, "cuda", "cuda:0", torch.device("cuda", 0)):
+        assert ptwm_b200.operator_status(device) == 0
+    with pytest.raises(ptwm_b200.PtwmError):
+        ptwm_b200.operator_status(1000)

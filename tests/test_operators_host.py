@@ -194,3 +194,12 @@ def test_a_projection_keeps_its_norm_and_matrices(monkeypatch):
         with pytest.raises(AttributeError):
             setattr(p, name, value)
     assert [r for call, _ in p._calls for r in call] == [w._ref for w in p.weights]
+
+
+def test_the_status_of_a_device_that_is_none(L):
+    if torch.cuda.is_available():
+        pytest.skip("there are devices")
+    with pytest.raises(ptwm_b200.PtwmError):
+        ptwm_b200.operator_status(0)
+    with pytest.raises(ptwm_b200.PtwmError):
+        ptwm_b200.operator_status("cuda:1")
