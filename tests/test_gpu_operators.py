@@ -977,3 +977,55 @@ def test_the_status_from_python():
         assert ptwm_b200.operator_status(device) == 0
     with pytest.raises(ptwm_b200.PtwmError):
         ptwm_b200.operator_status(1000)
+
+
+def _one_to_a_row(n, k, kind, seed, along_columns=False):
+    """Ones, halves and fours, one to a row (and, where along_columns, rather one to a column): every sum has one product, which is exact."""
+    g = _gen(seed)
+    codes = torch.zeros(n, k, dtype=torch.uint8, device="cuda")
+    picks = torch.tensor([1, 2, 6, 9, 10, 14], dtype=torch.uint8, device="cuda")
+    if along_columns:
+        codes[torch.randint(0, n, (k,), generator=g, device="cuda"), torch.arange(k, device="cuda")] = picks[torch.randint(0, 6, (k,), generator=g, device="cuda")]
+    else:
+        codes[torch.arange(n, device="cuda"), torch.randint(0, k, (n,), generator=g, device="cuda")] = picks[torch.randint(0, 6, (n,), generator=g, device="cuda")]
+    _, scales, top = _matrix(n, k, kind, seed)
+    return codes[:, 0::2] | codes[:, 1::2] << 4, scales, top
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("tokens", [1, 2, 7, 16, 33, 130, 300])
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_every_bit_of_a_token_counts(kind, tokens, dtype):
+    """All significant bits of fp16 (11) and fp32 (24), which are several parts of fewer bits: each product and its sum are exact, but for fp32
+    where tokens are few, whose two parts of eleven bits and a sign hold a value to 2^-23."""
+    n, k = 200, 544
+    x = (torch.randn(tokens, k, generator=_gen(4), device="cuda") * 3).to(DT[dtype])
+    w = _one_to_a_row(n, k, kind, 5)
+    want = x.double() @ _weight64(*w).T
+    y = matvec(x, ScaledWeight(*w), out_dtype=torch.float32).double()
+    if dtype == "fp32" and tokens <= 16:
+        assert bool(((y - want).abs() <= (2.0 ** -23 + 2.0 ** -24) * want.abs()).all())  # and the sum of the two parts is rounded once
+    else:
+        assert torch.equal(y, want)
+    w = _one_to_a_row(n, k, kind, 6, along_columns=True)
+    dy = (torch.randn(tokens, n, generator=_gen(7), device="cuda") * 3).to(DT[dtype])
+    dx, = torch.autograd.grad(matvec(x.requires_grad_(), ScaledWeight(*w)), x, dy)
+    assert torch.equal(dx.double(), (dy.double() @ _weight64(*w)).to(dx.dtype).double())  # exact, but for what fp16 has below its normal numbers
+
+
+@pytest.mark.parametrize("tokens", [24, 200])
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_long_sum_in_fp32_does_not_lose_what_is_small(tokens, grad):
+    """2^28 and then ones: sixteen of them, what an MMA adds, are half a step of the sum.  Sums of 256 are apart, so all but the first 255 ones
+    count, and 256 are a multiple of the step; sums in one piece would lose all of them."""
+    n = 14336
+    codes = torch.full((128, n) if not grad else (n, 128), 0x22, dtype=torch.uint8, device="cuda")[:, ::2].contiguous()
+    w = ScaledWeight(codes, torch.full((codes.shape[0], codes.shape[1] // 16), 127, dtype=torch.uint8, device="cuda"))
+    v = torch.ones(tokens, n, device="cuda")
+    v[:, 0] = 2.0 ** 28
+    if grad:
+        x = torch.zeros(tokens, 128, device="cuda", requires_grad=True)
+        y, = torch.autograd.grad(matvec(x, w), x, v)
+    else:
+        y = matvec(v, w)
+    assert bool(((y.double() - (2.0 ** 28 + n - 1)).abs() <= 255 + 16).all())  # and the last rounding: half a step of 32
