@@ -10,6 +10,8 @@
 // values down to 2^-31 of it (fp16 2^-28, E4M3 2^-35).  Where the smallest is below, or tokens are fp32, what is left over goes through
 // the same products again as another part on a finer scale: one pass for nearly all bf16 tokens, two for fp32, and always as many
 // as bring the parts within 2^-23 of every value.
+//   MMAs cut what an fp32 sum does not hold.  Sums of fp32 tokens are therefore added up, rounded, after each group (MXFP4) or box (NVFP4): one token of
+// 4096 x 14336 is within 2e-7 of its sum (in one piece 1.4e-6, and no faster).
 //   A block per SM keeps its tokens in shared memory and has a run of row tiles.  Of up to 16 of them at a turn, its 16 warps take equal
 // runs of boxes, so a warp works on one tile or two and ends each with its share of the sums; tokens that do not fit are split
 // over the blocks of a cluster.  Shares are added in the order of the columns.
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
             // of a power below one is no normal number, since a group's scale may bring the product back.
             const int up = up0 + FINER * PARTS * int(pass), with_scales = min(max(up, 0), 126);
             const float down = power_of_two(-with_scales), rest = power_of_two(with_scales - up);
-            float sum[NT][4] = {}, sum2[NT][4] = {};
+            float sum[NT][4] = {};
             const uint32_t tile0 = over_n(run.lo);
             uint32_t col = run.lo - tile0 * block_n, scales_of = smem_u32(scale_lines) + (tile0 * 16 + g) * 128;
             // this warp's share of the tile that it has ended with: [token][row], in the first of its two places for its first tile
@@ -473,14 +475,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         float v = sum[m][j];
-                        if (PARTS == 2 && !MX) v += sum2[m][j] * (1.0f / float(1ull << FINER));
                         v = (MX ? v : v * down) * rest;
                         const uint32_t token = m * 8 + 2 * t + (j & 1);
                         if (token < a.tokens && (!SPREAD || token < P)) {
                             float* const to = my + token * 16 + g + (j >> 1) * 8;
                             *to = pass ? *to + v : v;
                         }
-                        sum[m][j] = sum2[m][j] = 0;
+                        sum[m][j] = 0;
                     }
                 my += per;
             };
@@ -528,6 +529,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
 #pragma unroll
                 for (int m = 0; m < NT; ++m) xt[m] = tokens_at[m] + col * (BOX_COLS * 2);
                 const uint32_t nib = t / 2;
+                float of_box[PARTS][NT][4];  // of fp32 tokens against NVFP4: MMAs cut what a sum does not hold, so their sums are added up, rounded, after each box
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {  // 32 columns: 16 bytes of a row, four to a lane
                     const uint32_t w = box ^ uint32_t(c << 4);
@@ -566,16 +568,25 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 1) matvec_few_kernel(const __g
                             sum[m][1] += d[1] * f0;
                             sum[m][2] += d[2] * f1;
                             sum[m][3] += d[3] * f1;
+                        } else if constexpr (PARTS == 2) {
+#pragma unroll
+                            for (int p = 0; p < PARTS; ++p) {
+                                const uint4& q = p ? b2 : b;
+                                if (c == 0) mma16816_first(of_box[p][m], h0[0], h1[0], h0[1], h1[1], q.x, q.y);
+                                else mma16816(of_box[p][m], h0[0], h1[0], h0[1], h1[1], q.x, q.y);
+                                mma16816(of_box[p][m], h0[2], h1[2], h0[3], h1[3], q.z, q.w);
+                            }
                         } else {
                             mma16816(sum[m], h0[0], h1[0], h0[1], h1[1], b.x, b.y);
                             mma16816(sum[m], h0[2], h1[2], h0[3], h1[3], b.z, b.w);
-                            if (PARTS == 2) {
-                                mma16816(sum2[m], h0[0], h1[0], h0[1], h1[1], b2.x, b2.y);
-                                mma16816(sum2[m], h0[2], h1[2], h0[3], h1[3], b2.z, b2.w);
-                            }
                         }
                     }
                 }
+                if constexpr (PARTS == 2 && !MX)
+#pragma unroll
+                    for (int m = 0; m < NT; ++m)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sum[m][j] += of_box[0][m][j] + of_box[1][m][j] * (1.0f / float(1ull << FINER));
                 }
                 __syncwarp();
                 if (lane == 0 && (ask_left || goes_on(passes)) && !*failed) load();

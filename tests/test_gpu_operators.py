@@ -1029,3 +1029,15 @@ def test_a_long_sum_in_fp32_does_not_lose_what_is_small(tokens, grad):
     else:
         y = matvec(v, w)
     assert bool(((y.double() - (2.0 ** 28 + n - 1)).abs() <= 255 + 16).all())  # and the last rounding: half a step of 32
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("tokens", [1, 3, 8, 16])
+def test_a_long_sum_of_few_fp32_tokens_does_not_lose_what_is_small(tokens, kind):
+    """As above: the sums of 256 columns are apart, and what the one with 2^28 in it loses is at most the ones in it."""
+    n, k = 4096, 14336
+    values = torch.full((n, k // 2), 0x22, dtype=torch.uint8, device="cuda")
+    w = ScaledWeight(values, torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda")) if kind == "mxfp4" else ScaledWeight(values, torch.ones(n, k // 16, device="cuda").to(torch.float8_e4m3fn))
+    x = torch.ones(tokens, k, device="cuda")
+    x[:, 0] = 2.0 ** 28
+    assert bool(((matvec(x, w).double() - (2.0 ** 28 + k - 1)).abs() <= 255 + 16).all())
