@@ -9,7 +9,8 @@
 //   Tokens become fp16 by a power of two that takes the largest of the block's share of them to [2^14, 2^15).  That is exact for bf16
 // values down to 2^-31 of it (fp16 2^-28, E4M3 2^-35).  Where the smallest is below, or tokens are fp32, what is left over goes through
 // the same products again as another part on a finer scale: one pass for nearly all bf16 tokens, two for fp32, and always as many
-// as bring the parts within 2^-23 of every value.
+// as bring the parts within 2^-23 of every value.  A pass goes over the matrix again: one token of 4096 x 14336 takes 12.5 us, 21.6 where one of its
+// values is 2^-50.
 //   MMAs cut what an fp32 sum does not hold.  Sums of fp32 tokens are therefore added up, rounded, after each group (MXFP4) or box (NVFP4): one token of
 // 4096 x 14336 is within 2e-7 of its sum (in one piece 1.4e-6, and no faster).
 //   A block per SM keeps its tokens in shared memory and has a run of row tiles.  Of up to 16 of them at a turn, its 16 warps take equal

@@ -279,7 +279,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residu
 
     ``quant``: None for y in x's type; "row" or "block" for ``ScaledActivations``, E4M3 values with a fp32 scale per row
     (max|y| / 448) or an E8M0 scale per 32 values (the smallest power of two that keeps them within 448).  A row or block
-    that is not finite has NaN for scale and values.
+    that is not finite has NaN for scale and values.  Squares are summed in fp32: a row whose squares pass its range, with values of some 10^19, has an infinite
+    root mean square, and y is zero.
 
     Without ``quant`` there are gradients for x, residual and weight: first ones, backwards."""
     try:
@@ -363,8 +364,10 @@ class _Matvec(torch.autograd.Function):
 def matvec(x, weight: ScaledWeight, *, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``y[..., n] = sum_k x[..., k] W[n, k]`` with a 4-bit matrix, for one token or many.
 
-    x is fp32, fp16 or bf16 of shape [..., cols], or ``ScaledActivations``.  Sums are fp32, rounded once to ``out_dtype``
-    (x's type; bf16 for ScaledActivations).  The gradient goes back to a plain x, from the output's type and rounded once to x's: the
+    x is fp32, fp16 or bf16 of shape [..., cols], or ``ScaledActivations``, at most 2^19 tokens.  Sums are fp32, rounded once to ``out_dtype``
+    (x's type; bf16 for ScaledActivations); tensor cores cut, in them, what fp32 does not hold: fp32 results are within some 1e-6 of their norm.  fp32 tokens
+    are taken to 2^-23 of their value where they are few, and whole otherwise.  Where tokens are few, values beyond 2^28 (fp32) or 2^31 (bf16) apart cost
+    another pass over the matrix.  The gradient goes back to a plain x, from the output's type and rounded once to x's: the
     first one, backwards.  ScaledActivations and the matrix have none."""
     if not isinstance(weight, ScaledWeight):
         raise TypeError(f"weight is a ScaledWeight, got {type(weight).__name__}")
