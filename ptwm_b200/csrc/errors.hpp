@@ -17,14 +17,21 @@ inline int64_t fail(int64_t rc, const std::string& m) { last_error_ref() = m; re
 #define CUDA_TRY(expr)                                                                                        \
     do {                                                                                                      \
         cudaError_t e_ = (expr);                                                                              \
-        if (e_ != cudaSuccess) return ::ptwm::fail(PTWM_RC_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e_)); \
+        if (e_ != cudaSuccess) {                                                                              \
+            cudaGetLastError(); /* reported here: the thread's next call does not find it again */            \
+            return ::ptwm::fail(PTWM_RC_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e_));            \
+        }                                                                                                     \
     } while (0)
 
 // Makes `dev` current for the scope and restores the previous device.
 struct DeviceGuard {
     int prev = -1;
     cudaError_t err;
-    explicit DeviceGuard(int dev) { err = cudaGetDevice(&prev); if (err == cudaSuccess && prev != dev) err = cudaSetDevice(dev); }
+    explicit DeviceGuard(int dev) {
+        err = cudaGetDevice(&prev);
+        if (err == cudaSuccess && prev != dev) err = cudaSetDevice(dev);
+        if (err != cudaSuccess) cudaGetLastError();  // `err` has it: the thread's next call does not find it again
+    }
     ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
 };
 

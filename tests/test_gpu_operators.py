@@ -1041,3 +1041,12 @@ def test_a_long_sum_of_few_fp32_tokens_does_not_lose_what_is_small(tokens, kind)
     x = torch.ones(tokens, k, device="cuda")
     x[:, 0] = 2.0 ** 28
     assert bool(((matvec(x, w).double() - (2.0 ** 28 + k - 1)).abs() <= 255 + 16).all())
+
+
+def test_a_call_that_failed_leaves_no_error_to_the_next():
+    blob = oracle.write_container([spec_norm("n.weight", 4096, 3)], chunk_size=4096, menu=(oracle.RANS,))
+    want = ptwm_b200.ContainerHandle(blob).decode("n.weight")
+    L = ptwm_b200._lib.lib()
+    for rc in (lambda: L.ptwm_b200_operator_status(1000), lambda: L.ptwm_b200_rms_norm(want.data_ptr(), 0, want.data_ptr(), 0, want.data_ptr(), 0, 1, 8, 1, 1, 0, 1e-6, 1000, 1)):
+        assert rc() == -7 and "ordinal" in ptwm_b200._lib.last_error()
+        assert torch.equal(ptwm_b200.ContainerHandle(blob).decode("n.weight"), want)
