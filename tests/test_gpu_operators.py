@@ -959,15 +959,15 @@ def test_8_bit_tokens_whose_gradient_would_be_lost_are_refused():
 
 
 def test_a_call_with_too_little_scratch_writes_nothing():
-    few, many = ScaledWeight(*_matrix(16, 6144, "mxfp4", 1)), ScaledWeight(*_matrix(14336, 6144, "mxfp4", 2))
-    x = _integers(16, 6144, torch.float16, 3)
-    ys = [torch.full((16, w.rows), 7.0, device="cuda", dtype=torch.float16) for w in (few, many)]
+    few, many = ScaledWeight(*_matrix(16, 8192, "mxfp4", 1)), ScaledWeight(*_matrix(14336, 8192, "mxfp4", 2))
+    x = _integers(12, 8192, torch.float16, 3)
+    ys = [torch.full((12, w.rows), 7.0, device="cuda", dtype=torch.float16) for w in (few, many)]
     refs, at = (ctypes.c_uint64 * 2)(few._ref, many._ref), (ctypes.c_uint64 * 2)(*[y.data_ptr() for y in ys])
     torch.cuda.synchronize()
-    assert ptwm_b200._lib.lib().ptwm_b200_matvec_group(refs, at, 2, x.data_ptr(), 0, 16, 4, 0, 4, 0, 0, 0, 1) == -2
+    assert ptwm_b200._lib.lib().ptwm_b200_matvec_group(refs, at, 2, x.data_ptr(), 0, 12, 4, 0, 4, 0, 0, 0, 1) == -2
     torch.cuda.synchronize()
     assert all(bool((y == 7.0).all()) for y in ys)
-    norm = torch.ones(6144, device="cuda", dtype=torch.float16)
+    norm = torch.ones(8192, device="cuda", dtype=torch.float16)
     for y, w in zip(Projection(norm, [few, many])(x)[0], (few, many)):
         assert torch.equal(y, matvec(rms_norm(x, norm), w))
 

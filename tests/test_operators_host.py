@@ -172,15 +172,15 @@ def test_norms_of_rows_that_32_bits_do_not_count(L, cols):
 
 
 def test_scratch_is_looked_at_before_any_launch(L):
-    """A few rows of 6144 columns want none for 16 tokens, many do: a call for both says so before it touches the device."""
-    few, many = _weight(rows=16, cols=6144, value_pitch=6144 // 2, scale_pitch=192), _weight(rows=14336, cols=6144, value_pitch=6144 // 2, scale_pitch=192)
-    assert L.ptwm_b200_matvec_scratch_bytes(C.addressof(few), A, 16, 4, 0) == 0
-    need = L.ptwm_b200_matvec_scratch_bytes(C.addressof(many), A, 16, 4, 0)
-    assert need == 2 * 16 * 6144 * 2
+    """A few rows of 8192 columns want none for 12 tokens, many do: a call for both says so before it touches the device."""
+    few, many = _weight(rows=16, cols=8192, value_pitch=4096, scale_pitch=256), _weight(rows=14336, cols=8192, value_pitch=4096, scale_pitch=256)
+    assert L.ptwm_b200_matvec_scratch_bytes(C.addressof(few), A, 12, 4, 0) == 0
+    need = L.ptwm_b200_matvec_scratch_bytes(C.addressof(many), A, 12, 4, 0)
+    assert need == 2 * 12 * 8192 * 2
     refs, ys = (C.c_uint64 * 2)(C.addressof(few), C.addressof(many)), (C.c_uint64 * 2)(A, A)
     for scratch, size, rc in [(0, 0, SMALL), (0, need, SMALL), (A, need - 1, SMALL), (A + 8, need, INVALID)]:
-        assert L.ptwm_b200_matvec_group(refs, ys, 2, A, 0, 16, 4, 0, 4, scratch, size, 0, 1) == rc
-    assert L.ptwm_b200_matvec(C.addressof(many), A, 0, A, 16, 4, 0, 4, 0, 0, 0, 1) == SMALL
+        assert L.ptwm_b200_matvec_group(refs, ys, 2, A, 0, 12, 4, 0, 4, scratch, size, 0, 1) == rc
+    assert L.ptwm_b200_matvec(C.addressof(many), A, 0, A, 12, 4, 0, 4, 0, 0, 0, 1) == SMALL
 
 
 def test_a_projection_keeps_its_norm_and_matrices(monkeypatch):
