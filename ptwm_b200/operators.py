@@ -47,7 +47,13 @@ def _on_cuda(what: str, t: Any, device: Optional[torch.device] = None) -> None:
 def operator_status(device: Union[None, int, str, torch.device] = None) -> int:
     """0, or 1 from when on a wait inside a kernel of these operators has given up on the device (the current one where it is None).
     Waits for the device."""
-    index = device if isinstance(device, int) or device is None else torch.device(device).index
+    if device is None or isinstance(device, int):
+        index = device
+    else:
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"{device} is no CUDA device")
+        index = device.index
     return _check(_lib.lib().ptwm_b200_operator_status(torch.cuda.current_device() if index is None else index))
 
 

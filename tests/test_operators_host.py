@@ -203,3 +203,8 @@ def test_the_status_of_a_device_that_is_none(L):
         ptwm_b200.operator_status(0)
     with pytest.raises(ptwm_b200.PtwmError):
         ptwm_b200.operator_status("cuda:1")
+
+
+def test_only_cuda_devices_have_a_status():
+    with pytest.raises(ValueError, match="cpu"):
+        ptwm_b200.operator_status("cpu")
